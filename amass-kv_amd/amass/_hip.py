@@ -20,6 +20,7 @@ _F64 = C.c_double
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libamass_hip.so")
 ABI_VERSION = 11    # AMASS_ABI_VERSION of include/amass_hip.h these mirrors follow
+CHUNK_ABI_VERSION = 1    # AMASS_CHUNK_ABI_VERSION of include/amass_chunk.h
 
 
 class AmassError(RuntimeError):
@@ -138,6 +139,35 @@ class ScatterArgs(C.Structure):
         "n_tokens:i32 n_kv:i32 d:i32 page:i32 nv:i32")
 
 
+# include/amass_chunk.h
+class ExtendArgs(C.Structure):
+    _fields_ = _fields(
+        "block_table:p bt_st:i64 seq_lens:p query_start:p free_list:p top:p top_out:p slots:p "
+        "positions:p n_req:i32 n_tokens:i32 max_pages:i32 page:i32 nb:i32 capacity:i32")
+
+
+class ReleaseArgs(C.Structure):
+    _fields_ = _fields(
+        "block_table:p bt_st:i64 seq_lens:p done:p free_list:p top:p n_req:i32 max_pages:i32 "
+        "page:i32 nb:i32 capacity:i32")
+
+
+class RopeArgs(C.Structure):
+    _fields_ = _fields(
+        "q:p q_st:i64 q_hs:i64 k:p k_st:i64 k_hs:i64 v:p v_st:i64 v_hs:i64 q_out:p qo_st:i64 "
+        "qo_hs:i64 k_cache:p kc_sb:i64 kc_st:i64 kc_sh:i64 v_cache:p vc_sb:i64 vc_st:i64 "
+        "vc_sh:i64 table:p tab_st:i64 positions:p slots:p n_tokens:i32 n_heads:i32 n_kv:i32 "
+        "d:i32 rot:i32 page:i32 nb:i32 max_pos:i32 interleaved:i32 dtype:i32")
+
+
+class ChunkArgs(C.Structure):
+    _fields_ = _fields(
+        "q:p q_st:i64 q_hs:i64 k:p k_sb:i64 k_st:i64 k_sh:i64 v:p v_sb:i64 v_st:i64 v_sh:i64 "
+        "block_table:p bt_st:i64 seq_lens:p query_start:p out:p o_st:i64 o_hs:i64 lse:p "
+        "l_st:i64 l_hs:i64 scratch:p scratch_bytes:i64 scale:f32 n_req:i32 n_tokens:i32 "
+        "n_kv:i32 G:i32 d:i32 page:i32 nb:i32 max_pages:i32 causal:i32 window:i32 dtype:i32")
+
+
 STRUCTS = {
     "amass_quad_score_args": (0, QuadScoreArgs),
     "amass_r8_score_args": (1, R8ScoreArgs),
@@ -153,6 +183,14 @@ STRUCTS = {
     "amass_invalidate_args": (11, InvalidateArgs),
     "amass_stage_args": (12, StageArgs),
     "amass_scatter_args": (13, ScatterArgs),
+}
+
+# those of include/amass_chunk.h (amass_chunk_struct_size)
+CHUNK_STRUCTS = {
+    "amass_extend_args": (0, ExtendArgs),
+    "amass_release_args": (1, ReleaseArgs),
+    "amass_rope_args": (2, RopeArgs),
+    "amass_chunk_args": (3, ChunkArgs),
 }
 
 # entry point -> argument struct (None = custom signature)
@@ -174,6 +212,10 @@ ENTRY_POINTS = {
     "amass_tier_invalidate": InvalidateArgs,
     "amass_stage_begin_step": StageArgs,
     "amass_stage_scatter": ScatterArgs,
+    "amass_extend": ExtendArgs,
+    "amass_release": ReleaseArgs,
+    "amass_rope_write": RopeArgs,
+    "amass_chunk_attention": ChunkArgs,
 }
 
 _CODES = {_P: "P", _I64: "q", _I32: "i", _F32: "f", _F64: "d"}
@@ -215,6 +257,14 @@ def _prototypes(lib) -> None:
     lib.amass_binding_block_list.restype = C.c_int
     lib.amass_binding_begin_step.argtypes = [C.POINTER(InvalidateArgs), C.POINTER(StageArgs), _P]
     lib.amass_binding_begin_step.restype = C.c_int
+    lib.amass_chunk_scratch_bytes.argtypes = [C.POINTER(ChunkArgs)]
+    lib.amass_chunk_scratch_bytes.restype = _I64
+    lib.amass_chunk_abi_version.restype = C.c_int
+    lib.amass_chunk_struct_size.argtypes = [C.c_int]
+    lib.amass_chunk_struct_size.restype = C.c_size_t
+    if lib.amass_chunk_abi_version() != CHUNK_ABI_VERSION:
+        raise AmassError(f"{LIB_PATH} has chunk ABI version {lib.amass_chunk_abi_version()}, "
+                         f"these bindings expect {CHUNK_ABI_VERSION}: rebuild it")
 
 
 def load_library(path: str = LIB_PATH) -> C.CDLL:
@@ -261,6 +311,27 @@ def call(name: str, args, stream: int) -> None:
     rc = getattr(_LIB or load_library(), name)(C.byref(args), stream)
     if rc != 0:
         check(rc, name)
+
+
+def call_on(device, name: str, args) -> None:
+    """`call` on torch's current stream of the tensors' `device`, which need not be the
+    current one."""
+    import torch
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        call(name, args, current_stream(device))
+    else:
+        with torch.cuda.device(index):
+            call(name, args, current_stream(device))
+
+
+def same_device(first, *others) -> None:
+    """The tensors of one call lie on one GPU."""
+    require_cuda(first, *others)
+    d = first.device
+    for t in others:
+        if t is not None and t.device != d:
+            raise ValueError(f"tensors on {d} and {t.device} in one call")
 
 
 def call_select_attend(score, select, decode, mode: int, tickets, wgs_per_unit: int,

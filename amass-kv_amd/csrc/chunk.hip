@@ -1,0 +1,1010 @@
+// Attention of a chunk of new tokens over the paged cache for gfx950 (amass_chunk_attention).
+//
+// Mathematics.  The rows of (request, kv head) are its n new tokens times the G query heads
+// of the group (row rho: token rho / G, head rho % G), so a K / V tile serves all of them.
+// A workgroup of four waves takes CK_BM rows (a row tile) and walks keys 64 at a time with
+// the running maximum m, sum l and unnormalised output O of a softmax:
+//   S^T[key][row] = K Q^T     v_mfma 32x32x16, A = K rows (LDS), B = Q^T (registers)
+//   p = 2^(c s - c m), c = scale log2 e        one fma and one exp2 per score
+//   O^T[d][row] += V^T P^T    A = V^T (LDS, transposing 64-bit reads), B = P^T
+// In S^T a lane holds one row's scores (column = lane % 32), so the row maximum is a chain of
+// v_max in the lane and one exchange with lane ^ 32, the rescale one factor per lane, and the
+// accumulator registers of S^T, packed to 16 bits, already are the B operand of the second
+// product: the contraction order over keys is free, and V^T is read in the order they have.
+//
+// K and V go from HBM to LDS with 16-byte direct loads (no registers), each lane's source
+// chosen so that the LDS image is swizzled: 16-byte chunk c of row t is at chunk
+// c ^ swz(t), which spreads both the K reads (16 rows, one chunk) and the transposing V reads
+// (4 rows, 2 chunks) over the banks.
+//
+// Two layouts, chosen per row tile:
+//   many (more than 32 rows): wave w owns rows 32 w .. 32 w + 31; the workgroup shares each
+//     64-key tile, double-buffered (2 x 32 KB at d = 128), one barrier per tile.
+//   few (32 rows or less: single tokens, drafts, a chunk's remainder): the rows fit one wave,
+//     so the waves take 32 keys each in turn, each with a K and a V buffer of its own and no
+//     barrier, and merge their (m, l, O) through LDS at the end.
+// Splitting.  A row tile of many keys is cut into S parts when the batch has fewer tiles
+// than the chip has room for (plan below, on the device: the launch needs no lengths on the
+// host and can be captured); parts leave (m, l, O) in scratch and a second launch joins them.
+#include "../../include/amass_chunk.h"
+#include "common.h"
+
+namespace amass {
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+constexpr int CK_WAVES = 4;
+constexpr int CK_BM = 32 * CK_WAVES;       // rows of a row tile
+constexpr int CK_FEW = 32;                 // rows up to which the waves share the rows
+constexpr int CK_KEYS = 64;                // keys of a tile
+constexpr int CK_MIN_SPLIT = 4;            // fewest tiles of a part
+constexpr float CK_LAZY = 8.f;             // a maximum may lag by this power of two
+
+// ------------------------------------------------------------------ the 16-bit types
+template <int DT>
+__device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+    if constexpr (DT == AMASS_BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                       __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
+                                                      __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {       // to nearest even
+    if constexpr (DT == AMASS_BF16) return pack_bf16x2(lo, hi);
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){lo, hi}, f16x2_t));
+}
+// bits 15 / 31 set where a half of x is an infinity or a NaN
+template <int DT>
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t x) {
+    return DT == AMASS_BF16 ? (x & 0x7F807F80u) + 0x00800080u : (x & 0x7C007C00u) + 0x04000400u;
+}
+
+// ------------------------------------------------------------------ LDS
+// XOR of a row's 16-byte chunks: the 16 rows of a K read land in 16 places of the 256 bytes
+// that the banks serve, and 4 rows of a transposing V read in different chunk pairs.
+template <int D>
+__device__ __forceinline__ int swz(int row) {
+    return D == 128 ? ((row & 7) << 1) | ((row >> 3) & 1)
+                    : (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
+}
+
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+// 16 bytes per lane from base + off (off per lane) to LDS at `to` + 16 lane (`to` uniform).
+// No register waits for it: the caller waits with dma_wait before anyone reads the place.
+__device__ __forceinline__ void dma16(uint32_t to, const char* base, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(to), "v"(off), "s"(base)
+                 : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void dma_wait() {        // all but the last N loads have arrived
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory");
+}
+// four 16-bit values down a column of a 4-row block (lane i of 16: row i / 4, chunk half i % 4;
+// returns column i)
+__device__ __forceinline__ u32x2_t lds_tr4(uint32_t addr) {
+    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4_t*)(uintptr_t)addr));
+}
+
+// ------------------------------------------------------------------ ranges and plan
+struct ChunkPlan {
+    int sh;              // log2 page
+    int cap;             // positions that a block-table row covers
+    int target;          // workgroups per kv head that fill the chip
+    int slots;           // scratch slots per kv head
+    int slot_rows;       // rows of a slot
+    int tiles_max;       // row tiles of the batch at most
+    int64_t flag_bytes;  // of the items' flags, before the slots
+};
+
+struct Span {            // keys [64 lo, 64 lo + 64 n) hold the visible ones below hi
+    int lo, n, hi;
+};
+
+struct Req {
+    int q0, n, len;      // first row, new tokens, tokens
+};
+
+__device__ __forceinline__ Req load_req(const amass_chunk_args& a, int r) {
+    Req q;
+    q.q0 = min(max(a.query_start[r], 0), a.n_tokens);
+    q.n = max(min(max(a.query_start[r + 1], 0), a.n_tokens) - q.q0, 0);
+    q.len = max(a.seq_lens[r], 0);
+    return q;
+}
+__device__ __forceinline__ int row_tiles(const amass_chunk_args& a, const Req& q) {
+    return (int)(((int64_t)q.n * a.G + CK_BM - 1) / CK_BM);
+}
+
+// visible keys [lo, hi) of the token at position p
+__device__ __forceinline__ int key_hi(const amass_chunk_args& a, const ChunkPlan& pl, int len, int p) {
+    const int l = min(len, pl.cap);
+    return p < 0 ? 0 : a.causal ? min(l, p + 1) : l;
+}
+__device__ __forceinline__ int key_lo(const amass_chunk_args& a, int p) {
+    return a.window > 0 ? max(0, p - a.window + 1) : 0;
+}
+__device__ __forceinline__ Span tile_span(const amass_chunk_args& a, const ChunkPlan& pl,
+                                          const Req& q, int tile) {
+    const int r0 = tile * CK_BM, r1 = min(q.n * a.G, r0 + CK_BM) - 1;
+    const int p0 = q.len - q.n + r0 / a.G, p1 = q.len - q.n + r1 / a.G;
+    Span s;
+    s.hi = key_hi(a, pl, q.len, p1);
+    s.lo = key_lo(a, p0) / CK_KEYS;
+    s.n = max(0, (s.hi + CK_KEYS - 1) / CK_KEYS - s.lo);
+    return s;
+}
+// the most tiles of keys that a row tile of the request has
+__device__ __forceinline__ int req_work(const amass_chunk_args& a, const ChunkPlan& pl,
+                                        const Req& q, int tiles) {
+    int w = 0;
+    if (tiles > 0) w = tile_span(a, pl, q, tiles - 1).n;
+    if (tiles > 1) w = max(w, tile_span(a, pl, q, tiles - 2).n);
+    return w;
+}
+
+struct Item {
+    int r, tile, part, parts;
+    int item, slot;      // of part 0 (MERGE) or of this part
+    Req q;
+};
+
+// Parts of a row tile: the request's longest tile decides, tiles S_r = ceil(w_r / len) for
+// the smallest part length `len` >= max(CK_MIN_SPLIT, sum_r tiles_r w_r / target) at which
+// the batch has at most `target` items (workgroups per kv head), or the first such length
+// where the row tiles alone are that many (only tiles much longer than the average are cut
+// then).  Item y of the batch: requests in order, a request's last (causal: longest) tile
+// first.
+__device__ __forceinline__ int count_items(const amass_chunk_args& a, const ChunkPlan& pl,
+                                           int t0, int w0, int len) {
+    const int lane = threadIdx.x & 63;
+    int tot = wave_sum_uniform(t0 * max(1, (w0 + len - 1) / len));
+    for (int base = WAVE; base < a.n_req; base += WAVE) {
+        int n = 0;
+        if (base + lane < a.n_req) {
+            const Req q = load_req(a, base + lane);
+            const int t = row_tiles(a, q), w = req_work(a, pl, q, t);
+            n = t * max(1, (w + len - 1) / len);
+        }
+        tot += wave_sum_uniform(n);
+    }
+    return tot;
+}
+
+// Item y (`merge`: row tile y) of the batch; false past the end.
+template <bool MERGE>
+__device__ __forceinline__ bool find_item(const amass_chunk_args& a, const ChunkPlan& pl, int y,
+                                          Item& it) {
+    const int lane = threadIdx.x & 63;
+    Req q = {0, 0, 0};
+    if (lane < a.n_req) q = load_req(a, lane);
+    const int t0 = row_tiles(a, q), w0 = req_work(a, pl, q, t0);
+    float work = (float)t0 * (float)w0;
+    int tiles = wave_sum_uniform(t0), longest = wave_max_uniform(w0);
+    for (int base = WAVE; base < a.n_req; base += WAVE) {
+        Req x = {0, 0, 0};
+        if (base + lane < a.n_req) x = load_req(a, base + lane);
+        const int t = row_tiles(a, x), w = req_work(a, pl, x, t);
+        work += (float)t * (float)w;
+        tiles += wave_sum_uniform(t);
+        longest = max(longest, wave_max_uniform(w));
+    }
+    int len = max(CK_MIN_SPLIT, (int)ceilf(wave_sumf(work) / (float)pl.target));
+    if (len >= longest) {
+        len = max(longest, 1);                          // no tile is cut
+    } else if (tiles < pl.target && count_items(a, pl, t0, w0, len) > pl.target) {
+        int lo = len + 1, hi = longest;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (count_items(a, pl, t0, w0, mid) <= pl.target) hi = mid;
+            else lo = mid + 1;
+        }
+        len = lo;
+    }
+    int before = 0, items = 0, slots = 0;                // those of earlier requests
+    for (int base = 0; base < a.n_req; base += WAVE) {
+        Req x = q;
+        int t = t0, w = w0;
+        if (base > 0) {
+            x = {0, 0, 0};
+            if (base + lane < a.n_req) x = load_req(a, base + lane);
+            t = row_tiles(a, x);
+            w = req_work(a, pl, x, t);
+        }
+        const int S = max(1, (w + len - 1) / len);
+        const int ni = t * S, n = MERGE ? t : ni, ns = S > 1 ? ni : 0;
+        const int incl_i = wave_incl_scan(ni), incl_s = wave_incl_scan(ns);
+        const int incl = MERGE ? wave_incl_scan(n) : incl_i;
+        const int all = __builtin_amdgcn_readlane(incl, WAVE - 1);
+        if (y < before + all) {
+            const int src = __ffsll((long long)__ballot(before + incl > y)) - 1;
+            const int at = y - before - __builtin_amdgcn_readlane(incl - n, src);
+            const int s = __builtin_amdgcn_readlane(S, src);
+            it.r = base + src;
+            it.parts = s;
+            it.tile = __builtin_amdgcn_readlane(t, src) - 1 - (MERGE ? at : at / s);
+            it.part = MERGE ? 0 : at % s;
+            const int in_req = MERGE ? at * s : at;
+            it.item = items + __builtin_amdgcn_readlane(incl_i - ni, src) + in_req;
+            it.slot = slots + __builtin_amdgcn_readlane(incl_s - ns, src) + in_req;
+            it.q.q0 = __builtin_amdgcn_readlane(x.q0, src);
+            it.q.n = __builtin_amdgcn_readlane(x.n, src);
+            it.q.len = __builtin_amdgcn_readlane(x.len, src);
+            return true;
+        }
+        before += all;
+        items += __builtin_amdgcn_readlane(incl_i, WAVE - 1);
+        slots += __builtin_amdgcn_readlane(incl_s, WAVE - 1);
+    }
+    return false;
+}
+
+// tiles of keys per part of a row tile of n, and its parts (a short tile has fewer than its
+// request's longest)
+__device__ __forceinline__ int part_len(int n, int parts) { return max(1, (n + parts - 1) / parts); }
+
+// ------------------------------------------------------------------ one wave's state
+template <int D>
+struct RowState {
+    f32x16_t o[D / 32];      // O^T: d = 32 x + 8 (i / 4) + 4 (lane / 32) + i % 4, row lane % 32
+    float m, l;              // maximum (raw score); this lane's half of the sum
+};
+
+template <int D>
+__device__ __forceinline__ void reset(RowState<D>& st) {
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st.o[x][i] = 0.f;
+    st.m = -__FLT_MAX__;
+    st.l = 0.f;
+}
+
+// Byte offset in a V image of lane (h, sub, i16)'s part of a transposing read: d tile x, the
+// four keys from 8 e + 4 h.
+template <int D>
+__device__ __forceinline__ uint32_t v_place(int x, int e, int i16, int h, int sub) {
+    const int t = 8 * e + 4 * h + (i16 >> 2);
+    const int c = 4 * x + 2 * sub + ((i16 >> 1) & 1);
+    return t * (2 * D) + ((c ^ swz<D>(t)) << 4) + (i16 & 1) * 8;
+}
+
+// Lane constants of the LDS reads (byte offsets within a K or V image).
+template <int D>
+struct LdsLane {
+    uint32_t k[D / 16];      // chunk of MFMA i, key row lane % 32
+    uint32_t v[D / 32][2];   // 4-row block (keys 4 h .. and 8 + 4 h ..), d tile x
+    __device__ __forceinline__ LdsLane(int lane) {
+        const int row = lane & 31, h = lane >> 5, i16 = lane & 15, sub = (lane >> 4) & 1;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+            k[i] = row * (2 * D) + (((2 * i + h) ^ swz<D>(row)) << 4);
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) v[x][e] = v_place<D>(x, e, i16, h, sub);
+    }
+};
+
+// S^T of 32 NK keys
+template <int DT, int D, int NK>
+__device__ __forceinline__ void scores(const char* ks, const LdsLane<D>& ll,
+                                       const u32x4_t (&q)[D / 16], f32x16_t (&s)[NK]) {
+#pragma unroll
+    for (int x = 0; x < NK; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[x][i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int x = 0; x < NK; ++x) {
+            const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(ks + ll.k[i] + x * (64 * D));
+            s[x] = mfma32<DT>(kf, q[i], s[x]);
+        }
+}
+
+// -inf for the keys (relative to the tile) outside [lo, hi) of this lane's row, and those of
+// 16-key groups without a block
+template <int NK>
+__device__ __forceinline__ void mask_scores(f32x16_t (&s)[NK], int lo, int hi, uint32_t groups,
+                                            int lane) {
+    const int h4 = 4 * (lane >> 5);
+    lo -= h4;
+    hi -= h4;
+#pragma unroll
+    for (int x = 0; x < NK; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int key = 32 * x + 8 * (i >> 2) + (i & 3);
+            const bool see = key >= lo && key < hi && (groups >> (2 * x + (i >> 3)) & 1);
+            s[x][i] = see ? s[x][i] : -INFINITY;
+        }
+}
+
+// Running softmax: s -> packed weights p (B operand of 16-key step y: p[y]), st.m, st.l and
+// the rescale of st.o.  The maximum may lag the true one by 2^CK_LAZY, which the weights (up
+// to 2^8) and fp32 sums hold exactly as well, so most tiles skip the rescale.
+template <int DT, int D, int NK>
+__device__ __forceinline__ void softmax(f32x16_t (&s)[NK], float c, RowState<D>& st,
+                                        u32x4_t (&p)[2 * NK]) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int x = 0; x < NK; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[x][i]);
+    mx = xor32_maxf(mx);
+    if (__any((mx - st.m) * c > CK_LAZY)) {
+        const float m = fmaxf(st.m, mx);
+        const float al = __builtin_amdgcn_exp2f((st.m - m) * c);
+        st.m = m;
+        st.l *= al;
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) st.o[x][i] *= al;
+    }
+    const float mc = fmaxf(st.m * c, -__FLT_MAX__);
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < NK; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[x][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], c, -mc));
+            sum[i & 3] += s[x][i];
+        }
+    st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+    for (int y = 0; y < 2 * NK; ++y)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            p[y][j] = pack2<DT>(s[y >> 1][8 * (y & 1) + 2 * j], s[y >> 1][8 * (y & 1) + 2 * j + 1]);
+}
+
+template <int D>
+__device__ __forceinline__ u32x4_t v_frag(uint32_t vs, const LdsLane<D>& ll, int x, int y) {
+    const u32x2_t a = lds_tr4(vs + ll.v[x][0] + y * (32 * D));
+    const u32x2_t b = lds_tr4(vs + ll.v[x][1] + y * (32 * D));
+    return (u32x4_t){a[0], a[1], b[0], b[1]};
+}
+
+template <int DT, int D, int NK>
+__device__ __forceinline__ void weigh(uint32_t vs, const LdsLane<D>& ll, const u32x4_t (&p)[2 * NK],
+                                      RowState<D>& st) {
+#pragma unroll
+    for (int y = 0; y < 2 * NK; ++y)
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+            st.o[x] = mfma32<DT>(v_frag<D>(vs, ll, x, y), p[y], st.o[x]);
+}
+
+// whether any V value of the 32 NK keys is an infinity or a NaN
+template <int DT, int D, int NK>
+__device__ __forceinline__ bool any_nonfinite(uint32_t vs, const LdsLane<D>& ll) {
+    uint32_t bad = 0;
+#pragma unroll
+    for (int y = 0; y < 2 * NK; ++y)
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {
+            const u32x4_t v = v_frag<D>(vs, ll, x, y);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bad |= nonfinite2<DT>(v[j]);
+        }
+    return __any((bad & 0x80008000u) != 0);
+}
+
+// ------------------------------------------------------------------ staging
+// The 16 keys from t of one request: K rows to LDS at `kd`, V rows at `vd` (16 rows of 2 D
+// bytes, swizzled).  Rows at or past `len` hold nothing of the request: their V is zero (the
+// weight of a masked key is zero, and zero times what lies there could be NaN).
+template <int D>
+struct Stage {
+    static constexpr int ROWS = 512 / D;           // rows of one 1-KB load
+    static constexpr int LOADS = 16 / ROWS;
+    uint32_t k[LOADS], v[LOADS];                   // this lane's source offsets
+    int lane;
+    __device__ __forceinline__ Stage(const amass_chunk_args& a, int lane_) : lane(lane_) {
+        const int chunk = lane & (D / 8 - 1), lr = lane / (D / 8);
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) {
+            const int row = ROWS * n + lr;
+            const uint32_t c = (chunk ^ swz<D>(row)) << 4;
+            k[n] = (uint32_t)(2 * row * a.k_st) + c;
+            v[n] = (uint32_t)(2 * row * a.v_st) + c;
+        }
+    }
+    __device__ __forceinline__ void load_k(uint32_t to, const char* src) const {
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) dma16(to + 1024 * n, src, k[n]);
+    }
+    __device__ __forceinline__ void load_v(uint32_t to, const char* src) const {
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) dma16(to + 1024 * n, src, v[n]);
+    }
+    // the first `rows` rows, zero behind them
+    __device__ __forceinline__ void load_v_part(char* dst, uint32_t to, const char* src,
+                                                int rows) const {
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) {
+            if (ROWS * n + lane / (D / 8) < rows) dma16(to + 1024 * n, src, v[n]);
+            else *reinterpret_cast<u32x4_t*>(dst + 1024 * n + 16 * lane) = (u32x4_t){0u, 0u, 0u, 0u};
+        }
+    }
+};
+
+// Uniform view of a unit's pages.
+struct Pages {
+    const __attribute__((address_space(4))) int32_t* table;   // the request's row
+    const char* k;
+    const char* v;                                            // of the kv head
+    int64_t k_sb, k_st, v_sb, v_st;                           // bytes
+    int sh, nb;
+    // block of the 16 keys from t, -1 if the pool has none such
+    __device__ __forceinline__ int block(int t) const {
+        const int b = table[t >> sh];
+        return b >= 0 && b < nb ? b : -1;
+    }
+    __device__ __forceinline__ const char* k_at(int b, int t) const {
+        return k + b * k_sb + (t & ((1 << sh) - 1)) * k_st;
+    }
+    __device__ __forceinline__ const char* v_at(int b, int t) const {
+        return v + b * v_sb + (t & ((1 << sh) - 1)) * v_st;
+    }
+};
+
+// ------------------------------------------------------------------ results
+// Rows of a wave, normalised: 16 bytes per store after an exchange between the half waves
+// (lane l: d 32 x + 16 u .. + 7, lane l + 32: the next 8).
+template <int DT, int D>
+__device__ __forceinline__ void store_row(uint16_t* out, int x, const float (&o)[16], int lane) {
+    // (out: the row, null for none; x: the d tile)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        uint32_t e[2], f[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const auto s = __builtin_amdgcn_permlane32_swap(
+                pack2<DT>(o[8 * u + 2 * j], o[8 * u + 2 * j + 1]),
+                pack2<DT>(o[8 * u + 4 + 2 * j], o[8 * u + 4 + 2 * j + 1]), false, false);
+            e[j] = s[0];
+            f[j] = s[1];
+        }
+        if (out)
+            *reinterpret_cast<u32x4_t*>(out + 32 * x + 16 * u + 8 * (lane >> 5)) =
+                (u32x4_t){e[0], e[1], f[0], f[1]};
+    }
+}
+
+// scratch: four bytes per item (a wave's `bad`), then the slots.  A slot: per group of 32 rows D / 32 tiles of 16 x 64 floats, then m and l of 64 lanes
+template <int D>
+__device__ __forceinline__ float* slot_group(const amass_chunk_args& a, const ChunkPlan& pl, int kh,
+                                             int slot, int group) {
+    const int64_t at = ((int64_t)kh * pl.slots + slot) * (pl.slot_rows / 32) + group;
+    return reinterpret_cast<float*>((char*)a.scratch + pl.flag_bytes) + at * (32 * D + 2 * WAVE);
+}
+__device__ __forceinline__ uint8_t* item_flags(const amass_chunk_args& a, const ChunkPlan& pl, int kh,
+                                               int item) {
+    return (uint8_t*)a.scratch + ((int64_t)kh * (pl.tiles_max + pl.target) + item) * CK_WAVES;
+}
+
+template <int D>
+__device__ __forceinline__ void save_tile(float* g, int x, const float (&o)[16], int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4*>(g + (x * 4 + i) * 4 * WAVE + 4 * lane) =
+            make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+}
+
+struct RowOut {
+    uint16_t* out;       // the row, null for none
+    float* lse;
+};
+
+__device__ __forceinline__ RowOut row_out(const amass_chunk_args& a, const Req& q, int kh, int row) {
+    RowOut w = {nullptr, nullptr};
+    if (row < q.n * a.G) {
+        const int64_t t = q.q0 + row / a.G;
+        const int64_t h = kh * a.G + row % a.G;
+        w.out = (uint16_t*)a.out + t * a.o_st + h * a.o_hs;
+        if (a.lse) w.lse = a.lse + t * a.l_st + h * a.l_hs;
+    }
+    return w;
+}
+
+__device__ __forceinline__ void store_lse(const RowOut& w, float m, float l, float c, int lane) {
+    if (w.lse && lane < 32) {
+        const float mc = fmaxf(m * c, -__FLT_MAX__);
+        *w.lse = l == 0.f ? -INFINITY : (mc + __log2f(l)) * 0.693147180559945309f;
+    }
+}
+
+template <int D>
+struct __align__(1024) ChunkLds {
+    char kv[2 * 2 * CK_KEYS * 2 * D];              // staging, then the waves' O
+    float m[CK_WAVES][WAVE], l[CK_WAVES][WAVE];
+};
+
+// ------------------------------------------------------------------ kernel
+// grid: kv head fastest (workgroups of one kv head share an XCD's L2 where n_kv is a multiple
+// of 8), then the items.
+template <int DT, int D>
+__global__ __launch_bounds__(CK_WAVES * WAVE, 2) void chunk_kernel(const amass_chunk_args a,
+                                                                   const ChunkPlan pl) {
+    __shared__ ChunkLds<D> lds;
+    constexpr int KB = CK_KEYS * 2 * D;            // bytes of a K (or V) tile
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kh = blockIdx.x % a.n_kv;
+    Item it;
+    if (!find_item<false>(a, pl, blockIdx.x / a.n_kv, it)) return;
+    const Span sp = tile_span(a, pl, it.q, it.tile);
+    const int per = part_len(sp.n, it.parts);
+    const int j0 = min(sp.n, it.part * per), j1 = min(sp.n, j0 + per);   // tiles of this part
+    if (it.part > 0 && j0 >= j1) return;
+    const bool whole = per >= sp.n;                // no other part has keys
+    if (!whole && it.slot >= pl.slots) return;     // (only a query_start that does not ascend)
+    const int rows = min(CK_BM, it.q.n * a.G - it.tile * CK_BM);
+    const bool few = rows <= CK_FEW;
+    const int group = few ? 0 : w;                 // 32-row group of this wave
+    const int row = it.tile * CK_BM + 32 * group + (lane & 31);
+    const int last = it.tile * CK_BM + min(rows, 32 * group + 32) - 1;    // of the wave
+    const int start = it.q.len - it.q.n;
+    const float c = a.scale * 1.44269504088896341f;
+    Pages pg;
+    pg.table = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.block_table +
+                                                                             it.r * a.bt_st);
+    pg.k = (const char*)a.k + kh * a.k_sh * 2;
+    pg.v = (const char*)a.v + kh * a.v_sh * 2;
+    pg.k_sb = a.k_sb * 2;
+    pg.k_st = a.k_st * 2;
+    pg.v_sb = a.v_sb * 2;
+    pg.v_st = a.v_st * 2;
+    pg.sh = pl.sh;
+    pg.nb = a.nb;
+    const int len = min(it.q.len, pl.cap);
+    // this lane's visible keys; the wave's rows see at least [lo_hi, hi_lo), at most [lo_lo, hi_hi)
+    const bool live = row < it.q.n * a.G;
+    const int pos = start + row / a.G;
+    const int hi = live ? key_hi(a, pl, it.q.len, pos) : 0, lo = live ? key_lo(a, pos) : 0;
+    const int first = it.tile * CK_BM + 32 * group;
+    const bool idle = first > last;
+    const int p_first = start + first / a.G, p_last = start + last / a.G;
+    const int hi_lo = key_hi(a, pl, it.q.len, p_first), hi_hi = key_hi(a, pl, it.q.len, p_last);
+    const int lo_lo = key_lo(a, p_first), lo_hi = key_lo(a, p_last);
+
+    u32x4_t q[D / 16];
+    {
+        const uint16_t* src = (const uint16_t*)a.q + (int64_t)(it.q.q0 + row / a.G) * a.q_st +
+                              (int64_t)(kh * a.G + row % a.G) * a.q_hs + 8 * (lane >> 5);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+            q[i] = live ? *reinterpret_cast<const u32x4_t*>(src + 16 * i) : (u32x4_t){0u, 0u, 0u, 0u};
+    }
+    // (waited for here: a wait inside the key loop would also wait for the next tile's loads)
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(q[i]));
+    const LdsLane<D> ll(lane);
+    const Stage<D> stage(a, lane);
+    RowState<D> st;
+    reset(st);
+    bool bad = false;                              // a masked tile's V is not finite
+
+    if (!few) {
+        // ---- many rows: the workgroup shares the tiles -------------------------------------
+        const uint32_t base = lds_addr(lds.kv);
+        // wave w stages the 16 keys 64 j + 16 w ..; every wave knows which of the four have a block
+        const auto issue = [&](int j, int buf) -> uint32_t {
+            const int t0 = CK_KEYS * (sp.lo + j);
+            uint32_t ok = 0;
+            int mine = -1;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int t = t0 + 16 * g;
+                const int b = pg.block(t < sp.hi ? t : t0);
+                if (b >= 0 || t >= sp.hi) ok |= 1u << g;
+                if (g == w) mine = t < sp.hi ? b : -1;
+            }
+            const int t = t0 + 16 * w;
+            const uint32_t kd = base + 2 * KB * buf + 16 * w * 2 * D, vd = kd + KB;
+            if (mine >= 0) {
+                stage.load_k(kd, pg.k_at(mine, t));
+                if (t + 16 <= len) stage.load_v(vd, pg.v_at(mine, t));
+                else stage.load_v_part(lds.kv + (vd - base), vd, pg.v_at(mine, t), len - t);
+            } else {
+                stage.load_v_part(lds.kv + (vd - base), vd, pg.v, 0);
+            }
+            return ok;
+        };
+        uint32_t ok = j0 < j1 ? issue(j0, 0) : 0;
+        for (int j = j0; j < j1; ++j) {
+            const int buf = (j - j0) & 1;
+            dma_wait<0>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            const uint32_t groups = ok;
+            if (j + 1 < j1) ok = issue(j + 1, buf ^ 1);
+            const int t0 = CK_KEYS * (sp.lo + j);
+            if (idle || t0 >= hi_hi || t0 + CK_KEYS <= lo_lo) continue;
+            const char* ks = lds.kv + 2 * KB * buf;
+            const uint32_t vs = base + 2 * KB * buf + KB;
+            f32x16_t s[2];
+            u32x4_t p[4];
+            scores<DT, D, 2>(ks, ll, q, s);
+            const bool masked = t0 < lo_hi || t0 + CK_KEYS > hi_lo || groups != 15u;
+            if (masked) mask_scores<2>(s, lo - t0, hi - t0, groups, lane);
+            softmax<DT, D, 2>(s, c, st, p);
+            if (masked) bad |= any_nonfinite<DT, D, 2>(vs, ll);
+            weigh<DT, D, 2>(vs, ll, p, st);
+        }
+    } else {
+        // ---- few rows: each wave its own 32 keys, w + 4, w + 8, ... ------------------------
+        constexpr int HB = KB / 2;                 // 32 keys
+        char* own = lds.kv + 2 * HB * w;           // K, then V
+        const uint32_t base = lds_addr(own);
+        constexpr int LOADS = 2 * Stage<D>::LOADS;
+        const int b0 = 2 * (sp.lo + j0) + w, b1 = 2 * (sp.lo + j1);
+        uint32_t ok = 0;
+        int blk[2] = {-1, -1};
+        const auto find = [&](int b) {
+            ok = 0;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const int t = 32 * b + 16 * g;
+                blk[g] = t < sp.hi ? pg.block(t) : -1;
+                if (blk[g] >= 0 || t >= sp.hi) ok |= 1u << g;
+            }
+        };
+        // both return whether the usual number of loads is in flight
+        const auto issue_k = [&](int b) -> bool {
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+                if (blk[g] >= 0) stage.load_k(base + g * (HB / 2), pg.k_at(blk[g], 32 * b + 16 * g));
+            return blk[0] >= 0 && blk[1] >= 0;
+        };
+        const auto issue_v = [&](int b) -> bool {
+            if (blk[0] >= 0 && blk[1] >= 0 && 32 * b + 32 <= len) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+                    stage.load_v(base + HB + g * (HB / 2), pg.v_at(blk[g], 32 * b + 16 * g));
+                return true;
+            }
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const int t = 32 * b + 16 * g;
+                stage.load_v_part(own + HB + g * (HB / 2), base + HB + g * (HB / 2),
+                                  blk[g] >= 0 ? pg.v_at(blk[g], t) : pg.v,
+                                  blk[g] >= 0 ? len - t : 0);
+            }
+            return false;
+        };
+        bool kfull = false, vfull = false;
+        if (b0 < b1) {
+            find(b0);
+            issue_k(b0);
+            vfull = issue_v(b0);
+        }
+        for (int b = b0; b < b1; b += CK_WAVES) {
+            const int t0 = 32 * b;
+            const uint32_t groups = ok;
+            const bool more = b + CK_WAVES < b1;
+            f32x16_t s[1];
+            u32x4_t p[2];
+            if (vfull) dma_wait<LOADS>();
+            else dma_wait<0>();
+            scores<DT, D, 1>(own, ll, q, s);
+            dma_wait<63>();                        // (the K reads have returned)
+            if (more) {
+                find(b + CK_WAVES);
+                kfull = issue_k(b + CK_WAVES);
+            }
+            const bool masked = t0 < lo_hi || t0 + 32 > hi_lo || groups != 3u;
+            if (masked) mask_scores<1>(s, lo - t0, hi - t0, groups, lane);
+            softmax<DT, D, 1>(s, c, st, p);
+            if (more && kfull) dma_wait<LOADS>();
+            else dma_wait<0>();
+            const uint32_t vs = base + HB;
+            if (masked) bad |= any_nonfinite<DT, D, 1>(vs, ll);
+            weigh<DT, D, 1>(vs, ll, p, st);
+            dma_wait<63>();
+            if (more) vfull = issue_v(b + CK_WAVES);
+        }
+        if (lane == 0) item_flags(a, pl, kh, it.item)[w] = bad;
+        // the waves' (m, l, O) through LDS: wave w takes d tile w of all of them
+        dma_wait<0>();
+        __syncthreads();
+        lds.m[w][lane] = st.m;
+        lds.l[w][lane] = st.l + xor32_f(st.l);
+        float* of = reinterpret_cast<float*>(lds.kv) + w * (32 * D);
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {
+            float o[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = st.o[x][i];
+            save_tile<D>(of, x, o, lane);
+        }
+        __syncthreads();
+        float m = -__FLT_MAX__, l = 0.f, wt[CK_WAVES];
+#pragma unroll
+        for (int v = 0; v < CK_WAVES; ++v) m = fmaxf(m, lds.m[v][lane]);
+#pragma unroll
+        for (int v = 0; v < CK_WAVES; ++v) {
+            // (a wave without a finite score has l = 0 and O = 0)
+            wt[v] = __builtin_amdgcn_exp2f((lds.m[v][lane] - m) * c);
+            l += lds.l[v][lane] * wt[v];
+        }
+        if (w >= D / 32) return;
+        float o[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int v = 0; v < CK_WAVES; ++v) {
+                const float4 y = *reinterpret_cast<const float4*>(
+                    reinterpret_cast<float*>(lds.kv) + v * (32 * D) + (w * 4 + i) * 4 * WAVE + 4 * lane);
+                z.x += y.x * wt[v];
+                z.y += y.y * wt[v];
+                z.z += y.z * wt[v];
+                z.w += y.w * wt[v];
+            }
+            o[4 * i] = z.x;
+            o[4 * i + 1] = z.y;
+            o[4 * i + 2] = z.z;
+            o[4 * i + 3] = z.w;
+        }
+        if (whole) {
+            const RowOut ro = row_out(a, it.q, kh, row);
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] *= inv;
+            store_row<DT, D>(ro.out, w, o, lane);
+            if (w == 0) store_lse(ro, m, l, c, lane);
+        } else {
+            float* g = slot_group<D>(a, pl, kh, it.slot, 0);
+            save_tile<D>(g, w, o, lane);
+            if (w == 0) {
+                g[32 * D + lane] = m;
+                g[32 * D + WAVE + lane] = l;
+            }
+        }
+        return;
+    }
+    if (lane == 0) item_flags(a, pl, kh, it.item)[w] = bad;
+    if (idle) return;
+    const float l = st.l + xor32_f(st.l);
+    const RowOut ro = row_out(a, it.q, kh, row);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float* g = whole ? nullptr : slot_group<D>(a, pl, kh, it.slot, group);
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) {
+        float o[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = st.o[x][i] * (whole ? inv : 1.f);
+        if (whole) store_row<DT, D>(ro.out, x, o, lane);
+        else save_tile<D>(g, x, o, lane);
+    }
+    if (whole) {
+        store_lse(ro, st.m, l, c, lane);
+    } else {
+        g[32 * D + lane] = st.m;
+        g[32 * D + WAVE + lane] = l;
+    }
+}
+
+// One row over the keys it sees and no others: the way for a row tile in whose masked places V is
+// not finite (there a weight of zero gives NaN in a matrix product).  A wave takes 64 keys at a
+// time, a key per lane for the score, then d across the lanes for the values.  Slow, and rare.
+template <int DT, int D>
+__device__ __forceinline__ void attend_row(const amass_chunk_args& a, const ChunkPlan& pl,
+                                           const Req& q, int r, int kh, int row, float c, int lane) {
+    constexpr int PER = D / WAVE;                  // channels per lane
+    const int p = q.len - q.n + row / a.G;
+    const int lo = key_lo(a, p), hi = key_hi(a, pl, q.len, p);
+    const uint16_t* qr = (const uint16_t*)a.q + (int64_t)(q.q0 + row / a.G) * a.q_st +
+                         (int64_t)(kh * a.G + row % a.G) * a.q_hs;
+    const int32_t* table = a.block_table + r * a.bt_st;
+    const auto value = [](uint16_t h) { return DT == AMASS_BF16 ? bf16_to_f32(h) : fp16_to_f32(h); };
+    const auto place = [&](int t, int64_t sb, int64_t st, int64_t sh) -> int64_t {
+        const int b = table[t >> pl.sh];
+        return b >= 0 && b < a.nb ? b * sb + (t & ((1 << pl.sh) - 1)) * st + kh * sh : -1;
+    };
+    float m = -__FLT_MAX__, l = 0.f, o[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] = 0.f;
+    for (int t0 = lo; t0 < hi; t0 += WAVE) {
+        const int t = t0 + lane;
+        const int64_t at = t < hi ? place(t, a.k_sb, a.k_st, a.k_sh) : -1;
+        float s = -INFINITY;
+        if (at >= 0) {
+            s = 0.f;
+            const uint16_t* k = (const uint16_t*)a.k + at;
+            for (int i = 0; i < D; ++i) s = __builtin_fmaf(value(qr[i]), value(k[i]), s);
+        }
+        const float mx = fmaxf(m, wave_maxf_uniform(s));
+        const float al = __builtin_amdgcn_exp2f((m - mx) * c);
+        m = mx;
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -fmaxf(m * c, -__FLT_MAX__)));
+        l = l * al + wave_sumf(e);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) o[i] *= al;
+        for (int j = 0; j < WAVE && t0 + j < hi; ++j) {
+            const int64_t va = place(t0 + j, a.v_sb, a.v_st, a.v_sh);
+            if (va < 0) continue;
+            const float w = __shfl(e, j, WAVE);
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                o[i] += w * value(((const uint16_t*)a.v)[va + WAVE * i + lane]);
+        }
+    }
+    const RowOut ro = row_out(a, q, kh, row);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        ro.out[WAVE * i + lane] = (uint16_t)pack2<DT>(o[i] * inv, 0.f);
+    if (lane == 0) store_lse(ro, m, l, c, 0);
+}
+
+// Joins the parts of row tile blockIdx.x / n_kv (grid y: its 32-row groups): wave w takes d
+// tile w.
+template <int DT, int D>
+__global__ __launch_bounds__((D / 32) * WAVE) void chunk_merge_kernel(const amass_chunk_args a,
+                                                                      const ChunkPlan pl) {
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kh = blockIdx.x % a.n_kv, group = blockIdx.y;
+    Item it;
+    if (!find_item<true>(a, pl, blockIdx.x / a.n_kv, it)) return;
+    const Span sp = tile_span(a, pl, it.q, it.tile);
+    const int per = part_len(sp.n, it.parts);
+    const int parts = max(1, (sp.n + per - 1) / per);
+    const int rows = min(CK_BM, it.q.n * a.G - it.tile * CK_BM);
+    if (32 * group >= rows || it.item + parts > pl.tiles_max + pl.target ||
+        (parts > 1 && it.slot + parts > pl.slots))
+        return;
+    const float c = a.scale * 1.44269504088896341f;
+    const int row0 = it.tile * CK_BM + 32 * group;
+    const uint32_t* flags = reinterpret_cast<const uint32_t*>(item_flags(a, pl, kh, it.item));
+    uint32_t bad = 0;
+    for (int s = 0; s < parts; ++s) bad |= flags[s];
+    if (bad) {
+        for (int i = w; i < min(32, rows - 32 * group); i += D / 32)
+            attend_row<DT, D>(a, pl, it.q, it.r, kh, row0 + i, c, lane);
+        return;
+    }
+    if (parts < 2) return;
+    float m = -__FLT_MAX__;
+    for (int s = 0; s < parts; ++s)
+        m = fmaxf(m, slot_group<D>(a, pl, kh, it.slot + s, group)[32 * D + lane]);
+    float l = 0.f, o[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = 0.f;
+    for (int s = 0; s < parts; ++s) {
+        const float* g = slot_group<D>(a, pl, kh, it.slot + s, group);
+        const float wt = __builtin_amdgcn_exp2f((g[32 * D + lane] - m) * c);
+        l += g[32 * D + WAVE + lane] * wt;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 y = *reinterpret_cast<const float4*>(g + (w * 4 + i) * 4 * WAVE + 4 * lane);
+            o[4 * i] += y.x * wt;
+            o[4 * i + 1] += y.y * wt;
+            o[4 * i + 2] += y.z * wt;
+            o[4 * i + 3] += y.w * wt;
+        }
+    }
+    const RowOut ro = row_out(a, it.q, kh, row0 + (lane & 31));
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] *= inv;
+    store_row<DT, D>(ro.out, w, o, lane);
+    if (w == 0) store_lse(ro, m, l, c, lane);
+}
+
+// ------------------------------------------------------------------ host
+static int chunk_cus() {
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1)
+        return 256;
+    return n;
+}
+
+static bool chunk_empty(const amass_chunk_args& a) { return a.n_tokens == 0 || a.n_req == 0; }
+
+static int chunk_check(const amass_chunk_args& a) {
+    if (chunk_empty(a)) return AMASS_OK;
+    if (!a.q || !a.k || !a.v || !a.block_table || !a.seq_lens || !a.query_start || !a.out)
+        return AMASS_ERR_NULL;
+    if (a.dtype != AMASS_BF16 && a.dtype != AMASS_FP16) return AMASS_ERR_UNSUPPORTED;
+    if (a.d != 64 && a.d != 128) return AMASS_ERR_UNSUPPORTED;
+    if (a.page < 16 || a.page > (1 << 20) || (a.page & (a.page - 1))) return AMASS_ERR_GEOMETRY;
+    if (a.n_req < 0 || a.n_tokens < 0 || a.n_kv < 1 || a.G < 1 || a.nb < 1 || a.max_pages < 1 ||
+        a.window < 0 || !(a.scale > 0.f) || a.scale > 3e38f)
+        return AMASS_ERR_GEOMETRY;
+    if (a.n_kv > 4096 || a.G > 4096 || (int64_t)a.n_tokens * a.G > (1 << 30)) return AMASS_ERR_GEOMETRY;
+    const auto off = [](const void* p) { return ((uintptr_t)p & 15) != 0; };
+    if (off(a.q) || off(a.k) || off(a.v) || off(a.out) ||
+        ((a.q_st | a.q_hs | a.k_sb | a.k_st | a.k_sh | a.v_sb | a.v_st | a.v_sh | a.o_st | a.o_hs) & 7))
+        return AMASS_ERR_GEOMETRY;
+    // a row's offset within its 16 keys is 32 bits in the kernel
+    if (a.k_st < 0 || a.v_st < 0 || a.k_st > (1 << 26) || a.v_st > (1 << 26)) return AMASS_ERR_GEOMETRY;
+    return AMASS_OK;
+}
+
+static ChunkPlan chunk_plan(const amass_chunk_args& a) {
+    ChunkPlan p;
+    p.sh = 0;
+    while ((1 << p.sh) < a.page) ++p.sh;
+    const int64_t cap = (int64_t)a.max_pages << p.sh;
+    p.cap = cap > 0x7FFFFFC0 ? 0x7FFFFFC0 : (int)cap;
+    p.target = 2 * chunk_cus() / a.n_kv;
+    if (p.target < 1) p.target = 1;
+    const int64_t rows = (int64_t)a.n_tokens * a.G;
+    p.tiles_max = (int)(rows / CK_BM) + (a.n_req < a.n_tokens ? a.n_req : a.n_tokens);
+    // fewer tiles than `target`: the plan has at most `target` items; else those of cut tiles
+    // are at most twice sum_r tiles_r w_r / len <= target
+    p.slots = p.tiles_max < p.target ? p.target : 2 * p.target;
+    p.slot_rows = rows <= CK_FEW ? CK_FEW : CK_BM;
+    p.flag_bytes = ((int64_t)a.n_kv * (p.tiles_max + p.target) * CK_WAVES + 255) & ~(int64_t)255;
+    return p;
+}
+
+static int64_t chunk_scratch(const amass_chunk_args& a, const ChunkPlan& p) {
+    return p.flag_bytes + (int64_t)a.n_kv * p.slots * (p.slot_rows / 32) * (32 * a.d + 2 * WAVE) * sizeof(float);
+}
+
+template <int DT, int D>
+static int launch_chunk(const amass_chunk_args& a, const ChunkPlan& p, hipStream_t s) {
+    const int64_t items = (int64_t)(p.tiles_max + p.target) * a.n_kv;
+    if (items > 0x7FFFFFFF) return AMASS_ERR_GEOMETRY;
+    hipLaunchKernelGGL((chunk_kernel<DT, D>), dim3((unsigned)items), dim3(CK_WAVES * WAVE), 0, s, a, p);
+    const int rc = check_launch();
+    if (rc) return rc;
+    hipLaunchKernelGGL((chunk_merge_kernel<DT, D>), dim3(p.tiles_max * a.n_kv, p.slot_rows / 32),
+                       dim3((D / 32) * WAVE), 0, s, a, p);
+    return check_launch();
+}
+
+}  // namespace amass
+
+using namespace amass;
+
+extern "C" int64_t amass_chunk_scratch_bytes(const amass_chunk_args* a) {
+    if (!a) return AMASS_ERR_NULL;
+    const int rc = chunk_check(*a);
+    return rc || chunk_empty(*a) ? rc : chunk_scratch(*a, chunk_plan(*a));
+}
+
+extern "C" int amass_chunk_attention(const amass_chunk_args* ain, void* stream) {
+    if (!ain) return AMASS_ERR_NULL;
+    const amass_chunk_args& a = *ain;
+    const int rc = chunk_check(a);
+    if (rc) return rc;
+    if (chunk_empty(a)) return AMASS_OK;
+    if (!a.scratch) return AMASS_ERR_NULL;
+    const ChunkPlan p = chunk_plan(a);
+    if (((uintptr_t)a.scratch & 255) || a.scratch_bytes < chunk_scratch(a, p)) return AMASS_ERR_CAPACITY;
+    hipStream_t s = (hipStream_t)stream;
+    if (a.dtype == AMASS_BF16) return a.d == 128 ? launch_chunk<0, 128>(a, p, s) : launch_chunk<0, 64>(a, p, s);
+    return a.d == 128 ? launch_chunk<1, 128>(a, p, s) : launch_chunk<1, 64>(a, p, s);
+}
+
+extern "C" int amass_chunk_abi_version(void) { return AMASS_CHUNK_ABI_VERSION; }
+
+extern "C" size_t amass_chunk_struct_size(int which) {
+    switch (which) {
+        case 0: return sizeof(amass_extend_args);
+        case 1: return sizeof(amass_release_args);
+        case 2: return sizeof(amass_rope_args);
+        case 3: return sizeof(amass_chunk_args);
+        default: return 0;
+    }
+}
