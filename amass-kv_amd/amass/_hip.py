@@ -313,25 +313,46 @@ def call(name: str, args, stream: int) -> None:
         check(rc, name)
 
 
-def call_on(device, name: str, args) -> None:
-    """`call` on torch's current stream of the tensors' `device`, which need not be the
-    current one."""
+def device_index(first, *others) -> int:
+    """The GPU that all tensors of a call lie on (None stands for no tensor)."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            require_cuda(first, t)
+            raise ValueError(f"tensors on {first.device} and {t.device} in one call")
+    if index < 0:
+        require_cuda(first)
+    return index
+
+
+def call_on(index: int, name: str, args) -> None:
+    """`call` on torch's current stream of GPU `index`, which need not be the current one."""
     import torch
-    index = device.index
-    if index is None or index == torch.cuda.current_device():
-        call(name, args, current_stream(device))
+    if index == torch._C._cuda_getDevice():
+        call(name, args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            call(name, args, current_stream(device))
+            call(name, args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def same_device(first, *others) -> None:
-    """The tensors of one call lie on one GPU."""
-    require_cuda(first, *others)
-    d = first.device
-    for t in others:
-        if t is not None and t.device != d:
-            raise ValueError(f"tensors on {d} and {t.device} in one call")
+def vector(t, dtype, n: int, name: str) -> None:
+    """Refuse a `t` that is no contiguous vector of `dtype` with n entries or more."""
+    if t.dtype is not dtype or t.stride() != (1,) or t.numel() < n:
+        if t.dtype is not dtype or t.dim() != 1 or not t.is_contiguous() or t.numel() < n:
+            raise ValueError(f"{name} must be a contiguous vector of {n} {dtype}")
+
+
+def cache_halves(kv_cache):
+    """(blocks, page, n_kv, d), K's and V's addresses (V's 0 for a cache without V) and the
+    strides of a block, a row, a head and a channel, of a 16-bit (2, NB, page, n_kv, d),
+    (NB, 2, ...) or (NB, 1, ...) cache, without making the views."""
+    shape, st, at = kv_cache.shape, kv_cache.stride(), kv_cache.data_ptr()
+    if len(shape) != 5 or (shape[0] != 2 and shape[1] > 2):
+        raise ValueError("the cache must be (2, NB, page, n_kv, d), (NB, 2, ...) or (NB, 1, ...)")
+    if shape[0] == 2:
+        return shape[1:], at, at + 2 * st[0], st[1:]
+    v = 0 if shape[1] == 1 else at + 2 * st[1]
+    return (shape[0], *shape[2:]), at, v, (st[0], *st[2:])
 
 
 def call_select_attend(score, select, decode, mode: int, tickets, wgs_per_unit: int,

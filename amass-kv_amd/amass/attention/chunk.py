@@ -14,28 +14,29 @@ from __future__ import annotations
 
 import torch
 
-from .._hip import ChunkArgs, call_on, check, load_library, packer, same_device
-from .decode import _split_kv
+from .._hip import (ChunkArgs, cache_halves, call_on, check, device_index, load_library, packer,
+                    vector)
 from .rope import DTYPES
 
 HEAD_DIMS = (64, 128)
 _pack_chunk = packer(ChunkArgs)
+_SCRATCH = {}            # (GPU, requests, rows, kv heads, group, head dim) -> scratch bytes
 
 
 def _chunk_args(q, kv_cache, block_table, seq_lens, query_start, out, scale, causal, window,
-                lse) -> ChunkArgs:
-    same_device(q, kv_cache, block_table, seq_lens, query_start, out, lse)
-    k, v = _split_kv(kv_cache)
-    if v is None:
-        raise ValueError("the cache has no V half")
+                lse):
+    """(the argument struct's values up to the scratch, those behind it) of a checked call."""
     dt = q.dtype
-    if dt not in DTYPES or k.dtype != dt or out.dtype != dt:
+    if not (dt in DTYPES and dt is kv_cache.dtype is out.dtype):
         raise ValueError("q, the cache and out must all be bf16 or all fp16")
-    nb, page, n_kv, d = k.shape
-    if q.dim() != 3 or q.shape[2] != d or out.shape != q.shape:
+    (nb, page, n_kv, d), k, v, cs = cache_halves(kv_cache)
+    if v == 0:
+        raise ValueError("the cache has no V half")
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != d or out.shape != shape:
         raise ValueError(f"q and out must be (T, H, {d})")
-    T, H = q.shape[:2]
-    if H % n_kv or H == 0:
+    T, H, _ = shape
+    if H == 0 or H % n_kv:
         raise ValueError(f"{H} query heads are not a multiple of {n_kv} kv heads")
     if d not in HEAD_DIMS:
         raise ValueError(f"head dim {d} (built for {HEAD_DIMS})")
@@ -46,43 +47,52 @@ def _chunk_args(q, kv_cache, block_table, seq_lens, query_start, out, scale, cau
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 3e38:
         raise ValueError(f"scale {scale} must be positive and finite")
-    n_req = seq_lens.shape[0]
-    for t, name, n in ((seq_lens, "seq_lens", n_req), (query_start, "query_start", n_req + 1)):
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.shape[0] < n:
-            raise ValueError(f"{name} must be a contiguous int32 vector of {n} entries")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or \
-            block_table.stride(1) != 1 or block_table.shape[0] < n_req or \
-            block_table.shape[1] < 1:
+    n_req = seq_lens.numel()
+    vector(seq_lens, torch.int32, n_req, "seq_lens")
+    vector(query_start, torch.int32, n_req + 1, "query_start")
+    rows, width = block_table.shape
+    bt_st, unit = block_table.stride()
+    if block_table.dtype is not torch.int32 or (unit != 1 and width > 1) or rows < n_req or \
+            width < 1:
         raise ValueError("block_table must be (R, max_pages) int32 with unit column stride")
-    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), out.stride()
-    if qs[2] != 1 or ks[3] != 1 or vs[3] != 1 or os_[2] != 1:
+    q_st, q_hs, q_unit = q.stride()
+    o_st, o_hs, o_unit = out.stride()
+    sb, st, sh, c_unit = cs
+    if not q_unit == o_unit == c_unit == 1:
         raise ValueError("q / cache / out need unit stride on the head dim")
-    ls = (0, 0)
+    l_at = l_st = l_hs = 0
     if lse is not None:
-        if lse.dtype != torch.float32 or lse.shape != (T, H):
+        if lse.dtype is not torch.float32 or lse.shape != (T, H):
             raise ValueError("lse must be (T, H) fp32")
-        ls = lse.stride()
-    return _pack_chunk(                # in the struct's order
-        q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0],
-        vs[1], vs[2], block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(),
-        query_start.data_ptr(), out.data_ptr(), os_[0], os_[1],
-        0 if lse is None else lse.data_ptr(), ls[0], ls[1], 0, 0, scale, n_req, T, n_kv,
-        H // n_kv, d, page, nb, block_table.shape[1], 1 if causal else 0, window or 0,
-        DTYPES[dt])
+        l_at = lse.data_ptr()
+        l_st, l_hs = lse.stride()
+    return ((q.data_ptr(), q_st, q_hs, k, sb, st, sh, v, sb, st, sh, block_table.data_ptr(),
+             bt_st, seq_lens.data_ptr(), query_start.data_ptr(), out.data_ptr(), o_st, o_hs,
+             l_at, l_st, l_hs),
+            (scale, n_req, T, n_kv, H // n_kv, d, page, nb, width, 1 if causal else 0,
+             window or 0, DTYPES[dt]))
 
 
-def _scratch_bytes(a: ChunkArgs) -> int:
-    n = load_library().amass_chunk_scratch_bytes(a)
-    if n < 0:
-        check(n, "amass_chunk_scratch_bytes")
+def _scratch_bytes(index, head, tail) -> int:
+    key = (index, *tail[1:6])
+    n = _SCRATCH.get(key)
+    if n is None:
+        with torch.cuda.device(index):
+            n = load_library().amass_chunk_scratch_bytes(_pack_chunk(*head, 0, 0, *tail))
+        if n < 0:
+            check(n, "amass_chunk_scratch_bytes")
+        if len(_SCRATCH) >= 4096:
+            _SCRATCH.clear()
+        _SCRATCH[key] = n
     return n
 
 
 def chunk_scratch_bytes(q, kv_cache, block_table, seq_lens, query_start, out, *, scale=None,
                         causal: bool = True, window=None, lse=None) -> int:
     """Bytes of scratch that ``paged_chunk_attention`` takes for these shapes."""
-    return _scratch_bytes(_chunk_args(q, kv_cache, block_table, seq_lens, query_start, out,
-                                      scale, causal, window, lse))
+    index = device_index(q, kv_cache, block_table, seq_lens, query_start, out, lse)
+    return _scratch_bytes(index, *_chunk_args(q, kv_cache, block_table, seq_lens, query_start,
+                                              out, scale, causal, window, lse))
 
 
 def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start, out, *, scale=None,
@@ -103,16 +113,18 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start, out, 
 
     ``scratch``: a uint8 tensor of ``chunk_scratch_bytes`` for programs that keep their own;
     calls that may run at the same time need one each."""
-    a = _chunk_args(q, kv_cache, block_table, seq_lens, query_start, out, scale, causal, window,
-                    lse)
-    need = _scratch_bytes(a)
+    index = device_index(q, kv_cache, block_table, seq_lens, query_start, out, lse, scratch)
+    head, tail = _chunk_args(q, kv_cache, block_table, seq_lens, query_start, out, scale,
+                             causal, window, lse)
+    need = _scratch_bytes(index, head, tail)
     if scratch is None:
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+        scratch = q.new_empty(need // 2)
+        size = need
     else:
-        same_device(q, scratch)
-        if scratch.dtype != torch.uint8 or not scratch.is_contiguous():
+        if scratch.dtype is not torch.uint8 or not scratch.is_contiguous():
             raise ValueError("scratch must be a contiguous uint8 tensor")
-        if scratch.numel() < need:
-            raise ValueError(f"scratch of {scratch.numel()} bytes, {need} needed")
-    a.scratch, a.scratch_bytes = scratch.data_ptr(), scratch.numel()
-    call_on(q.device, "amass_chunk_attention", a)
+        size = scratch.numel()
+        if size < need:
+            raise ValueError(f"scratch of {size} bytes, {need} needed")
+    call_on(index, "amass_chunk_attention",
+            _pack_chunk(*head, scratch.data_ptr(), size, *tail))

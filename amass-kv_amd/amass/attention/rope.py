@@ -27,12 +27,11 @@ import math
 
 import torch
 
-from .._hip import RopeArgs, call_on, packer, same_device
+from .._hip import RopeArgs, cache_halves, call_on, device_index, packer, vector
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 DTYPES = {torch.bfloat16: 0, torch.float16: 1}      # AMASS_BF16, AMASS_FP16
 _pack_rope = packer(RopeArgs)
-_NO_VIEW = (0, 0, 0)
 
 
 def rope_frequencies(rot: int, *, base: float = 10000.0, scaling: str | None = None,
@@ -96,46 +95,47 @@ def rope_paged_write(q, k, v, positions, table, kv_cache, slots, q_out=None, *,
     ``rope_table``, ``kv_cache`` one layer's (2, NB, page, n_kv, d), (NB, 2, ...) or, without V,
     (NB, 1, ...).  A row whose position is outside the table is passed over; one whose slot is
     outside the cache has its q turned and is not written.  bf16 or fp16."""
-    from .decode import _split_kv
     q_out = q if q_out is None else q_out
-    same_device(q, k, v, positions, table, kv_cache, slots, q_out)
-    kc, vc = _split_kv(kv_cache)
+    index = device_index(q, k, v, positions, table, kv_cache, slots, q_out)
     dt = q.dtype
-    if dt not in DTYPES or k.dtype != dt or kc.dtype != dt or q_out.dtype != dt or \
-            (v is not None and v.dtype != dt):
+    if not (dt in DTYPES and dt is k.dtype is kv_cache.dtype is q_out.dtype
+            and (v is None or dt is v.dtype)):
         raise ValueError("q, k, v, q_out and the cache must all be bf16 or all fp16")
     if layout not in LAYOUTS:
         raise ValueError(f"layout {layout!r}: 'half' or 'interleaved'")
-    if (v is None) != (vc is None):
+    (nb, page, n_kv, d), kc, vc, cs = cache_halves(kv_cache)
+    if (v is None) != (vc == 0):
         raise ValueError("v comes with a cache that has V, and only with one")
-    nb, page, n_kv, d = kc.shape
-    T, H = q.shape[:2]
-    if q.shape != (T, H, d) or q_out.shape != q.shape or k.shape != (T, n_kv, d) or \
-            (v is not None and v.shape != k.shape):
+    shape, k_shape = q.shape, k.shape
+    if len(shape) != 3 or shape[2] != d or q_out.shape != shape or \
+            k_shape != (shape[0], n_kv, d) or (v is not None and v.shape != k_shape):
         raise ValueError(f"q (T, H, {d}) and k, v (T, {n_kv}, {d}) expected, q_out like q")
+    T, H, _ = shape
     max_pos, rot = table.shape
-    if table.dtype != torch.float32 or table.stride(1) != 1 or rot % 2 or not 2 <= rot <= d:
+    tab_st, unit = table.stride()
+    if table.dtype is not torch.float32 or unit != 1 or rot % 2 or not 2 <= rot <= d:
         raise ValueError(f"table must be (max_pos, rot) fp32 with an even rot of at most {d}")
     if d % 2 or page & (page - 1):
         raise ValueError(f"head dim {d} must be even and page {page} a power of two")
-    if positions.dtype != torch.int32 or slots.dtype != torch.int64 or \
-            not (positions.is_contiguous() and slots.is_contiguous()) or \
-            positions.dim() != 1 or slots.dim() != 1 or positions.shape[0] < T or \
-            slots.shape[0] < T:
-        raise ValueError("positions (T,) int32 and slots (T,) int64 must be contiguous")
-    qs, ks, os_, cs = q.stride(), k.stride(), q_out.stride(), kc.stride()
-    if qs[2] != 1 or ks[2] != 1 or os_[2] != 1 or cs[3] != 1:
+    vector(positions, torch.int32, T, "positions")
+    vector(slots, torch.int64, T, "slots")
+    if T == 0:
+        return
+    q_st, q_hs, q_unit = q.stride()
+    k_st, k_hs, k_unit = k.stride()
+    o_st, o_hs, o_unit = q_out.stride()
+    sb, st, sh, c_unit = cs
+    if not q_unit == k_unit == o_unit == c_unit == 1:
         raise ValueError("q / k / q_out / cache need unit stride on the head dim")
-    v_at = vc_at = 0
-    vs = vcs = _NO_VIEW
+    v_at = v_st = v_hs = 0
     if v is not None:
-        v_at, vs, vc_at, vcs = v.data_ptr(), v.stride(), vc.data_ptr(), vc.stride()
-        if vs[2] != 1 or vcs[3] != 1:
-            raise ValueError("v and its cache need unit stride on the head dim")
+        v_at = v.data_ptr()
+        v_st, v_hs, v_unit = v.stride()
+        if v_unit != 1:
+            raise ValueError("v needs unit stride on the head dim")
     a = _pack_rope(                    # in the struct's order
-        q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v_at, vs[0], vs[1],
-        q_out.data_ptr(), os_[0], os_[1], kc.data_ptr(), cs[0], cs[1], cs[2],
-        vc_at, vcs[0], vcs[1], vcs[2], table.data_ptr(), table.stride(0),
+        q.data_ptr(), q_st, q_hs, k.data_ptr(), k_st, k_hs, v_at, v_st, v_hs,
+        q_out.data_ptr(), o_st, o_hs, kc, sb, st, sh, vc, sb, st, sh, table.data_ptr(), tab_st,
         positions.data_ptr(), slots.data_ptr(), T, H, n_kv, d, rot, page, nb, max_pos,
         LAYOUTS[layout], DTYPES[dt])
-    call_on(q.device, "amass_rope_write", a)
+    call_on(index, "amass_rope_write", a)

@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import torch
 
-from .._hip import ExtendArgs, ReleaseArgs, call_on, packer, same_device
+from .._hip import ExtendArgs, ReleaseArgs, call_on, device_index, packer, vector
 
 MAX_REQS = 4096      # requests of one call (the kernels rank them in LDS)
 _pack_extend = packer(ExtendArgs)
@@ -30,24 +30,21 @@ def free_blocks(num_blocks: int, device):
     return free, torch.tensor([num_blocks, 0, 0], dtype=torch.int32, device=device)
 
 
-def _check_step(block_table, seq_lens, free, top, page, num_blocks):
-    for t, name in ((seq_lens, "seq_lens"), (free, "free"), (top, "top")):
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 vector")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+def _table(block_table, n_req, page, num_blocks):
+    """(row stride, width) of a checked block table."""
+    rows, width = block_table.shape
+    st, unit = block_table.stride()
+    if block_table.dtype is not torch.int32 or (unit != 1 and width > 1):
         raise ValueError("block_table must be (R, max_pages) int32 with unit column stride")
-    n_req = seq_lens.shape[0]
-    if block_table.shape[0] < n_req or block_table.shape[1] < 1:
+    if rows < n_req or width < 1:
         raise ValueError("block_table needs a row per request")
     if n_req > MAX_REQS:
         raise ValueError(f"{n_req} requests in one call (at most {MAX_REQS})")
-    if top.shape[0] < 3:
-        raise ValueError("top has three words (free_blocks)")
     if page < 1 or page & (page - 1):
         raise ValueError(f"page {page} is not a power of two")
     if num_blocks < 1:
         raise ValueError("num_blocks must be positive")
-    return n_req
+    return st, width
 
 
 def extend_block_tables(block_table, seq_lens, query_start, free, top, slots, positions, *,
@@ -64,25 +61,25 @@ def extend_block_tables(block_table, seq_lens, query_start, free, top, slots, po
 
     ``top`` becomes the blocks left (``top[2]``: those that were short).  With ``top_out``,
     another such tensor, they go there and ``top`` stays, so that the step may be dropped."""
-    same_device(block_table, seq_lens, query_start, free, top, slots, positions, top_out)
-    n_req = _check_step(block_table, seq_lens, free, top, page, num_blocks)
-    if query_start.dtype != torch.int32 or query_start.dim() != 1 or \
-            not query_start.is_contiguous() or query_start.shape[0] < n_req + 1:
-        raise ValueError("query_start must be a contiguous int32 vector of R + 1 rows")
-    if slots.dtype != torch.int64 or positions.dtype != torch.int32 or slots.dim() != 1 or \
-            positions.dim() != 1 or not (slots.is_contiguous() and positions.is_contiguous()) \
-            or positions.shape[0] < slots.shape[0]:
-        raise ValueError("slots (T,) int64 and positions (T,) int32 must be contiguous")
+    index = device_index(block_table, seq_lens, query_start, free, top, slots, positions,
+                         top_out)
+    n_req, n_tokens, n_free = seq_lens.numel(), slots.numel(), free.numel()
+    st, width = _table(block_table, n_req, page, num_blocks)
+    vector(seq_lens, torch.int32, n_req, "seq_lens")
+    vector(query_start, torch.int32, n_req + 1, "query_start")
+    vector(free, torch.int32, n_free, "free")
+    vector(top, torch.int32, 3, "top")
+    vector(slots, torch.int64, n_tokens, "slots")
+    vector(positions, torch.int32, n_tokens, "positions")
     if top_out is None:
         top_out = top
-    elif top_out.dtype != torch.int32 or not top_out.is_contiguous() or top_out.numel() < 3:
-        raise ValueError("top_out must be three contiguous int32 words")
+    else:
+        vector(top_out, torch.int32, 3, "top_out")
     a = _pack_extend(                  # in the struct's order
-        block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(),
-        query_start.data_ptr(), free.data_ptr(), top.data_ptr(), top_out.data_ptr(),
-        slots.data_ptr(), positions.data_ptr(), n_req, slots.shape[0], block_table.shape[1],
-        page, num_blocks, free.shape[0])
-    call_on(block_table.device, "amass_extend", a)
+        block_table.data_ptr(), st, seq_lens.data_ptr(), query_start.data_ptr(),
+        free.data_ptr(), top.data_ptr(), top_out.data_ptr(), slots.data_ptr(),
+        positions.data_ptr(), n_req, n_tokens, width, page, num_blocks, n_free)
+    call_on(index, "amass_extend", a)
 
 
 def release_blocks(block_table, seq_lens, done, free, top, *, page: int,
@@ -90,13 +87,14 @@ def release_blocks(block_table, seq_lens, done, free, top, *, page: int,
     """The blocks of the first ``ceil(seq_lens[r] / page)`` pages of every request with
     ``done[r]`` (bool) go behind the free list, in (request, page) order, and their table
     entries become -1.  Blocks past the list's length are dropped (``top[2]``)."""
-    same_device(block_table, seq_lens, done, free, top)
-    n_req = _check_step(block_table, seq_lens, free, top, page, num_blocks)
-    if done.dtype not in (torch.bool, torch.uint8) or done.dim() != 1 or \
-            not done.is_contiguous() or done.shape[0] < n_req:
-        raise ValueError("done must be a contiguous bool vector, an entry per request")
+    index = device_index(block_table, seq_lens, done, free, top)
+    n_req, n_free = seq_lens.numel(), free.numel()
+    st, width = _table(block_table, n_req, page, num_blocks)
+    vector(seq_lens, torch.int32, n_req, "seq_lens")
+    vector(free, torch.int32, n_free, "free")
+    vector(top, torch.int32, 3, "top")
+    vector(done, torch.uint8 if done.dtype is torch.uint8 else torch.bool, n_req, "done")
     a = _pack_release(                 # in the struct's order
-        block_table.data_ptr(), block_table.stride(0), seq_lens.data_ptr(), done.data_ptr(),
-        free.data_ptr(), top.data_ptr(), n_req, block_table.shape[1], page, num_blocks,
-        free.shape[0])
-    call_on(block_table.device, "amass_release", a)
+        block_table.data_ptr(), st, seq_lens.data_ptr(), done.data_ptr(), free.data_ptr(),
+        top.data_ptr(), n_req, width, page, num_blocks, n_free)
+    call_on(index, "amass_release", a)

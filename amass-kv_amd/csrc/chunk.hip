@@ -26,6 +26,8 @@
 // Splitting.  A row tile of many keys is cut into S parts when the batch has fewer tiles
 // than the chip has room for (plan below, on the device: the launch needs no lengths on the
 // host and can be captured); parts leave (m, l, O) in scratch and a second launch joins them.
+#include <atomic>
+
 #include "../../include/amass_chunk.h"
 #include "common.h"
 
@@ -105,7 +107,8 @@ struct ChunkPlan {
     int slots;           // scratch slots per kv head
     int slot_rows;       // rows of a slot
     int tiles_max;       // row tiles of the batch at most
-    int64_t flag_bytes;  // of the items' flags, before the slots
+    uint32_t g_mul;      // x / G = x g_mul >> (30 + g_sh) for x < 2^30
+    int g_sh;
 };
 
 struct Span {            // keys [64 lo, 64 lo + 64 n) hold the visible ones below hi
@@ -116,6 +119,9 @@ struct Req {
     int q0, n, len;      // first row, new tokens, tokens
 };
 
+__device__ __forceinline__ int div_g(const ChunkPlan& pl, int x) {
+    return (int)(((uint64_t)(uint32_t)x * pl.g_mul) >> (30 + pl.g_sh));
+}
 __device__ __forceinline__ Req load_req(const amass_chunk_args& a, int r) {
     Req q;
     q.q0 = min(max(a.query_start[r], 0), a.n_tokens);
@@ -124,7 +130,7 @@ __device__ __forceinline__ Req load_req(const amass_chunk_args& a, int r) {
     return q;
 }
 __device__ __forceinline__ int row_tiles(const amass_chunk_args& a, const Req& q) {
-    return (int)(((int64_t)q.n * a.G + CK_BM - 1) / CK_BM);
+    return (int)((uint32_t)(q.n * a.G + CK_BM - 1) / CK_BM);
 }
 
 // visible keys [lo, hi) of the token at position p
@@ -138,121 +144,150 @@ __device__ __forceinline__ int key_lo(const amass_chunk_args& a, int p) {
 __device__ __forceinline__ Span tile_span(const amass_chunk_args& a, const ChunkPlan& pl,
                                           const Req& q, int tile) {
     const int r0 = tile * CK_BM, r1 = min(q.n * a.G, r0 + CK_BM) - 1;
-    const int p0 = q.len - q.n + r0 / a.G, p1 = q.len - q.n + r1 / a.G;
+    const int p0 = q.len - q.n + div_g(pl, r0), p1 = q.len - q.n + div_g(pl, r1);
     Span s;
     s.hi = key_hi(a, pl, q.len, p1);
     s.lo = key_lo(a, p0) / CK_KEYS;
     s.n = max(0, (s.hi + CK_KEYS - 1) / CK_KEYS - s.lo);
     return s;
 }
-// the most tiles of keys that a row tile of the request has
+// the most tiles of keys that a row tile of the request has (the last one's, or under a
+// window that of the last whole one)
 __device__ __forceinline__ int req_work(const amass_chunk_args& a, const ChunkPlan& pl,
                                         const Req& q, int tiles) {
     int w = 0;
     if (tiles > 0) w = tile_span(a, pl, q, tiles - 1).n;
-    if (tiles > 1) w = max(w, tile_span(a, pl, q, tiles - 2).n);
+    if (tiles > 1 && a.window > 0) w = max(w, tile_span(a, pl, q, tiles - 2).n);
     return w;
+}
+
+// Parts of a row tile: S_r = ceil(w_r / len), w_r the request's longest tile, for the
+// smallest part length `len` >= max(CK_MIN_SPLIT, sum_r tiles_r w_r / target) at which the
+// batch has at most `target` items (workgroups per kv head), or the first such length where
+// the row tiles alone are that many (only tiles much longer than the average are cut then).
+// Every workgroup computes it from the lengths, 64 requests at a time, one per lane.
+struct LaneReq {
+    Req q;
+    int tiles, work;
+};
+__device__ __forceinline__ LaneReq lane_req(const amass_chunk_args& a, const ChunkPlan& pl, int r) {
+    LaneReq x = {{0, 0, 0}, 0, 0};
+    if (r < a.n_req) x.q = load_req(a, r);
+    x.tiles = row_tiles(a, x.q);
+    x.work = req_work(a, pl, x.q, x.tiles);
+    return x;
+}
+__device__ __forceinline__ int parts_of(int w, int len) { return max(1, (w + len - 1) / len); }
+
+__device__ __forceinline__ int count_items(const amass_chunk_args& a, const ChunkPlan& pl,
+                                           const LaneReq& x0, int len) {
+    const int lane = threadIdx.x & 63;
+    int tot = wave_sum_uniform(x0.tiles * parts_of(x0.work, len));
+    for (int base = WAVE; base < a.n_req; base += WAVE) {
+        const LaneReq x = lane_req(a, pl, base + lane);
+        tot += wave_sum_uniform(x.tiles * parts_of(x.work, len));
+    }
+    return tot;
+}
+__device__ __forceinline__ int part_length(const amass_chunk_args& a, const ChunkPlan& pl,
+                                           const LaneReq& x0) {
+    const int lane = threadIdx.x & 63;
+    float work = (float)x0.tiles * (float)x0.work;
+    int tiles = wave_sum_uniform(x0.tiles), longest = wave_max_uniform(x0.work);
+    for (int base = WAVE; base < a.n_req; base += WAVE) {
+        const LaneReq x = lane_req(a, pl, base + lane);
+        work += (float)x.tiles * (float)x.work;
+        tiles += wave_sum_uniform(x.tiles);
+        longest = max(longest, wave_max_uniform(x.work));
+    }
+    int len = max(CK_MIN_SPLIT, (int)ceilf(wave_sumf_uniform(work) / (float)pl.target));
+    if (len >= longest) return max(longest, 1);          // no tile is cut
+    if (tiles >= pl.target || count_items(a, pl, x0, len) <= pl.target) return len;
+    int lo = len + 1, hi = longest;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (count_items(a, pl, x0, mid) <= pl.target) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
 }
 
 struct Item {
     int r, tile, part, parts;
-    int item, slot;      // of part 0 (MERGE) or of this part
+    int slot;            // of this part, where parts > 1
+    int cut;             // index of the row tile among those cut
     Req q;
 };
 
-// Parts of a row tile: the request's longest tile decides, tiles S_r = ceil(w_r / len) for
-// the smallest part length `len` >= max(CK_MIN_SPLIT, sum_r tiles_r w_r / target) at which
-// the batch has at most `target` items (workgroups per kv head), or the first such length
-// where the row tiles alone are that many (only tiles much longer than the average are cut
-// then).  Item y of the batch: requests in order, a request's last (causal: longest) tile
-// first.
-__device__ __forceinline__ int count_items(const amass_chunk_args& a, const ChunkPlan& pl,
-                                           int t0, int w0, int len) {
+// Item y of the batch (requests in order, a request's last -- causal: longest -- tile first);
+// false past the end.
+__device__ __forceinline__ bool find_item(const amass_chunk_args& a, const ChunkPlan& pl,
+                                          const LaneReq& x0, int len, int y, Item& it) {
     const int lane = threadIdx.x & 63;
-    int tot = wave_sum_uniform(t0 * max(1, (w0 + len - 1) / len));
-    for (int base = WAVE; base < a.n_req; base += WAVE) {
-        int n = 0;
-        if (base + lane < a.n_req) {
-            const Req q = load_req(a, base + lane);
-            const int t = row_tiles(a, q), w = req_work(a, pl, q, t);
-            n = t * max(1, (w + len - 1) / len);
-        }
-        tot += wave_sum_uniform(n);
-    }
-    return tot;
-}
-
-// Item y (`merge`: row tile y) of the batch; false past the end.
-template <bool MERGE>
-__device__ __forceinline__ bool find_item(const amass_chunk_args& a, const ChunkPlan& pl, int y,
-                                          Item& it) {
-    const int lane = threadIdx.x & 63;
-    Req q = {0, 0, 0};
-    if (lane < a.n_req) q = load_req(a, lane);
-    const int t0 = row_tiles(a, q), w0 = req_work(a, pl, q, t0);
-    float work = (float)t0 * (float)w0;
-    int tiles = wave_sum_uniform(t0), longest = wave_max_uniform(w0);
-    for (int base = WAVE; base < a.n_req; base += WAVE) {
-        Req x = {0, 0, 0};
-        if (base + lane < a.n_req) x = load_req(a, base + lane);
-        const int t = row_tiles(a, x), w = req_work(a, pl, x, t);
-        work += (float)t * (float)w;
-        tiles += wave_sum_uniform(t);
-        longest = max(longest, wave_max_uniform(w));
-    }
-    int len = max(CK_MIN_SPLIT, (int)ceilf(wave_sumf(work) / (float)pl.target));
-    if (len >= longest) {
-        len = max(longest, 1);                          // no tile is cut
-    } else if (tiles < pl.target && count_items(a, pl, t0, w0, len) > pl.target) {
-        int lo = len + 1, hi = longest;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (count_items(a, pl, t0, w0, mid) <= pl.target) hi = mid;
-            else lo = mid + 1;
-        }
-        len = lo;
-    }
-    int before = 0, items = 0, slots = 0;                // those of earlier requests
+    int before = 0, slots = 0, cuts = 0;                 // those of earlier requests
     for (int base = 0; base < a.n_req; base += WAVE) {
-        Req x = q;
-        int t = t0, w = w0;
-        if (base > 0) {
-            x = {0, 0, 0};
-            if (base + lane < a.n_req) x = load_req(a, base + lane);
-            t = row_tiles(a, x);
-            w = req_work(a, pl, x, t);
-        }
-        const int S = max(1, (w + len - 1) / len);
-        const int ni = t * S, n = MERGE ? t : ni, ns = S > 1 ? ni : 0;
-        const int incl_i = wave_incl_scan(ni), incl_s = wave_incl_scan(ns);
-        const int incl = MERGE ? wave_incl_scan(n) : incl_i;
+        const LaneReq x = base == 0 ? x0 : lane_req(a, pl, base + lane);
+        const int S = parts_of(x.work, len);
+        const int n = x.tiles * S, ns = S > 1 ? n : 0, nc = S > 1 ? x.tiles : 0;
+        const int incl = wave_incl_scan(n), incl_s = wave_incl_scan(ns), incl_c = wave_incl_scan(nc);
         const int all = __builtin_amdgcn_readlane(incl, WAVE - 1);
         if (y < before + all) {
             const int src = __ffsll((long long)__ballot(before + incl > y)) - 1;
             const int at = y - before - __builtin_amdgcn_readlane(incl - n, src);
-            const int s = __builtin_amdgcn_readlane(S, src);
+            const int s = __builtin_amdgcn_readlane(S, src), t = at / s;
             it.r = base + src;
             it.parts = s;
-            it.tile = __builtin_amdgcn_readlane(t, src) - 1 - (MERGE ? at : at / s);
-            it.part = MERGE ? 0 : at % s;
-            const int in_req = MERGE ? at * s : at;
-            it.item = items + __builtin_amdgcn_readlane(incl_i - ni, src) + in_req;
-            it.slot = slots + __builtin_amdgcn_readlane(incl_s - ns, src) + in_req;
-            it.q.q0 = __builtin_amdgcn_readlane(x.q0, src);
-            it.q.n = __builtin_amdgcn_readlane(x.n, src);
-            it.q.len = __builtin_amdgcn_readlane(x.len, src);
+            it.tile = __builtin_amdgcn_readlane(x.tiles, src) - 1 - t;
+            it.part = at - t * s;
+            it.slot = slots + __builtin_amdgcn_readlane(incl_s - ns, src) + at;
+            it.cut = cuts + __builtin_amdgcn_readlane(incl_c - nc, src) + t;
+            it.q.q0 = __builtin_amdgcn_readlane(x.q.q0, src);
+            it.q.n = __builtin_amdgcn_readlane(x.q.n, src);
+            it.q.len = __builtin_amdgcn_readlane(x.q.len, src);
             return true;
         }
         before += all;
-        items += __builtin_amdgcn_readlane(incl_i, WAVE - 1);
         slots += __builtin_amdgcn_readlane(incl_s, WAVE - 1);
+        cuts += __builtin_amdgcn_readlane(incl_c, WAVE - 1);
     }
     return false;
 }
+__device__ __forceinline__ int count_cut(const amass_chunk_args& a, const ChunkPlan& pl,
+                                         const LaneReq& x0, int len) {
+    const int lane = threadIdx.x & 63;
+    int tot = 0;
+    for (int base = 0; base < a.n_req; base += WAVE) {
+        const LaneReq x = base == 0 ? x0 : lane_req(a, pl, base + lane);
+        tot += wave_sum_uniform(parts_of(x.work, len) > 1 ? x.tiles : 0);
+    }
+    return tot;
+}
 
-// tiles of keys per part of a row tile of n, and its parts (a short tile has fewer than its
-// request's longest)
+// tiles of keys per part of a row tile of n (a short tile has fewer parts than its request's
+// longest)
 __device__ __forceinline__ int part_len(int n, int parts) { return max(1, (n + parts - 1) / parts); }
+
+// ------------------------------------------------------------------ scratch
+// The number of cut row tiles, a record of each, then the slots of their parts, by kv head.  A
+// slot: per group of 32 rows D / 32 tiles of 16 x 64 floats, the rows' m and l, and whether
+// the part met V values that are not finite in a masked place.
+struct CutTile {
+    int r, tile, parts, slot;
+    Req q;
+    int pad;
+};
+constexpr int CK_HEAD = 256;
+constexpr int CK_STATS = 128;            // floats: m (32), l (32), bad
+
+__device__ __forceinline__ CutTile* cut_tile(const amass_chunk_args& a, int i) {
+    return reinterpret_cast<CutTile*>((char*)a.scratch + CK_HEAD) + i;
+}
+template <int D>
+__device__ __forceinline__ float* slot_group(const amass_chunk_args& a, const ChunkPlan& pl, int kh,
+                                             int slot, int group) {
+    const int64_t at = ((int64_t)kh * pl.slots + slot) * (pl.slot_rows / 32) + group;
+    return reinterpret_cast<float*>(cut_tile(a, pl.slots)) + at * (32 * D + CK_STATS);
+}
 
 // ------------------------------------------------------------------ one wave's state
 template <int D>
@@ -485,18 +520,6 @@ __device__ __forceinline__ void store_row(uint16_t* out, int x, const float (&o)
     }
 }
 
-// scratch: four bytes per item (a wave's `bad`), then the slots.  A slot: per group of 32 rows D / 32 tiles of 16 x 64 floats, then m and l of 64 lanes
-template <int D>
-__device__ __forceinline__ float* slot_group(const amass_chunk_args& a, const ChunkPlan& pl, int kh,
-                                             int slot, int group) {
-    const int64_t at = ((int64_t)kh * pl.slots + slot) * (pl.slot_rows / 32) + group;
-    return reinterpret_cast<float*>((char*)a.scratch + pl.flag_bytes) + at * (32 * D + 2 * WAVE);
-}
-__device__ __forceinline__ uint8_t* item_flags(const amass_chunk_args& a, const ChunkPlan& pl, int kh,
-                                               int item) {
-    return (uint8_t*)a.scratch + ((int64_t)kh * (pl.tiles_max + pl.target) + item) * CK_WAVES;
-}
-
 template <int D>
 __device__ __forceinline__ void save_tile(float* g, int x, const float (&o)[16], int lane) {
 #pragma unroll
@@ -505,16 +528,24 @@ __device__ __forceinline__ void save_tile(float* g, int x, const float (&o)[16],
             make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
 }
 
+template <int D>
+__device__ __forceinline__ void save_stats(float* g, float m, float l, bool bad, int lane) {
+    g[32 * D + lane] = lane < 32 ? m : l;        // (both halves of the wave hold the rows)
+    if (lane == 0) g[32 * D + WAVE] = bad ? 1.f : 0.f;
+}
+
 struct RowOut {
     uint16_t* out;       // the row, null for none
     float* lse;
 };
 
-__device__ __forceinline__ RowOut row_out(const amass_chunk_args& a, const Req& q, int kh, int row) {
+__device__ __forceinline__ RowOut row_out(const amass_chunk_args& a, const ChunkPlan& pl,
+                                          const Req& q, int kh, int row) {
     RowOut w = {nullptr, nullptr};
     if (row < q.n * a.G) {
-        const int64_t t = q.q0 + row / a.G;
-        const int64_t h = kh * a.G + row % a.G;
+        const int i = div_g(pl, row);
+        const int64_t t = q.q0 + i;
+        const int64_t h = kh * a.G + (row - i * a.G);
         w.out = (uint16_t*)a.out + t * a.o_st + h * a.o_hs;
         if (a.lse) w.lse = a.lse + t * a.l_st + h * a.l_hs;
     }
@@ -528,10 +559,65 @@ __device__ __forceinline__ void store_lse(const RowOut& w, float m, float l, flo
     }
 }
 
+// One row over the keys it sees and no others: the way for a row tile in whose masked places V is
+// not finite (there a weight of zero gives NaN in a matrix product).  A wave takes 64 keys at a
+// time, a key per lane for the score, then d across the lanes for the values.  Slow, and rare.
+template <int DT, int D>
+__device__ __forceinline__ void attend_row(const amass_chunk_args& a, const ChunkPlan& pl,
+                                           const Req& q, int r, int kh, int row, float c, int lane) {
+    constexpr int PER = D / WAVE;                  // channels per lane
+    const int i = div_g(pl, row);
+    const int p = q.len - q.n + i;
+    const int lo = key_lo(a, p), hi = key_hi(a, pl, q.len, p);
+    const uint16_t* qr = (const uint16_t*)a.q + (int64_t)(q.q0 + i) * a.q_st +
+                         (int64_t)(kh * a.G + (row - i * a.G)) * a.q_hs;
+    const int32_t* table = a.block_table + r * a.bt_st;
+    const auto value = [](uint16_t h) { return DT == AMASS_BF16 ? bf16_to_f32(h) : fp16_to_f32(h); };
+    const auto place = [&](int t, int64_t sb, int64_t st, int64_t sh) -> int64_t {
+        const int b = table[t >> pl.sh];
+        return b >= 0 && b < a.nb ? b * sb + (t & ((1 << pl.sh) - 1)) * st + kh * sh : -1;
+    };
+    float m = -__FLT_MAX__, l = 0.f, o[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] = 0.f;
+    for (int t0 = lo; t0 < hi; t0 += WAVE) {
+        const int t = t0 + lane;
+        const int64_t at = t < hi ? place(t, a.k_sb, a.k_st, a.k_sh) : -1;
+        float s = -INFINITY;
+        if (at >= 0) {
+            s = 0.f;
+            const uint16_t* k = (const uint16_t*)a.k + at;
+            for (int x = 0; x < D; ++x) s = __builtin_fmaf(value(qr[x]), value(k[x]), s);
+        }
+        const float mx = fmaxf(m, wave_maxf_uniform(s));
+        const float al = __builtin_amdgcn_exp2f((m - mx) * c);
+        m = mx;
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -fmaxf(m * c, -__FLT_MAX__)));
+        l = l * al + wave_sumf(e);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) o[i] *= al;
+        for (int j = 0; j < WAVE && t0 + j < hi; ++j) {
+            const int64_t va = place(t0 + j, a.v_sb, a.v_st, a.v_sh);
+            if (va < 0) continue;
+            const float w = __shfl(e, j, WAVE);
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                o[i] += w * value(((const uint16_t*)a.v)[va + WAVE * i + lane]);
+        }
+    }
+    const RowOut ro = row_out(a, pl, q, kh, row);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        ro.out[WAVE * i + lane] = (uint16_t)pack2<DT>(o[i] * inv, 0.f);
+    if (lane == 0) store_lse(ro, m, l, c, 0);
+}
+
 template <int D>
 struct __align__(1024) ChunkLds {
     char kv[2 * 2 * CK_KEYS * 2 * D];              // staging, then the waves' O
     float m[CK_WAVES][WAVE], l[CK_WAVES][WAVE];
+    int bad[CK_WAVES];
 };
 
 // ------------------------------------------------------------------ kernel
@@ -546,13 +632,23 @@ __global__ __launch_bounds__(CK_WAVES * WAVE, 2) void chunk_kernel(const amass_c
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kh = blockIdx.x % a.n_kv;
     Item it;
-    if (!find_item<false>(a, pl, blockIdx.x / a.n_kv, it)) return;
+    {
+        const LaneReq x0 = lane_req(a, pl, lane);
+        const int plen = part_length(a, pl, x0);
+        if (blockIdx.x == 0 && w == 0) {
+            const int cuts = count_cut(a, pl, x0, plen);
+            if (lane == 0) *(int*)a.scratch = cuts;
+        }
+        if (!find_item(a, pl, x0, plen, blockIdx.x / a.n_kv, it)) return;
+    }
     const Span sp = tile_span(a, pl, it.q, it.tile);
     const int per = part_len(sp.n, it.parts);
     const int j0 = min(sp.n, it.part * per), j1 = min(sp.n, j0 + per);   // tiles of this part
     if (it.part > 0 && j0 >= j1) return;
     const bool whole = per >= sp.n;                // no other part has keys
-    if (!whole && it.slot >= pl.slots) return;     // (only a query_start that does not ascend)
+    if (it.parts > 1 && it.slot >= pl.slots) return;    // (a query_start that does not ascend)
+    if (it.parts > 1 && it.part == 0 && kh == 0 && threadIdx.x == 0)
+        *cut_tile(a, it.cut) = {it.r, it.tile, (sp.n + per - 1) / per, it.slot, it.q, 0};
     const int rows = min(CK_BM, it.q.n * a.G - it.tile * CK_BM);
     const bool few = rows <= CK_FEW;
     const int group = few ? 0 : w;                 // 32-row group of this wave
@@ -574,18 +670,19 @@ __global__ __launch_bounds__(CK_WAVES * WAVE, 2) void chunk_kernel(const amass_c
     const int len = min(it.q.len, pl.cap);
     // this lane's visible keys; the wave's rows see at least [lo_hi, hi_lo), at most [lo_lo, hi_hi)
     const bool live = row < it.q.n * a.G;
-    const int pos = start + row / a.G;
+    const int tok = div_g(pl, row);
+    const int pos = start + tok;
     const int hi = live ? key_hi(a, pl, it.q.len, pos) : 0, lo = live ? key_lo(a, pos) : 0;
     const int first = it.tile * CK_BM + 32 * group;
     const bool idle = first > last;
-    const int p_first = start + first / a.G, p_last = start + last / a.G;
+    const int p_first = start + div_g(pl, first), p_last = start + div_g(pl, last);
     const int hi_lo = key_hi(a, pl, it.q.len, p_first), hi_hi = key_hi(a, pl, it.q.len, p_last);
     const int lo_lo = key_lo(a, p_first), lo_hi = key_lo(a, p_last);
 
     u32x4_t q[D / 16];
     {
-        const uint16_t* src = (const uint16_t*)a.q + (int64_t)(it.q.q0 + row / a.G) * a.q_st +
-                              (int64_t)(kh * a.G + row % a.G) * a.q_hs + 8 * (lane >> 5);
+        const uint16_t* src = (const uint16_t*)a.q + (int64_t)(it.q.q0 + tok) * a.q_st +
+                              (int64_t)(kh * a.G + (row - tok * a.G)) * a.q_hs + 8 * (lane >> 5);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
             q[i] = live ? *reinterpret_cast<const u32x4_t*>(src + 16 * i) : (u32x4_t){0u, 0u, 0u, 0u};
@@ -718,7 +815,7 @@ __global__ __launch_bounds__(CK_WAVES * WAVE, 2) void chunk_kernel(const amass_c
             dma_wait<63>();
             if (more) vfull = issue_v(b + CK_WAVES);
         }
-        if (lane == 0) item_flags(a, pl, kh, it.item)[w] = bad;
+        if (lane == 0) lds.bad[w] = bad;
         // the waves' (m, l, O) through LDS: wave w takes d tile w of all of them
         dma_wait<0>();
         __syncthreads();
@@ -742,6 +839,14 @@ __global__ __launch_bounds__(CK_WAVES * WAVE, 2) void chunk_kernel(const amass_c
             wt[v] = __builtin_amdgcn_exp2f((lds.m[v][lane] - m) * c);
             l += lds.l[v][lane] * wt[v];
         }
+        bad = false;
+#pragma unroll
+        for (int v = 0; v < CK_WAVES; ++v) bad |= lds.bad[v] != 0;
+        if (whole && bad) {
+            for (int i = w; i < rows; i += CK_WAVES)
+                attend_row<DT, D>(a, pl, it.q, it.r, kh, it.tile * CK_BM + i, c, lane);
+            return;
+        }
         if (w >= D / 32) return;
         float o[16];
 #pragma unroll
@@ -762,7 +867,7 @@ __global__ __launch_bounds__(CK_WAVES * WAVE, 2) void chunk_kernel(const amass_c
             o[4 * i + 3] = z.w;
         }
         if (whole) {
-            const RowOut ro = row_out(a, it.q, kh, row);
+            const RowOut ro = row_out(a, pl, it.q, kh, row);
             const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] *= inv;
@@ -771,17 +876,17 @@ __global__ __launch_bounds__(CK_WAVES * WAVE, 2) void chunk_kernel(const amass_c
         } else {
             float* g = slot_group<D>(a, pl, kh, it.slot, 0);
             save_tile<D>(g, w, o, lane);
-            if (w == 0) {
-                g[32 * D + lane] = m;
-                g[32 * D + WAVE + lane] = l;
-            }
+            if (w == 0) save_stats<D>(g, m, l, bad, lane);
         }
         return;
     }
-    if (lane == 0) item_flags(a, pl, kh, it.item)[w] = bad;
     if (idle) return;
+    if (whole && bad) {
+        for (int i = first; i <= last; ++i) attend_row<DT, D>(a, pl, it.q, it.r, kh, i, c, lane);
+        return;
+    }
     const float l = st.l + xor32_f(st.l);
-    const RowOut ro = row_out(a, it.q, kh, row);
+    const RowOut ro = row_out(a, pl, it.q, kh, row);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     float* g = whole ? nullptr : slot_group<D>(a, pl, kh, it.slot, group);
 #pragma unroll
@@ -792,128 +897,128 @@ __global__ __launch_bounds__(CK_WAVES * WAVE, 2) void chunk_kernel(const amass_c
         if (whole) store_row<DT, D>(ro.out, x, o, lane);
         else save_tile<D>(g, x, o, lane);
     }
-    if (whole) {
-        store_lse(ro, st.m, l, c, lane);
-    } else {
-        g[32 * D + lane] = st.m;
-        g[32 * D + WAVE + lane] = l;
-    }
+    if (whole) store_lse(ro, st.m, l, c, lane);
+    else save_stats<D>(g, st.m, l, bad, lane);
 }
 
-// One row over the keys it sees and no others: the way for a row tile in whose masked places V is
-// not finite (there a weight of zero gives NaN in a matrix product).  A wave takes 64 keys at a
-// time, a key per lane for the score, then d across the lanes for the values.  Slow, and rare.
-template <int DT, int D>
-__device__ __forceinline__ void attend_row(const amass_chunk_args& a, const ChunkPlan& pl,
-                                           const Req& q, int r, int kh, int row, float c, int lane) {
-    constexpr int PER = D / WAVE;                  // channels per lane
-    const int p = q.len - q.n + row / a.G;
-    const int lo = key_lo(a, p), hi = key_hi(a, pl, q.len, p);
-    const uint16_t* qr = (const uint16_t*)a.q + (int64_t)(q.q0 + row / a.G) * a.q_st +
-                         (int64_t)(kh * a.G + row % a.G) * a.q_hs;
-    const int32_t* table = a.block_table + r * a.bt_st;
-    const auto value = [](uint16_t h) { return DT == AMASS_BF16 ? bf16_to_f32(h) : fp16_to_f32(h); };
-    const auto place = [&](int t, int64_t sb, int64_t st, int64_t sh) -> int64_t {
-        const int b = table[t >> pl.sh];
-        return b >= 0 && b < a.nb ? b * sb + (t & ((1 << pl.sh) - 1)) * st + kh * sh : -1;
-    };
-    float m = -__FLT_MAX__, l = 0.f, o[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = 0.f;
-    for (int t0 = lo; t0 < hi; t0 += WAVE) {
-        const int t = t0 + lane;
-        const int64_t at = t < hi ? place(t, a.k_sb, a.k_st, a.k_sh) : -1;
-        float s = -INFINITY;
-        if (at >= 0) {
-            s = 0.f;
-            const uint16_t* k = (const uint16_t*)a.k + at;
-            for (int i = 0; i < D; ++i) s = __builtin_fmaf(value(qr[i]), value(k[i]), s);
-        }
-        const float mx = fmaxf(m, wave_maxf_uniform(s));
-        const float al = __builtin_amdgcn_exp2f((m - mx) * c);
-        m = mx;
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -fmaxf(m * c, -__FLT_MAX__)));
-        l = l * al + wave_sumf(e);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) o[i] *= al;
-        for (int j = 0; j < WAVE && t0 + j < hi; ++j) {
-            const int64_t va = place(t0 + j, a.v_sb, a.v_st, a.v_sh);
-            if (va < 0) continue;
-            const float w = __shfl(e, j, WAVE);
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                o[i] += w * value(((const uint16_t*)a.v)[va + WAVE * i + lane]);
-        }
-    }
-    const RowOut ro = row_out(a, q, kh, row);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-        ro.out[WAVE * i + lane] = (uint16_t)pack2<DT>(o[i] * inv, 0.f);
-    if (lane == 0) store_lse(ro, m, l, c, 0);
-}
+// Joins the parts of cut row tiles: workgroup (cut tile and kv head, 32-row group, d tile).
+// Bound by the latency of its loads: record, statistics, O.  Wave w takes parts w, w + 4, ... in
+// batches whose loads are all issued before any is used, and the waves join through LDS.
+constexpr int CM_WAVES = 4;
+constexpr int CM_BATCH = 4;
 
-// Joins the parts of row tile blockIdx.x / n_kv (grid y: its 32-row groups): wave w takes d
-// tile w.
 template <int DT, int D>
-__global__ __launch_bounds__((D / 32) * WAVE) void chunk_merge_kernel(const amass_chunk_args a,
+__global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amass_chunk_args a,
                                                                       const ChunkPlan pl) {
+    __shared__ float ms[CM_WAVES][32], ls[CM_WAVES][32], os[CM_WAVES][16][WAVE];
+    __shared__ int bads[CM_WAVES];
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kh = blockIdx.x % a.n_kv, group = blockIdx.y;
-    Item it;
-    if (!find_item<true>(a, pl, blockIdx.x / a.n_kv, it)) return;
-    const Span sp = tile_span(a, pl, it.q, it.tile);
-    const int per = part_len(sp.n, it.parts);
-    const int parts = max(1, (sp.n + per - 1) / per);
-    const int rows = min(CK_BM, it.q.n * a.G - it.tile * CK_BM);
-    if (32 * group >= rows || it.item + parts > pl.tiles_max + pl.target ||
-        (parts > 1 && it.slot + parts > pl.slots))
-        return;
+    const int kh = blockIdx.x % a.n_kv, i = blockIdx.x / a.n_kv;
+    const int group = blockIdx.y, x = blockIdx.z;
+    const int cuts = *(const int*)a.scratch;
+    const CutTile ct = *cut_tile(a, i);            // (inside the scratch; read before it is known)
+    if (i >= cuts || ct.parts < 2 || ct.slot + ct.parts > pl.slots) return;
+    const int rows = min(CK_BM, ct.q.n * a.G - ct.tile * CK_BM);
+    if (32 * group >= rows) return;
     const float c = a.scale * 1.44269504088896341f;
-    const int row0 = it.tile * CK_BM + 32 * group;
-    const uint32_t* flags = reinterpret_cast<const uint32_t*>(item_flags(a, pl, kh, it.item));
-    uint32_t bad = 0;
-    for (int s = 0; s < parts; ++s) bad |= flags[s];
+    const float* g0 = slot_group<D>(a, pl, kh, ct.slot, group);
+    const int64_t step = (int64_t)(pl.slot_rows / 32) * (32 * D + CK_STATS);
+    const int rl = lane & 31;
+    float m = -__FLT_MAX__, l = 0.f, o[16];
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j] = 0.f;
+    for (int s0 = w; s0 < ct.parts; s0 += CM_WAVES * CM_BATCH) {
+        float pm[CM_BATCH], ps[CM_BATCH], pb[CM_BATCH];
+        float4 y[CM_BATCH][4];
+#pragma unroll
+        for (int u = 0; u < CM_BATCH; ++u) {
+            const int s = s0 + u * CM_WAVES;
+            pm[u] = -__FLT_MAX__;
+            ps[u] = pb[u] = 0.f;
+            if (s < ct.parts) {                    // (scalar)
+                const float* g = g0 + s * step;
+                pm[u] = g[32 * D + rl];
+                ps[u] = g[32 * D + 32 + rl];
+                pb[u] = g[32 * D + WAVE];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    y[u][j] = *reinterpret_cast<const float4*>(g + (x * 4 + j) * 4 * WAVE + 4 * lane);
+            }
+        }
+        float mx = m;
+#pragma unroll
+        for (int u = 0; u < CM_BATCH; ++u) mx = fmaxf(mx, pm[u]);
+        const float al = __builtin_amdgcn_exp2f((m - mx) * c);
+        m = mx;
+        l *= al;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] *= al;
+#pragma unroll
+        for (int u = 0; u < CM_BATCH; ++u)
+            if (s0 + u * CM_WAVES < ct.parts) {
+                const float wt = __builtin_amdgcn_exp2f((pm[u] - m) * c);
+                bad |= pb[u] != 0.f;
+                l += ps[u] * wt;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    o[4 * j] += y[u][j].x * wt;
+                    o[4 * j + 1] += y[u][j].y * wt;
+                    o[4 * j + 2] += y[u][j].z * wt;
+                    o[4 * j + 3] += y[u][j].w * wt;
+                }
+            }
+    }
+    if (lane < 32) {
+        ms[w][lane] = m;
+        ls[w][lane] = l;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) os[w][j][lane] = o[j];
+    if (lane == 0) bads[w] = bad;
+    __syncthreads();
+    bad = false;
+#pragma unroll
+    for (int v = 0; v < CM_WAVES; ++v) bad |= bads[v] != 0;
+    const int row0 = ct.tile * CK_BM + 32 * group;
     if (bad) {
-        for (int i = w; i < min(32, rows - 32 * group); i += D / 32)
-            attend_row<DT, D>(a, pl, it.q, it.r, kh, row0 + i, c, lane);
+        for (int j = w + CM_WAVES * x; j < min(32, rows - 32 * group); j += CM_WAVES * (D / 32))
+            attend_row<DT, D>(a, pl, ct.q, ct.r, kh, row0 + j, c, lane);
         return;
     }
-    if (parts < 2) return;
-    float m = -__FLT_MAX__;
-    for (int s = 0; s < parts; ++s)
-        m = fmaxf(m, slot_group<D>(a, pl, kh, it.slot + s, group)[32 * D + lane]);
-    float l = 0.f, o[16];
+    if (w != 0) return;
+    m = -__FLT_MAX__;
+    l = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] = 0.f;
-    for (int s = 0; s < parts; ++s) {
-        const float* g = slot_group<D>(a, pl, kh, it.slot + s, group);
-        const float wt = __builtin_amdgcn_exp2f((g[32 * D + lane] - m) * c);
-        l += g[32 * D + WAVE + lane] * wt;
+    for (int v = 0; v < CM_WAVES; ++v) m = fmaxf(m, ms[v][rl]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 y = *reinterpret_cast<const float4*>(g + (w * 4 + i) * 4 * WAVE + 4 * lane);
-            o[4 * i] += y.x * wt;
-            o[4 * i + 1] += y.y * wt;
-            o[4 * i + 2] += y.z * wt;
-            o[4 * i + 3] += y.w * wt;
-        }
+    for (int j = 0; j < 16; ++j) o[j] = 0.f;
+#pragma unroll
+    for (int v = 0; v < CM_WAVES; ++v) {
+        const float wt = __builtin_amdgcn_exp2f((ms[v][rl] - m) * c);
+        l += ls[v][rl] * wt;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] += os[v][j][lane] * wt;
     }
-    const RowOut ro = row_out(a, it.q, kh, row0 + (lane & 31));
+    const RowOut ro = row_out(a, pl, ct.q, kh, row0 + rl);
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] *= inv;
-    store_row<DT, D>(ro.out, w, o, lane);
-    if (w == 0) store_lse(ro, m, l, c, lane);
+    for (int j = 0; j < 16; ++j) o[j] *= inv;
+    store_row<DT, D>(ro.out, x, o, lane);
+    if (x == 0) store_lse(ro, m, l, c, lane);
 }
 
 // ------------------------------------------------------------------ host
+// compute units of the current device, asked for once per device
 static int chunk_cus() {
+    static std::atomic<int> known[64];
     int dev = 0, n = 0;
-    if (hipGetDevice(&dev) != hipSuccess ||
-        hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1)
+    if (hipGetDevice(&dev) != hipSuccess) return 256;
+    if (dev >= 0 && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1)
         return 256;
+    if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 
@@ -953,12 +1058,15 @@ static ChunkPlan chunk_plan(const amass_chunk_args& a) {
     // are at most twice sum_r tiles_r w_r / len <= target
     p.slots = p.tiles_max < p.target ? p.target : 2 * p.target;
     p.slot_rows = rows <= CK_FEW ? CK_FEW : CK_BM;
-    p.flag_bytes = ((int64_t)a.n_kv * (p.tiles_max + p.target) * CK_WAVES + 255) & ~(int64_t)255;
+    p.g_sh = 0;
+    while ((1 << p.g_sh) < a.G) ++p.g_sh;
+    p.g_mul = (uint32_t)((((uint64_t)1 << (30 + p.g_sh)) + a.G - 1) / a.G);
     return p;
 }
 
 static int64_t chunk_scratch(const amass_chunk_args& a, const ChunkPlan& p) {
-    return p.flag_bytes + (int64_t)a.n_kv * p.slots * (p.slot_rows / 32) * (32 * a.d + 2 * WAVE) * sizeof(float);
+    return CK_HEAD + (int64_t)p.slots * sizeof(CutTile) +
+           (int64_t)a.n_kv * p.slots * (p.slot_rows / 32) * (32 * a.d + CK_STATS) * sizeof(float);
 }
 
 template <int DT, int D>
@@ -968,8 +1076,10 @@ static int launch_chunk(const amass_chunk_args& a, const ChunkPlan& p, hipStream
     hipLaunchKernelGGL((chunk_kernel<DT, D>), dim3((unsigned)items), dim3(CK_WAVES * WAVE), 0, s, a, p);
     const int rc = check_launch();
     if (rc) return rc;
-    hipLaunchKernelGGL((chunk_merge_kernel<DT, D>), dim3(p.tiles_max * a.n_kv, p.slot_rows / 32),
-                       dim3((D / 32) * WAVE), 0, s, a, p);
+    // a cut tile has two slots at least
+    const int cuts = p.tiles_max < (p.slots + 1) / 2 ? p.tiles_max : (p.slots + 1) / 2;
+    hipLaunchKernelGGL((chunk_merge_kernel<DT, D>), dim3(cuts * a.n_kv, p.slot_rows / 32, D / 32),
+                       dim3(CM_WAVES * WAVE), 0, s, a, p);
     return check_launch();
 }
 

@@ -127,6 +127,13 @@ __device__ __forceinline__ float wave_maxf_uniform(float v) {
     return fmaxf(fmaxf(readlane_f(v, 0), readlane_f(v, 16)),
                  fmaxf(readlane_f(v, 32), readlane_f(v, 48)));
 }
+__device__ __forceinline__ float wave_sumf_uniform(float v) {
+    v += dpp_f<DPP_HALF_MIRROR>(v);
+    v += dpp_f<DPP_XOR2>(v);
+    v += dpp_f<DPP_XOR1>(v);
+    v += dpp_f<DPP_ROW_MIRROR>(v);
+    return (readlane_f(v, 0) + readlane_f(v, 16)) + (readlane_f(v, 32) + readlane_f(v, 48));
+}
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
     return (uint32_t)dpp_i<CTRL>((int)v);
