@@ -162,7 +162,7 @@ class RopeArgs(C.Structure):
 
 class ChunkArgs(C.Structure):
     _fields_ = _fields(
-        "q:p q_st:i64 q_hs:i64 k:p k_sb:i64 k_st:i64 k_sh:i64 v:p v_sb:i64 v_st:i64 v_sh:i64 "
+        "q:p q_st:i64 q_hs:i64 k:p v:p kv_sb:i64 kv_st:i64 kv_sh:i64 "
         "block_table:p bt_st:i64 seq_lens:p query_start:p out:p o_st:i64 o_hs:i64 lse:p "
         "l_st:i64 l_hs:i64 scratch:p scratch_bytes:i64 scale:f32 n_req:i32 n_tokens:i32 "
         "n_kv:i32 G:i32 d:i32 page:i32 nb:i32 max_pages:i32 causal:i32 window:i32 dtype:i32")

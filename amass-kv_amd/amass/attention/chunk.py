@@ -66,8 +66,8 @@ def _chunk_args(q, kv_cache, block_table, seq_lens, query_start, out, scale, cau
             raise ValueError("lse must be (T, H) fp32")
         l_at = lse.data_ptr()
         l_st, l_hs = lse.stride()
-    return ((q.data_ptr(), q_st, q_hs, k, sb, st, sh, v, sb, st, sh, block_table.data_ptr(),
-             bt_st, seq_lens.data_ptr(), query_start.data_ptr(), out.data_ptr(), o_st, o_hs,
+    return ((q.data_ptr(), q_st, q_hs, k, v, sb, st, sh, block_table.data_ptr(), bt_st,
+             seq_lens.data_ptr(), query_start.data_ptr(), out.data_ptr(), o_st, o_hs,
              l_at, l_st, l_hs),
             (scale, n_req, T, n_kv, H // n_kv, d, page, nb, width, 1 if causal else 0,
              window or 0, DTYPES[dt]))

@@ -306,35 +306,36 @@ __device__ __forceinline__ void reset(RowState<D>& st) {
     st.l = 0.f;
 }
 
-// Byte offset in a V image of lane (h, sub, i16)'s part of a transposing read: d tile x, the
-// four keys from 8 e + 4 h.
-template <int D>
-__device__ __forceinline__ uint32_t v_place(int x, int e, int i16, int h, int sub) {
-    const int t = 8 * e + 4 * h + (i16 >> 2);
-    const int c = 4 * x + 2 * sub + ((i16 >> 1) & 1);
-    return t * (2 * D) + ((c ^ swz<D>(t)) << 4) + (i16 & 1) * 8;
-}
-
-// Lane constants of the LDS reads (byte offsets within a K or V image).
+// This lane's LDS reads, as byte offsets within a K or V image.  The swizzle only turns bits of
+// the 16-byte chunk, and so does going to another chunk of the same row, so one offset each
+// and an XOR reach all of them.
 template <int D>
 struct LdsLane {
-    uint32_t k[D / 16];      // chunk of MFMA i, key row lane % 32
-    uint32_t v[D / 32][2];   // 4-row block (keys 4 h .. and 8 + 4 h ..), d tile x
+    uint32_t k, v;
     __device__ __forceinline__ LdsLane(int lane) {
         const int row = lane & 31, h = lane >> 5, i16 = lane & 15, sub = (lane >> 4) & 1;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-            k[i] = row * (2 * D) + (((2 * i + h) ^ swz<D>(row)) << 4);
-#pragma unroll
-        for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) v[x][e] = v_place<D>(x, e, i16, h, sub);
+        k = row * (2 * D) + ((h ^ swz<D>(row)) << 4);
+        const int t = 4 * h + (i16 >> 2), c = 2 * sub + ((i16 >> 1) & 1);
+        v = t * (2 * D) + ((c ^ swz<D>(t)) << 4) + (i16 & 1) * 8;
+    }
+    // channels 16 i + 8 h .. of key row % 32 + 32 x
+    __device__ __forceinline__ u32x4_t k_frag(uint32_t ks, int i, int x) const {
+        return *(const __attribute__((address_space(3))) u32x4_t*)(uintptr_t)(
+            ((ks + k) ^ (uint32_t)(i << 5)) + x * (64 * D));
+    }
+    // d tile x of the 16 keys from 16 y: four keys from 4 h, four from 8 + 4 h (whose rows
+    // turn the chunk's lowest bit)
+    __device__ __forceinline__ u32x4_t v_frag(uint32_t vs, int x, int y) const {
+        const uint32_t at = (vs + v) ^ (uint32_t)(x << 6);
+        const u32x2_t a = lds_tr4(at + y * (32 * D));
+        const u32x2_t b = lds_tr4((at ^ 16u) + y * (32 * D) + 16 * D);
+        return (u32x4_t){a[0], a[1], b[0], b[1]};
     }
 };
 
 // S^T of 32 NK keys
 template <int DT, int D, int NK>
-__device__ __forceinline__ void scores(const char* ks, const LdsLane<D>& ll,
+__device__ __forceinline__ void scores(uint32_t ks, const LdsLane<D>& ll,
                                        const u32x4_t (&q)[D / 16], f32x16_t (&s)[NK]) {
 #pragma unroll
     for (int x = 0; x < NK; ++x)
@@ -343,10 +344,8 @@ __device__ __forceinline__ void scores(const char* ks, const LdsLane<D>& ll,
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-        for (int x = 0; x < NK; ++x) {
-            const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(ks + ll.k[i] + x * (64 * D));
-            s[x] = mfma32<DT>(kf, q[i], s[x]);
-        }
+        for (int x = 0; x < NK; ++x)
+            s[x] = mfma32<DT>(ll.k_frag(ks, i, x), q[i], s[x]);
 }
 
 // -inf for the keys (relative to the tile) outside [lo, hi) of this lane's row, and those of
@@ -367,60 +366,164 @@ __device__ __forceinline__ void mask_scores(f32x16_t (&s)[NK], int lo, int hi, u
         }
 }
 
-// Running softmax: s -> packed weights p (B operand of 16-key step y: p[y]), st.m, st.l and
-// the rescale of st.o.  The maximum may lag the true one by 2^CK_LAZY, which the weights (up
-// to 2^8) and fp32 sums hold exactly as well, so most tiles skip the rescale.
-template <int DT, int D, int NK>
-__device__ __forceinline__ void softmax(f32x16_t (&s)[NK], float c, RowState<D>& st,
-                                        u32x4_t (&p)[2 * NK]) {
-    float mx = s[0][0];
+// The running maximum after these scores, and the rescale of what was summed.  The maximum
+// may lag the true one by 2^CK_LAZY, which the weights (up to 2^8) and fp32 sums hold exactly
+// as well, so most tiles skip the rescale.
+__device__ __forceinline__ float row_max(const f32x16_t& s) {
+    float mx = s[0];
 #pragma unroll
-    for (int x = 0; x < NK; ++x)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[x][i]);
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    return mx;
+}
+// O times al, passed over where every lane's is 1.  Written out with its own skip, on registers
+// of its own choice: as a branch of the program the products would be new values, and the compiler moves
+// all of O (64 registers) twice a tile to join them.  The waits cover a matrix product's result
+// before, and its operand after.
+#define CK_MUL1(r) "v_mul_f32 v" #r ", %[al], v" #r "\n\t"
+#define CK_MUL16(a, b, c, d, e, f, g, h, i, j, k, l, m, n, o, p)                               \
+    CK_MUL1(a) CK_MUL1(b) CK_MUL1(c) CK_MUL1(d) CK_MUL1(e) CK_MUL1(f) CK_MUL1(g) CK_MUL1(h)     \
+    CK_MUL1(i) CK_MUL1(j) CK_MUL1(k) CK_MUL1(l) CK_MUL1(m) CK_MUL1(n) CK_MUL1(o) CK_MUL1(p)
+#define CK_MUL_0 CK_MUL16(128, 129, 130, 131, 132, 133, 134, 135, 136, 137, 138, 139, 140, 141, 142, 143)
+#define CK_MUL_1 CK_MUL16(144, 145, 146, 147, 148, 149, 150, 151, 152, 153, 154, 155, 156, 157, 158, 159)
+#define CK_MUL_2 CK_MUL16(160, 161, 162, 163, 164, 165, 166, 167, 168, 169, 170, 171, 172, 173, 174, 175)
+#define CK_MUL_3 CK_MUL16(176, 177, 178, 179, 180, 181, 182, 183, 184, 185, 186, 187, 188, 189, 190, 191)
+#define CK_SKIP "v_cmp_neq_f32 vcc, 1.0, %[al]\n\ts_cbranch_vccz 1f\n\ts_nop 15\n\ts_nop 15\n\t"
+template <int D>
+__device__ __forceinline__ void scale_o(RowState<D>& st, float al) {
+    if constexpr (D == 128)
+        asm volatile(CK_SKIP CK_MUL_0 CK_MUL_1 CK_MUL_2 CK_MUL_3 "s_nop 7\n1:"
+                     : "+{v[128:143]}"(st.o[0]), "+{v[144:159]}"(st.o[1]),
+                       "+{v[160:175]}"(st.o[D / 32 - 2]), "+{v[176:191]}"(st.o[D / 32 - 1])
+                     : [al] "v"(al)
+                     : "vcc");
+    else
+        asm volatile(CK_SKIP CK_MUL_0 CK_MUL_1 "s_nop 7\n1:"
+                     : "+{v[128:143]}"(st.o[0]), "+{v[144:159]}"(st.o[1])
+                     : [al] "v"(al)
+                     : "vcc");
+}
+// the maximum and the sum for a higher maximum; the factor for O
+template <int D>
+__device__ __forceinline__ float raise(float mx, float c, RowState<D>& st) {
+    const float m = fmaxf(st.m, mx);
+    const float al = __builtin_amdgcn_exp2f((st.m - m) * c);
+    st.m = m;
+    st.l *= al;
+    return al;
+}
+template <int D>
+__device__ __forceinline__ bool lags(float mx, float c, const RowState<D>& st) {
+    return __any((mx - st.m) * c > CK_LAZY);
+}
+template <int D, int NK>
+__device__ __forceinline__ void maximum(const f32x16_t (&s)[NK], float c, RowState<D>& st) {
+    float mx = row_max(s[0]);
+    if constexpr (NK == 2) mx = fmaxf(mx, row_max(s[1]));
     mx = xor32_maxf(mx);
-    if (__any((mx - st.m) * c > CK_LAZY)) {
-        const float m = fmaxf(st.m, mx);
-        const float al = __builtin_amdgcn_exp2f((st.m - m) * c);
-        st.m = m;
-        st.l *= al;
-#pragma unroll
-        for (int x = 0; x < D / 32; ++x)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) st.o[x][i] *= al;
-    }
+    float al = 1.f;
+    const bool lag = lags(mx, c, st);
+    if (lag) al = raise(mx, c, st);
+    scale_o(st, al);
+}
+
+// Weights p = 2^(c s - c m) and O^T += V^T P^T, 32 keys at a time: the exponentials of the
+// second 32 run under the products of the first.  Scores (2 x, 8 y ..) packed are the B operand of
+// 16-key step 2 x + y.
+template <int DT, int D, int NK>
+__device__ __forceinline__ void weigh(uint32_t vs, const LdsLane<D>& ll, const f32x16_t (&s)[NK],
+                                      float c, RowState<D>& st) {
     const float mc = fmaxf(st.m * c, -__FLT_MAX__);
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int x = 0; x < NK; ++x)
+    for (int x = 0; x < NK; ++x) {
+        u32x4_t p[2];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[x][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], c, -mc));
-            sum[i & 3] += s[x][i];
+        for (int i = 0; i < 16; i += 2) {
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], c, -mc));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i + 1], c, -mc));
+            sum[i & 2] += e0;
+            sum[(i & 2) + 1] += e1;
+            p[i >> 3][(i >> 1) & 3] = pack2<DT>(e0, e1);
         }
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int z = 0; z < D / 32; ++z)
+                st.o[z] = mfma32<DT>(ll.v_frag(vs, z, 2 * x + y), p[y], st.o[z]);
+    }
     st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-    for (int y = 0; y < 2 * NK; ++y)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            p[y][j] = pack2<DT>(s[y >> 1][8 * (y & 1) + 2 * j], s[y >> 1][8 * (y & 1) + 2 * j + 1]);
 }
 
-template <int D>
-__device__ __forceinline__ u32x4_t v_frag(uint32_t vs, const LdsLane<D>& ll, int x, int y) {
-    const u32x2_t a = lds_tr4(vs + ll.v[x][0] + y * (32 * D));
-    const u32x2_t b = lds_tr4(vs + ll.v[x][1] + y * (32 * D));
-    return (u32x4_t){a[0], a[1], b[0], b[1]};
-}
-
-template <int DT, int D, int NK>
-__device__ __forceinline__ void weigh(uint32_t vs, const LdsLane<D>& ll, const u32x4_t (&p)[2 * NK],
-                                      RowState<D>& st) {
+// A whole tile of 64 keys that every row sees, in a fixed order (each step ends in a scheduling
+// barrier): the matrix products follow each other with four fragments in flight, and the
+// vector work runs under them:
+//   scores of keys 0..31 | scores of 32..63, weights of 0..31 | maximum |
+//   products with V of 0..31, weights of 32..63 | products with V of 32..63
+// The first weights are made with the maximum so far and made again in the rare tile whose
+// scores exceed it by more than it may lag.
+template <int DT, int D>
+__device__ __forceinline__ void whole_tile(uint32_t ks, uint32_t vs, const LdsLane<D>& ll,
+                                           const u32x4_t (&q)[D / 16], float c, RowState<D>& st) {
+    constexpr int N = D / 16, Z = D / 32;      // products of 32 keys with K or V; d tiles
+    u32x4_t f[4], p[4];
+    f32x16_t s[2], zero;
 #pragma unroll
-    for (int y = 0; y < 2 * NK; ++y)
+    for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+    const auto k_frag = [&](int n) { return ll.k_frag(ks, n % N, n / N); };
+    const auto step = [] { __builtin_amdgcn_sched_barrier(0); };
+    float mc = fmaxf(st.m * c, -__FLT_MAX__), sum[4] = {0.f, 0.f, 0.f, 0.f};
+    const auto weight = [&](int x, int i) {    // weights 2 i and 2 i + 1 of half x
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][2 * i], c, -mc));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][2 * i + 1], c, -mc));
+        sum[2 * (i & 1)] += e0;
+        sum[2 * (i & 1) + 1] += e1;
+        uint32_t w = pack2<DT>(e0, e1);
+        asm volatile("" : "+v"(w));            // (made here, not behind the branch below)
+        p[2 * x + (i >> 2)][i & 3] = w;
+    };
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x)
-            st.o[x] = mfma32<DT>(v_frag<D>(vs, ll, x, y), p[y], st.o[x]);
+    for (int n = 0; n < 4; ++n) f[n] = k_frag(n);
+    step();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        s[0] = mfma32<DT>(f[n & 3], q[n], n ? s[0] : zero);
+        f[n & 3] = k_frag(n + 4);
+        step();
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        s[1] = mfma32<DT>(f[n & 3], q[n], n ? s[1] : zero);
+        if (n + 4 < N) f[n & 3] = k_frag(N + n + 4);
+        else f[n & 3] = ll.v_frag(vs, (n + 4 - N) % Z, (n + 4 - N) / Z);
+#pragma unroll
+        for (int i = 8 * n / N; i < 8 * (n + 1) / N; ++i) weight(0, i);
+        step();
+    }
+    const float mx = xor32_maxf(fmaxf(row_max(s[0]), row_max(s[1])));
+    const bool lag = lags(mx, c, st);
+    float al = 1.f;
+    if (lag) {
+        al = raise(mx, c, st);
+        mc = fmaxf(st.m * c, -__FLT_MAX__);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weight(0, i);
+    }
+    scale_o(st, al);
+    step();
+    // V fragment n: 16-key step n / Z, d tile n % Z
+#pragma unroll
+    for (int n = 0; n < 2 * N; ++n) {
+        st.o[n % Z] = mfma32<DT>(f[n & 3], p[n / Z], st.o[n % Z]);
+        if (n + 4 < 2 * N) f[n & 3] = ll.v_frag(vs, (n + 4) % Z, (n + 4) / Z);
+        if (n < N) {
+#pragma unroll
+            for (int i = 8 * n / N; i < 8 * (n + 1) / N; ++i) weight(1, i);
+        }
+        step();
+    }
+    st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 // whether any V value of the 32 NK keys is an infinity or a NaN
@@ -431,7 +534,7 @@ __device__ __forceinline__ bool any_nonfinite(uint32_t vs, const LdsLane<D>& ll)
     for (int y = 0; y < 2 * NK; ++y)
 #pragma unroll
         for (int x = 0; x < D / 32; ++x) {
-            const u32x4_t v = v_frag<D>(vs, ll, x, y);
+            const u32x4_t v = ll.v_frag(vs, x, y);
 #pragma unroll
             for (int j = 0; j < 4; ++j) bad |= nonfinite2<DT>(v[j]);
         }
@@ -439,61 +542,53 @@ __device__ __forceinline__ bool any_nonfinite(uint32_t vs, const LdsLane<D>& ll)
 }
 
 // ------------------------------------------------------------------ staging
-// The 16 keys from t of one request: K rows to LDS at `kd`, V rows at `vd` (16 rows of 2 D
-// bytes, swizzled).  Rows at or past `len` hold nothing of the request: their V is zero (the
-// weight of a masked key is zero, and zero times what lies there could be NaN).
+// One request's pages of one kv head.  Everything but the lane offsets is uniform.
 template <int D>
-struct Stage {
+struct Pages {
     static constexpr int ROWS = 512 / D;           // rows of one 1-KB load
-    static constexpr int LOADS = 16 / ROWS;
-    uint32_t k[LOADS], v[LOADS];                   // this lane's source offsets
+    static constexpr int LOADS = 16 / ROWS;        // loads of 16 rows
+    const __attribute__((address_space(4))) int32_t* table;   // the request's row
+    const char* k;                                 // of the kv head
+    int64_t to_v;                                  // from a K row to its V row
+    uint32_t sb, st;                               // bytes of a block, a row
+    int sh, nb, last;                              // last: a position that has a table entry
+    uint32_t lane_off[LOADS];                      // this lane's source in a 16-row group
     int lane;
-    __device__ __forceinline__ Stage(const amass_chunk_args& a, int lane_) : lane(lane_) {
+
+    __device__ __forceinline__ Pages(const amass_chunk_args& a, const ChunkPlan& pl, int r, int kh,
+                                     int hi, int lane_)
+        : table((const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.block_table +
+                                                                              r * a.bt_st)),
+          k((const char*)a.k + kh * a.kv_sh * 2), to_v((const char*)a.v - (const char*)a.k),
+          sb((uint32_t)a.kv_sb * 2), st((uint32_t)a.kv_st * 2), sh(pl.sh), nb(a.nb),
+          last(max(hi - 1, 0)), lane(lane_) {
         const int chunk = lane & (D / 8 - 1), lr = lane / (D / 8);
 #pragma unroll
         for (int n = 0; n < LOADS; ++n) {
             const int row = ROWS * n + lr;
-            const uint32_t c = (chunk ^ swz<D>(row)) << 4;
-            k[n] = (uint32_t)(2 * row * a.k_st) + c;
-            v[n] = (uint32_t)(2 * row * a.v_st) + c;
+            lane_off[n] = (uint32_t)row * st + ((uint32_t)(chunk ^ swz<D>(row)) << 4);
         }
     }
-    __device__ __forceinline__ void load_k(uint32_t to, const char* src) const {
-#pragma unroll
-        for (int n = 0; n < LOADS; ++n) dma16(to + 1024 * n, src, k[n]);
+    // table entry of position t (of `last` behind it) and whether the pool has that block
+    __device__ __forceinline__ int entry(int t) const { return table[min(t, last) >> sh]; }
+    __device__ __forceinline__ bool has(int id) const { return (uint32_t)id < (uint32_t)nb; }
+    __device__ __forceinline__ const char* row(int id, int t) const {
+        return k + (uint64_t)(uint32_t)id * sb + (uint32_t)(t & ((1 << sh) - 1)) * st;
     }
-    __device__ __forceinline__ void load_v(uint32_t to, const char* src) const {
+    // 16 rows to LDS
+    __device__ __forceinline__ void load(uint32_t to, const char* src) const {
 #pragma unroll
-        for (int n = 0; n < LOADS; ++n) dma16(to + 1024 * n, src, v[n]);
+        for (int n = 0; n < LOADS; ++n) dma16(to + 1024 * n, src, lane_off[n]);
     }
-    // the first `rows` rows, zero behind them
-    __device__ __forceinline__ void load_v_part(char* dst, uint32_t to, const char* src,
-                                                int rows) const {
+    // the first `rows` of 16 rows, zero behind them (the weight of a masked key is zero, and
+    // zero times what lies behind a request's last token could be NaN)
+    __device__ __forceinline__ void load_part(char* dst, uint32_t to, const char* src,
+                                              int rows) const {
 #pragma unroll
         for (int n = 0; n < LOADS; ++n) {
-            if (ROWS * n + lane / (D / 8) < rows) dma16(to + 1024 * n, src, v[n]);
+            if (ROWS * n + lane / (D / 8) < rows) dma16(to + 1024 * n, src, lane_off[n]);
             else *reinterpret_cast<u32x4_t*>(dst + 1024 * n + 16 * lane) = (u32x4_t){0u, 0u, 0u, 0u};
         }
-    }
-};
-
-// Uniform view of a unit's pages.
-struct Pages {
-    const __attribute__((address_space(4))) int32_t* table;   // the request's row
-    const char* k;
-    const char* v;                                            // of the kv head
-    int64_t k_sb, k_st, v_sb, v_st;                           // bytes
-    int sh, nb;
-    // block of the 16 keys from t, -1 if the pool has none such
-    __device__ __forceinline__ int block(int t) const {
-        const int b = table[t >> sh];
-        return b >= 0 && b < nb ? b : -1;
-    }
-    __device__ __forceinline__ const char* k_at(int b, int t) const {
-        return k + b * k_sb + (t & ((1 << sh) - 1)) * k_st;
-    }
-    __device__ __forceinline__ const char* v_at(int b, int t) const {
-        return v + b * v_sb + (t & ((1 << sh) - 1)) * v_st;
     }
 };
 
@@ -573,16 +668,17 @@ __device__ __forceinline__ void attend_row(const amass_chunk_args& a, const Chun
                          (int64_t)(kh * a.G + (row - i * a.G)) * a.q_hs;
     const int32_t* table = a.block_table + r * a.bt_st;
     const auto value = [](uint16_t h) { return DT == AMASS_BF16 ? bf16_to_f32(h) : fp16_to_f32(h); };
-    const auto place = [&](int t, int64_t sb, int64_t st, int64_t sh) -> int64_t {
+    const auto place = [&](int t) -> int64_t {
         const int b = table[t >> pl.sh];
-        return b >= 0 && b < a.nb ? b * sb + (t & ((1 << pl.sh) - 1)) * st + kh * sh : -1;
+        return b >= 0 && b < a.nb ? b * a.kv_sb + (t & ((1 << pl.sh) - 1)) * a.kv_st + kh * a.kv_sh
+                                  : -1;
     };
     float m = -__FLT_MAX__, l = 0.f, o[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) o[i] = 0.f;
     for (int t0 = lo; t0 < hi; t0 += WAVE) {
         const int t = t0 + lane;
-        const int64_t at = t < hi ? place(t, a.k_sb, a.k_st, a.k_sh) : -1;
+        const int64_t at = t < hi ? place(t) : -1;
         float s = -INFINITY;
         if (at >= 0) {
             s = 0.f;
@@ -597,7 +693,7 @@ __device__ __forceinline__ void attend_row(const amass_chunk_args& a, const Chun
 #pragma unroll
         for (int i = 0; i < PER; ++i) o[i] *= al;
         for (int j = 0; j < WAVE && t0 + j < hi; ++j) {
-            const int64_t va = place(t0 + j, a.v_sb, a.v_st, a.v_sh);
+            const int64_t va = place(t0 + j);
             if (va < 0) continue;
             const float w = __shfl(e, j, WAVE);
 #pragma unroll
@@ -624,7 +720,8 @@ struct __align__(1024) ChunkLds {
 // grid: kv head fastest (workgroups of one kv head share an XCD's L2 where n_kv is a multiple
 // of 8), then the items.
 template <int DT, int D>
-__global__ __launch_bounds__(CK_WAVES * WAVE, 2) void chunk_kernel(const amass_chunk_args a,
+__global__ __launch_bounds__(CK_WAVES * WAVE) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+chunk_kernel(const amass_chunk_args a,
                                                                    const ChunkPlan pl) {
     __shared__ ChunkLds<D> lds;
     constexpr int KB = CK_KEYS * 2 * D;            // bytes of a K (or V) tile
@@ -656,17 +753,7 @@ __global__ __launch_bounds__(CK_WAVES * WAVE, 2) void chunk_kernel(const amass_c
     const int last = it.tile * CK_BM + min(rows, 32 * group + 32) - 1;    // of the wave
     const int start = it.q.len - it.q.n;
     const float c = a.scale * 1.44269504088896341f;
-    Pages pg;
-    pg.table = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.block_table +
-                                                                             it.r * a.bt_st);
-    pg.k = (const char*)a.k + kh * a.k_sh * 2;
-    pg.v = (const char*)a.v + kh * a.v_sh * 2;
-    pg.k_sb = a.k_sb * 2;
-    pg.k_st = a.k_st * 2;
-    pg.v_sb = a.v_sb * 2;
-    pg.v_st = a.v_st * 2;
-    pg.sh = pl.sh;
-    pg.nb = a.nb;
+    const Pages<D> pg(a, pl, it.r, kh, sp.hi, lane);
     const int len = min(it.q.len, pl.cap);
     // this lane's visible keys; the wave's rows see at least [lo_hi, hi_lo), at most [lo_lo, hi_hi)
     const bool live = row < it.q.n * a.G;
@@ -691,96 +778,119 @@ __global__ __launch_bounds__(CK_WAVES * WAVE, 2) void chunk_kernel(const amass_c
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(q[i]));
     const LdsLane<D> ll(lane);
-    const Stage<D> stage(a, lane);
     RowState<D> st;
     reset(st);
     bool bad = false;                              // a masked tile's V is not finite
 
     if (!few) {
         // ---- many rows: the workgroup shares the tiles -------------------------------------
+        // Wave w requests the 16 keys 64 j + 16 w .. of tile j, one tile ahead; their table entry
+        // is looked up another tile ahead, so that no request waits for it.
         const uint32_t base = lds_addr(lds.kv);
-        // wave w stages the 16 keys 64 j + 16 w ..; every wave knows which of the four have a block
-        const auto issue = [&](int j, int buf) -> uint32_t {
-            const int t0 = CK_KEYS * (sp.lo + j);
-            uint32_t ok = 0;
-            int mine = -1;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int t = t0 + 16 * g;
-                const int b = pg.block(t < sp.hi ? t : t0);
-                if (b >= 0 || t >= sp.hi) ok |= 1u << g;
-                if (g == w) mine = t < sp.hi ? b : -1;
-            }
-            const int t = t0 + 16 * w;
+        int t_next = CK_KEYS * (sp.lo + j0) + 16 * w, id = pg.entry(t_next);
+        const auto request = [&](int buf) {
             const uint32_t kd = base + 2 * KB * buf + 16 * w * 2 * D, vd = kd + KB;
-            if (mine >= 0) {
-                stage.load_k(kd, pg.k_at(mine, t));
-                if (t + 16 <= len) stage.load_v(vd, pg.v_at(mine, t));
-                else stage.load_v_part(lds.kv + (vd - base), vd, pg.v_at(mine, t), len - t);
+            const char* src = pg.row(id, t_next);
+            if (t_next + 16 <= len && pg.has(id)) {
+                pg.load(kd, src);
+                pg.load(vd, src + pg.to_v);
             } else {
-                stage.load_v_part(lds.kv + (vd - base), vd, pg.v, 0);
+                const int rows = pg.has(id) ? min(len - t_next, 16) : 0;
+                if (rows > 0) pg.load(kd, src);
+                pg.load_part(lds.kv + (vd - base), vd, src + pg.to_v, rows);
             }
-            return ok;
+            t_next += CK_KEYS;
+            id = pg.entry(t_next);
         };
-        uint32_t ok = j0 < j1 ? issue(j0, 0) : 0;
-        for (int j = j0; j < j1; ++j) {
-            const int buf = (j - j0) & 1;
+        // whether every page that a row of the workgroup sees in this part has a block
+        {
+            bool has = true;
+            const int from = max(CK_KEYS * (sp.lo + j0), key_lo(a, start + div_g(pl, it.tile * CK_BM)));
+            const int to = min(CK_KEYS * (sp.lo + j1), sp.hi);
+            for (int p = (from >> pg.sh) + threadIdx.x; p << pg.sh < to; p += CK_WAVES * WAVE)
+                has &= pg.has(a.block_table[it.r * a.bt_st + p]);
+            const bool all = __all(has);
+            if (lane == 0) lds.bad[w] = !all;
+        }
+        const auto turn = [&](int j) {
             dma_wait<0>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            const uint32_t groups = ok;
-            if (j + 1 < j1) ok = issue(j + 1, buf ^ 1);
+            if (j + 1 < j1) request((j + 1 - j0) & 1);
+        };
+        // tiles [f0, f1) hold only keys that all of the wave's rows see
+        bool sound = false;
+        const auto step = [&](int j) {             // a tile with masks
             const int t0 = CK_KEYS * (sp.lo + j);
-            if (idle || t0 >= hi_hi || t0 + CK_KEYS <= lo_lo) continue;
-            const char* ks = lds.kv + 2 * KB * buf;
-            const uint32_t vs = base + 2 * KB * buf + KB;
+            if (idle || t0 >= hi_hi || t0 + CK_KEYS <= lo_lo) return;
+            const uint32_t ks = base + 2 * KB * ((j - j0) & 1), vs = ks + KB;
+            uint32_t groups = 15;
+            if (!sound) {
+                groups = 0;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) groups |= (pg.has(pg.entry(t0 + 16 * g)) ? 1u : 0u) << g;
+            }
             f32x16_t s[2];
-            u32x4_t p[4];
             scores<DT, D, 2>(ks, ll, q, s);
-            const bool masked = t0 < lo_hi || t0 + CK_KEYS > hi_lo || groups != 15u;
-            if (masked) mask_scores<2>(s, lo - t0, hi - t0, groups, lane);
-            softmax<DT, D, 2>(s, c, st, p);
-            if (masked) bad |= any_nonfinite<DT, D, 2>(vs, ll);
-            weigh<DT, D, 2>(vs, ll, p, st);
+            mask_scores<2>(s, lo - t0, hi - t0, groups, lane);
+            if (t0 < lo_hi || t0 + CK_KEYS > hi_lo) bad |= any_nonfinite<DT, D, 2>(vs, ll);
+            maximum<D, 2>(s, c, st);
+            weigh<DT, D, 2>(vs, ll, s, c, st);
+        };
+        if (j0 < j1) {
+            request(0);
+            turn(j0);
+            sound = __builtin_amdgcn_readfirstlane(lds.bad[0] | lds.bad[1] | lds.bad[2] |
+                                                   lds.bad[3]) == 0;
+        }
+        const bool fast = sound && !idle;
+        const int f1 = fast ? min(j1, hi_lo / CK_KEYS - sp.lo) : j1;
+        const int f0 = fast ? min(f1, max(j0, (lo_hi + CK_KEYS - 1) / CK_KEYS - sp.lo)) : j1;
+        int j = j0;
+        while (j < f0) {
+            step(j);
+            if (++j < j1) turn(j);
+        }
+        while (j < f1) {
+            const uint32_t ks = base + 2 * KB * ((j - j0) & 1);
+            whole_tile<DT, D>(ks, ks + KB, ll, q, c, st);
+            if (++j < j1) turn(j);
+        }
+        while (j < j1) {
+            step(j);
+            if (++j < j1) turn(j);
         }
     } else {
         // ---- few rows: each wave its own 32 keys, w + 4, w + 8, ... ------------------------
         constexpr int HB = KB / 2;                 // 32 keys
         char* own = lds.kv + 2 * HB * w;           // K, then V
         const uint32_t base = lds_addr(own);
-        constexpr int LOADS = 2 * Stage<D>::LOADS;
+        constexpr int LOADS = 2 * Pages<D>::LOADS;
         const int b0 = 2 * (sp.lo + j0) + w, b1 = 2 * (sp.lo + j1);
-        uint32_t ok = 0;
-        int blk[2] = {-1, -1};
+        int id[2];
         const auto find = [&](int b) {
-            ok = 0;
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const int t = 32 * b + 16 * g;
-                blk[g] = t < sp.hi ? pg.block(t) : -1;
-                if (blk[g] >= 0 || t >= sp.hi) ok |= 1u << g;
-            }
+            for (int g = 0; g < 2; ++g) id[g] = pg.entry(32 * b + 16 * g);
         };
         // both return whether the usual number of loads is in flight
         const auto issue_k = [&](int b) -> bool {
 #pragma unroll
             for (int g = 0; g < 2; ++g)
-                if (blk[g] >= 0) stage.load_k(base + g * (HB / 2), pg.k_at(blk[g], 32 * b + 16 * g));
-            return blk[0] >= 0 && blk[1] >= 0;
+                if (pg.has(id[g])) pg.load(base + g * (HB / 2), pg.row(id[g], 32 * b + 16 * g));
+            return pg.has(id[0]) && pg.has(id[1]);
         };
         const auto issue_v = [&](int b) -> bool {
-            if (blk[0] >= 0 && blk[1] >= 0 && 32 * b + 32 <= len) {
+            if (pg.has(id[0]) && pg.has(id[1]) && 32 * b + 32 <= len) {
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
-                    stage.load_v(base + HB + g * (HB / 2), pg.v_at(blk[g], 32 * b + 16 * g));
+                    pg.load(base + HB + g * (HB / 2), pg.row(id[g], 32 * b + 16 * g) + pg.to_v);
                 return true;
             }
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 const int t = 32 * b + 16 * g;
-                stage.load_v_part(own + HB + g * (HB / 2), base + HB + g * (HB / 2),
-                                  blk[g] >= 0 ? pg.v_at(blk[g], t) : pg.v,
-                                  blk[g] >= 0 ? len - t : 0);
+                pg.load_part(own + HB + g * (HB / 2), base + HB + g * (HB / 2),
+                             pg.row(id[g], t) + pg.to_v, pg.has(id[g]) ? len - t : 0);
             }
             return false;
         };
@@ -792,13 +902,12 @@ __global__ __launch_bounds__(CK_WAVES * WAVE, 2) void chunk_kernel(const amass_c
         }
         for (int b = b0; b < b1; b += CK_WAVES) {
             const int t0 = 32 * b;
-            const uint32_t groups = ok;
+            const uint32_t groups = (pg.has(id[0]) ? 1u : 0u) | (pg.has(id[1]) ? 2u : 0u);
             const bool more = b + CK_WAVES < b1;
             f32x16_t s[1];
-            u32x4_t p[2];
             if (vfull) dma_wait<LOADS>();
             else dma_wait<0>();
-            scores<DT, D, 1>(own, ll, q, s);
+            scores<DT, D, 1>(base, ll, q, s);
             dma_wait<63>();                        // (the K reads have returned)
             if (more) {
                 find(b + CK_WAVES);
@@ -806,12 +915,12 @@ __global__ __launch_bounds__(CK_WAVES * WAVE, 2) void chunk_kernel(const amass_c
             }
             const bool masked = t0 < lo_hi || t0 + 32 > hi_lo || groups != 3u;
             if (masked) mask_scores<1>(s, lo - t0, hi - t0, groups, lane);
-            softmax<DT, D, 1>(s, c, st, p);
+            maximum<D, 1>(s, c, st);
             if (more && kfull) dma_wait<LOADS>();
             else dma_wait<0>();
             const uint32_t vs = base + HB;
             if (masked) bad |= any_nonfinite<DT, D, 1>(vs, ll);
-            weigh<DT, D, 1>(vs, ll, p, st);
+            weigh<DT, D, 1>(vs, ll, s, c, st);
             dma_wait<63>();
             if (more) vfull = issue_v(b + CK_WAVES);
         }
@@ -1037,10 +1146,11 @@ static int chunk_check(const amass_chunk_args& a) {
     if (a.n_kv > 4096 || a.G > 4096 || (int64_t)a.n_tokens * a.G > (1 << 30)) return AMASS_ERR_GEOMETRY;
     const auto off = [](const void* p) { return ((uintptr_t)p & 15) != 0; };
     if (off(a.q) || off(a.k) || off(a.v) || off(a.out) ||
-        ((a.q_st | a.q_hs | a.k_sb | a.k_st | a.k_sh | a.v_sb | a.v_st | a.v_sh | a.o_st | a.o_hs) & 7))
+        ((a.q_st | a.q_hs | a.kv_sb | a.kv_st | a.kv_sh | a.o_st | a.o_hs) & 7))
         return AMASS_ERR_GEOMETRY;
-    // a row's offset within its 16 keys is 32 bits in the kernel
-    if (a.k_st < 0 || a.v_st < 0 || a.k_st > (1 << 26) || a.v_st > (1 << 26)) return AMASS_ERR_GEOMETRY;
+    // the kernel has 32 bits for a row's offset (bytes) within its block
+    if (a.kv_sb < 0 || a.kv_sb >= (1 << 30) || a.kv_st < 0 || a.kv_st * a.page >= (1 << 30))
+        return AMASS_ERR_GEOMETRY;
     return AMASS_OK;
 }
 

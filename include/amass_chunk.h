@@ -109,7 +109,7 @@ int amass_rope_write(const amass_rope_args* a, void* stream);
  * not used, whatever it holds (infinities and NaN among it).  A row that sees no finite score (a
  * position below 0, an empty request, only scores of -inf) gets zeros and lse = -inf.  Rows of no request are left as
  * they are.  scale > 0.  d 64 or 128, page >= 16, G >= 1, K and V views 16-byte aligned with
- * strides of multiples of 8 elements, q likewise, out 16-byte aligned with strides of
+ * strides of multiples of 8 elements (a block below 2^30 of them), q likewise, out 16-byte aligned with strides of
  * multiples of 8.
  *
  * scratch: amass_chunk_scratch_bytes(a) bytes, 256-byte aligned, for the parts of rows whose
@@ -117,8 +117,8 @@ int amass_rope_write(const amass_rope_args* a, void* stream);
  * same time need one each. */
 typedef struct amass_chunk_args {
     const void*    q; int64_t q_st, q_hs;                /* (T,H,d) */
-    const void*    k; int64_t k_sb, k_st, k_sh;          /* (NB,page,n_kv,d) views */
-    const void*    v; int64_t v_sb, v_st, v_sh;
+    const void*    k; const void* v;                     /* (NB,page,n_kv,d) views of */
+    int64_t        kv_sb, kv_st, kv_sh;                  /* the same strides */
     const int32_t* block_table; int64_t bt_st;
     const int32_t* seq_lens;
     const int32_t* query_start;

@@ -52,8 +52,8 @@ def test_structs_and_symbols_mirror_the_header():
 
 def _chunk(**over):
     a = _hip.ChunkArgs()
-    base = dict(q=0x1000, q_st=512, q_hs=128, k=0x1000, k_sb=32768, k_st=1024, k_sh=128, v=0x1000,
-                v_sb=32768, v_st=1024, v_sh=128, block_table=0x1000, bt_st=4, seq_lens=0x1000,
+    base = dict(q=0x1000, q_st=512, q_hs=128, k=0x1000, v=0x1000,
+                kv_sb=32768, kv_st=1024, kv_sh=128, block_table=0x1000, bt_st=4, seq_lens=0x1000,
                 query_start=0x1000, out=0x1000, o_st=512, o_hs=128, scale=0.1, n_req=1,
                 n_tokens=3, n_kv=8, G=4, d=128, page=16, nb=4, max_pages=4, causal=1)
     for k, v in {**base, **over}.items():
@@ -66,8 +66,8 @@ def _chunk(**over):
     (dict(dtype=2), -3), (dict(page=8), -2), (dict(page=24), -2), (dict(scale=0.0), -2),
     (dict(scale=-1.0), -2), (dict(scale=math.nan), -2), (dict(scale=math.inf), -2),
     (dict(window=-1), -2), (dict(G=0), -2), (dict(n_kv=0), -2), (dict(nb=0), -2),
-    (dict(q=0x1008), -2), (dict(k_st=1028), -2), (dict(o_hs=124), -2), (dict(k_st=1 << 30), -2),
-    (dict(k_st=-1024), -2), (dict(n_tokens=1 << 29), -2), (dict(max_pages=0), -2)])
+    (dict(q=0x1008), -2), (dict(kv_st=1028), -2), (dict(o_hs=124), -2), (dict(kv_st=1 << 30), -2),
+    (dict(kv_st=-1024), -2), (dict(kv_sb=1 << 30), -2), (dict(kv_sb=-32768), -2), (dict(n_tokens=1 << 29), -2), (dict(max_pages=0), -2)])
 def test_chunk_attention_refuses(over, status):
     lib = _hip.load_library()
     a = _chunk(**over)
