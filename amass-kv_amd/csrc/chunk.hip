@@ -41,10 +41,16 @@ typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int CK_WAVES = 4;
+// workgroups per CU (waves per SIMD): 256 registers a lane at d = 128, 170 at d = 64
+constexpr int ck_wgs(int d) { return d == 128 ? 2 : 3; }
 constexpr int CK_BM = 32 * CK_WAVES;       // rows of a row tile
 constexpr int CK_FEW = 32;                 // rows up to which the waves share the rows
 constexpr int CK_KEYS = 64;                // keys of a tile
 constexpr int CK_MIN_SPLIT = 4;            // fewest tiles of a part
+// A tile of 64 keys costs a workgroup of few rows what the memory takes for it, 32 KB (d 128) at
+// 5 TB/s over 512 workgroups, 3.3 us, and one of many rows its products, 1.0 us.
+constexpr int CK_FEW_COST = 3;
+constexpr int CK_WORTH = 3;                // cut tiles for parts of at most 2 / 3 of the longest
 constexpr float CK_LAZY = 8.f;             // a maximum may lag by this power of two
 
 // ------------------------------------------------------------------ the 16-bit types
@@ -70,23 +76,32 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t x) {
 
 // ------------------------------------------------------------------ LDS
 // XOR of a row's 16-byte chunks: the 16 rows of a K read land in 16 places of the 256 bytes
-// that the banks serve, and 4 rows of a transposing V read in different chunk pairs.
+// that the banks serve, and the 4 rows (of 64 bytes) of half a wave's transposing V read in
+// different quarters of them.
 template <int D>
 __device__ __forceinline__ int swz(int row) {
-    return D == 128 ? ((row & 7) << 1) | ((row >> 3) & 1)
-                    : (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
+    return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3)
+                    : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
 }
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 // 16 bytes per lane from base + off (off per lane) to LDS at `to` + 16 lane (`to` uniform).
-// No register waits for it: the caller waits with dma_wait before anyone reads the place.
+// No register waits for it: the caller waits with dma_wait before anyone reads the place.  ONCE:
+// what nobody reads again soon (it need not stay in the L2).
+template <bool ONCE>
 __device__ __forceinline__ void dma16(uint32_t to, const char* base, uint32_t off) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(to), "v"(off), "s"(base)
-                 : "memory", "m0");
+    if constexpr (ONCE)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                     :
+                     : "s"(to), "v"(off), "s"(base)
+                     : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :
+                     : "s"(to), "v"(off), "s"(base)
+                     : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void dma_wait() {        // all but the last N loads have arrived
@@ -161,55 +176,66 @@ __device__ __forceinline__ int req_work(const amass_chunk_args& a, const ChunkPl
     return w;
 }
 
-// Parts of a row tile: S_r = ceil(w_r / len), w_r the request's longest tile, for the
-// smallest part length `len` >= max(CK_MIN_SPLIT, sum_r tiles_r w_r / target) at which the
-// batch has at most `target` items (workgroups per kv head), or the first such length where
-// the row tiles alone are that many (only tiles much longer than the average are cut then).
+// Parts of a row tile: S_r = ceil(w_r / len), w_r the cost of the request's longest tile (its
+// tiles of keys times CK_FEW_COST where the tile has few rows), for the smallest part length
+// `len` >= max(CK_MIN_SPLIT, sum_r tiles_r w_r / target) at which the batch has at most
+// `target` items (workgroups per kv head), or the first such length where the row tiles alone
+// are that many (only tiles much longer than the average are cut then).  No part has fewer
+// than CK_MIN_SPLIT tiles of keys.
 // Every workgroup computes it from the lengths, 64 requests at a time, one per lane.
 struct LaneReq {
     Req q;
-    int tiles, work;
+    int tiles, work;     // row tiles; the longest's tiles of keys
+    int cost;            // of a tile of keys
 };
 __device__ __forceinline__ LaneReq lane_req(const amass_chunk_args& a, const ChunkPlan& pl, int r) {
-    LaneReq x = {{0, 0, 0}, 0, 0};
+    LaneReq x = {{0, 0, 0}, 0, 0, 1};
     if (r < a.n_req) x.q = load_req(a, r);
     x.tiles = row_tiles(a, x.q);
     x.work = req_work(a, pl, x.q, x.tiles);
+    x.cost = x.q.n * a.G <= CK_FEW ? CK_FEW_COST : 1;
     return x;
 }
-__device__ __forceinline__ int parts_of(int w, int len) { return max(1, (w + len - 1) / len); }
+__device__ __forceinline__ int parts_of(const LaneReq& x, int len) {
+    const int most = (x.work + CK_MIN_SPLIT - 1) / CK_MIN_SPLIT;
+    return max(1, min(most, (x.work * x.cost + len - 1) / len));
+}
 
 __device__ __forceinline__ int count_items(const amass_chunk_args& a, const ChunkPlan& pl,
                                            const LaneReq& x0, int len) {
     const int lane = threadIdx.x & 63;
-    int tot = wave_sum_uniform(x0.tiles * parts_of(x0.work, len));
+    int tot = wave_sum_uniform(x0.tiles * parts_of(x0, len));
     for (int base = WAVE; base < a.n_req; base += WAVE) {
         const LaneReq x = lane_req(a, pl, base + lane);
-        tot += wave_sum_uniform(x.tiles * parts_of(x.work, len));
+        tot += wave_sum_uniform(x.tiles * parts_of(x, len));
     }
     return tot;
 }
 __device__ __forceinline__ int part_length(const amass_chunk_args& a, const ChunkPlan& pl,
                                            const LaneReq& x0) {
     const int lane = threadIdx.x & 63;
-    float work = (float)x0.tiles * (float)x0.work;
-    int tiles = wave_sum_uniform(x0.tiles), longest = wave_max_uniform(x0.work);
+    float work = (float)x0.tiles * (float)(x0.work * x0.cost);
+    int tiles = wave_sum_uniform(x0.tiles), longest = wave_max_uniform(x0.work * x0.cost);
     for (int base = WAVE; base < a.n_req; base += WAVE) {
         const LaneReq x = lane_req(a, pl, base + lane);
-        work += (float)x.tiles * (float)x.work;
+        work += (float)x.tiles * (float)(x.work * x.cost);
         tiles += wave_sum_uniform(x.tiles);
-        longest = max(longest, wave_max_uniform(x.work));
+        longest = max(longest, wave_max_uniform(x.work * x.cost));
     }
-    int len = max(CK_MIN_SPLIT, (int)ceilf(wave_sumf_uniform(work) / (float)pl.target));
-    if (len >= longest) return max(longest, 1);          // no tile is cut
-    if (tiles >= pl.target || count_items(a, pl, x0, len) <= pl.target) return len;
-    int lo = len + 1, hi = longest;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (count_items(a, pl, x0, mid) <= pl.target) hi = mid;
-        else lo = mid + 1;
+    const int len = max(CK_MIN_SPLIT, (int)ceilf(wave_sumf_uniform(work) / (float)pl.target));
+    const int none = max(longest, 1);                    // no tile is cut
+    if (len >= longest) return none;
+    int lo = len, hi = longest;
+    if (tiles < pl.target && count_items(a, pl, x0, len) > pl.target) {
+        ++lo;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (count_items(a, pl, x0, mid) <= pl.target) hi = mid;
+            else lo = mid + 1;
+        }
     }
-    return lo;
+    // joining costs what two or three tiles do: cut only for a part well below the longest tile
+    return CK_WORTH * lo > longest * (CK_WORTH - 1) ? none : lo;
 }
 
 struct Item {
@@ -227,7 +253,7 @@ __device__ __forceinline__ bool find_item(const amass_chunk_args& a, const Chunk
     int before = 0, slots = 0, cuts = 0;                 // those of earlier requests
     for (int base = 0; base < a.n_req; base += WAVE) {
         const LaneReq x = base == 0 ? x0 : lane_req(a, pl, base + lane);
-        const int S = parts_of(x.work, len);
+        const int S = parts_of(x, len);
         const int n = x.tiles * S, ns = S > 1 ? n : 0, nc = S > 1 ? x.tiles : 0;
         const int incl = wave_incl_scan(n), incl_s = wave_incl_scan(ns), incl_c = wave_incl_scan(nc);
         const int all = __builtin_amdgcn_readlane(incl, WAVE - 1);
@@ -258,7 +284,7 @@ __device__ __forceinline__ int count_cut(const amass_chunk_args& a, const ChunkP
     int tot = 0;
     for (int base = 0; base < a.n_req; base += WAVE) {
         const LaneReq x = base == 0 ? x0 : lane_req(a, pl, base + lane);
-        tot += wave_sum_uniform(parts_of(x.work, len) > 1 ? x.tiles : 0);
+        tot += wave_sum_uniform(parts_of(x, len) > 1 ? x.tiles : 0);
     }
     return tot;
 }
@@ -324,11 +350,11 @@ struct LdsLane {
             ((ks + k) ^ (uint32_t)(i << 5)) + x * (64 * D));
     }
     // d tile x of the 16 keys from 16 y: four keys from 4 h, four from 8 + 4 h (whose rows
-    // turn the chunk's lowest bit)
+    // turn the chunk's second bit)
     __device__ __forceinline__ u32x4_t v_frag(uint32_t vs, int x, int y) const {
         const uint32_t at = (vs + v) ^ (uint32_t)(x << 6);
         const u32x2_t a = lds_tr4(at + y * (32 * D));
-        const u32x2_t b = lds_tr4((at ^ 16u) + y * (32 * D) + 16 * D);
+        const u32x2_t b = lds_tr4((at ^ 32u) + y * (32 * D) + 16 * D);
         return (u32x4_t){a[0], a[1], b[0], b[1]};
     }
 };
@@ -484,6 +510,7 @@ __device__ __forceinline__ void whole_tile(uint32_t ks, uint32_t vs, const LdsLa
 #pragma unroll
     for (int n = 0; n < 4; ++n) f[n] = k_frag(n);
     step();
+    __builtin_amdgcn_s_setprio(1);             // (products before the other wave's vector work)
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         s[0] = mfma32<DT>(f[n & 3], q[n], n ? s[0] : zero);
@@ -499,6 +526,7 @@ __device__ __forceinline__ void whole_tile(uint32_t ks, uint32_t vs, const LdsLa
         for (int i = 8 * n / N; i < 8 * (n + 1) / N; ++i) weight(0, i);
         step();
     }
+    __builtin_amdgcn_s_setprio(0);
     const float mx = xor32_maxf(fmaxf(row_max(s[0]), row_max(s[1])));
     const bool lag = lags(mx, c, st);
     float al = 1.f;
@@ -511,6 +539,7 @@ __device__ __forceinline__ void whole_tile(uint32_t ks, uint32_t vs, const LdsLa
         for (int i = 0; i < 8; ++i) weight(0, i);
     }
     scale_o(st, al);
+    __builtin_amdgcn_s_setprio(1);
     step();
     // V fragment n: 16-key step n / Z, d tile n % Z
 #pragma unroll
@@ -523,6 +552,7 @@ __device__ __forceinline__ void whole_tile(uint32_t ks, uint32_t vs, const LdsLa
         }
         step();
     }
+    __builtin_amdgcn_s_setprio(0);
     st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
@@ -575,10 +605,14 @@ struct Pages {
     __device__ __forceinline__ const char* row(int id, int t) const {
         return k + (uint64_t)(uint32_t)id * sb + (uint32_t)(t & ((1 << sh) - 1)) * st;
     }
-    // 16 rows to LDS
+    // 16 rows to LDS (load_once: that no other workgroup is about to read)
     __device__ __forceinline__ void load(uint32_t to, const char* src) const {
 #pragma unroll
-        for (int n = 0; n < LOADS; ++n) dma16(to + 1024 * n, src, lane_off[n]);
+        for (int n = 0; n < LOADS; ++n) dma16<false>(to + 1024 * n, src, lane_off[n]);
+    }
+    __device__ __forceinline__ void load_once(uint32_t to, const char* src) const {
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) dma16<true>(to + 1024 * n, src, lane_off[n]);
     }
     // the first `rows` of 16 rows, zero behind them (the weight of a masked key is zero, and
     // zero times what lies behind a request's last token could be NaN)
@@ -586,7 +620,7 @@ struct Pages {
                                               int rows) const {
 #pragma unroll
         for (int n = 0; n < LOADS; ++n) {
-            if (ROWS * n + lane / (D / 8) < rows) dma16(to + 1024 * n, src, lane_off[n]);
+            if (ROWS * n + lane / (D / 8) < rows) dma16<false>(to + 1024 * n, src, lane_off[n]);
             else *reinterpret_cast<u32x4_t*>(dst + 1024 * n + 16 * lane) = (u32x4_t){0u, 0u, 0u, 0u};
         }
     }
@@ -720,7 +754,7 @@ struct __align__(1024) ChunkLds {
 // grid: kv head fastest (workgroups of one kv head share an XCD's L2 where n_kv is a multiple
 // of 8), then the items.
 template <int DT, int D>
-__global__ __launch_bounds__(CK_WAVES * WAVE) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+__global__ __launch_bounds__(CK_WAVES * WAVE) __attribute__((amdgpu_waves_per_eu(ck_wgs(D), ck_wgs(D)))) void
 chunk_kernel(const amass_chunk_args a,
                                                                    const ChunkPlan pl) {
     __shared__ ChunkLds<D> lds;
@@ -774,9 +808,12 @@ chunk_kernel(const amass_chunk_args a,
         for (int i = 0; i < D / 16; ++i)
             q[i] = live ? *reinterpret_cast<const u32x4_t*>(src + 16 * i) : (u32x4_t){0u, 0u, 0u, 0u};
     }
-    // (waited for here: a wait inside the key loop would also wait for the next tile's loads)
+    // (called before the loop over the keys: a wait in there would also wait for the next tile's
+    // loads)
+    const auto have_q = [&] {
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(q[i]));
+        for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(q[i]));
+    };
     const LdsLane<D> ll(lane);
     RowState<D> st;
     reset(st);
@@ -838,6 +875,7 @@ chunk_kernel(const amass_chunk_args a,
             weigh<DT, D, 2>(vs, ll, s, c, st);
         };
         if (j0 < j1) {
+            have_q();
             request(0);
             turn(j0);
             sound = __builtin_amdgcn_readfirstlane(lds.bad[0] | lds.bad[1] | lds.bad[2] |
@@ -876,14 +914,14 @@ chunk_kernel(const amass_chunk_args a,
         const auto issue_k = [&](int b) -> bool {
 #pragma unroll
             for (int g = 0; g < 2; ++g)
-                if (pg.has(id[g])) pg.load(base + g * (HB / 2), pg.row(id[g], 32 * b + 16 * g));
+                if (pg.has(id[g])) pg.load_once(base + g * (HB / 2), pg.row(id[g], 32 * b + 16 * g));
             return pg.has(id[0]) && pg.has(id[1]);
         };
         const auto issue_v = [&](int b) -> bool {
             if (pg.has(id[0]) && pg.has(id[1]) && 32 * b + 32 <= len) {
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
-                    pg.load(base + HB + g * (HB / 2), pg.row(id[g], 32 * b + 16 * g) + pg.to_v);
+                    pg.load_once(base + HB + g * (HB / 2), pg.row(id[g], 32 * b + 16 * g) + pg.to_v);
                 return true;
             }
 #pragma unroll
@@ -900,6 +938,7 @@ chunk_kernel(const amass_chunk_args a,
             issue_k(b0);
             vfull = issue_v(b0);
         }
+        have_q();
         for (int b = b0; b < b1; b += CK_WAVES) {
             const int t0 = 32 * b;
             const uint32_t groups = (pg.has(id[0]) ? 1u : 0u) | (pg.has(id[1]) ? 2u : 0u);
@@ -1010,9 +1049,9 @@ chunk_kernel(const amass_chunk_args a,
     else save_stats<D>(g, st.m, l, bad, lane);
 }
 
-// Joins the parts of cut row tiles: workgroup (cut tile and kv head, 32-row group, d tile).
-// Bound by the latency of its loads: record, statistics, O.  Wave w takes parts w, w + 4, ... in
-// batches whose loads are all issued before any is used, and the waves join through LDS.
+// Joins the parts of cut row tiles: a workgroup per cut tile, kv head, 32-row group and d tile.  Bound by the latency of its loads: record, statistics, O.  Wave
+// w takes parts w, w + 4, ... in batches whose loads are all issued before any is used, and the
+// waves join through LDS.  Large batches have nothing to join: their launch reads the count.
 constexpr int CM_WAVES = 4;
 constexpr int CM_BATCH = 4;
 
@@ -1021,19 +1060,18 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
                                                                       const ChunkPlan pl) {
     __shared__ float ms[CM_WAVES][32], ls[CM_WAVES][32], os[CM_WAVES][16][WAVE];
     __shared__ int bads[CM_WAVES];
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, rl = lane & 31;
+    const int group = blockIdx.y, x = blockIdx.z;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kh = blockIdx.x % a.n_kv, i = blockIdx.x / a.n_kv;
-    const int group = blockIdx.y, x = blockIdx.z;
     const int cuts = *(const int*)a.scratch;
     const CutTile ct = *cut_tile(a, i);            // (inside the scratch; read before it is known)
     if (i >= cuts || ct.parts < 2 || ct.slot + ct.parts > pl.slots) return;
     const int rows = min(CK_BM, ct.q.n * a.G - ct.tile * CK_BM);
-    if (32 * group >= rows) return;
     const float c = a.scale * 1.44269504088896341f;
-    const float* g0 = slot_group<D>(a, pl, kh, ct.slot, group);
     const int64_t step = (int64_t)(pl.slot_rows / 32) * (32 * D + CK_STATS);
-    const int rl = lane & 31;
+    if (32 * group >= rows) return;
+    const float* g0 = slot_group<D>(a, pl, kh, ct.slot, group);
     float m = -__FLT_MAX__, l = 0.f, o[16];
     bool bad = false;
 #pragma unroll
@@ -1046,7 +1084,7 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
             const int s = s0 + u * CM_WAVES;
             pm[u] = -__FLT_MAX__;
             ps[u] = pb[u] = 0.f;
-            if (s < ct.parts) {                    // (scalar)
+            if (s < ct.parts) {                // (scalar)
                 const float* g = g0 + s * step;
                 pm[u] = g[32 * D + rl];
                 ps[u] = g[32 * D + 32 + rl];
@@ -1094,28 +1132,27 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
     if (bad) {
         for (int j = w + CM_WAVES * x; j < min(32, rows - 32 * group); j += CM_WAVES * (D / 32))
             attend_row<DT, D>(a, pl, ct.q, ct.r, kh, row0 + j, c, lane);
-        return;
+    } else if (w == 0) {
+        m = -__FLT_MAX__;
+        l = 0.f;
+#pragma unroll
+        for (int v = 0; v < CM_WAVES; ++v) m = fmaxf(m, ms[v][rl]);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] = 0.f;
+#pragma unroll
+        for (int v = 0; v < CM_WAVES; ++v) {
+            const float wt = __builtin_amdgcn_exp2f((ms[v][rl] - m) * c);
+            l += ls[v][rl] * wt;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] += os[v][j][lane] * wt;
+        }
+        const RowOut ro = row_out(a, pl, ct.q, kh, row0 + rl);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] *= inv;
+        store_row<DT, D>(ro.out, x, o, lane);
+        if (x == 0) store_lse(ro, m, l, c, lane);
     }
-    if (w != 0) return;
-    m = -__FLT_MAX__;
-    l = 0.f;
-#pragma unroll
-    for (int v = 0; v < CM_WAVES; ++v) m = fmaxf(m, ms[v][rl]);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) o[j] = 0.f;
-#pragma unroll
-    for (int v = 0; v < CM_WAVES; ++v) {
-        const float wt = __builtin_amdgcn_exp2f((ms[v][rl] - m) * c);
-        l += ls[v][rl] * wt;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) o[j] += os[v][j][lane] * wt;
-    }
-    const RowOut ro = row_out(a, pl, ct.q, kh, row0 + rl);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) o[j] *= inv;
-    store_row<DT, D>(ro.out, x, o, lane);
-    if (x == 0) store_lse(ro, m, l, c, lane);
 }
 
 // ------------------------------------------------------------------ host
@@ -1160,7 +1197,7 @@ static ChunkPlan chunk_plan(const amass_chunk_args& a) {
     while ((1 << p.sh) < a.page) ++p.sh;
     const int64_t cap = (int64_t)a.max_pages << p.sh;
     p.cap = cap > 0x7FFFFFC0 ? 0x7FFFFFC0 : (int)cap;
-    p.target = 2 * chunk_cus() / a.n_kv;
+    p.target = ck_wgs(a.d) * chunk_cus() / a.n_kv;
     if (p.target < 1) p.target = 1;
     const int64_t rows = (int64_t)a.n_tokens * a.G;
     p.tiles_max = (int)(rows / CK_BM) + (a.n_req < a.n_tokens ? a.n_req : a.n_tokens);
