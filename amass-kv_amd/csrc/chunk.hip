@@ -808,12 +808,9 @@ chunk_kernel(const amass_chunk_args a,
         for (int i = 0; i < D / 16; ++i)
             q[i] = live ? *reinterpret_cast<const u32x4_t*>(src + 16 * i) : (u32x4_t){0u, 0u, 0u, 0u};
     }
-    // (called before the loop over the keys: a wait in there would also wait for the next tile's
-    // loads)
-    const auto have_q = [&] {
+    // (here, not in the loop over the keys, where a wait would also wait for the next tile's loads)
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(q[i]));
-    };
+    for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(q[i]));
     const LdsLane<D> ll(lane);
     RowState<D> st;
     reset(st);
@@ -875,7 +872,6 @@ chunk_kernel(const amass_chunk_args a,
             weigh<DT, D, 2>(vs, ll, s, c, st);
         };
         if (j0 < j1) {
-            have_q();
             request(0);
             turn(j0);
             sound = __builtin_amdgcn_readfirstlane(lds.bad[0] | lds.bad[1] | lds.bad[2] |
@@ -938,7 +934,6 @@ chunk_kernel(const amass_chunk_args a,
             issue_k(b0);
             vfull = issue_v(b0);
         }
-        have_q();
         for (int b = b0; b < b1; b += CK_WAVES) {
             const int t0 = 32 * b;
             const uint32_t groups = (pg.has(id[0]) ? 1u : 0u) | (pg.has(id[1]) ? 2u : 0u);

@@ -108,6 +108,23 @@ CASES = {
     "empty requests": dict(new=[0, 9, 0, 40, 0], lens=[33, 9, 0, 77, 5], pad=6),
     "many requests": dict(new=[1 + i % 3 for i in range(150)], lens=[3 + 5 * i for i in range(150)],
                           n_kv=1, G=2),
+    # prompts of many row tiles
+    "long prompt": dict(new=[300], lens=[300]),
+    "long prompt, one head": dict(new=[1030], lens=[1030], G=1, n_kv=1),
+    "long prompt d64 fp16": dict(new=[270], lens=[420], d=64, dtype="fp16", n_kv=1),
+    "long prompt d64 bf16": dict(new=[520], lens=[520], d=64, G=2, n_kv=1),
+    "long prompt fp16": dict(new=[257], lens=[600], dtype="fp16", n_kv=1),
+    "long, keys split": dict(new=[260], lens=[4000], n_kv=1),
+    "long ragged": dict(new=[700, 1, 33, 300], lens=[700, 500, 90, 1000], G=5, n_kv=1, pad=9),
+    "long window": dict(new=[600], lens=[900], window=130, G=2, n_kv=1),
+    "long window of one": dict(new=[300], lens=[390], window=1, n_kv=1),
+    "long, not causal": dict(new=[300], lens=[470], causal=False, n_kv=1),
+    "long, rows before position 0": dict(new=[400], lens=[130], n_kv=1),
+    "long, pages of 64": dict(new=[290], lens=[777], page=64, n_kv=1, halves_first=True),
+    "long, forty heads": dict(new=[30], lens=[150], G=40, n_kv=1),
+    "long, peaked": dict(new=[300], lens=[500], loud=12.0, n_kv=1),
+    "long, peaked fp16": dict(new=[300], lens=[500], loud=12.0, n_kv=1, dtype="fp16"),
+    "long, very peaked": dict(new=[300], lens=[400], loud=60.0, n_kv=1),
     # shapes
     "five heads per kv head": dict(new=[61, 3], lens=[90, 50], G=5, n_kv=3),
     "forty heads per kv head": dict(new=[7], lens=[150], G=40, n_kv=1),
@@ -136,7 +153,7 @@ def test_matches_float64(name):
     c.check(*c.run())
 
 
-@pytest.mark.parametrize("new,lens", [([1, 20], [70, 50]), ([40], [150])])
+@pytest.mark.parametrize("new,lens", [([1, 20], [70, 50]), ([40], [150]), ([260], [333])])
 def test_what_is_not_visible_is_not_used(new, lens):
     """Infinities and NaN behind a request's last token, in blocks of nobody and in K of masked
     positions."""
@@ -158,7 +175,8 @@ def test_what_is_not_visible_is_not_used(new, lens):
 
 @pytest.mark.parametrize("dtype,d", [("bf16", 128), ("fp16", 64)])
 @pytest.mark.parametrize("new,lens,at", [([100], [230], 180), ([6], [300], 297),
-                                         ([3, 90], [80, 90], 40), ([5], [6000], 5998)])
+                                         ([3, 90], [80, 90], 40), ([5], [6000], 5998),
+                                         ([270], [400], 250), ([1100], [1100], 700)])
 def test_not_finite_tokens_reach_only_rows_that_see_them(new, lens, at, dtype, d):
     """A token of the last request has infinities in V and NaN in K: earlier rows are as if it
     were not there, the rows that see it are not finite."""
@@ -178,7 +196,8 @@ def test_not_finite_tokens_reach_only_rows_that_see_them(new, lens, at, dtype, d
     c.check(out, lse, rows=rest)
 
 
-@pytest.mark.parametrize("new,lens", [([1, 3], [300, 200]), ([70], [300]), ([4], [5000])])
+@pytest.mark.parametrize("new,lens", [([1, 3], [300, 200]), ([70], [300]), ([4], [5000]),
+                                      ([280], [400])])
 def test_pages_without_a_block_are_masked(new, lens):
     announce(f"chunk attention: blocks outside the pool, {new} of {lens}")
     c = Case(new=new, lens=lens, n_kv=1, spare=0)
@@ -191,7 +210,7 @@ def test_pages_without_a_block_are_masked(new, lens):
 
 def test_no_visible_page_at_all():
     announce("chunk attention: every block outside the pool")
-    for new, lens in (([2], [40]), ([50], [90])):
+    for new, lens in (([2], [40]), ([50], [90]), ([260], [300])):
         c = Case(new=new, lens=lens, n_kv=1)
         c.table.fill_(-1)
         out, lse = c.run()
