@@ -185,57 +185,64 @@ __device__ __forceinline__ int req_work(const amass_chunk_args& a, const ChunkPl
 // Every workgroup computes it from the lengths, 64 requests at a time, one per lane.
 struct LaneReq {
     Req q;
-    int tiles, work;     // row tiles; the longest's tiles of keys
-    int cost;            // of a tile of keys
+    int tiles;           // row tiles
+    int most;            // parts of at least CK_MIN_SPLIT tiles of keys that the longest has
+    float cost;          // of the longest
 };
 __device__ __forceinline__ LaneReq lane_req(const amass_chunk_args& a, const ChunkPlan& pl, int r) {
-    LaneReq x = {{0, 0, 0}, 0, 0, 1};
+    LaneReq x = {{0, 0, 0}, 0, 0, 0.f};
     if (r < a.n_req) x.q = load_req(a, r);
     x.tiles = row_tiles(a, x.q);
-    x.work = req_work(a, pl, x.q, x.tiles);
-    x.cost = x.q.n * a.G <= CK_FEW ? CK_FEW_COST : 1;
+    const int work = req_work(a, pl, x.q, x.tiles);
+    x.most = (work + CK_MIN_SPLIT - 1) / CK_MIN_SPLIT;
+    x.cost = (float)work * (x.q.n * a.G <= CK_FEW ? CK_FEW_COST : 1);
     return x;
 }
-__device__ __forceinline__ int parts_of(const LaneReq& x, int len) {
-    const int most = (x.work + CK_MIN_SPLIT - 1) / CK_MIN_SPLIT;
-    return max(1, min(most, (x.work * x.cost + len - 1) / len));
+// (inv: 1 / len, a little less, so that no rounding makes a part more)
+__device__ __forceinline__ int parts_of(const LaneReq& x, float inv) {
+    return max(1, min(x.most, (int)ceilf(x.cost * inv)));
 }
 
 __device__ __forceinline__ int count_items(const amass_chunk_args& a, const ChunkPlan& pl,
-                                           const LaneReq& x0, int len) {
+                                           const LaneReq& x0, float inv) {
     const int lane = threadIdx.x & 63;
-    int tot = wave_sum_uniform(x0.tiles * parts_of(x0, len));
+    int tot = wave_sum_uniform(x0.tiles * parts_of(x0, inv));
     for (int base = WAVE; base < a.n_req; base += WAVE) {
         const LaneReq x = lane_req(a, pl, base + lane);
-        tot += wave_sum_uniform(x.tiles * parts_of(x, len));
+        tot += wave_sum_uniform(x.tiles * parts_of(x, inv));
     }
     return tot;
 }
-__device__ __forceinline__ int part_length(const amass_chunk_args& a, const ChunkPlan& pl,
-                                           const LaneReq& x0) {
+// 1 / len, for a part length within 1 / 32 of the one described above
+__device__ __forceinline__ float part_inverse(const amass_chunk_args& a, const ChunkPlan& pl,
+                                              const LaneReq& x0) {
+    constexpr float LESS = 1.f - 0x1p-20f;
     const int lane = threadIdx.x & 63;
-    float work = (float)x0.tiles * (float)(x0.work * x0.cost);
-    int tiles = wave_sum_uniform(x0.tiles), longest = wave_max_uniform(x0.work * x0.cost);
+    float work = (float)x0.tiles * x0.cost;
+    int tiles = wave_sum_uniform(x0.tiles);
+    float longest = wave_maxf_uniform(x0.cost);
     for (int base = WAVE; base < a.n_req; base += WAVE) {
         const LaneReq x = lane_req(a, pl, base + lane);
-        work += (float)x.tiles * (float)(x.work * x.cost);
+        work += (float)x.tiles * x.cost;
         tiles += wave_sum_uniform(x.tiles);
-        longest = max(longest, wave_max_uniform(x.work * x.cost));
+        longest = fmaxf(longest, wave_maxf_uniform(x.cost));
     }
-    const int len = max(CK_MIN_SPLIT, (int)ceilf(wave_sumf_uniform(work) / (float)pl.target));
-    const int none = max(longest, 1);                    // no tile is cut
-    if (len >= longest) return none;
-    int lo = len, hi = longest;
-    if (tiles < pl.target && count_items(a, pl, x0, len) > pl.target) {
-        ++lo;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (count_items(a, pl, x0, mid) <= pl.target) hi = mid;
-            else lo = mid + 1;
+    work = wave_sumf_uniform(work);
+    const float none = LESS / fmaxf(longest, 1.f);       // no tile is cut
+    float lo = fmaxf((float)CK_MIN_SPLIT, work / ((float)pl.target * LESS));
+    if (lo >= longest) return none;
+    if (tiles < pl.target && count_items(a, pl, x0, LESS / lo) > pl.target) {
+        // parts <= cost / len + 1 each: at this length the items are few enough
+        float hi = fminf(longest, work / ((float)(pl.target - tiles) * LESS) + 1.f);
+        while (hi - lo > lo * (1.f / 32)) {
+            const float mid = 0.5f * (lo + hi);
+            if (count_items(a, pl, x0, LESS / mid) <= pl.target) hi = mid;
+            else lo = mid;
         }
+        lo = hi;
     }
     // joining costs what two or three tiles do: cut only for a part well below the longest tile
-    return CK_WORTH * lo > longest * (CK_WORTH - 1) ? none : lo;
+    return CK_WORTH * lo > longest * (CK_WORTH - 1) ? none : LESS / lo;
 }
 
 struct Item {
@@ -248,12 +255,12 @@ struct Item {
 // Item y of the batch (requests in order, a request's last -- causal: longest -- tile first);
 // false past the end.
 __device__ __forceinline__ bool find_item(const amass_chunk_args& a, const ChunkPlan& pl,
-                                          const LaneReq& x0, int len, int y, Item& it) {
+                                          const LaneReq& x0, float inv, int y, Item& it) {
     const int lane = threadIdx.x & 63;
     int before = 0, slots = 0, cuts = 0;                 // those of earlier requests
     for (int base = 0; base < a.n_req; base += WAVE) {
         const LaneReq x = base == 0 ? x0 : lane_req(a, pl, base + lane);
-        const int S = parts_of(x, len);
+        const int S = parts_of(x, inv);
         const int n = x.tiles * S, ns = S > 1 ? n : 0, nc = S > 1 ? x.tiles : 0;
         const int incl = wave_incl_scan(n), incl_s = wave_incl_scan(ns), incl_c = wave_incl_scan(nc);
         const int all = __builtin_amdgcn_readlane(incl, WAVE - 1);
@@ -279,12 +286,12 @@ __device__ __forceinline__ bool find_item(const amass_chunk_args& a, const Chunk
     return false;
 }
 __device__ __forceinline__ int count_cut(const amass_chunk_args& a, const ChunkPlan& pl,
-                                         const LaneReq& x0, int len) {
+                                         const LaneReq& x0, float inv) {
     const int lane = threadIdx.x & 63;
     int tot = 0;
     for (int base = 0; base < a.n_req; base += WAVE) {
         const LaneReq x = base == 0 ? x0 : lane_req(a, pl, base + lane);
-        tot += wave_sum_uniform(parts_of(x, len) > 1 ? x.tiles : 0);
+        tot += wave_sum_uniform(parts_of(x, inv) > 1 ? x.tiles : 0);
     }
     return tot;
 }
@@ -765,12 +772,12 @@ chunk_kernel(const amass_chunk_args a,
     Item it;
     {
         const LaneReq x0 = lane_req(a, pl, lane);
-        const int plen = part_length(a, pl, x0);
+        const float inv = part_inverse(a, pl, x0);
         if (blockIdx.x == 0 && w == 0) {
-            const int cuts = count_cut(a, pl, x0, plen);
+            const int cuts = count_cut(a, pl, x0, inv);
             if (lane == 0) *(int*)a.scratch = cuts;
         }
-        if (!find_item(a, pl, x0, plen, blockIdx.x / a.n_kv, it)) return;
+        if (!find_item(a, pl, x0, inv, blockIdx.x / a.n_kv, it)) return;
     }
     const Span sp = tile_span(a, pl, it.q, it.tile);
     const int per = part_len(sp.n, it.parts);
