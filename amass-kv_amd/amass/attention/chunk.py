@@ -19,6 +19,7 @@ from .._hip import (ChunkArgs, cache_halves, call_on, check, device_index, load_
 from .rope import DTYPES
 
 HEAD_DIMS = (64, 128)
+MAX_INT = 2 ** 31 - 1
 _pack_chunk = packer(ChunkArgs)
 _SCRATCH = {}            # (GPU, requests, rows, kv heads, group, head dim) -> scratch bytes
 
@@ -60,17 +61,21 @@ def _chunk_args(q, kv_cache, block_table, seq_lens, query_start, out, scale, cau
     sb, st, sh, c_unit = cs
     if not q_unit == o_unit == c_unit == 1:
         raise ValueError("q / cache / out need unit stride on the head dim")
+    if not (o_st or T == 1) or not (o_hs or H == 1):
+        raise ValueError("rows or heads of out share memory")
     l_at = l_st = l_hs = 0
     if lse is not None:
         if lse.dtype is not torch.float32 or lse.shape != (T, H):
             raise ValueError("lse must be (T, H) fp32")
         l_at = lse.data_ptr()
         l_st, l_hs = lse.stride()
+        if not (l_st or T == 1) or not (l_hs or H == 1):
+            raise ValueError("rows or heads of lse share memory")
     return ((q.data_ptr(), q_st, q_hs, k, v, sb, st, sh, block_table.data_ptr(), bt_st,
              seq_lens.data_ptr(), query_start.data_ptr(), out.data_ptr(), o_st, o_hs,
              l_at, l_st, l_hs),
             (scale, n_req, T, n_kv, H // n_kv, d, page, nb, width, 1 if causal else 0,
-             window or 0, DTYPES[dt]))
+             min(window or 0, MAX_INT), DTYPES[dt]))
 
 
 def _scratch_bytes(index, head, tail) -> int:
@@ -106,7 +111,7 @@ def paged_chunk_attention(q, kv_cache, block_table, seq_lens, query_start, out, 
     ``j <= p``, with ``window`` those ``j > p - window``, and nothing in pages whose block is
     outside the cache or beyond the table's width.  Rows that see nothing get zeros (``lse``:
     -inf); rows of no request stay as they are.  ``scale`` defaults to ``d ** -0.5``; ``lse``
-    (T, H) fp32 receives the rows' log-sum-exp of the scaled scores.
+    (T, H) fp32 receives the rows' log-sum-exp of the scaled scores.  ``out`` may be q.
 
     bf16 or fp16, d 64 or 128, pages of 16 or a larger power of two, any number of query heads
     per kv head.  K and V need 16-byte aligned rows, as q and out do.

@@ -94,7 +94,8 @@ def rope_paged_write(q, k, v, positions, table, kv_cache, slots, q_out=None, *,
     ``positions`` (T,) int32, ``slots`` (T,) int64 (``extend_block_tables``), ``table`` from
     ``rope_table``, ``kv_cache`` one layer's (2, NB, page, n_kv, d), (NB, 2, ...) or, without V,
     (NB, 1, ...).  A row whose position is outside the table is passed over; one whose slot is
-    outside the cache has its q turned and is not written.  bf16 or fp16."""
+    outside the cache has its q turned and is not written.  A slot belongs to one row of a call.
+    ``q_out`` is q or shares no memory with it.  bf16 or fp16."""
     q_out = q if q_out is None else q_out
     index = device_index(q, k, v, positions, table, kv_cache, slots, q_out)
     dt = q.dtype
@@ -127,6 +128,10 @@ def rope_paged_write(q, k, v, positions, table, kv_cache, slots, q_out=None, *,
     sb, st, sh, c_unit = cs
     if not q_unit == k_unit == o_unit == c_unit == 1:
         raise ValueError("q / k / q_out / cache need unit stride on the head dim")
+    if not (o_st or T == 1) or not (o_hs or H == 1):
+        raise ValueError("rows or heads of q_out share memory")
+    if not (sb or nb == 1) or not (st or page == 1) or not (sh or n_kv == 1):
+        raise ValueError("rows of the cache share memory")
     v_at = v_st = v_hs = 0
     if v is not None:
         v_at = v.data_ptr()

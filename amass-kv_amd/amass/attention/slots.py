@@ -11,7 +11,8 @@ at rest, blocks short of the last call).  ``free_blocks`` makes both.
 One launch each, fixed-shape, without allocation or host synchronisation, so both can be
 captured in a HIP graph.  ``query_start`` (R + 1,) are the rows where the requests' tokens
 start, ``seq_lens`` (R,) the requests' lengths with the new tokens, as the attention backend's
-metadata has them.  A block belongs to one request.
+metadata has them.  A block belongs to one request, and calls on one list run one after the
+other (on one stream, or ordered by events).
 """
 from __future__ import annotations
 
@@ -36,6 +37,8 @@ def _table(block_table, n_req, page, num_blocks):
     st, unit = block_table.stride()
     if block_table.dtype is not torch.int32 or (unit != 1 and width > 1):
         raise ValueError("block_table must be (R, max_pages) int32 with unit column stride")
+    if st < width and rows > 1:
+        raise ValueError("rows of block_table share memory")
     if rows < n_req or width < 1:
         raise ValueError("block_table needs a row per request")
     if n_req > MAX_REQS:

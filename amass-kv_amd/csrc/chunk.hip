@@ -5,7 +5,8 @@
 // A workgroup of four waves takes CK_BM rows (a row tile) and walks keys 64 at a time with
 // the running maximum m, sum l and unnormalised output O of a softmax:
 //   S^T[key][row] = K Q^T     v_mfma 32x32x16, A = K rows (LDS), B = Q^T (registers)
-//   p = 2^(c s - c m), c = scale log2 e        one fma and one exp2 per score
+//   p = 2^(c s - c m), c = scale log2 e        one fma and one exp2 per score, rounded to the
+//                                              element type for the second product, summed as fp32
 //   O^T[d][row] += V^T P^T    A = V^T (LDS, transposing 64-bit reads), B = P^T
 // In S^T a lane holds one row's scores (column = lane % 32), so the row maximum is a chain of
 // v_max in the lane and one exchange with lane ^ 32, the rescale one factor per lane, and the
@@ -52,6 +53,11 @@ constexpr int CK_MIN_SPLIT = 4;            // fewest tiles of a part
 constexpr int CK_FEW_COST = 3;
 constexpr int CK_WORTH = 3;                // cut tiles for parts of at most 2 / 3 of the longest
 constexpr float CK_LAZY = 8.f;             // a maximum may lag by this power of two
+// Weights are 2^CK_LIFT times those of the formula (sums too, so the result is the same): fp16
+// has no bits below 2^-24, and thousands of keys that far down a row count together.  2^15, the
+// largest with the lag, is below fp16's largest; bf16 has the exponents of fp32.
+template <int DT>
+constexpr float CK_LIFT = DT == AMASS_FP16 ? 7.f : 0.f;
 
 // ------------------------------------------------------------------ the 16-bit types
 template <int DT>
@@ -154,7 +160,7 @@ __device__ __forceinline__ int key_hi(const amass_chunk_args& a, const ChunkPlan
     return p < 0 ? 0 : a.causal ? min(l, p + 1) : l;
 }
 __device__ __forceinline__ int key_lo(const amass_chunk_args& a, int p) {
-    return a.window > 0 ? max(0, p - a.window + 1) : 0;
+    return a.window > 0 && p >= a.window ? p - a.window + 1 : 0;
 }
 __device__ __forceinline__ Span tile_span(const amass_chunk_args& a, const ChunkPlan& pl,
                                           const Req& q, int tile) {
@@ -465,7 +471,7 @@ __device__ __forceinline__ void maximum(const f32x16_t (&s)[NK], float c, RowSta
 template <int DT, int D, int NK>
 __device__ __forceinline__ void weigh(uint32_t vs, const LdsLane<D>& ll, const f32x16_t (&s)[NK],
                                       float c, RowState<D>& st) {
-    const float mc = fmaxf(st.m * c, -__FLT_MAX__);
+    const float mc = fmaxf(st.m * c, -__FLT_MAX__) - CK_LIFT<DT>;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < NK; ++x) {
@@ -504,7 +510,7 @@ __device__ __forceinline__ void whole_tile(uint32_t ks, uint32_t vs, const LdsLa
     for (int i = 0; i < 16; ++i) zero[i] = 0.f;
     const auto k_frag = [&](int n) { return ll.k_frag(ks, n % N, n / N); };
     const auto step = [] { __builtin_amdgcn_sched_barrier(0); };
-    float mc = fmaxf(st.m * c, -__FLT_MAX__), sum[4] = {0.f, 0.f, 0.f, 0.f};
+    float mc = fmaxf(st.m * c, -__FLT_MAX__) - CK_LIFT<DT>, sum[4] = {0.f, 0.f, 0.f, 0.f};
     const auto weight = [&](int x, int i) {    // weights 2 i and 2 i + 1 of half x
         const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][2 * i], c, -mc));
         const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][2 * i + 1], c, -mc));
@@ -539,7 +545,7 @@ __device__ __forceinline__ void whole_tile(uint32_t ks, uint32_t vs, const LdsLa
     float al = 1.f;
     if (lag) {
         al = raise(mx, c, st);
-        mc = fmaxf(st.m * c, -__FLT_MAX__);
+        mc = fmaxf(st.m * c, -__FLT_MAX__) - CK_LIFT<DT>;
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] = 0.f;
 #pragma unroll
@@ -688,9 +694,10 @@ __device__ __forceinline__ RowOut row_out(const amass_chunk_args& a, const Chunk
     return w;
 }
 
+template <int DT>
 __device__ __forceinline__ void store_lse(const RowOut& w, float m, float l, float c, int lane) {
     if (w.lse && lane < 32) {
-        const float mc = fmaxf(m * c, -__FLT_MAX__);
+        const float mc = fmaxf(m * c, -__FLT_MAX__) - CK_LIFT<DT>;
         *w.lse = l == 0.f ? -INFINITY : (mc + __log2f(l)) * 0.693147180559945309f;
     }
 }
@@ -729,7 +736,8 @@ __device__ __forceinline__ void attend_row(const amass_chunk_args& a, const Chun
         const float mx = fmaxf(m, wave_maxf_uniform(s));
         const float al = __builtin_amdgcn_exp2f((m - mx) * c);
         m = mx;
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -fmaxf(m * c, -__FLT_MAX__)));
+        const float mc = fmaxf(m * c, -__FLT_MAX__) - CK_LIFT<DT>;
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -mc));
         l = l * al + wave_sumf(e);
 #pragma unroll
         for (int i = 0; i < PER; ++i) o[i] *= al;
@@ -747,7 +755,7 @@ __device__ __forceinline__ void attend_row(const amass_chunk_args& a, const Chun
 #pragma unroll
     for (int i = 0; i < PER; ++i)
         ro.out[WAVE * i + lane] = (uint16_t)pack2<DT>(o[i] * inv, 0.f);
-    if (lane == 0) store_lse(ro, m, l, c, 0);
+    if (lane == 0) store_lse<DT>(ro, m, l, c, 0);
 }
 
 template <int D>
@@ -847,8 +855,8 @@ chunk_kernel(const amass_chunk_args a,
         {
             bool has = true;
             const int from = max(CK_KEYS * (sp.lo + j0), key_lo(a, start + div_g(pl, it.tile * CK_BM)));
-            const int to = min(CK_KEYS * (sp.lo + j1), sp.hi);
-            for (int p = (from >> pg.sh) + threadIdx.x; p << pg.sh < to; p += CK_WAVES * WAVE)
+            const int to = (min(CK_KEYS * (sp.lo + j1), sp.hi) - 1) >> pg.sh;    // the last page
+            for (int p = (from >> pg.sh) + threadIdx.x; p <= to; p += CK_WAVES * WAVE)
                 has &= pg.has(a.block_table[it.r * a.bt_st + p]);
             const bool all = __all(has);
             if (lane == 0) lds.bad[w] = !all;
@@ -1022,7 +1030,7 @@ chunk_kernel(const amass_chunk_args a,
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] *= inv;
             store_row<DT, D>(ro.out, w, o, lane);
-            if (w == 0) store_lse(ro, m, l, c, lane);
+            if (w == 0) store_lse<DT>(ro, m, l, c, lane);
         } else {
             float* g = slot_group<D>(a, pl, kh, it.slot, 0);
             save_tile<D>(g, w, o, lane);
@@ -1047,7 +1055,7 @@ chunk_kernel(const amass_chunk_args a,
         if (whole) store_row<DT, D>(ro.out, x, o, lane);
         else save_tile<D>(g, x, o, lane);
     }
-    if (whole) store_lse(ro, st.m, l, c, lane);
+    if (whole) store_lse<DT>(ro, st.m, l, c, lane);
     else save_stats<D>(g, st.m, l, bad, lane);
 }
 
@@ -1153,7 +1161,7 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[j] *= inv;
         store_row<DT, D>(ro.out, x, o, lane);
-        if (x == 0) store_lse(ro, m, l, c, lane);
+        if (x == 0) store_lse<DT>(ro, m, l, c, lane);
     }
 }
 
@@ -1198,7 +1206,7 @@ static ChunkPlan chunk_plan(const amass_chunk_args& a) {
     p.sh = 0;
     while ((1 << p.sh) < a.page) ++p.sh;
     const int64_t cap = (int64_t)a.max_pages << p.sh;
-    p.cap = cap > 0x7FFFFFC0 ? 0x7FFFFFC0 : (int)cap;
+    p.cap = cap > 0x7FFF0000 ? 0x7FFF0000 : (int)cap;    // (positions a tile ahead fit an int)
     p.target = ck_wgs(a.d) * chunk_cus() / a.n_kv;
     if (p.target < 1) p.target = 1;
     const int64_t rows = (int64_t)a.n_tokens * a.G;
@@ -1221,7 +1229,7 @@ static int64_t chunk_scratch(const amass_chunk_args& a, const ChunkPlan& p) {
 template <int DT, int D>
 static int launch_chunk(const amass_chunk_args& a, const ChunkPlan& p, hipStream_t s) {
     const int64_t items = (int64_t)(p.tiles_max + p.target) * a.n_kv;
-    if (items > 0x7FFFFFFF) return AMASS_ERR_GEOMETRY;
+    if (items * CK_WAVES * WAVE > 0xFFFFFFFFll) return AMASS_ERR_GEOMETRY;    // (threads of a launch)
     hipLaunchKernelGGL((chunk_kernel<DT, D>), dim3((unsigned)items), dim3(CK_WAVES * WAVE), 0, s, a, p);
     const int rc = check_launch();
     if (rc) return rc;

@@ -94,7 +94,7 @@ static int launch_rope(const amass_rope_args& a, hipStream_t s) {
     const int64_t units = (int64_t)(a.n_heads + a.n_kv * (a.v ? 2 : 1)) * (a.d / (2 * N));
     const int chunks = (int)((units + ROPE_THREADS - 1) / ROPE_THREADS);
     const int threads = (int)(((units + chunks - 1) / chunks + WAVE - 1) / WAVE) * WAVE;
-    if (chunks > 65535) return AMASS_ERR_GEOMETRY;
+    if (chunks > 65535 || (int64_t)a.n_tokens * threads > 0xFFFFFFFFll) return AMASS_ERR_GEOMETRY;
     const dim3 grid(a.n_tokens, chunks);
     if (a.interleaved)
         hipLaunchKernelGGL((rope_kernel<DT, N, true>), grid, dim3(threads), 0, s, a, sh);

@@ -107,7 +107,7 @@ __global__ __launch_bounds__(SL_THREADS) void extend_kernel(const amass_extend_a
                 int blk;
                 if (k >= 0) {
                     const int at = top - 1 - (before[lo] + k);
-                    blk = at >= 0 ? a.free_list[at] : -1;
+                    blk = at >= 0 && at < a.capacity ? a.free_list[at] : -1;
                     if (blk < 0 || blk >= a.nb) blk = -1;
                     if ((pos & ((1 << sh) - 1)) == 0) *entry = blk;   // its first token
                 } else {

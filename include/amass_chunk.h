@@ -84,7 +84,8 @@ int amass_release(const amass_release_args* a, void* stream);
  * d-1 are copied.  q_out may be q.  k_cache / v_cache are one layer's (NB, page, n_kv, d)
  * views; v NULL writes no V.  A token whose position is outside [0, max_pos) is passed over
  * (q_out and the cache keep what they have there); one whose slot is outside [0, nb * page)
- * only has its q turned.  Two tokens of one slot leave one of the two rows' values there. */
+ * only has its q turned.  Two tokens of one slot leave values of either there, in pieces.  q_out
+ * is q or shares no memory with it. */
 typedef struct amass_rope_args {
     const void* q;     int64_t q_st, q_hs;               /* (T,H,d)    */
     const void* k;     int64_t k_st, k_hs;               /* (T,n_kv,d) */
@@ -106,11 +107,11 @@ int amass_rope_write(const amass_rope_args* a, void* stream);
  *   s_j = scale q . k_j,  out = sum_j e^(s_j - m) v_j / l,  lse = m + ln l  (natural log)
  * with m = max_j s_j and l = sum_j e^(s_j - m), sums and statistics in fp32, the weights
  * e^(s_j - m) rounded to the element type for the second product.  What is not visible is
- * not used, whatever it holds (infinities and NaN among it).  A row that sees no finite score (a
- * position below 0, an empty request, only scores of -inf) gets zeros and lse = -inf.  Rows of no request are left as
- * they are.  scale > 0.  d 64 or 128, page >= 16, G >= 1, K and V views 16-byte aligned with
- * strides of multiples of 8 elements (a block below 2^30 of them), q likewise, out 16-byte aligned with strides of
- * multiples of 8.
+ * not used, whatever it holds (infinities and NaN among it).  A row that sees no finite score
+ * (a position below 0, an empty request, only scores of -inf) gets zeros and lse = -inf.  Rows
+ * of no request are left as they are.  out may be q.  scale > 0.  d 64 or 128, page >= 16,
+ * G >= 1; q, out and the K and V views 16-byte aligned with strides of multiples of 8 elements
+ * (a block below 2^30 of them).
  *
  * scratch: amass_chunk_scratch_bytes(a) bytes, 256-byte aligned, for the parts of rows whose
  * keys several workgroups share.  It holds nothing between calls; calls that may run at the

@@ -67,7 +67,8 @@ def _chunk(**over):
     (dict(scale=-1.0), -2), (dict(scale=math.nan), -2), (dict(scale=math.inf), -2),
     (dict(window=-1), -2), (dict(G=0), -2), (dict(n_kv=0), -2), (dict(nb=0), -2),
     (dict(q=0x1008), -2), (dict(kv_st=1028), -2), (dict(o_hs=124), -2), (dict(kv_st=1 << 30), -2),
-    (dict(kv_st=-1024), -2), (dict(kv_sb=1 << 30), -2), (dict(kv_sb=-32768), -2), (dict(n_tokens=1 << 29), -2), (dict(max_pages=0), -2)])
+    (dict(kv_st=-1024), -2), (dict(kv_sb=1 << 30), -2), (dict(kv_sb=-32768), -2),
+    (dict(n_tokens=1 << 29), -2), (dict(max_pages=0), -2)])
 def test_chunk_attention_refuses(over, status):
     lib = _hip.load_library()
     a = _chunk(**over)
@@ -91,6 +92,14 @@ def test_chunk_attention_refuses_a_small_or_missing_scratch():
         a = _chunk(**empty)
         assert lib.amass_chunk_scratch_bytes(ctypes.byref(a)) == 0
         assert lib.amass_chunk_attention(ctypes.byref(a), None) == 0
+
+
+def test_chunk_attention_refuses_more_workgroups_than_a_launch_has():
+    lib = _hip.load_library()
+    a = _chunk(n_tokens=1 << 20, n_kv=4096)
+    a.scratch, a.scratch_bytes = 0x1000, lib.amass_chunk_scratch_bytes(ctypes.byref(a))
+    assert a.scratch_bytes > 0
+    assert lib.amass_chunk_attention(ctypes.byref(a), None) == -2
 
 
 def _fill(st, **over):
@@ -121,7 +130,8 @@ def test_extend_release_and_rope_refuse():
                 nb=4, max_pos=9)
     for over, status in ((dict(q=None), -1), (dict(v=P), -1), (dict(rot=130), -2),
                          (dict(rot=3), -2), (dict(d=127), -2), (dict(page=10), -2),
-                         (dict(dtype=5), -3), (dict(max_pos=0), -2), (dict(nb=0), -2)):
+                         (dict(dtype=5), -3), (dict(max_pos=0), -2), (dict(nb=0), -2),
+                         (dict(n_tokens=1 << 30), -2)):       # more threads than a launch has
         a = _fill(_hip.RopeArgs, **{**rope, **over})
         assert lib.amass_rope_write(ctypes.byref(a), None) == status, over
     a = _fill(_hip.RopeArgs, **{**rope, "n_tokens": 0})

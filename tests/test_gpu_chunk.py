@@ -5,7 +5,8 @@ Tolerance, per element.  With u = eps / 2 of the element type: the weights are r
 fp32 (off by at most d 2^-24 sum |q k| <= d 2^-24 `reach` once scaled), which moves a weight and its
 sum by that much each; exponentials, sums and joins in fp32 add less than 2^-16 of `size` for
 the lengths here (each at most 2^-24 per term).  fp16 adds its subnormal half steps: 2^-25 of
-a weight (of a sum that is at least 1) per key seen, and of the result.  lse: the scores' and
+a weight (of weights that are 2^7 times the formula's, so of a sum that is at least 2^7) per
+key seen, and of the result.  lse: the scores' and
 the sums' error, and one rounding of its own size."""
 import numpy as np
 import pytest
@@ -74,7 +75,7 @@ class Case:
         tol = u * (1.01 * size + np.abs(want)) + (2.0 * moved[:, :, None] + 2.0 ** -16) * size
         if self.dt == torch.float16:
             vmax = float(self.v.abs().max())
-            tol += 2.0 ** -25 * (1.0 + seen[:, None, None] * vmax)
+            tol += 2.0 ** -25 + 2.0 ** -32 * seen[:, None, None] * vmax
         err = np.abs(out - want)
         bad = ~(err <= tol)
         assert not bad[rows].any(), (np.argwhere(bad[rows])[:4], err[rows].max())
@@ -124,6 +125,8 @@ CASES = {
     "long, forty heads": dict(new=[30], lens=[150], G=40, n_kv=1),
     "long, peaked": dict(new=[300], lens=[500], loud=12.0, n_kv=1),
     "long, peaked fp16": dict(new=[300], lens=[500], loud=12.0, n_kv=1, dtype="fp16"),
+    "long, a window beyond everything": dict(new=[400], lens=[130], n_kv=1, window=2 ** 31 - 1),
+    "a window past 32 bits": dict(new=[3, 40], lens=[50, 30], window=2 ** 40),
     "long, very peaked": dict(new=[300], lens=[400], loud=60.0, n_kv=1),
     # shapes
     "five heads per kv head": dict(new=[61, 3], lens=[90, 50], G=5, n_kv=3),
@@ -300,6 +303,31 @@ def test_same_rows_in_any_batch_are_near():
         both.check(both_full, lse)
 
 
+@pytest.mark.parametrize("new,lens", [([2], [9000]), ([60], [9000])])
+def test_keys_far_down_an_fp16_row_count_together(new, lens):
+    """One key with V = 0, and thousands of weight e^-17.5, below half of fp16's least step."""
+    announce(f"chunk attention: faint keys, {new}")
+    c = Case(new=new, lens=lens, dtype="fp16", n_kv=1, G=2)
+    c.q.zero_(), c.k.zero_(), c.v.abs_()
+    c.q[:, :, 0] = 16.0
+    c.k[..., 0] = -12.375                           # 16 * 12.375 / sqrt(128) = 17.5
+    first = int(c.table[0, 0])
+    c.k[first, 5, :, 0] = 0.0
+    c.v[first, 5] = 0.0
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("new,lens", [([4, 1], [3000, 70]), ([150, 3], [500, 90])])
+def test_out_may_be_q(new, lens):
+    announce(f"chunk attention: in place, {new} of {lens}")
+    c = Case(new=new, lens=lens, n_kv=2)
+    apart, alse = c.run()
+    q, kv, table, ln, qs = c.dev()
+    lse = torch.full(q.shape[:2], 7.0, device=DEV)
+    paged_chunk_attention(q, kv, table, ln, qs, q, lse=lse)
+    assert torch.equal(q, apart) and torch.equal(lse, alse)
+
+
 def test_repeats_bit_for_bit():
     announce("chunk attention: the same bits every time")
     c = Case(new=[4, 60, 1], lens=[3000, 500, 2500], n_kv=2)
@@ -391,7 +419,10 @@ def test_wrapper_refuses():
                  dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
                  dict(lse=torch.zeros(3, 8, dtype=torch.float64, device=DEV)),
                  dict(lse=torch.zeros(3, 7, device=DEV)),
-                 dict(q=q.transpose(1, 2).contiguous().transpose(1, 2))):
+                 dict(q=q.transpose(1, 2).contiguous().transpose(1, 2)),
+                 dict(out=good["out"][:1].expand(3, 8, 128)),
+                 dict(out=good["out"][:, :1].expand(3, 8, 128)),
+                 dict(lse=torch.zeros(3, 1, device=DEV).expand(3, 8))):
         with pytest.raises(ValueError):
             paged_chunk_attention(**{**good, **over})
     from amass._hip import AmassError

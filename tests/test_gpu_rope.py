@@ -184,7 +184,9 @@ def test_wrapper_refuses():
                  dict(slots=slots.int()), dict(table=table.double()),
                  dict(table=rope_table(66, 8, device=DEV)), dict(q=wide), dict(layout="other"),
                  dict(q_out=torch.zeros(4, 3, 64, dtype=dt, device=DEV)),
-                 dict(kv_cache=kv[:, :1])):
+                 dict(kv_cache=kv[:, :1]), dict(q_out=q[:1].expand(4, 2, 64)),
+                 dict(q_out=q[:, :1].expand(4, 2, 64)), dict(kv_cache=kv[:1].expand(3, 2, 16, 1, 64)),
+                 dict(kv_cache=kv[:, :, :1].expand(3, 2, 16, 1, 64))):
         with pytest.raises(ValueError):
             rope_paged_write(**{**good, **over})
     rope_paged_write(q[:0], k[:0], v[:0], pos[:0], table, kv, slots[:0])      # nothing to do

@@ -219,6 +219,9 @@ def test_wrapper_refuses():
                      (dict(seq_lens=_i32([1, 2])), {}), ({}, dict(top_out=top[:2]))):
         with pytest.raises(ValueError):
             extend_block_tables(**{**good, **over}, **{**dict(page=16, num_blocks=4), **kw})
+    with pytest.raises(ValueError, match="share memory"):
+        extend_block_tables(table.expand(2, 2), _i32([1, 1]), _i32([0, 1, 2]), free, top, slots, pos,
+                            page=16, num_blocks=4)
     with pytest.raises(ValueError, match="at most 4096"):
         n = 4097
         extend_block_tables(torch.zeros(n, 2, dtype=torch.int32, device=DEV), _i32([1] * n),
