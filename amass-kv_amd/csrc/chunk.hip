@@ -1059,9 +1059,13 @@ chunk_kernel(const amass_chunk_args a,
     else save_stats<D>(g, st.m, l, bad, lane);
 }
 
-// Joins the parts of cut row tiles: a workgroup per cut tile, kv head, 32-row group and d tile.  Bound by the latency of its loads: record, statistics, O.  Wave
-// w takes parts w, w + 4, ... in batches whose loads are all issued before any is used, and the
-// waves join through LDS.  Large batches have nothing to join: their launch reads the count.
+// Joins the parts of cut row tiles, a d tile per workgroup (grid: cut tile x kv head, 32-row group, d
+// tile).  Bound by the latency of its loads: record, statistics and O, 3.3 us at 16 parts of one
+// tile, 6.2 us at 310 tiles of two or three parts (20 MB).  A wave issues the loads of
+// CM_BATCH parts before it uses any.  Up to that many parts it joins a group alone, and one
+// workgroup takes all groups of the tile (a workgroup of waves with a part each, joining in LDS,
+// took 8.7 us there); beyond, wave w takes parts w, w + 4, ... of one group and the waves join
+// through LDS.  Batches without cut tiles leave a launch that reads the count, 4 us.
 constexpr int CM_WAVES = 4;
 constexpr int CM_BATCH = 4;
 
@@ -1071,7 +1075,7 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
     __shared__ float ms[CM_WAVES][32], ls[CM_WAVES][32], os[CM_WAVES][16][WAVE];
     __shared__ int bads[CM_WAVES];
     const int lane = threadIdx.x & 63, rl = lane & 31;
-    const int group = blockIdx.y, x = blockIdx.z;
+    const int x = blockIdx.z;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kh = blockIdx.x % a.n_kv, i = blockIdx.x / a.n_kv;
     const int cuts = *(const int*)a.scratch;
@@ -1080,18 +1084,20 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
     const int rows = min(CK_BM, ct.q.n * a.G - ct.tile * CK_BM);
     const float c = a.scale * 1.44269504088896341f;
     const int64_t step = (int64_t)(pl.slot_rows / 32) * (32 * D + CK_STATS);
-    if (32 * group >= rows) return;
+    const bool alone = ct.parts <= CM_BATCH;
+    const int group = alone ? w : blockIdx.y, w0 = alone ? 0 : w, waves = alone ? 1 : CM_WAVES;
+    if (32 * group >= rows || (alone && blockIdx.y > 0)) return;
     const float* g0 = slot_group<D>(a, pl, kh, ct.slot, group);
     float m = -__FLT_MAX__, l = 0.f, o[16];
     bool bad = false;
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[j] = 0.f;
-    for (int s0 = w; s0 < ct.parts; s0 += CM_WAVES * CM_BATCH) {
+    for (int s0 = w0; s0 < ct.parts; s0 += waves * CM_BATCH) {
         float pm[CM_BATCH], ps[CM_BATCH], pb[CM_BATCH];
         float4 y[CM_BATCH][4];
 #pragma unroll
         for (int u = 0; u < CM_BATCH; ++u) {
-            const int s = s0 + u * CM_WAVES;
+            const int s = s0 + u * waves;
             pm[u] = -__FLT_MAX__;
             ps[u] = pb[u] = 0.f;
             if (s < ct.parts) {                // (scalar)
@@ -1114,7 +1120,7 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
         for (int j = 0; j < 16; ++j) o[j] *= al;
 #pragma unroll
         for (int u = 0; u < CM_BATCH; ++u)
-            if (s0 + u * CM_WAVES < ct.parts) {
+            if (s0 + u * waves < ct.parts) {
                 const float wt = __builtin_amdgcn_exp2f((pm[u] - m) * c);
                 bad |= pb[u] != 0.f;
                 l += ps[u] * wt;
@@ -1127,22 +1133,21 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
                 }
             }
     }
-    if (lane < 32) {
-        ms[w][lane] = m;
-        ls[w][lane] = l;
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) os[w][j][lane] = o[j];
-    if (lane == 0) bads[w] = bad;
-    __syncthreads();
-    bad = false;
-#pragma unroll
-    for (int v = 0; v < CM_WAVES; ++v) bad |= bads[v] != 0;
     const int row0 = ct.tile * CK_BM + 32 * group;
-    if (bad) {
-        for (int j = w + CM_WAVES * x; j < min(32, rows - 32 * group); j += CM_WAVES * (D / 32))
-            attend_row<DT, D>(a, pl, ct.q, ct.r, kh, row0 + j, c, lane);
-    } else if (w == 0) {
+    const int some = min(32, rows - 32 * group);
+    if (!alone) {
+        if (lane < 32) {
+            ms[w][lane] = m;
+            ls[w][lane] = l;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) os[w][j][lane] = o[j];
+        if (lane == 0) bads[w] = bad;
+        __syncthreads();
+        bad = false;
+#pragma unroll
+        for (int v = 0; v < CM_WAVES; ++v) bad |= bads[v] != 0;
+        if (w > 0 && !bad) return;
         m = -__FLT_MAX__;
         l = 0.f;
 #pragma unroll
@@ -1156,13 +1161,18 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
 #pragma unroll
             for (int j = 0; j < 16; ++j) o[j] += os[v][j][lane] * wt;
         }
-        const RowOut ro = row_out(a, pl, ct.q, kh, row0 + rl);
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) o[j] *= inv;
-        store_row<DT, D>(ro.out, x, o, lane);
-        if (x == 0) store_lse<DT>(ro, m, l, c, lane);
     }
+    if (bad) {
+        for (int j = w0 + waves * x; j < some; j += waves * (D / 32))
+            attend_row<DT, D>(a, pl, ct.q, ct.r, kh, row0 + j, c, lane);
+        return;
+    }
+    const RowOut ro = row_out(a, pl, ct.q, kh, row0 + rl);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j] *= inv;
+    store_row<DT, D>(ro.out, x, o, lane);
+    if (x == 0) store_lse<DT>(ro, m, l, c, lane);
 }
 
 // ------------------------------------------------------------------ host
