@@ -28,6 +28,7 @@
 // than the chip has room for (plan below, on the device: the launch needs no lengths on the
 // host and can be captured); parts leave (m, l, O) in scratch and a second launch joins them.
 #include <atomic>
+#include <type_traits>
 
 #include "../../include/amass_chunk.h"
 #include "common.h"
@@ -308,15 +309,14 @@ __device__ __forceinline__ int part_len(int n, int parts) { return max(1, (n + p
 
 // ------------------------------------------------------------------ scratch
 // The number of cut row tiles, a record of each, then the slots of their parts, by kv head.  A
-// slot: per group of 32 rows D / 32 tiles of 16 x 64 floats, the rows' m and l, and whether
-// the part met V values that are not finite in a masked place.
+// slot: per group of 32 rows D / 32 tiles of 16 x 64 floats, then the rows' m and l.
 struct CutTile {
     int r, tile, parts, slot;
     Req q;
     int pad;
 };
 constexpr int CK_HEAD = 256;
-constexpr int CK_STATS = 128;            // floats: m (32), l (32), bad
+constexpr int CK_STATS = 64;             // floats: m (32), l (32)
 
 __device__ __forceinline__ CutTile* cut_tile(const amass_chunk_args& a, int i) {
     return reinterpret_cast<CutTile*>((char*)a.scratch + CK_HEAD) + i;
@@ -584,6 +584,53 @@ __device__ __forceinline__ bool any_nonfinite(uint32_t vs, const LdsLane<D>& ll)
     return __any((bad & 0x80008000u) != 0);
 }
 
+// `weigh` for V that is not finite everywhere, where the weight zero of a key that a row does not see
+// would make NaN.  The products take zeros in place of what is not finite; then products of
+// the largest bf16 values (where a row sees a key that is not finite in the channel; zeros
+// elsewhere) of either sign make an infinity and NaN of that row's channel.  Rare, and written for few registers.
+template <int DT, int D, int NK>
+__device__ __forceinline__ void weigh_careful(uint32_t vs, const LdsLane<D>& ll,
+                                              const f32x16_t (&s)[NK], float c, RowState<D>& st) {
+    constexpr uint32_t MOST = 0x7F7Fu;
+    const float mc = fmaxf(st.m * c, -__FLT_MAX__) - CK_LIFT<DT>;
+    const auto step = [] { __builtin_amdgcn_sched_barrier(0); };
+    const auto bad_halves = [](uint32_t x) {
+        return ((nonfinite2<DT>(x) >> 15) & 0x00010001u) * 0xFFFFu;
+    };
+    float sum = 0.f;
+#pragma unroll
+    for (int y = 0; y < 2 * NK; ++y) {
+        u32x4_t p, see;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const float s0 = s[y >> 1][8 * (y & 1) + i], s1 = s[y >> 1][8 * (y & 1) + i + 1];
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s0, c, -mc));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s1, c, -mc));
+            sum += e0 + e1;
+            p[i >> 1] = pack2<DT>(e0, e1);
+            see[i >> 1] = (s0 != -INFINITY ? MOST : 0u) | (s1 != -INFINITY ? MOST << 16 : 0u);
+            step();
+        }
+#pragma unroll
+        for (int z = 0; z < D / 32; ++z) {
+            u32x4_t v = ll.v_frag(vs, z, y), most;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t halves = bad_halves(v[j]);
+                most[j] = halves & (MOST << 16 | MOST);
+                v[j] &= ~halves;
+            }
+            st.o[z] = mfma32<DT>(v, p, st.o[z]);
+            st.o[z] = mfma32<AMASS_BF16>(most, see, st.o[z]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most[j] |= (most[j] & 0x00010001u) << 15;
+            st.o[z] = mfma32<AMASS_BF16>(most, see, st.o[z]);
+            step();
+        }
+    }
+    st.l += sum;
+}
+
 // ------------------------------------------------------------------ staging
 // One request's pages of one kv head.  Everything but the lane offsets is uniform.
 template <int D>
@@ -671,9 +718,8 @@ __device__ __forceinline__ void save_tile(float* g, int x, const float (&o)[16],
 }
 
 template <int D>
-__device__ __forceinline__ void save_stats(float* g, float m, float l, bool bad, int lane) {
+__device__ __forceinline__ void save_stats(float* g, float m, float l, int lane) {
     g[32 * D + lane] = lane < 32 ? m : l;        // (both halves of the wave hold the rows)
-    if (lane == 0) g[32 * D + WAVE] = bad ? 1.f : 0.f;
 }
 
 struct RowOut {
@@ -702,67 +748,12 @@ __device__ __forceinline__ void store_lse(const RowOut& w, float m, float l, flo
     }
 }
 
-// One row over the keys it sees and no others: the way for a row tile in whose masked places V is
-// not finite (there a weight of zero gives NaN in a matrix product).  A wave takes 64 keys at a
-// time, a key per lane for the score, then d across the lanes for the values.  Slow, and rare.
-template <int DT, int D>
-__device__ __forceinline__ void attend_row(const amass_chunk_args& a, const ChunkPlan& pl,
-                                           const Req& q, int r, int kh, int row, float c, int lane) {
-    constexpr int PER = D / WAVE;                  // channels per lane
-    const int i = div_g(pl, row);
-    const int p = q.len - q.n + i;
-    const int lo = key_lo(a, p), hi = key_hi(a, pl, q.len, p);
-    const uint16_t* qr = (const uint16_t*)a.q + (int64_t)(q.q0 + i) * a.q_st +
-                         (int64_t)(kh * a.G + (row - i * a.G)) * a.q_hs;
-    const int32_t* table = a.block_table + r * a.bt_st;
-    const auto value = [](uint16_t h) { return DT == AMASS_BF16 ? bf16_to_f32(h) : fp16_to_f32(h); };
-    const auto place = [&](int t) -> int64_t {
-        const int b = table[t >> pl.sh];
-        return b >= 0 && b < a.nb ? b * a.kv_sb + (t & ((1 << pl.sh) - 1)) * a.kv_st + kh * a.kv_sh
-                                  : -1;
-    };
-    float m = -__FLT_MAX__, l = 0.f, o[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = 0.f;
-    for (int t0 = lo; t0 < hi; t0 += WAVE) {
-        const int t = t0 + lane;
-        const int64_t at = t < hi ? place(t) : -1;
-        float s = -INFINITY;
-        if (at >= 0) {
-            s = 0.f;
-            const uint16_t* k = (const uint16_t*)a.k + at;
-            for (int x = 0; x < D; ++x) s = __builtin_fmaf(value(qr[x]), value(k[x]), s);
-        }
-        const float mx = fmaxf(m, wave_maxf_uniform(s));
-        const float al = __builtin_amdgcn_exp2f((m - mx) * c);
-        m = mx;
-        const float mc = fmaxf(m * c, -__FLT_MAX__) - CK_LIFT<DT>;
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s, c, -mc));
-        l = l * al + wave_sumf(e);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) o[i] *= al;
-        for (int j = 0; j < WAVE && t0 + j < hi; ++j) {
-            const int64_t va = place(t0 + j);
-            if (va < 0) continue;
-            const float w = __shfl(e, j, WAVE);
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                o[i] += w * value(((const uint16_t*)a.v)[va + WAVE * i + lane]);
-        }
-    }
-    const RowOut ro = row_out(a, pl, q, kh, row);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-        ro.out[WAVE * i + lane] = (uint16_t)pack2<DT>(o[i] * inv, 0.f);
-    if (lane == 0) store_lse<DT>(ro, m, l, c, 0);
-}
-
 template <int D>
 struct __align__(1024) ChunkLds {
     char kv[2 * 2 * CK_KEYS * 2 * D];              // staging, then the waves' O
     float m[CK_WAVES][WAVE], l[CK_WAVES][WAVE];
-    int bad[CK_WAVES];
+    int gaps[CK_WAVES];                            // a page without a block
+    int bad[CK_WAVES];                             // V that is not finite in a masked place
 };
 
 // ------------------------------------------------------------------ kernel
@@ -859,7 +850,7 @@ chunk_kernel(const amass_chunk_args a,
             for (int p = (from >> pg.sh) + threadIdx.x; p <= to; p += CK_WAVES * WAVE)
                 has &= pg.has(a.block_table[it.r * a.bt_st + p]);
             const bool all = __all(has);
-            if (lane == 0) lds.bad[w] = !all;
+            if (lane == 0) lds.gaps[w] = !all;
         }
         const auto turn = [&](int j) {
             dma_wait<0>();
@@ -869,7 +860,7 @@ chunk_kernel(const amass_chunk_args a,
         };
         // tiles [f0, f1) hold only keys that all of the wave's rows see
         bool sound = false;
-        const auto step = [&](int j) {             // a tile with masks
+        const auto step = [&](int j, auto careful) {    // a tile with masks
             const int t0 = CK_KEYS * (sp.lo + j);
             if (idle || t0 >= hi_hi || t0 + CK_KEYS <= lo_lo) return;
             const uint32_t ks = base + 2 * KB * ((j - j0) & 1), vs = ks + KB;
@@ -882,22 +873,26 @@ chunk_kernel(const amass_chunk_args a,
             f32x16_t s[2];
             scores<DT, D, 2>(ks, ll, q, s);
             mask_scores<2>(s, lo - t0, hi - t0, groups, lane);
-            if (t0 < lo_hi || t0 + CK_KEYS > hi_lo) bad |= any_nonfinite<DT, D, 2>(vs, ll);
             maximum<D, 2>(s, c, st);
-            weigh<DT, D, 2>(vs, ll, s, c, st);
+            if constexpr (careful) {
+                weigh_careful<DT, D, 2>(vs, ll, s, c, st);
+            } else {
+                if (t0 < lo_hi || t0 + CK_KEYS > hi_lo) bad |= any_nonfinite<DT, D, 2>(vs, ll);
+                weigh<DT, D, 2>(vs, ll, s, c, st);
+            }
         };
         if (j0 < j1) {
             request(0);
             turn(j0);
-            sound = __builtin_amdgcn_readfirstlane(lds.bad[0] | lds.bad[1] | lds.bad[2] |
-                                                   lds.bad[3]) == 0;
+            sound = __builtin_amdgcn_readfirstlane(lds.gaps[0] | lds.gaps[1] | lds.gaps[2] |
+                                                   lds.gaps[3]) == 0;
         }
         const bool fast = sound && !idle;
         const int f1 = fast ? min(j1, hi_lo / CK_KEYS - sp.lo) : j1;
         const int f0 = fast ? min(f1, max(j0, (lo_hi + CK_KEYS - 1) / CK_KEYS - sp.lo)) : j1;
         int j = j0;
         while (j < f0) {
-            step(j);
+            step(j, std::false_type());
             if (++j < j1) turn(j);
         }
         while (j < f1) {
@@ -906,8 +901,22 @@ chunk_kernel(const amass_chunk_args a,
             if (++j < j1) turn(j);
         }
         while (j < j1) {
-            step(j);
+            step(j, std::false_type());
             if (++j < j1) turn(j);
+        }
+        // V that is not finite where a row does not see it: all over again, with care
+        if (lane == 0) lds.bad[w] = bad;
+        __syncthreads();
+        if (lds.bad[0] | lds.bad[1] | lds.bad[2] | lds.bad[3]) {
+            sound = false;
+            reset(st);
+            t_next = CK_KEYS * (sp.lo + j0) + 16 * w;
+            id = pg.entry(t_next);
+            request(0);
+            for (j = j0; j < j1; ++j) {
+                turn(j);
+                step(j, std::true_type());
+            }
         }
     } else {
         // ---- few rows: each wave its own 32 keys, w + 4, w + 8, ... ------------------------
@@ -973,7 +982,23 @@ chunk_kernel(const amass_chunk_args a,
             dma_wait<63>();
             if (more) vfull = issue_v(b + CK_WAVES);
         }
-        if (lane == 0) lds.bad[w] = bad;
+        if (bad) {                                 // (as above, this wave alone)
+            reset(st);
+            for (int b = b0; b < b1; b += CK_WAVES) {
+                const int t0 = 32 * b;
+                find(b);
+                issue_k(b);
+                issue_v(b);
+                dma_wait<0>();
+                const uint32_t groups = (pg.has(id[0]) ? 1u : 0u) | (pg.has(id[1]) ? 2u : 0u);
+                f32x16_t s[1];
+                scores<DT, D, 1>(base, ll, q, s);
+                mask_scores<1>(s, lo - t0, hi - t0, groups, lane);
+                maximum<D, 1>(s, c, st);
+                weigh_careful<DT, D, 1>(base + HB, ll, s, c, st);
+                dma_wait<0>();                     // (the reads have returned)
+            }
+        }
         // the waves' (m, l, O) through LDS: wave w takes d tile w of all of them
         dma_wait<0>();
         __syncthreads();
@@ -996,14 +1021,6 @@ chunk_kernel(const amass_chunk_args a,
             // (a wave without a finite score has l = 0 and O = 0)
             wt[v] = __builtin_amdgcn_exp2f((lds.m[v][lane] - m) * c);
             l += lds.l[v][lane] * wt[v];
-        }
-        bad = false;
-#pragma unroll
-        for (int v = 0; v < CK_WAVES; ++v) bad |= lds.bad[v] != 0;
-        if (whole && bad) {
-            for (int i = w; i < rows; i += CK_WAVES)
-                attend_row<DT, D>(a, pl, it.q, it.r, kh, it.tile * CK_BM + i, c, lane);
-            return;
         }
         if (w >= D / 32) return;
         float o[16];
@@ -1034,15 +1051,11 @@ chunk_kernel(const amass_chunk_args a,
         } else {
             float* g = slot_group<D>(a, pl, kh, it.slot, 0);
             save_tile<D>(g, w, o, lane);
-            if (w == 0) save_stats<D>(g, m, l, bad, lane);
+            if (w == 0) save_stats<D>(g, m, l, lane);
         }
         return;
     }
     if (idle) return;
-    if (whole && bad) {
-        for (int i = first; i <= last; ++i) attend_row<DT, D>(a, pl, it.q, it.r, kh, i, c, lane);
-        return;
-    }
     const float l = st.l + xor32_f(st.l);
     const RowOut ro = row_out(a, pl, it.q, kh, row);
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -1056,7 +1069,7 @@ chunk_kernel(const amass_chunk_args a,
         else save_tile<D>(g, x, o, lane);
     }
     if (whole) store_lse<DT>(ro, st.m, l, c, lane);
-    else save_stats<D>(g, st.m, l, bad, lane);
+    else save_stats<D>(g, st.m, l, lane);
 }
 
 // Joins the parts of cut row tiles, a d tile per workgroup (grid: cut tile x kv head, 32-row group, d
@@ -1073,7 +1086,6 @@ template <int DT, int D>
 __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amass_chunk_args a,
                                                                       const ChunkPlan pl) {
     __shared__ float ms[CM_WAVES][32], ls[CM_WAVES][32], os[CM_WAVES][16][WAVE];
-    __shared__ int bads[CM_WAVES];
     const int lane = threadIdx.x & 63, rl = lane & 31;
     const int x = blockIdx.z;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1089,22 +1101,20 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
     if (32 * group >= rows || (alone && blockIdx.y > 0)) return;
     const float* g0 = slot_group<D>(a, pl, kh, ct.slot, group);
     float m = -__FLT_MAX__, l = 0.f, o[16];
-    bool bad = false;
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[j] = 0.f;
     for (int s0 = w0; s0 < ct.parts; s0 += waves * CM_BATCH) {
-        float pm[CM_BATCH], ps[CM_BATCH], pb[CM_BATCH];
+        float pm[CM_BATCH], ps[CM_BATCH];
         float4 y[CM_BATCH][4];
 #pragma unroll
         for (int u = 0; u < CM_BATCH; ++u) {
             const int s = s0 + u * waves;
             pm[u] = -__FLT_MAX__;
-            ps[u] = pb[u] = 0.f;
+            ps[u] = 0.f;
             if (s < ct.parts) {                // (scalar)
                 const float* g = g0 + s * step;
                 pm[u] = g[32 * D + rl];
                 ps[u] = g[32 * D + 32 + rl];
-                pb[u] = g[32 * D + WAVE];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     y[u][j] = *reinterpret_cast<const float4*>(g + (x * 4 + j) * 4 * WAVE + 4 * lane);
@@ -1122,7 +1132,6 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
         for (int u = 0; u < CM_BATCH; ++u)
             if (s0 + u * waves < ct.parts) {
                 const float wt = __builtin_amdgcn_exp2f((pm[u] - m) * c);
-                bad |= pb[u] != 0.f;
                 l += ps[u] * wt;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -1133,8 +1142,6 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
                 }
             }
     }
-    const int row0 = ct.tile * CK_BM + 32 * group;
-    const int some = min(32, rows - 32 * group);
     if (!alone) {
         if (lane < 32) {
             ms[w][lane] = m;
@@ -1142,12 +1149,8 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
         }
 #pragma unroll
         for (int j = 0; j < 16; ++j) os[w][j][lane] = o[j];
-        if (lane == 0) bads[w] = bad;
         __syncthreads();
-        bad = false;
-#pragma unroll
-        for (int v = 0; v < CM_WAVES; ++v) bad |= bads[v] != 0;
-        if (w > 0 && !bad) return;
+        if (w > 0) return;
         m = -__FLT_MAX__;
         l = 0.f;
 #pragma unroll
@@ -1162,12 +1165,7 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
             for (int j = 0; j < 16; ++j) o[j] += os[v][j][lane] * wt;
         }
     }
-    if (bad) {
-        for (int j = w0 + waves * x; j < some; j += waves * (D / 32))
-            attend_row<DT, D>(a, pl, ct.q, ct.r, kh, row0 + j, c, lane);
-        return;
-    }
-    const RowOut ro = row_out(a, pl, ct.q, kh, row0 + rl);
+    const RowOut ro = row_out(a, pl, ct.q, kh, ct.tile * CK_BM + 32 * group + rl);
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[j] *= inv;

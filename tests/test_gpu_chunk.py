@@ -199,6 +199,34 @@ def test_not_finite_tokens_reach_only_rows_that_see_them(new, lens, at, dtype, d
     c.check(out, lse, rows=rest)
 
 
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("fp16", 64)])
+@pytest.mark.parametrize("new,lens,at", [([100], [230], 180), ([6], [300], 297), ([5], [6000], 5998),
+                                         ([300], [2500], 2300), ([1], [40], 39)])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_one_channel_of_v_that_is_not_finite(new, lens, at, dtype, d, value):
+    """It reaches that channel of the rows that see its token, and nothing else."""
+    announce(f"chunk attention: {value} in a channel, {new} of {lens}, {dtype}")
+    c = Case(new=new, lens=lens, n_kv=1, dtype=dtype, d=d)
+    block, row = int(c.table[0, at // 16]), at % 16
+    keep = c.v[block, row, 0, 37].clone()
+    c.v[block, row, 0, 37] = value
+    out, lse = c.run()
+    sees = at - (lens[0] - new[0])                  # the first row that does
+    c.v[block, row, 0, 37] = keep
+    assert not torch.isfinite(out[sees:, :, 37].float()).any()
+    out[sees:, :, 37] = torch.tensor(c.want()[0][sees:, :, 37], dtype=c.dt, device=DEV)
+    c.check(out, lse)
+
+
+@pytest.mark.parametrize("new,lens", [([3, 1], [70, 400]), ([500], [3000])])
+def test_a_cache_of_nans(new, lens):
+    announce(f"chunk attention: V of NaN, {new} of {lens}")
+    c = Case(new=new, lens=lens, n_kv=1)
+    c.v.fill_(float("nan"))
+    out, lse = c.run()
+    assert torch.isnan(out.float()).all() and torch.isfinite(lse).all()
+
+
 @pytest.mark.parametrize("new,lens", [([1, 3], [300, 200]), ([70], [300]), ([4], [5000]),
                                       ([280], [400])])
 def test_pages_without_a_block_are_masked(new, lens):
