@@ -18,15 +18,22 @@
 // c ^ swz(t), which spreads both the K reads (16 rows, one chunk) and the transposing V reads
 // (4 rows, 2 chunks) over the banks.
 //
-// Two layouts, chosen per row tile:
+// Two layouts, chosen per row tile (d = 128, bf16, 8 kv heads of 4 query heads unless stated):
 //   many (more than 32 rows): wave w owns rows 32 w .. 32 w + 31; the workgroup shares each
-//     64-key tile, double-buffered (2 x 32 KB at d = 128), one barrier per tile.
+//     64-key tile, double-buffered (2 x 32 KB at d = 128), one barrier per tile.  The matrix cores
+//     bound it: a prompt of 8192 tokens 511 us, 1.08 PFLOP/s (61 % of the matrix cores' cycles,
+//     6.7 vector instructions beside every product), 2048 tokens behind 63488
+//     1880 us, 1.15 PFLOP/s (67 %); a product of 8192^3 reaches 1.28 to 1.46 here.  One wave of
+//     64 rows (O and Q in the accumulator half of the registers) took 549 and 2005 us.
 //   few (32 rows or less: single tokens, drafts, a chunk's remainder): the rows fit one wave,
 //     so the waves take 32 keys each in turn, each with a K and a V buffer of its own and no
-//     barrier, and merge their (m, l, O) through LDS at the end.
+//     barrier, and merge their (m, l, O) through LDS at the end.  Memory bounds it: 8 requests of 4
+//     drafted tokens with 8k to 24k keys 104 us, 5.6 TB/s; 64 single tokens with 8k keys 330 us,
+//     6.4 TB/s.  The many-row layout, three of four waves idle, takes 116 for the drafts.
 // Splitting.  A row tile of many keys is cut into S parts when the batch has fewer tiles
 // than the chip has room for (plan below, on the device: the launch needs no lengths on the
 // host and can be captured); parts leave (m, l, O) in scratch and a second launch joins them.
+// 5 drafted tokens behind 4096: 8.4 us of 16 parts and 3.2 us of joining.
 #include <atomic>
 #include <type_traits>
 
@@ -48,11 +55,12 @@ constexpr int ck_wgs(int d) { return d == 128 ? 2 : 3; }
 constexpr int CK_BM = 32 * CK_WAVES;       // rows of a row tile
 constexpr int CK_FEW = 32;                 // rows up to which the waves share the rows
 constexpr int CK_KEYS = 64;                // keys of a tile
-constexpr int CK_MIN_SPLIT = 4;            // fewest tiles of a part
-// A tile of 64 keys costs a workgroup of few rows what the memory takes for it, 32 KB (d 128) at
-// 5 TB/s over 512 workgroups, 3.3 us, and one of many rows its products, 1.0 us.
-constexpr int CK_FEW_COST = 3;
-constexpr int CK_WORTH = 3;                // cut tiles for parts of at most 2 / 3 of the longest
+// fewest tiles of a part: joining costs what two do (5 tokens behind 4096: 13.1 us at 4, 14.7 at 2,
+// 13.7 at 8)
+constexpr int CK_MIN_SPLIT = 4;
+// cut tiles for parts of at most 2 / 3 of the longest (at most half: 1000 tokens behind 1600 with 7
+// heads per kv head 49.8 -> 59.8 us, ragged chunks under a sliding window 33.4 -> 32.0)
+constexpr int CK_WORTH = 3;
 constexpr float CK_LAZY = 8.f;             // a maximum may lag by this power of two
 // Weights are 2^CK_LIFT times those of the formula (sums too, so the result is the same): fp16
 // has no bits below 2^-24, and thousands of keys that far down a row count together.  2^15, the
@@ -129,6 +137,7 @@ struct ChunkPlan {
     int slots;           // scratch slots per kv head
     int slot_rows;       // rows of a slot
     int tiles_max;       // row tiles of the batch at most
+    int items;           // items of the batch at most
     uint32_t g_mul;      // x / G = x g_mul >> (30 + g_sh) for x < 2^30
     int g_sh;
 };
@@ -183,73 +192,103 @@ __device__ __forceinline__ int req_work(const amass_chunk_args& a, const ChunkPl
     return w;
 }
 
-// Parts of a row tile: S_r = ceil(w_r / len), w_r the cost of the request's longest tile (its
-// tiles of keys times CK_FEW_COST where the tile has few rows), for the smallest part length
-// `len` >= max(CK_MIN_SPLIT, sum_r tiles_r w_r / target) at which the batch has at most
-// `target` items (workgroups per kv head), or the first such length where the row tiles alone
-// are that many (only tiles much longer than the average are cut then).  No part has fewer
-// than CK_MIN_SPLIT tiles of keys.
-// Every workgroup computes it from the lengths, 64 requests at a time, one per lane.
+// The batch's row tiles per kv head, `target` of which the chip takes at a time, are dispatched in
+// the requests' order, a request's last (causal: longest) first.  Whole rounds of `target` tiles
+// are left whole; the `rest` behind them (all of them where they are fewer than a round) is cut
+// so that it fills the chip once: S_r = ceil(w_r / len) parts of a request's tiles, w_r the
+// longest's tiles of keys, for the smallest len >= max(CK_MIN_SPLIT, sum_r rest_r w_r / target)
+// with at most `target` parts, none shorter than CK_MIN_SPLIT tiles of keys.  Where some
+// tile is much longer than a workgroup's share of all the work, that share is `len`, and there are
+// no whole rounds.  (2100 tokens behind 60k, 66 tiles for 64: 3037 us uncut, 1951 with the rest cut.)
+// Every wave computes it from the lengths, 64 requests at a time, one per lane.
 struct LaneReq {
     Req q;
-    int tiles;           // row tiles
+    int tiles, rest;     // row tiles; those behind the whole rounds (the first `rest` of them)
     int most;            // parts of at least CK_MIN_SPLIT tiles of keys that the longest has
-    float cost;          // of the longest
+    float cost;          // the longest's tiles of keys
 };
-__device__ __forceinline__ LaneReq lane_req(const amass_chunk_args& a, const ChunkPlan& pl, int r) {
-    LaneReq x = {{0, 0, 0}, 0, 0, 0.f};
+__device__ __forceinline__ LaneReq lane_req(const amass_chunk_args& a, const ChunkPlan& pl, int r,
+                                            int whole, int before) {
+    // (whole: tiles of the whole rounds; before: tiles of the requests before this wave's 64)
+    LaneReq x = {{0, 0, 0}, 0, 0, 0, 0.f};
     if (r < a.n_req) x.q = load_req(a, r);
-    x.tiles = row_tiles(a, x.q);
-    const int work = req_work(a, pl, x.q, x.tiles);
+    x.tiles = x.rest = row_tiles(a, x.q);
+    if (whole > 0) x.rest = min(max(before + wave_incl_scan(x.tiles) - whole, 0), x.tiles);
+    const int work = req_work(a, pl, x.q, x.rest);
     x.most = (work + CK_MIN_SPLIT - 1) / CK_MIN_SPLIT;
-    x.cost = (float)work * (x.q.n * a.G <= CK_FEW ? CK_FEW_COST : 1);
+    x.cost = (float)work;
     return x;
 }
-// (inv: 1 / len, a little less, so that no rounding makes a part more)
+
+struct Parts {
+    int whole;
+    float inv;           // 1 / len, a little less, so that no rounding makes a part more
+    LaneReq x0;          // of the first 64 requests
+};
 __device__ __forceinline__ int parts_of(const LaneReq& x, float inv) {
     return max(1, min(x.most, (int)ceilf(x.cost * inv)));
 }
-
-__device__ __forceinline__ int count_items(const amass_chunk_args& a, const ChunkPlan& pl,
-                                           const LaneReq& x0, float inv) {
-    const int lane = threadIdx.x & 63;
-    int tot = wave_sum_uniform(x0.tiles * parts_of(x0, inv));
+template <class F>
+__device__ __forceinline__ void every_req(const amass_chunk_args& a, const ChunkPlan& pl,
+                                          const Parts& p, F f) {
+    f(p.x0);
+    if (a.n_req <= WAVE) return;
+    int before = wave_sum_uniform(p.x0.tiles);
     for (int base = WAVE; base < a.n_req; base += WAVE) {
-        const LaneReq x = lane_req(a, pl, base + lane);
-        tot += wave_sum_uniform(x.tiles * parts_of(x, inv));
+        const LaneReq x = lane_req(a, pl, base + (threadIdx.x & 63), p.whole, before);
+        before += wave_sum_uniform(x.tiles);
+        f(x);
     }
+}
+__device__ __forceinline__ int count_items(const amass_chunk_args& a, const ChunkPlan& pl,
+                                           const Parts& p, float inv) {
+    int tot = 0;
+    every_req(a, pl, p, [&](const LaneReq& x) { tot += wave_sum_uniform(x.rest * parts_of(x, inv)); });
     return tot;
 }
-// 1 / len, for a part length within 1 / 32 of the one described above
-__device__ __forceinline__ float part_inverse(const amass_chunk_args& a, const ChunkPlan& pl,
-                                              const LaneReq& x0) {
+__device__ __forceinline__ Parts plan_parts(const amass_chunk_args& a, const ChunkPlan& pl) {
     constexpr float LESS = 1.f - 0x1p-20f;
     const int lane = threadIdx.x & 63;
-    float work = (float)x0.tiles * x0.cost;
-    int tiles = wave_sum_uniform(x0.tiles);
-    float longest = wave_maxf_uniform(x0.cost);
-    for (int base = WAVE; base < a.n_req; base += WAVE) {
-        const LaneReq x = lane_req(a, pl, base + lane);
-        work += (float)x.tiles * x.cost;
-        tiles += wave_sum_uniform(x.tiles);
-        longest = fmaxf(longest, wave_maxf_uniform(x.cost));
-    }
-    work = wave_sumf_uniform(work);
-    const float none = LESS / fmaxf(longest, 1.f);       // no tile is cut
-    float lo = fmaxf((float)CK_MIN_SPLIT, work / ((float)pl.target * LESS));
-    if (lo >= longest) return none;
-    if (tiles < pl.target && count_items(a, pl, x0, LESS / lo) > pl.target) {
-        // parts <= cost / len + 1 each: at this length the items are few enough
-        float hi = fminf(longest, work / ((float)(pl.target - tiles) * LESS) + 1.f);
-        while (hi - lo > lo * (1.f / 32)) {
-            const float mid = 0.5f * (lo + hi);
-            if (count_items(a, pl, x0, LESS / mid) <= pl.target) hi = mid;
-            else lo = mid;
-        }
-        lo = hi;
-    }
+    Parts p = {0, 0.f, lane_req(a, pl, lane, 0, 0)};
+    int tiles;
+    float longest, share;
+    const auto add_up = [&] {
+        float work = 0.f;
+        tiles = 0;
+        longest = 0.f;
+        every_req(a, pl, p, [&](const LaneReq& x) {
+            work += (float)x.rest * x.cost;
+            tiles += wave_sum_uniform(x.rest);
+            longest = fmaxf(longest, wave_maxf_uniform(x.cost));
+        });
+        work = wave_sumf_uniform(work);
+        share = fmaxf((float)CK_MIN_SPLIT, work / ((float)pl.target * LESS));
+    };
     // joining costs what two or three tiles do: cut only for a part well below the longest tile
-    return CK_WORTH * lo > longest * (CK_WORTH - 1) ? none : LESS / lo;
+    const auto pays = [&](float len) { return CK_WORTH * len <= longest * (CK_WORTH - 1); };
+    add_up();
+    if (tiles >= pl.target) {
+        if (pays(share)) {
+            p.inv = LESS / share;
+            return p;
+        }
+        p.whole = tiles - tiles % pl.target;
+        p.x0 = lane_req(a, pl, lane, p.whole, 0);
+        add_up();
+    }
+    float len = share;
+    if (len < longest && count_items(a, pl, p, LESS / len) > pl.target) {
+        // parts <= cost / len + 1 each: at this length the items are few enough
+        float few = fminf(longest, share * (float)pl.target / (float)(pl.target - tiles) + 1.f);
+        while (few - len > len * (1.f / 32)) {
+            const float mid = 0.5f * (len + few);
+            if (count_items(a, pl, p, LESS / mid) <= pl.target) few = mid;
+            else len = mid;
+        }
+        len = few;
+    }
+    p.inv = pays(len) ? LESS / len : LESS / fmaxf(longest, 1.f);      // (else no tile is cut)
+    return p;
 }
 
 struct Item {
@@ -259,47 +298,46 @@ struct Item {
     Req q;
 };
 
-// Item y of the batch (requests in order, a request's last -- causal: longest -- tile first);
-// false past the end.
+// Item y of the batch; false past the end.
 __device__ __forceinline__ bool find_item(const amass_chunk_args& a, const ChunkPlan& pl,
-                                          const LaneReq& x0, float inv, int y, Item& it) {
-    const int lane = threadIdx.x & 63;
-    int before = 0, slots = 0, cuts = 0;                 // those of earlier requests
-    for (int base = 0; base < a.n_req; base += WAVE) {
-        const LaneReq x = base == 0 ? x0 : lane_req(a, pl, base + lane);
-        const int S = parts_of(x, inv);
-        const int n = x.tiles * S, ns = S > 1 ? n : 0, nc = S > 1 ? x.tiles : 0;
+                                          const Parts& p, int y, Item& it) {
+    int base = 0, before = 0, slots = 0, cuts = 0;       // those of earlier requests
+    bool found = false;
+    every_req(a, pl, p, [&](const LaneReq& x) {
+        const int S = parts_of(x, p.inv), full = x.tiles - x.rest;
+        const int n = full + x.rest * S, ns = S > 1 ? x.rest * S : 0, nc = S > 1 ? x.rest : 0;
         const int incl = wave_incl_scan(n), incl_s = wave_incl_scan(ns), incl_c = wave_incl_scan(nc);
         const int all = __builtin_amdgcn_readlane(incl, WAVE - 1);
-        if (y < before + all) {
+        if (!found && y < before + all) {
+            found = true;
             const int src = __ffsll((long long)__ballot(before + incl > y)) - 1;
             const int at = y - before - __builtin_amdgcn_readlane(incl - n, src);
-            const int s = __builtin_amdgcn_readlane(S, src), t = at / s;
+            const int f = __builtin_amdgcn_readlane(full, src), b = at - f;
+            const int s = b < 0 ? 1 : __builtin_amdgcn_readlane(S, src), t = b / s;
             it.r = base + src;
             it.parts = s;
-            it.tile = __builtin_amdgcn_readlane(x.tiles, src) - 1 - t;
-            it.part = at - t * s;
-            it.slot = slots + __builtin_amdgcn_readlane(incl_s - ns, src) + at;
+            it.tile = b < 0 ? __builtin_amdgcn_readlane(x.tiles, src) - 1 - at
+                            : __builtin_amdgcn_readlane(x.rest, src) - 1 - t;
+            it.part = b < 0 ? 0 : b - t * s;
+            it.slot = slots + __builtin_amdgcn_readlane(incl_s - ns, src) + b;
             it.cut = cuts + __builtin_amdgcn_readlane(incl_c - nc, src) + t;
             it.q.q0 = __builtin_amdgcn_readlane(x.q.q0, src);
             it.q.n = __builtin_amdgcn_readlane(x.q.n, src);
             it.q.len = __builtin_amdgcn_readlane(x.q.len, src);
-            return true;
         }
+        base += WAVE;
         before += all;
         slots += __builtin_amdgcn_readlane(incl_s, WAVE - 1);
         cuts += __builtin_amdgcn_readlane(incl_c, WAVE - 1);
-    }
-    return false;
+    });
+    return found;
 }
 __device__ __forceinline__ int count_cut(const amass_chunk_args& a, const ChunkPlan& pl,
-                                         const LaneReq& x0, float inv) {
-    const int lane = threadIdx.x & 63;
+                                         const Parts& p) {
     int tot = 0;
-    for (int base = 0; base < a.n_req; base += WAVE) {
-        const LaneReq x = base == 0 ? x0 : lane_req(a, pl, base + lane);
-        tot += wave_sum_uniform(parts_of(x, inv) > 1 ? x.tiles : 0);
-    }
+    every_req(a, pl, p, [&](const LaneReq& x) {
+        tot += wave_sum_uniform(parts_of(x, p.inv) > 1 ? x.rest : 0);
+    });
     return tot;
 }
 
@@ -770,13 +808,12 @@ chunk_kernel(const amass_chunk_args a,
     const int kh = blockIdx.x % a.n_kv;
     Item it;
     {
-        const LaneReq x0 = lane_req(a, pl, lane);
-        const float inv = part_inverse(a, pl, x0);
+        const Parts p = plan_parts(a, pl);
         if (blockIdx.x == 0 && w == 0) {
-            const int cuts = count_cut(a, pl, x0, inv);
+            const int cuts = count_cut(a, pl, p);
             if (lane == 0) *(int*)a.scratch = cuts;
         }
-        if (!find_item(a, pl, x0, inv, blockIdx.x / a.n_kv, it)) return;
+        if (!find_item(a, pl, p, blockIdx.x / a.n_kv, it)) return;
     }
     const Span sp = tile_span(a, pl, it.q, it.tile);
     const int per = part_len(sp.n, it.parts);
@@ -1219,9 +1256,10 @@ static ChunkPlan chunk_plan(const amass_chunk_args& a) {
     if (p.target < 1) p.target = 1;
     const int64_t rows = (int64_t)a.n_tokens * a.G;
     p.tiles_max = (int)(rows / CK_BM) + (a.n_req < a.n_tokens ? a.n_req : a.n_tokens);
-    // fewer tiles than `target`: the plan has at most `target` items; else those of cut tiles
-    // are at most twice sum_r tiles_r w_r / len <= target
+    // the rest's parts are at most `target`; without whole rounds those of cut tiles are at most twice
+    // sum_r tiles_r w_r / len <= target
     p.slots = p.tiles_max < p.target ? p.target : 2 * p.target;
+    p.items = p.tiles_max < p.target ? p.target : p.tiles_max + p.target;
     p.slot_rows = rows <= CK_FEW ? CK_FEW : CK_BM;
     p.g_sh = 0;
     while ((1 << p.g_sh) < a.G) ++p.g_sh;
@@ -1236,7 +1274,7 @@ static int64_t chunk_scratch(const amass_chunk_args& a, const ChunkPlan& p) {
 
 template <int DT, int D>
 static int launch_chunk(const amass_chunk_args& a, const ChunkPlan& p, hipStream_t s) {
-    const int64_t items = (int64_t)(p.tiles_max + p.target) * a.n_kv;
+    const int64_t items = (int64_t)p.items * a.n_kv;
     if (items * CK_WAVES * WAVE > 0xFFFFFFFFll) return AMASS_ERR_GEOMETRY;    // (threads of a launch)
     hipLaunchKernelGGL((chunk_kernel<DT, D>), dim3((unsigned)items), dim3(CK_WAVES * WAVE), 0, s, a, p);
     const int rc = check_launch();

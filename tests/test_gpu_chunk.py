@@ -356,6 +356,62 @@ def test_out_may_be_q(new, lens):
     assert torch.equal(q, apart) and torch.equal(lse, alse)
 
 
+def want_on_gpu(c):
+    """Case.want for batches that fill the chip: the same formulas in float64 on the GPU."""
+    q, k, v = (x.double().to(DEV) for x in (c.q, c.k, c.v))
+    T, H, d = q.shape
+    n_kv, G = k.shape[2], H // k.shape[2]
+    out, size = torch.full_like(q, float("nan")), torch.zeros_like(q)
+    lse, reach = (torch.zeros(T, H, dtype=torch.float64, device=DEV) for _ in range(2))
+    seen = torch.zeros(T, dtype=torch.int64, device=DEV)
+    lse[int(c.qs[-1]):] = float("nan")
+    for r, L in enumerate(c.lens.tolist()):
+        a, b = int(c.qs[r]), int(c.qs[r + 1])
+        n, block = b - a, c.table[r, :-(-L // c.page)].long().to(DEV)
+        p, j = torch.arange(L - n, L, device=DEV), torch.arange(L, device=DEV)
+        see = (j <= p[:, None]) & (j > p[:, None] - (c.window or 2 ** 40))
+        seen[a:b] = see.sum(1)
+        see = see.repeat_interleave(G, 0)
+        for h in range(n_kv):
+            kk, vv = (x[block, :, h].reshape(-1, d)[:L] for x in (k, v))
+            heads = slice(h * G, (h + 1) * G)
+            qq = q[a:b, heads].reshape(-1, d)
+            s = (c.scale * (qq @ kk.T.contiguous())).masked_fill(~see, -float("inf"))
+            m = s.amax(1, keepdim=True)
+            e = (s - m).exp()
+            l = e.sum(1, keepdim=True)
+            out[a:b, heads] = (e @ vv / l).view(n, G, d)
+            size[a:b, heads] = (e @ vv.abs() / l).view(n, G, d)
+            lse[a:b, heads] = (m + l.log()).view(n, G)
+            t = c.scale * (qq.abs() @ kk.abs().T.contiguous())
+            reach[a:b, heads] = t.masked_fill(~see, 0.0).amax(1).view(n, G)
+    return tuple(x.cpu().numpy() for x in (out, lse, seen, size, reach))
+
+
+ROUNDS = {        # 64 row tiles of 8 kv heads fill the chip once
+    "66 tiles": dict(new=[2100], lens=[2400]),
+    "the rest is a request's": dict(new=[100, 1900, 150], lens=[1500, 2000, 3000]),
+    "the rest is of two requests": dict(new=[1950, 90, 130], lens=[1950, 2500, 1300], pad=3),
+    "two rounds, 70 requests": dict(new=[40] * 70, lens=[100 + 37 * (i % 23) for i in range(70)]),
+    "a row far longer than its share": dict(new=[4, 1900, 200], lens=[9000, 1900, 300]),
+    "window": dict(new=[1500, 900], lens=[1500, 2900], window=700),
+    "fp16": dict(new=[1950, 300], lens=[1950, 2000], dtype="fp16"),
+}
+
+
+@pytest.mark.parametrize("name", ["small"] + list(ROUNDS))
+def test_more_tiles_than_the_chip_takes(name):
+    announce(f"chunk attention: {name}, more tiles than the chip takes at a time")
+    if name == "small":                             # the reference here against the oracle
+        c = Case(new=[20, 3], lens=[70, 33], window=40)
+        for x, y in zip(want_on_gpu(c), c.want()):
+            assert np.allclose(x, y, rtol=1e-11, atol=1e-12)
+        return
+    c = Case(**{**dict(n_kv=8, G=4), **ROUNDS[name]})
+    c.want = lambda: want_on_gpu(c)
+    c.check(*c.run())
+
+
 def test_repeats_bit_for_bit():
     announce("chunk attention: the same bits every time")
     c = Case(new=[4, 60, 1], lens=[3000, 500, 2500], n_kv=2)
