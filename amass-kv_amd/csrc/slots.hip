@@ -6,7 +6,9 @@
 // then its stores.  One launch does it: every workgroup ranks all requests' new pages
 // itself (a block scan over the lengths, which the L2 holds) and finds its tokens' requests
 // by bisection in LDS, and a token of a new page computes its block from its rank, so
-// nothing waits for the table that the launch writes.
+// nothing waits for the table that the launch writes.  64 requests of one token 2.8 us, 24
+// prompts of 34 thousand tokens (0.4 MB) 3.9 us; with four tokens per thread, in turn or side by
+// side, these are 2.8 and 6.6, and 4.2 and 6.2: rounds are what costs, not workgroups.
 #include "../../include/amass_chunk.h"
 #include "common.h"
 
@@ -14,7 +16,6 @@ namespace amass {
 
 constexpr int SL_THREADS = 256;
 constexpr int SL_WAVES = SL_THREADS / WAVE;
-constexpr int SL_TOKENS = 4 * SL_THREADS;          // tokens per workgroup
 constexpr int REL_THREADS = 1024;
 
 // exclusive prefix of v over the workgroup's threads; the sum in `total`
@@ -40,7 +41,7 @@ __device__ __forceinline__ int pages_of(int len, int sh) {
     return len > 0 ? ((len - 1) >> sh) + 1 : 0;
 }
 
-// grid (chunks of SL_TOKENS tokens), dynamic LDS: query_start (R+1), lengths (R), new pages
+// grid (chunks of SL_THREADS tokens), dynamic LDS: query_start (R+1), lengths (R), new pages
 // of the requests before (R).
 __global__ __launch_bounds__(SL_THREADS) void extend_kernel(const amass_extend_args a, int sh) {
     extern __shared__ int lds[];
@@ -70,55 +71,38 @@ __global__ __launch_bounds__(SL_THREADS) void extend_kernel(const amass_extend_a
     }
     __syncthreads();
     const int top = top_s;
-    if (tid == 0) {
-        // every workgroup reads top[0] before its arrival; the last one may overwrite it
-        bool last = true;
-        if (a.top_out == a.top && gridDim.x > 1) {
-            last = atomicAdd(&a.top[1], 1) == (int)gridDim.x - 1;
-            if (last) atomicExch(&a.top[1], 0);
-        } else {
-            last = blockIdx.x == 0;
-        }
-        if (last) {
-            a.top_out[0] = max(top - fresh, 0);
-            a.top_out[2] = max(fresh - top, 0);
+    // every workgroup reads top[0] before its arrival; the last one may overwrite it (below: the
+    // arrival's answer is not waited for here)
+    int arrived = blockIdx.x == 0 ? (int)gridDim.x - 1 : 0;
+    const bool count = a.top_out == a.top && gridDim.x > 1;
+    if (count && tid == 0) arrived = atomicAdd(&a.top[1], 1);
+    const int t = blockIdx.x * SL_THREADS + tid;
+    // the last request that starts at or before the token
+    int r = 0;
+    for (int step = a.n_req > 1 ? 1 << (31 - __clz(a.n_req - 1)) : 0; step > 0; step >>= 1)
+        if (r + step < a.n_req && qs[r + step] <= t) r += step;
+    int pos = -1, blk = -1;
+    if (a.n_req > 0 && t >= qs[r] && t < qs[r + 1]) {
+        const int start = len[r] - (qs[r + 1] - qs[r]);
+        pos = max(start + (t - qs[r]), -1);
+        const int p = pos >> sh;
+        if (pos >= 0 && p < a.max_pages) {
+            int32_t* entry = a.block_table + (int64_t)r * a.bt_st + p;
+            const int k = p - pages_of(start, sh), at = top - 1 - (before[r] + k);
+            if (k < 0) blk = *entry;
+            else if (at >= 0 && at < a.capacity) blk = a.free_list[at];
+            if (blk >= a.nb) blk = -1;
+            if (k >= 0 && (pos & ((1 << sh) - 1)) == 0) *entry = max(blk, -1);    // a page's first token
         }
     }
-#pragma unroll
-    for (int u = 0; u < SL_TOKENS / SL_THREADS; ++u) {
-        const int t = blockIdx.x * SL_TOKENS + u * SL_THREADS + tid;
-        if (t >= a.n_tokens) return;
-        // the last request that starts at or before t
-        int lo = 0, hi = a.n_req;        // qs[lo] <= t or lo = 0; qs[hi] > t or hi = R
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (qs[mid] <= t) lo = mid;
-            else hi = mid;
-        }
-        int pos = -1;
-        int64_t slot = -1;
-        if (a.n_req > 0 && t >= qs[lo] && t < qs[lo + 1]) {
-            const int start = len[lo] - (qs[lo + 1] - qs[lo]);
-            pos = max(start + (t - qs[lo]), -1);
-            const int p = pos >> sh;
-            if (pos >= 0 && p < a.max_pages) {
-                int32_t* entry = a.block_table + (int64_t)lo * a.bt_st + p;
-                const int k = p - pages_of(start, sh);
-                int blk;
-                if (k >= 0) {
-                    const int at = top - 1 - (before[lo] + k);
-                    blk = at >= 0 && at < a.capacity ? a.free_list[at] : -1;
-                    if (blk < 0 || blk >= a.nb) blk = -1;
-                    if ((pos & ((1 << sh) - 1)) == 0) *entry = blk;   // its first token
-                } else {
-                    blk = *entry;
-                }
-                if (blk >= 0 && blk < a.nb)
-                    slot = ((int64_t)blk << sh) + (pos & ((1 << sh) - 1));
-            }
-        }
+    if (t < a.n_tokens) {
         a.positions[t] = pos;
-        a.slots[t] = slot;
+        a.slots[t] = blk < 0 ? -1 : ((int64_t)blk << sh) + (pos & ((1 << sh) - 1));
+    }
+    if (tid == 0 && arrived == (int)gridDim.x - 1) {
+        if (count) atomicExch(&a.top[1], 0);
+        a.top_out[0] = max(top - fresh, 0);
+        a.top_out[2] = max(fresh - top, 0);
     }
 }
 
@@ -189,7 +173,7 @@ extern "C" int amass_extend(const amass_extend_args* a, void* stream) {
         return AMASS_ERR_GEOMETRY;
     if (a->n_req > AMASS_MAX_STEP_REQS) return AMASS_ERR_CAPACITY;
     // a step without tokens or requests still writes top_out and its rows' -1
-    const int chunks = a->n_tokens > 0 ? (a->n_tokens - 1) / SL_TOKENS + 1 : 1;
+    const int chunks = a->n_tokens > 0 ? (a->n_tokens - 1) / SL_THREADS + 1 : 1;
     hipLaunchKernelGGL(extend_kernel, dim3(chunks), dim3(SL_THREADS),
                        sizeof(int) * (3 * a->n_req + 1), (hipStream_t)stream, *a,
                        log2_of(a->page));
