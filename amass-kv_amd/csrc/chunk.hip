@@ -531,16 +531,25 @@ __device__ __forceinline__ void weigh(uint32_t vs, const LdsLane<D>& ll, const f
     st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// A whole tile of 64 keys that every row sees, in a fixed order (each step ends in a scheduling
+// A tile of 64 keys, in a fixed order (each step ends in a scheduling
 // barrier): the matrix products follow each other with four fragments in flight, and the
 // vector work runs under them:
 //   scores of keys 0..31 | scores of 32..63, weights of 0..31 | maximum |
 //   products with V of 0..31, weights of 32..63 | products with V of 32..63
 // The first weights are made with the maximum so far and made again in the rare tile whose
-// scores exceed it by more than it may lag.
-template <int DT, int D>
-__device__ __forceinline__ void whole_tile(uint32_t ks, uint32_t vs, const LdsLane<D>& ll,
-                                           const u32x4_t (&q)[D / 16], float c, RowState<D>& st) {
+// scores exceed it by more than it may lag.  MASKS: the lane's row sees the keys [lo, hi) of the
+// tile; without, all.
+template <int DT, int D, bool MASKS>
+__device__ __forceinline__ void ordered_tile(uint32_t ks, uint32_t vs, const LdsLane<D>& ll,
+                                             const u32x4_t (&q)[D / 16], float c, RowState<D>& st,
+                                             int lo, int hi, int lane) {
+    lo -= 4 * (lane >> 5);
+    hi -= 4 * (lane >> 5);
+    const uint32_t seen = (uint32_t)max(hi - lo, 0);
+    const auto masked = [&](float v, int x, int i) {
+        const int key = 32 * x + 8 * (i >> 2) + (i & 3);
+        return !MASKS || (uint32_t)(key - lo) < seen ? v : -INFINITY;
+    };
     constexpr int N = D / 16, Z = D / 32;      // products of 32 keys with K or V; d tiles
     u32x4_t f[4], p[4];
     f32x16_t s[2], zero;
@@ -549,7 +558,11 @@ __device__ __forceinline__ void whole_tile(uint32_t ks, uint32_t vs, const LdsLa
     const auto k_frag = [&](int n) { return ll.k_frag(ks, n % N, n / N); };
     const auto step = [] { __builtin_amdgcn_sched_barrier(0); };
     float mc = fmaxf(st.m * c, -__FLT_MAX__) - CK_LIFT<DT>, sum[4] = {0.f, 0.f, 0.f, 0.f};
-    const auto weight = [&](int x, int i) {    // weights 2 i and 2 i + 1 of half x
+    const auto weight = [&](int x, int i, bool fresh = true) {    // weights 2 i and 2 i + 1 of half x
+        if (x == 0 && fresh) {                 // (half 1 is masked before the maximum)
+            s[0][2 * i] = masked(s[0][2 * i], 0, 2 * i);
+            s[0][2 * i + 1] = masked(s[0][2 * i + 1], 0, 2 * i + 1);
+        }
         const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][2 * i], c, -mc));
         const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][2 * i + 1], c, -mc));
         sum[2 * (i & 1)] += e0;
@@ -578,6 +591,10 @@ __device__ __forceinline__ void whole_tile(uint32_t ks, uint32_t vs, const LdsLa
         step();
     }
     __builtin_amdgcn_s_setprio(0);
+    if constexpr (MASKS) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[1][i] = masked(s[1][i], 1, i);
+    }
     const float mx = xor32_maxf(fmaxf(row_max(s[0]), row_max(s[1])));
     const bool lag = lags(mx, c, st);
     float al = 1.f;
@@ -587,7 +604,7 @@ __device__ __forceinline__ void whole_tile(uint32_t ks, uint32_t vs, const LdsLa
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) weight(0, i);
+        for (int i = 0; i < 8; ++i) weight(0, i, false);
     }
     scale_o(st, al);
     __builtin_amdgcn_s_setprio(1);
@@ -607,19 +624,17 @@ __device__ __forceinline__ void whole_tile(uint32_t ks, uint32_t vs, const LdsLa
     st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// whether any V value of the 32 NK keys is an infinity or a NaN
-template <int DT, int D, int NK>
-__device__ __forceinline__ bool any_nonfinite(uint32_t vs, const LdsLane<D>& ll) {
-    uint32_t bad = 0;
+// whether O of a row that is there is not finite: V of keys that it sees is not, or of keys that it
+// does not see (zero times that is NaN, and stays).  Asked once per row tile: asking V of every
+// tile with masks instead took 0.4 us of such a tile.
+template <int D>
+__device__ __forceinline__ bool not_finite(const RowState<D>& st, bool live) {
+    float z[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int y = 0; y < 2 * NK; ++y)
+    for (int x = 0; x < D / 32; ++x)
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x) {
-            const u32x4_t v = ll.v_frag(vs, x, y);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) bad |= nonfinite2<DT>(v[j]);
-        }
-    return __any((bad & 0x80008000u) != 0);
+        for (int i = 0; i < 16; ++i) z[i & 3] = __builtin_fmaf(st.o[x][i], 0.f, z[i & 3]);
+    return __any(live && !((z[0] + z[1]) + (z[2] + z[3]) == 0.f));
 }
 
 // `weigh` for V that is not finite everywhere, where the weight zero of a key that a row does not see
@@ -791,7 +806,7 @@ struct __align__(1024) ChunkLds {
     char kv[2 * 2 * CK_KEYS * 2 * D];              // staging, then the waves' O
     float m[CK_WAVES][WAVE], l[CK_WAVES][WAVE];
     int gaps[CK_WAVES];                            // a page without a block
-    int bad[CK_WAVES];                             // V that is not finite in a masked place
+    int bad[CK_WAVES];                             // O that is not finite
 };
 
 // ------------------------------------------------------------------ kernel
@@ -857,7 +872,6 @@ chunk_kernel(const amass_chunk_args a,
     const LdsLane<D> ll(lane);
     RowState<D> st;
     reset(st);
-    bool bad = false;                              // a masked tile's V is not finite
 
     if (!few) {
         // ---- many rows: the workgroup shares the tiles -------------------------------------
@@ -895,64 +909,64 @@ chunk_kernel(const amass_chunk_args a,
             asm volatile("" ::: "memory");
             if (j + 1 < j1) request((j + 1 - j0) & 1);
         };
-        // tiles [f0, f1) hold only keys that all of the wave's rows see
-        bool sound = false;
-        const auto step = [&](int j, auto careful) {    // a tile with masks
+        const auto seen = [&](int j) {             // by some row of the wave
             const int t0 = CK_KEYS * (sp.lo + j);
-            if (idle || t0 >= hi_hi || t0 + CK_KEYS <= lo_lo) return;
-            const uint32_t ks = base + 2 * KB * ((j - j0) & 1), vs = ks + KB;
-            uint32_t groups = 15;
-            if (!sound) {
-                groups = 0;
-#pragma unroll
-                for (int g = 0; g < 4; ++g) groups |= (pg.has(pg.entry(t0 + 16 * g)) ? 1u : 0u) << g;
-            }
-            f32x16_t s[2];
-            scores<DT, D, 2>(ks, ll, q, s);
-            mask_scores<2>(s, lo - t0, hi - t0, groups, lane);
-            maximum<D, 2>(s, c, st);
-            if constexpr (careful) {
-                weigh_careful<DT, D, 2>(vs, ll, s, c, st);
-            } else {
-                if (t0 < lo_hi || t0 + CK_KEYS > hi_lo) bad |= any_nonfinite<DT, D, 2>(vs, ll);
-                weigh<DT, D, 2>(vs, ll, s, c, st);
-            }
+            return !idle && t0 < hi_hi && t0 + CK_KEYS > lo_lo;
         };
+        const auto tile = [&](int j, auto masks) {
+            const uint32_t ks = base + 2 * KB * ((j - j0) & 1);
+            const int t0 = CK_KEYS * (sp.lo + j);
+            ordered_tile<DT, D, masks>(ks, ks + KB, ll, q, c, st, lo - t0, hi - t0, lane);
+        };
+        bool again = false;
         if (j0 < j1) {
             request(0);
             turn(j0);
-            sound = __builtin_amdgcn_readfirstlane(lds.gaps[0] | lds.gaps[1] | lds.gaps[2] |
-                                                   lds.gaps[3]) == 0;
+            again = __builtin_amdgcn_readfirstlane(lds.gaps[0] | lds.gaps[1] | lds.gaps[2] |
+                                                   lds.gaps[3]) != 0;
         }
-        const bool fast = sound && !idle;
-        const int f1 = fast ? min(j1, hi_lo / CK_KEYS - sp.lo) : j1;
-        const int f0 = fast ? min(f1, max(j0, (lo_hi + CK_KEYS - 1) / CK_KEYS - sp.lo)) : j1;
-        int j = j0;
-        while (j < f0) {
-            step(j, std::false_type());
-            if (++j < j1) turn(j);
+        if (!again) {
+            // tiles [f0, f1) hold only keys that all of the wave's rows see
+            const int f1 = idle ? j1 : min(j1, hi_lo / CK_KEYS - sp.lo);
+            const int f0 = idle ? j1 : min(f1, max(j0, (lo_hi + CK_KEYS - 1) / CK_KEYS - sp.lo));
+            int j = j0;
+            while (j < f0) {
+                if (seen(j)) tile(j, std::true_type());
+                if (++j < j1) turn(j);
+            }
+            while (j < f1) {
+                tile(j, std::false_type());
+                if (++j < j1) turn(j);
+            }
+            while (j < j1) {
+                if (seen(j)) tile(j, std::true_type());
+                if (++j < j1) turn(j);
+            }
+            const bool bad = not_finite(st, live);
+            if (lane == 0) lds.bad[w] = bad;
+            __syncthreads();
+            again = __builtin_amdgcn_readfirstlane(lds.bad[0] | lds.bad[1] | lds.bad[2] |
+                                                   lds.bad[3]) != 0;
         }
-        while (j < f1) {
-            const uint32_t ks = base + 2 * KB * ((j - j0) & 1);
-            whole_tile<DT, D>(ks, ks + KB, ll, q, c, st);
-            if (++j < j1) turn(j);
-        }
-        while (j < j1) {
-            step(j, std::false_type());
-            if (++j < j1) turn(j);
-        }
-        // V that is not finite where a row does not see it: all over again, with care
-        if (lane == 0) lds.bad[w] = bad;
-        __syncthreads();
-        if (lds.bad[0] | lds.bad[1] | lds.bad[2] | lds.bad[3]) {
-            sound = false;
+        // Pages without a block, or something that is not finite: (all over again) with care
+        if (again) {
             reset(st);
             t_next = CK_KEYS * (sp.lo + j0) + 16 * w;
             id = pg.entry(t_next);
             request(0);
-            for (j = j0; j < j1; ++j) {
+            for (int j = j0; j < j1; ++j) {
                 turn(j);
-                step(j, std::true_type());
+                if (!seen(j)) continue;
+                const uint32_t ks = base + 2 * KB * ((j - j0) & 1);
+                const int t0 = CK_KEYS * (sp.lo + j);
+                uint32_t groups = 0;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) groups |= (pg.has(pg.entry(t0 + 16 * g)) ? 1u : 0u) << g;
+                f32x16_t s[2];
+                scores<DT, D, 2>(ks, ll, q, s);
+                mask_scores<2>(s, lo - t0, hi - t0, groups, lane);
+                maximum<D, 2>(s, c, st);
+                weigh_careful<DT, D, 2>(ks + KB, ll, s, c, st);
             }
         }
     } else {
@@ -1014,12 +1028,11 @@ chunk_kernel(const amass_chunk_args a,
             if (more && kfull) dma_wait<LOADS>();
             else dma_wait<0>();
             const uint32_t vs = base + HB;
-            if (masked) bad |= any_nonfinite<DT, D, 1>(vs, ll);
             weigh<DT, D, 1>(vs, ll, s, c, st);
             dma_wait<63>();
             if (more) vfull = issue_v(b + CK_WAVES);
         }
-        if (bad) {                                 // (as above, this wave alone)
+        if (not_finite(st, live)) {                // (as above, this wave alone)
             reset(st);
             for (int b = b0; b < b1; b += CK_WAVES) {
                 const int t0 = 32 * b;
