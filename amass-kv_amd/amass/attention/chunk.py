@@ -46,7 +46,7 @@ def _chunk_args(q, kv_cache, block_table, seq_lens, query_start, out, scale, cau
     if window is not None and window < 1:
         raise ValueError("window must be positive (None: no window)")
     scale = d ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 3e38:
+    if not 0.0 < scale <= 2e38:                 # (times log2 e it stays finite)
         raise ValueError(f"scale {scale} must be positive and finite")
     n_req = seq_lens.numel()
     vector(seq_lens, torch.int32, n_req, "seq_lens")

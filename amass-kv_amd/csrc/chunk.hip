@@ -200,31 +200,49 @@ __device__ __forceinline__ int req_work(const amass_chunk_args& a, const ChunkPl
 // with at most `target` parts, none shorter than CK_MIN_SPLIT tiles of keys.  Where some
 // tile is much longer than a workgroup's share of all the work, that share is `len`, and there are
 // no whole rounds.  (2100 tokens behind 60k, 66 tiles for 64: 3037 us uncut, 1951 with the rest cut.)
-// Every wave computes it from the lengths, 64 requests at a time, one per lane.
+// Every wave computes it from the lengths, 64 requests at a time, one per lane; of more than 64
+// requests the workgroup holds what that takes in LDS (256 single tokens with 500 keys each: 111 us
+// with a round of memory per pass and 64 requests, 105 so).
+struct Held {            // in LDS
+    Req q;
+    int tiles, work;     // row tiles, and the most tiles of keys that one has
+};
 struct LaneReq {
     Req q;
     int tiles, rest;     // row tiles; those behind the whole rounds (the first `rest` of them)
     int most;            // parts of at least CK_MIN_SPLIT tiles of keys that the longest has
     float cost;          // the longest's tiles of keys
 };
-__device__ __forceinline__ LaneReq lane_req(const amass_chunk_args& a, const ChunkPlan& pl, int r,
-                                            int whole, int before) {
-    // (whole: tiles of the whole rounds; before: tiles of the requests before this wave's 64)
-    LaneReq x = {{0, 0, 0}, 0, 0, 0, 0.f};
-    if (r < a.n_req) x.q = load_req(a, r);
-    x.tiles = x.rest = row_tiles(a, x.q);
-    if (whole > 0) x.rest = min(max(before + wave_incl_scan(x.tiles) - whole, 0), x.tiles);
-    const int work = req_work(a, pl, x.q, x.rest);
-    x.most = (work + CK_MIN_SPLIT - 1) / CK_MIN_SPLIT;
-    x.cost = (float)work;
-    return x;
+__device__ __forceinline__ Held held_req(const amass_chunk_args& a, const ChunkPlan& pl, int r) {
+    Held h = {{0, 0, 0}, 0, 0};
+    if (r < a.n_req) h.q = load_req(a, r);
+    h.tiles = row_tiles(a, h.q);
+    h.work = req_work(a, pl, h.q, h.tiles);
+    return h;
 }
 
 struct Parts {
-    int whole;
+    const Held* held;    // the first n_held requests'
+    int n_held;
+    int whole;           // tiles of the whole rounds
     float inv;           // 1 / len, a little less, so that no rounding makes a part more
     LaneReq x0;          // of the first 64 requests
 };
+// (before: tiles of the requests before the 64)
+__device__ __forceinline__ LaneReq lane_req(const amass_chunk_args& a, const ChunkPlan& pl,
+                                            const Parts& p, int r, int before) {
+    Held h;
+    if (r < p.n_held) h = p.held[r];
+    else h = held_req(a, pl, r);
+    LaneReq x = {h.q, h.tiles, h.tiles, 0, 0.f};
+    if (p.whole > 0) {
+        x.rest = min(max(before + wave_incl_scan(h.tiles) - p.whole, 0), h.tiles);
+        if (x.rest < h.tiles) h.work = x.rest > 0 ? req_work(a, pl, h.q, x.rest) : 0;
+    }
+    x.most = (h.work + CK_MIN_SPLIT - 1) / CK_MIN_SPLIT;
+    x.cost = (float)h.work;
+    return x;
+}
 __device__ __forceinline__ int parts_of(const LaneReq& x, float inv) {
     return max(1, min(x.most, (int)ceilf(x.cost * inv)));
 }
@@ -235,7 +253,7 @@ __device__ __forceinline__ void every_req(const amass_chunk_args& a, const Chunk
     if (a.n_req <= WAVE) return;
     int before = wave_sum_uniform(p.x0.tiles);
     for (int base = WAVE; base < a.n_req; base += WAVE) {
-        const LaneReq x = lane_req(a, pl, base + (threadIdx.x & 63), p.whole, before);
+        const LaneReq x = lane_req(a, pl, p, base + (threadIdx.x & 63), before);
         before += wave_sum_uniform(x.tiles);
         f(x);
     }
@@ -246,10 +264,12 @@ __device__ __forceinline__ int count_items(const amass_chunk_args& a, const Chun
     every_req(a, pl, p, [&](const LaneReq& x) { tot += wave_sum_uniform(x.rest * parts_of(x, inv)); });
     return tot;
 }
-__device__ __forceinline__ Parts plan_parts(const amass_chunk_args& a, const ChunkPlan& pl) {
+__device__ __forceinline__ Parts plan_parts(const amass_chunk_args& a, const ChunkPlan& pl,
+                                            const Held* held, int n_held) {
     constexpr float LESS = 1.f - 0x1p-20f;
     const int lane = threadIdx.x & 63;
-    Parts p = {0, 0.f, lane_req(a, pl, lane, 0, 0)};
+    Parts p = {held, n_held, 0, 0.f, {{0, 0, 0}, 0, 0, 0, 0.f}};
+    p.x0 = lane_req(a, pl, p, lane, 0);
     int tiles;
     float longest, share;
     const auto add_up = [&] {
@@ -273,7 +293,7 @@ __device__ __forceinline__ Parts plan_parts(const amass_chunk_args& a, const Chu
             return p;
         }
         p.whole = tiles - tiles % pl.target;
-        p.x0 = lane_req(a, pl, lane, p.whole, 0);
+        p.x0 = lane_req(a, pl, p, lane, 0);
         add_up();
     }
     float len = share;
@@ -625,8 +645,8 @@ __device__ __forceinline__ void ordered_tile(uint32_t ks, uint32_t vs, const Lds
 }
 
 // whether O of a row that is there is not finite: V of keys that it sees is not, or of keys that it
-// does not see (zero times that is NaN, and stays).  Asked once per row tile: asking V of every
-// tile with masks instead took 0.4 us of such a tile.
+// does not see (zero times that is NaN, and stays).  Asked once per row tile, 64 products a lane;
+// asking V of every tile with masks takes 160 instructions and 32 LDS reads each time.
 template <int D>
 __device__ __forceinline__ bool not_finite(const RowState<D>& st, bool live) {
     float z[4] = {0.f, 0.f, 0.f, 0.f};
@@ -814,8 +834,7 @@ struct __align__(1024) ChunkLds {
 // of 8), then the items.
 template <int DT, int D>
 __global__ __launch_bounds__(CK_WAVES * WAVE) __attribute__((amdgpu_waves_per_eu(ck_wgs(D), ck_wgs(D)))) void
-chunk_kernel(const amass_chunk_args a,
-                                                                   const ChunkPlan pl) {
+chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
     __shared__ ChunkLds<D> lds;
     constexpr int KB = CK_KEYS * 2 * D;            // bytes of a K (or V) tile
     const int lane = threadIdx.x & 63;
@@ -823,12 +842,17 @@ chunk_kernel(const amass_chunk_args a,
     const int kh = blockIdx.x % a.n_kv;
     Item it;
     {
-        const Parts p = plan_parts(a, pl);
+        Held* held = reinterpret_cast<Held*>(lds.kv);
+        const int n_held = a.n_req > WAVE ? min(a.n_req, (int)(sizeof(lds.kv) / sizeof(Held))) : 0;
+        for (int r = threadIdx.x; r < n_held; r += CK_WAVES * WAVE) held[r] = held_req(a, pl, r);
+        if (n_held > 0) __syncthreads();
+        const Parts p = plan_parts(a, pl, held, n_held);
         if (blockIdx.x == 0 && w == 0) {
             const int cuts = count_cut(a, pl, p);
             if (lane == 0) *(int*)a.scratch = cuts;
         }
         if (!find_item(a, pl, p, blockIdx.x / a.n_kv, it)) return;
+        if (n_held > 0) __syncthreads();           // (before the keys take its place)
     }
     const Span sp = tile_span(a, pl, it.q, it.tile);
     const int per = part_len(sp.n, it.parts);
@@ -1246,7 +1270,7 @@ static int chunk_check(const amass_chunk_args& a) {
     if (a.d != 64 && a.d != 128) return AMASS_ERR_UNSUPPORTED;
     if (a.page < 16 || a.page > (1 << 20) || (a.page & (a.page - 1))) return AMASS_ERR_GEOMETRY;
     if (a.n_req < 0 || a.n_tokens < 0 || a.n_kv < 1 || a.G < 1 || a.nb < 1 || a.max_pages < 1 ||
-        a.window < 0 || !(a.scale > 0.f) || a.scale > 3e38f)
+        a.window < 0 || !(a.scale > 0.f) || a.scale > 2e38f)
         return AMASS_ERR_GEOMETRY;
     if (a.n_kv > 4096 || a.G > 4096 || (int64_t)a.n_tokens * a.G > (1 << 30)) return AMASS_ERR_GEOMETRY;
     const auto off = [](const void* p) { return ((uintptr_t)p & 15) != 0; };

@@ -109,7 +109,7 @@ int amass_rope_write(const amass_rope_args* a, void* stream);
  * e^(s_j - m) rounded to the element type for the second product.  What is not visible is
  * not used, whatever it holds (infinities and NaN among it).  A row that sees no finite score
  * (a position below 0, an empty request, only scores of -inf) gets zeros and lse = -inf.  Rows
- * of no request are left as they are.  out may be q.  scale > 0.  d 64 or 128, page >= 16,
+ * of no request are left as they are.  out may be q.  0 < scale <= 2e38.  d 64 or 128, page >= 16,
  * G >= 1; q, out and the K and V views 16-byte aligned with strides of multiples of 8 elements
  * (a block below 2^30 of them).
  *
