@@ -61,6 +61,10 @@ constexpr int CK_MIN_SPLIT = 4;
 // cut tiles for parts of at most 2 / 3 of the longest (at most half: 1000 tokens behind 1600 with 7
 // heads per kv head 49.8 -> 59.8 us, ragged chunks under a sliding window 33.4 -> 32.0)
 constexpr int CK_WORTH = 3;
+// Keys that one row tile alone reads are loaded past the caches where the batch's row tiles read
+// more bytes of K and V than this, half of the memory-side cache: 4 drafted tokens of 8 requests, 580 MB, 118 ->
+// 103 us, 8 tokens with 8 heads per kv head, 164 MB, 43.7 -> 40.4, but 41 MB 21.8 -> 22.1 to 24.1 -> 29.1.
+constexpr float CK_ONCE = 128e6f;
 constexpr float CK_LAZY = 8.f;             // a maximum may lag by this power of two
 // Weights are 2^CK_LIFT times those of the formula (sums too, so the result is the same): fp16
 // has no bits below 2^-24, and thousands of keys that far down a row count together.  2^15, the
@@ -104,7 +108,7 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 }
 // 16 bytes per lane from base + off (off per lane) to LDS at `to` + 16 lane (`to` uniform).
 // No register waits for it: the caller waits with dma_wait before anyone reads the place.  ONCE:
-// what nobody reads again soon (it need not stay in the L2).
+// what nobody reads again soon (it need not stay in a cache).
 template <bool ONCE>
 __device__ __forceinline__ void dma16(uint32_t to, const char* base, uint32_t off) {
     if constexpr (ONCE)
@@ -226,6 +230,7 @@ struct Parts {
     int n_held;
     int whole;           // tiles of the whole rounds
     float inv;           // 1 / len, a little less, so that no rounding makes a part more
+    float keys;          // tiles of keys of all row tiles
     LaneReq x0;          // of the first 64 requests
 };
 // (before: tiles of the requests before the 64)
@@ -268,12 +273,12 @@ __device__ __forceinline__ Parts plan_parts(const amass_chunk_args& a, const Chu
                                             const Held* held, int n_held) {
     constexpr float LESS = 1.f - 0x1p-20f;
     const int lane = threadIdx.x & 63;
-    Parts p = {held, n_held, 0, 0.f, {{0, 0, 0}, 0, 0, 0, 0.f}};
+    Parts p = {held, n_held, 0, 0.f, 0.f, {{0, 0, 0}, 0, 0, 0, 0.f}};
     p.x0 = lane_req(a, pl, p, lane, 0);
     int tiles;
-    float longest, share;
+    float work, longest, share;
     const auto add_up = [&] {
-        float work = 0.f;
+        work = 0.f;
         tiles = 0;
         longest = 0.f;
         every_req(a, pl, p, [&](const LaneReq& x) {
@@ -287,6 +292,7 @@ __device__ __forceinline__ Parts plan_parts(const amass_chunk_args& a, const Chu
     // joining costs what two or three tiles do: cut only for a part well below the longest tile
     const auto pays = [&](float len) { return CK_WORTH * len <= longest * (CK_WORTH - 1); };
     add_up();
+    p.keys = work;
     if (tiles >= pl.target) {
         if (pays(share)) {
             p.inv = LESS / share;
@@ -738,14 +744,15 @@ struct Pages {
     __device__ __forceinline__ const char* row(int id, int t) const {
         return k + (uint64_t)(uint32_t)id * sb + (uint32_t)(t & ((1 << sh) - 1)) * st;
     }
-    // 16 rows to LDS (load_once: that no other workgroup is about to read)
-    __device__ __forceinline__ void load(uint32_t to, const char* src) const {
+    // 16 rows to LDS
+    __device__ __forceinline__ void load(uint32_t to, const char* src, bool once) const {
+        if (once) {
 #pragma unroll
-        for (int n = 0; n < LOADS; ++n) dma16<false>(to + 1024 * n, src, lane_off[n]);
-    }
-    __device__ __forceinline__ void load_once(uint32_t to, const char* src) const {
+            for (int n = 0; n < LOADS; ++n) dma16<true>(to + 1024 * n, src, lane_off[n]);
+        } else {
 #pragma unroll
-        for (int n = 0; n < LOADS; ++n) dma16<true>(to + 1024 * n, src, lane_off[n]);
+            for (int n = 0; n < LOADS; ++n) dma16<false>(to + 1024 * n, src, lane_off[n]);
+        }
     }
     // the first `rows` of 16 rows, zero behind them (the weight of a masked key is zero, and
     // zero times what lies behind a request's last token could be NaN)
@@ -841,6 +848,7 @@ chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kh = blockIdx.x % a.n_kv;
     Item it;
+    float keys;
     {
         Held* held = reinterpret_cast<Held*>(lds.kv);
         const int n_held = a.n_req > WAVE ? min(a.n_req, (int)(sizeof(lds.kv) / sizeof(Held))) : 0;
@@ -851,6 +859,7 @@ chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
             const int cuts = count_cut(a, pl, p);
             if (lane == 0) *(int*)a.scratch = cuts;
         }
+        keys = p.keys;
         if (!find_item(a, pl, p, blockIdx.x / a.n_kv, it)) return;
         if (n_held > 0) __syncthreads();           // (before the keys take its place)
     }
@@ -864,6 +873,7 @@ chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
         *cut_tile(a, it.cut) = {it.r, it.tile, (sp.n + per - 1) / per, it.slot, it.q, 0};
     const int rows = min(CK_BM, it.q.n * a.G - it.tile * CK_BM);
     const bool few = rows <= CK_FEW;
+    const bool once = it.q.n * a.G <= CK_BM && keys * (float)(2 * KB) * (float)a.n_kv > CK_ONCE;
     const int group = few ? 0 : w;                 // 32-row group of this wave
     const int row = it.tile * CK_BM + 32 * group + (lane & 31);
     const int last = it.tile * CK_BM + min(rows, 32 * group + 32) - 1;    // of the wave
@@ -907,11 +917,11 @@ chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
             const uint32_t kd = base + 2 * KB * buf + 16 * w * 2 * D, vd = kd + KB;
             const char* src = pg.row(id, t_next);
             if (t_next + 16 <= len && pg.has(id)) {
-                pg.load(kd, src);
-                pg.load(vd, src + pg.to_v);
+                pg.load(kd, src, once);
+                pg.load(vd, src + pg.to_v, once);
             } else {
                 const int rows = pg.has(id) ? min(len - t_next, 16) : 0;
-                if (rows > 0) pg.load(kd, src);
+                if (rows > 0) pg.load(kd, src, false);
                 pg.load_part(lds.kv + (vd - base), vd, src + pg.to_v, rows);
             }
             t_next += CK_KEYS;
@@ -1009,14 +1019,14 @@ chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
         const auto issue_k = [&](int b) -> bool {
 #pragma unroll
             for (int g = 0; g < 2; ++g)
-                if (pg.has(id[g])) pg.load_once(base + g * (HB / 2), pg.row(id[g], 32 * b + 16 * g));
+                if (pg.has(id[g])) pg.load(base + g * (HB / 2), pg.row(id[g], 32 * b + 16 * g), once);
             return pg.has(id[0]) && pg.has(id[1]);
         };
         const auto issue_v = [&](int b) -> bool {
             if (pg.has(id[0]) && pg.has(id[1]) && 32 * b + 32 <= len) {
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
-                    pg.load_once(base + HB + g * (HB / 2), pg.row(id[g], 32 * b + 16 * g) + pg.to_v);
+                    pg.load(base + HB + g * (HB / 2), pg.row(id[g], 32 * b + 16 * g) + pg.to_v, once);
                 return true;
             }
 #pragma unroll

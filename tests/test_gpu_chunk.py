@@ -109,6 +109,10 @@ CASES = {
     "empty requests": dict(new=[0, 9, 0, 40, 0], lens=[33, 9, 0, 77, 5], pad=6),
     "many requests": dict(new=[1 + i % 3 for i in range(150)], lens=[3 + 5 * i for i in range(150)],
                           n_kv=1, G=2),
+    "thousands of requests": dict(new=[1] * 3400, lens=[1 + i % 29 for i in range(3400)], n_kv=1,
+                                  G=1),
+    "thousands of requests d64": dict(new=[1] * 1800, lens=[1 + i % 29 for i in range(1800)],
+                                      n_kv=1, G=2, d=64),
     # prompts of many row tiles
     "long prompt": dict(new=[300], lens=[300]),
     "long prompt, one head": dict(new=[1030], lens=[1030], G=1, n_kv=1),
