@@ -107,20 +107,38 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
 // 16 bytes per lane from base + off (off per lane) to LDS at `to` + 16 lane (`to` uniform).
-// No register waits for it: the caller waits with dma_wait before anyone reads the place.  ONCE:
-// what nobody reads again soon (it need not stay in a cache).
-template <bool ONCE>
+// No register waits for it: the caller waits with dma_wait before anyone reads the place.
 __device__ __forceinline__ void dma16(uint32_t to, const char* base, uint32_t off) {
-    if constexpr (ONCE)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(to), "v"(off), "s"(base)
+                 : "memory", "m0");
+}
+// N of them, load n from base + off[n] + 1024 n to `to` + 1024 n + 16 lane: the instruction's offset counts
+// on both sides, so `to` is set once.  ONCE: what nobody reads again soon (it need not stay in
+// a cache).
+#define CK_LOAD(n, at, hint) "\n\tglobal_load_lds_dwordx4 %" #n ", %1 offset:" #at hint
+#define CK_LOADS2(hint) "s_mov_b32 m0, %0\n\ts_nop 0" CK_LOAD(2, 0, hint) CK_LOAD(3, 1024, hint)
+#define CK_LOADS4(hint) CK_LOADS2(hint) CK_LOAD(4, 2048, hint) CK_LOAD(5, 0xc00, hint)
+template <bool ONCE, int N>
+__device__ __forceinline__ void dma16_n(uint32_t to, const char* base, const uint32_t (&off)[N]) {
+    if constexpr (N == 4 && ONCE)
+        asm volatile(CK_LOADS4(" nt")
                      :
-                     : "s"(to), "v"(off), "s"(base)
+                     : "s"(to), "s"(base), "v"(off[0]), "v"(off[1]), "v"(off[N - 2]), "v"(off[N - 1])
+                     : "memory", "m0");
+    else if constexpr (N == 4)
+        asm volatile(CK_LOADS4("")
+                     :
+                     : "s"(to), "s"(base), "v"(off[0]), "v"(off[1]), "v"(off[N - 2]), "v"(off[N - 1])
+                     : "memory", "m0");
+    else if constexpr (ONCE)
+        asm volatile(CK_LOADS2(" nt")
+                     :
+                     : "s"(to), "s"(base), "v"(off[0]), "v"(off[1])
                      : "memory", "m0");
     else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                     :
-                     : "s"(to), "v"(off), "s"(base)
-                     : "memory", "m0");
+        asm volatile(CK_LOADS2("") : : "s"(to), "s"(base), "v"(off[0]), "v"(off[1]) : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void dma_wait() {        // all but the last N loads have arrived
@@ -716,26 +734,28 @@ template <int D>
 struct Pages {
     static constexpr int ROWS = 512 / D;           // rows of one 1-KB load
     static constexpr int LOADS = 16 / ROWS;        // loads of 16 rows
+    static constexpr int BACK = 1024 * (LOADS - 1);
     const __attribute__((address_space(4))) int32_t* table;   // the request's row
-    const char* k;                                 // of the kv head
+    const char* k;                                 // of the kv head, BACK before it
     int64_t to_v;                                  // from a K row to its V row
     uint32_t sb, st;                               // bytes of a block, a row
     int sh, nb, last;                              // last: a position that has a table entry
-    uint32_t lane_off[LOADS];                      // this lane's source in a 16-row group
+    uint32_t lane_off[LOADS];                      // this lane's source in a 16-row group, less the
+                                                   // load's own 1024 n, from BACK before it
     int lane;
 
     __device__ __forceinline__ Pages(const amass_chunk_args& a, const ChunkPlan& pl, int r, int kh,
                                      int hi, int lane_)
         : table((const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.block_table +
                                                                               r * a.bt_st)),
-          k((const char*)a.k + kh * a.kv_sh * 2), to_v((const char*)a.v - (const char*)a.k),
+          k((const char*)a.k + kh * a.kv_sh * 2 - BACK), to_v((const char*)a.v - (const char*)a.k),
           sb((uint32_t)a.kv_sb * 2), st((uint32_t)a.kv_st * 2), sh(pl.sh), nb(a.nb),
           last(max(hi - 1, 0)), lane(lane_) {
         const int chunk = lane & (D / 8 - 1), lr = lane / (D / 8);
 #pragma unroll
         for (int n = 0; n < LOADS; ++n) {
             const int row = ROWS * n + lr;
-            lane_off[n] = (uint32_t)row * st + ((uint32_t)(chunk ^ swz<D>(row)) << 4);
+            lane_off[n] = (uint32_t)row * st + ((uint32_t)(chunk ^ swz<D>(row)) << 4) + BACK - 1024 * n;
         }
     }
     // table entry of position t (of `last` behind it) and whether the pool has that block
@@ -745,14 +765,13 @@ struct Pages {
         return k + (uint64_t)(uint32_t)id * sb + (uint32_t)(t & ((1 << sh) - 1)) * st;
     }
     // 16 rows to LDS
+    template <bool ONCE = false>
+    __device__ __forceinline__ void load(uint32_t to, const char* src) const {
+        dma16_n<ONCE>(to, src, lane_off);
+    }
     __device__ __forceinline__ void load(uint32_t to, const char* src, bool once) const {
-        if (once) {
-#pragma unroll
-            for (int n = 0; n < LOADS; ++n) dma16<true>(to + 1024 * n, src, lane_off[n]);
-        } else {
-#pragma unroll
-            for (int n = 0; n < LOADS; ++n) dma16<false>(to + 1024 * n, src, lane_off[n]);
-        }
+        if (once) load<true>(to, src);
+        else load(to, src);
     }
     // the first `rows` of 16 rows, zero behind them (the weight of a masked key is zero, and
     // zero times what lies behind a request's last token could be NaN)
@@ -760,7 +779,7 @@ struct Pages {
                                               int rows) const {
 #pragma unroll
         for (int n = 0; n < LOADS; ++n) {
-            if (ROWS * n + lane / (D / 8) < rows) dma16<false>(to + 1024 * n, src, lane_off[n]);
+            if (ROWS * n + lane / (D / 8) < rows) dma16(to + 1024 * n, src + 1024 * n, lane_off[n]);
             else *reinterpret_cast<u32x4_t*>(dst + 1024 * n + 16 * lane) = (u32x4_t){0u, 0u, 0u, 0u};
         }
     }
@@ -873,7 +892,8 @@ chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
         *cut_tile(a, it.cut) = {it.r, it.tile, (sp.n + per - 1) / per, it.slot, it.q, 0};
     const int rows = min(CK_BM, it.q.n * a.G - it.tile * CK_BM);
     const bool few = rows <= CK_FEW;
-    const bool once = it.q.n * a.G <= CK_BM && keys * (float)(2 * KB) * (float)a.n_kv > CK_ONCE;
+    const bool once = it.q.n * a.G <= CK_BM &&
+                      __builtin_amdgcn_readfirstlane(keys * (float)(2 * KB) * (float)a.n_kv > CK_ONCE);
     const int group = few ? 0 : w;                 // 32-row group of this wave
     const int row = it.tile * CK_BM + 32 * group + (lane & 31);
     const int last = it.tile * CK_BM + min(rows, 32 * group + 32) - 1;    // of the wave
@@ -917,11 +937,16 @@ chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
             const uint32_t kd = base + 2 * KB * buf + 16 * w * 2 * D, vd = kd + KB;
             const char* src = pg.row(id, t_next);
             if (t_next + 16 <= len && pg.has(id)) {
-                pg.load(kd, src, once);
-                pg.load(vd, src + pg.to_v, once);
+                if (once) {
+                    pg.template load<true>(kd, src);
+                    pg.template load<true>(vd, src + pg.to_v);
+                } else {
+                    pg.load(kd, src);
+                    pg.load(vd, src + pg.to_v);
+                }
             } else {
                 const int rows = pg.has(id) ? min(len - t_next, 16) : 0;
-                if (rows > 0) pg.load(kd, src, false);
+                if (rows > 0) pg.load(kd, src);
                 pg.load_part(lds.kv + (vd - base), vd, src + pg.to_v, rows);
             }
             t_next += CK_KEYS;
