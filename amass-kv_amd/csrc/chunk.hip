@@ -21,10 +21,10 @@
 // Two layouts, chosen per row tile (d = 128, bf16, 8 kv heads of 4 query heads unless stated):
 //   many (more than 32 rows): wave w owns rows 32 w .. 32 w + 31; the workgroup shares each
 //     64-key tile, double-buffered (2 x 32 KB at d = 128), one barrier per tile.  The matrix cores
-//     bound it: a prompt of 8192 tokens 511 us, 1.08 PFLOP/s (61 % of the matrix cores' cycles,
+//     bound it: a prompt of 8192 tokens 517 us, 1.06 PFLOP/s (60 % of the matrix cores' cycles,
 //     6.7 vector instructions beside every product), 2048 tokens behind 63488
-//     1880 us, 1.15 PFLOP/s (67 %); a product of 8192^3 reaches 1.28 to 1.46 here.  One wave of
-//     64 rows (O and Q in the accumulator half of the registers) took 549 and 2005 us.
+//     1932 us, 1.12 PFLOP/s (66 %); a product of 8192^3 reaches 1.25 to 1.40 beside them.  A wave
+//     of 64 rows (O and Q in the accumulator half of the registers) took 549 and 2005 us.
 //   few (32 rows or less: single tokens, drafts, a chunk's remainder): the rows fit one wave,
 //     so the waves take 32 keys each in turn, each with a K and a V buffer of its own and no
 //     barrier, and merge their (m, l, O) through LDS at the end.  Memory bounds it: 8 requests of 4
