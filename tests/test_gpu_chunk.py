@@ -460,6 +460,43 @@ def test_captured_with_other_lengths():
         assert torch.equal(eager, out) and torch.equal(eager_lse, lse)
 
 
+def test_captured_prompts_and_padding():
+    """One captured call of 2200 rows: more tiles than the chip takes, then mostly rows of nobody, and
+    other requests."""
+    announce("chunk attention: captured, from full to mostly padding")
+    T, kw = 2200, dict(n_kv=8, G=4)
+    steps = [([2100, 0, 0], [2400, 1, 1]), ([40, 30, 10], [900, 3000, 77]),
+             ([1, 1900, 299], [2500, 1900, 800]), ([0, 0, 0], [5, 6, 7])]
+    q = torch.zeros(T, 32, 128, dtype=torch.bfloat16, device=DEV)
+    kv = torch.zeros(400, 2, 16, 8, 128, dtype=torch.bfloat16, device=DEV)
+    table = torch.zeros(3, 200, dtype=torch.int32, device=DEV)
+    lens = torch.zeros(3, dtype=torch.int32, device=DEV)
+    qs = torch.zeros(4, dtype=torch.int32, device=DEV)
+    out, lse = torch.zeros_like(q), torch.zeros(T, 32, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged_chunk_attention(q, kv, table, lens, qs, out, lse=lse)
+    for i in range(8):
+        new, ln = steps[i % 4]
+        c = Case(new=new, lens=ln, pad=T - sum(new), seed=i, **kw)
+        cq, ckv, ct, cl, cs = c.dev()
+        q.copy_(cq), lens.copy_(cl), qs.copy_(cs)
+        kv[:ckv.shape[0]] = ckv
+        table[:, :ct.shape[1]] = ct
+        out.fill_(7.0), lse.fill_(7.0)
+        graph.replay()
+        eager, eager_lse = torch.full_like(out, 7.0), torch.full_like(lse, 7.0)
+        paged_chunk_attention(q, kv, table, lens, qs, eager, lse=eager_lse)
+        assert torch.equal(eager, out) and torch.equal(eager_lse, lse)
+        if i < 4 and sum(new):
+            live = [r for r in range(3) if new[r]]
+            c.lens, c.table = c.lens[live], c.table[live]
+            c.qs = torch.tensor(np.concatenate([[0], np.cumsum([new[r] for r in live])]),
+                                dtype=torch.int32)
+            c.want = lambda c=c: want_on_gpu(c)
+            c.check(out, lse)
+
+
 def test_two_streams_at_once():
     announce("chunk attention: two streams")
     cases = [Case(new=[4, 1], lens=[6000, 3000], n_kv=2, seed=s) for s in (1, 2)]
