@@ -62,8 +62,9 @@ constexpr int CK_MIN_SPLIT = 4;
 // heads per kv head 49.8 -> 59.8 us, ragged chunks under a sliding window 33.4 -> 32.0)
 constexpr int CK_WORTH = 3;
 // Keys that one row tile alone reads are loaded past the caches where the batch's row tiles read
-// more bytes of K and V than this, half of the memory-side cache: 4 drafted tokens of 8 requests, 580 MB, 118 ->
-// 103 us, 8 tokens with 8 heads per kv head, 164 MB, 43.7 -> 40.4, but 41 MB 21.8 -> 22.1 to 24.1 -> 29.1.
+// more bytes of K and V than this, half of the memory-side cache: 4 drafted tokens of 8 requests,
+// 580 MB, 118 -> 103 us; 8 tokens with 8 heads per kv head, 164 MB, 43.7 -> 40.4; but 41 MB that the
+// last call left there 24.1 -> 29.1 (1 kv head) and 21.8 -> 22.1 (8).
 constexpr float CK_ONCE = 128e6f;
 constexpr float CK_LAZY = 8.f;             // a maximum may lag by this power of two
 // Weights are 2^CK_LIFT times those of the formula (sums too, so the result is the same): fp16
@@ -114,9 +115,9 @@ __device__ __forceinline__ void dma16(uint32_t to, const char* base, uint32_t of
                  : "s"(to), "v"(off), "s"(base)
                  : "memory", "m0");
 }
-// N of them, load n from base + off[n] + 1024 n to `to` + 1024 n + 16 lane: the instruction's offset counts
-// on both sides, so `to` is set once.  ONCE: what nobody reads again soon (it need not stay in
-// a cache).
+// N of them, load n from base + off[n] + 1024 n to `to` + 1024 n + 16 lane: the instruction's
+// offset counts on both sides, so `to` is set once.  ONCE: what nobody reads again soon (it need
+// not stay in a cache).
 #define CK_LOAD(n, at, hint) "\n\tglobal_load_lds_dwordx4 %" #n ", %1 offset:" #at hint
 #define CK_LOADS2(hint) "s_mov_b32 m0, %0\n\ts_nop 0" CK_LOAD(2, 0, hint) CK_LOAD(3, 1024, hint)
 #define CK_LOADS4(hint) CK_LOADS2(hint) CK_LOAD(4, 2048, hint) CK_LOAD(5, 0xc00, hint)
@@ -681,10 +682,11 @@ __device__ __forceinline__ bool not_finite(const RowState<D>& st, bool live) {
     return __any(live && !((z[0] + z[1]) + (z[2] + z[3]) == 0.f));
 }
 
-// `weigh` for V that is not finite everywhere, where the weight zero of a key that a row does not see
-// would make NaN.  The products take zeros in place of what is not finite; then products of
+// `weigh` for V that is not finite everywhere, where the weight zero of a key that a row does not
+// see would make NaN.  The products take zeros in place of what is not finite; then products of
 // the largest bf16 values (where a row sees a key that is not finite in the channel; zeros
-// elsewhere) of either sign make an infinity and NaN of that row's channel.  Rare, and written for few registers.
+// elsewhere) of either sign make an infinity and NaN of that row's channel.  Rare, and written
+// for few registers.
 template <int DT, int D, int NK>
 __device__ __forceinline__ void weigh_careful(uint32_t vs, const LdsLane<D>& ll,
                                               const f32x16_t (&s)[NK], float c, RowState<D>& st) {
@@ -859,7 +861,8 @@ struct __align__(1024) ChunkLds {
 // grid: kv head fastest (workgroups of one kv head share an XCD's L2 where n_kv is a multiple
 // of 8), then the items.
 template <int DT, int D>
-__global__ __launch_bounds__(CK_WAVES * WAVE) __attribute__((amdgpu_waves_per_eu(ck_wgs(D), ck_wgs(D)))) void
+__global__ __launch_bounds__(CK_WAVES * WAVE)
+__attribute__((amdgpu_waves_per_eu(ck_wgs(D), ck_wgs(D)))) void
 chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
     __shared__ ChunkLds<D> lds;
     constexpr int KB = CK_KEYS * 2 * D;            // bytes of a K (or V) tile
@@ -1378,7 +1381,8 @@ extern "C" int amass_chunk_attention(const amass_chunk_args* ain, void* stream) 
     const ChunkPlan p = chunk_plan(a);
     if (((uintptr_t)a.scratch & 255) || a.scratch_bytes < chunk_scratch(a, p)) return AMASS_ERR_CAPACITY;
     hipStream_t s = (hipStream_t)stream;
-    if (a.dtype == AMASS_BF16) return a.d == 128 ? launch_chunk<0, 128>(a, p, s) : launch_chunk<0, 64>(a, p, s);
+    if (a.dtype == AMASS_BF16)
+        return a.d == 128 ? launch_chunk<0, 128>(a, p, s) : launch_chunk<0, 64>(a, p, s);
     return a.d == 128 ? launch_chunk<1, 128>(a, p, s) : launch_chunk<1, 64>(a, p, s);
 }
 

@@ -92,7 +92,7 @@ __global__ __launch_bounds__(SL_THREADS) void extend_kernel(const amass_extend_a
             if (k < 0) blk = *entry;
             else if (at >= 0 && at < a.capacity) blk = a.free_list[at];
             if (blk >= a.nb) blk = -1;
-            if (k >= 0 && (pos & ((1 << sh) - 1)) == 0) *entry = max(blk, -1);    // a page's first token
+            if (k >= 0 && (pos & ((1 << sh) - 1)) == 0) *entry = max(blk, -1);    // its first token
         }
     }
     if (t < a.n_tokens) {
