@@ -113,6 +113,8 @@ CASES = {
                                   G=1),
     "thousands of requests d64": dict(new=[1] * 1800, lens=[1 + i % 29 for i in range(1800)],
                                       n_kv=1, G=2, d=64),
+    "pages of 256": dict(new=[5, 200], lens=[700, 300], page=256, n_kv=1),
+    "pages of 4096": dict(new=[2, 70, 1], lens=[5000, 90, 4097], page=4096, n_kv=1, d=64, G=3),
     # prompts of many row tiles
     "long prompt": dict(new=[300], lens=[300]),
     "long prompt, one head": dict(new=[1030], lens=[1030], G=1, n_kv=1),
