@@ -223,6 +223,9 @@ __device__ __forceinline__ int req_work(const amass_chunk_args& a, const ChunkPl
 // with at most `target` parts, none shorter than CK_MIN_SPLIT tiles of keys.  Where some
 // tile is much longer than a workgroup's share of all the work, that share is `len`, and there are
 // no whole rounds.  (2100 tokens behind 60k, 66 tiles for 64: 3037 us uncut, 1951 with the rest cut.)
+// Items, slots and records are bounded by the row tiles that ascending starts can make (chunk_plan
+// below).  Starts that do not ascend may make more, whose items no workgroup would take and
+// whose records nobody would write: such a batch is passed over whole (`fits`).
 // Every wave computes it from the lengths, 64 requests at a time, one per lane; of more than 64
 // requests the workgroup holds what that takes in LDS (256 single tokens with 500 keys each: 111 us
 // with a round of memory per pass and 64 requests, 105 so).
@@ -247,6 +250,7 @@ __device__ __forceinline__ Held held_req(const amass_chunk_args& a, const ChunkP
 struct Parts {
     const Held* held;    // the first n_held requests'
     int n_held;
+    bool fits;           // no more row tiles than ascending starts make
     int whole;           // tiles of the whole rounds
     float inv;           // 1 / len, a little less, so that no rounding makes a part more
     float keys;          // tiles of keys of all row tiles
@@ -292,7 +296,7 @@ __device__ __forceinline__ Parts plan_parts(const amass_chunk_args& a, const Chu
                                             const Held* held, int n_held) {
     constexpr float LESS = 1.f - 0x1p-20f;
     const int lane = threadIdx.x & 63;
-    Parts p = {held, n_held, 0, 0.f, 0.f, {{0, 0, 0}, 0, 0, 0, 0.f}};
+    Parts p = {held, n_held, true, 0, 0.f, 0.f, {{0, 0, 0}, 0, 0, 0, 0.f}};
     p.x0 = lane_req(a, pl, p, lane, 0);
     int tiles;
     float work, longest, share;
@@ -302,7 +306,7 @@ __device__ __forceinline__ Parts plan_parts(const amass_chunk_args& a, const Chu
         longest = 0.f;
         every_req(a, pl, p, [&](const LaneReq& x) {
             work += (float)x.rest * x.cost;
-            tiles += wave_sum_uniform(x.rest);
+            tiles = min(tiles + wave_sum_uniform(x.rest), 1 << 30);
             longest = fmaxf(longest, wave_maxf_uniform(x.cost));
         });
         work = wave_sumf_uniform(work);
@@ -312,6 +316,8 @@ __device__ __forceinline__ Parts plan_parts(const amass_chunk_args& a, const Chu
     const auto pays = [&](float len) { return CK_WORTH * len <= longest * (CK_WORTH - 1); };
     add_up();
     p.keys = work;
+    p.fits = tiles <= pl.tiles_max;
+    if (!p.fits) return p;
     if (tiles >= pl.target) {
         if (pays(share)) {
             p.inv = LESS / share;
@@ -878,11 +884,11 @@ chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
         if (n_held > 0) __syncthreads();
         const Parts p = plan_parts(a, pl, held, n_held);
         if (blockIdx.x == 0 && w == 0) {
-            const int cuts = count_cut(a, pl, p);
+            const int cuts = p.fits ? count_cut(a, pl, p) : 0;
             if (lane == 0) *(int*)a.scratch = cuts;
         }
         keys = p.keys;
-        if (!find_item(a, pl, p, blockIdx.x / a.n_kv, it)) return;
+        if (!p.fits || !find_item(a, pl, p, blockIdx.x / a.n_kv, it)) return;
         if (n_held > 0) __syncthreads();           // (before the keys take its place)
     }
     const Span sp = tile_span(a, pl, it.q, it.tile);
@@ -890,7 +896,6 @@ chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
     const int j0 = min(sp.n, it.part * per), j1 = min(sp.n, j0 + per);   // tiles of this part
     if (it.part > 0 && j0 >= j1) return;
     const bool whole = per >= sp.n;                // no other part has keys
-    if (it.parts > 1 && it.slot >= pl.slots) return;    // (a query_start that does not ascend)
     if (it.parts > 1 && it.part == 0 && kh == 0 && threadIdx.x == 0)
         *cut_tile(a, it.cut) = {it.r, it.tile, (sp.n + per - 1) / per, it.slot, it.q, 0};
     const int rows = min(CK_BM, it.q.n * a.G - it.tile * CK_BM);
@@ -1204,7 +1209,7 @@ __global__ __launch_bounds__(CM_WAVES * WAVE) void chunk_merge_kernel(const amas
     const int kh = blockIdx.x % a.n_kv, i = blockIdx.x / a.n_kv;
     const int cuts = *(const int*)a.scratch;
     const CutTile ct = *cut_tile(a, i);            // (inside the scratch; read before it is known)
-    if (i >= cuts || ct.parts < 2 || ct.slot + ct.parts > pl.slots) return;
+    if (i >= cuts || ct.parts < 2) return;
     const int rows = min(CK_BM, ct.q.n * a.G - ct.tile * CK_BM);
     const float c = a.scale * 1.44269504088896341f;
     const int64_t step = (int64_t)(pl.slot_rows / 32) * (32 * D + CK_STATS);

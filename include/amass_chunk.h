@@ -12,8 +12,9 @@
  * tokens it then has, so its row query_start[r] + i is at position
  * seq_lens[r] - (query_start[r+1] - query_start[r]) + i.  query_start has n_req + 1 ascending
  * entries; rows from query_start[n_req] to n_tokens-1 belong to no request (a padded batch).
- * Entries below 0 or above n_tokens are taken as those.  Position p of request r is in block
- * block_table[r][p / page], row p % page; `page` is a power of two.
+ * Entries below 0 or above n_tokens are taken as those.  With entries that do not ascend a call
+ * touches nothing outside its tensors, and what it leaves in them is not specified.  Position p
+ * of request r is in block block_table[r][p / page], row p % page; `page` is a power of two.
  */
 #ifndef AMASS_CHUNK_H
 #define AMASS_CHUNK_H
