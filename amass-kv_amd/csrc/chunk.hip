@@ -93,6 +93,11 @@ template <int DT>
 __device__ __forceinline__ uint32_t nonfinite2(uint32_t x) {
     return DT == AMASS_BF16 ? (x & 0x7F807F80u) + 0x00800080u : (x & 0x7C007C00u) + 0x04000400u;
 }
+// bits 15 / 31 set where a half of x is a NaN
+template <int DT>
+__device__ __forceinline__ uint32_t nan2(uint32_t x) {
+    return (x & 0x7FFF7FFFu) + (DT == AMASS_BF16 ? 0x007F007Fu : 0x03FF03FFu);
+}
 
 // ------------------------------------------------------------------ LDS
 // XOR of a row's 16-byte chunks: the 16 rows of a K read land in 16 places of the 256 bytes
@@ -691,17 +696,15 @@ __device__ __forceinline__ bool not_finite(const RowState<D>& st, bool live) {
 // `weigh` for V that is not finite everywhere, where the weight zero of a key that a row does not
 // see would make NaN.  The products take zeros in place of what is not finite; then products of
 // the largest bf16 values (where a row sees a key that is not finite in the channel; zeros
-// elsewhere) of either sign make an infinity and NaN of that row's channel.  Rare, and written
-// for few registers.
+// elsewhere) make an infinity of V's sign of that row's channel, and of the opposite sign too, NaN
+// with the first, where V is NaN.  Rare, and written for few registers.
 template <int DT, int D, int NK>
 __device__ __forceinline__ void weigh_careful(uint32_t vs, const LdsLane<D>& ll,
                                               const f32x16_t (&s)[NK], float c, RowState<D>& st) {
     constexpr uint32_t MOST = 0x7F7Fu;
     const float mc = fmaxf(st.m * c, -__FLT_MAX__) - CK_LIFT<DT>;
     const auto step = [] { __builtin_amdgcn_sched_barrier(0); };
-    const auto bad_halves = [](uint32_t x) {
-        return ((nonfinite2<DT>(x) >> 15) & 0x00010001u) * 0xFFFFu;
-    };
+    const auto halves = [](uint32_t tops) { return ((tops >> 15) & 0x00010001u) * 0xFFFFu; };
     float sum = 0.f;
 #pragma unroll
     for (int y = 0; y < 2 * NK; ++y) {
@@ -718,18 +721,17 @@ __device__ __forceinline__ void weigh_careful(uint32_t vs, const LdsLane<D>& ll,
         }
 #pragma unroll
         for (int z = 0; z < D / 32; ++z) {
-            u32x4_t v = ll.v_frag(vs, z, y), most;
+            u32x4_t v = ll.v_frag(vs, z, y), most, other;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t halves = bad_halves(v[j]);
-                most[j] = halves & (MOST << 16 | MOST);
-                v[j] &= ~halves;
+                const uint32_t bad = halves(nonfinite2<DT>(v[j])), nan = halves(nan2<DT>(v[j]));
+                most[j] = bad & (MOST << 16 | MOST | (v[j] & 0x80008000u));
+                other[j] = nan & (most[j] ^ 0x80008000u);
+                v[j] &= ~bad;
             }
             st.o[z] = mfma32<DT>(v, p, st.o[z]);
             st.o[z] = mfma32<AMASS_BF16>(most, see, st.o[z]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) most[j] |= (most[j] & 0x00010001u) << 15;
-            st.o[z] = mfma32<AMASS_BF16>(most, see, st.o[z]);
+            st.o[z] = mfma32<AMASS_BF16>(other, see, st.o[z]);
             step();
         }
     }

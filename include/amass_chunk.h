@@ -108,11 +108,13 @@ int amass_rope_write(const amass_rope_args* a, void* stream);
  *   s_j = scale q . k_j,  out = sum_j e^(s_j - m) v_j / l,  lse = m + ln l  (natural log)
  * with m = max_j s_j and l = sum_j e^(s_j - m), sums and statistics in fp32, the weights
  * e^(s_j - m) rounded to the element type for the second product.  What is not visible is
- * not used, whatever it holds (infinities and NaN among it).  A row that sees no finite score
- * (a position below 0, an empty request, only scores of -inf) gets zeros and lse = -inf.  Rows
- * of no request are left as they are.  out may be q.  0 < scale <= 2e38.  d 64 or 128, page >= 16,
- * G >= 1; q, out and the K and V views 16-byte aligned with strides of multiples of 8 elements
- * (a block below 2^30 of them).
+ * not used, whatever it holds (infinities and NaN among it).  A visible infinity in V
+ * makes its channel that infinity (NaN beside the opposite one, or where the key's weight is below
+ * fp32's least), a visible NaN makes it NaN; a key of score -inf counts as not visible.  A row
+ * that sees no finite score (a position below 0, an empty request, only scores of -inf) gets zeros
+ * and lse = -inf.  Rows of no request are left as they are.  out may be q.  0 < scale <= 2e38.
+ * d 64 or 128, page >= 16, G >= 1; q, out and the K and V views 16-byte aligned with strides of
+ * multiples of 8 elements (a block below 2^30 of them).
  *
  * scratch: amass_chunk_scratch_bytes(a) bytes, 256-byte aligned, for the parts of rows whose
  * keys several workgroups share.  It holds nothing between calls; calls that may run at the

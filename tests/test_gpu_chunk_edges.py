@@ -8,6 +8,7 @@ from helpers import announce
 from test_gpu_chunk import DEV, Case
 
 pytestmark = pytest.mark.gpu
+INF = float("inf")
 
 
 def test_starts_that_do_not_ascend_leave_other_memory_alone():
@@ -43,3 +44,47 @@ def test_rows_of_one_request_only_are_right_where_starts_do_not_ascend(T, starts
     c = Case(new=[T, 0, 0], lens=[150, 40, 230], n_kv=2)
     c.qs = torch.tensor(starts, dtype=torch.int32)
     c.check(*c.run(), rows=rows)
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("fp16", 64)])
+@pytest.mark.parametrize("new,lens,at", [([100], [230], 180), ([6], [300], 297), ([5], [6000], 5998),
+                                         ([300], [2500], 2300), ([1], [40], 39)])
+@pytest.mark.parametrize("value", [INF, -INF, float("nan")])
+def test_v_that_is_not_finite_arrives_as_itself(new, lens, at, dtype, d, value):
+    announce(f"chunk attention: {value} seen in a channel of V, {new} of {lens}, {dtype}")
+    c = Case(new=new, lens=lens, n_kv=1, dtype=dtype, d=d)
+    block, row = int(c.table[0, at // 16]), at % 16
+    c.v[block, row, 0, 37] = value
+    with np.errstate(invalid="ignore"):
+        want = torch.tensor(c.want()[0][:, :, 37])
+    out, _ = c.run()
+    sees = at - (lens[0] - new[0])                  # the first row that does
+    got = out[:, :, 37].double().cpu()
+    assert torch.isfinite(got[:sees]).all()
+    assert torch.equal(got[sees:].nan_to_num(nan=5.0, posinf=6.0, neginf=7.0),
+                       want[sees:].nan_to_num(nan=5.0, posinf=6.0, neginf=7.0))
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("fp16", 128)])
+@pytest.mark.parametrize("new,lens,first,second", [([90], [150], 70, 130), ([7], [2000], 1500, 1997),
+                                                   ([300], [900], 650, 652)])
+def test_opposite_infinities_in_v_make_nan(new, lens, first, second, dtype, d):
+    """Rows that see one of them have it, rows that see both NaN; in other channels nothing."""
+    announce(f"chunk attention: both infinities in V, {new} of {lens}, {dtype}")
+    c = Case(new=new, lens=lens, n_kv=1, dtype=dtype, d=d)
+    want = c.want()
+    kept = {}
+    for at, value in ((first, INF), (second, -INF)):
+        b, i = int(c.table[0, at // 16]), at % 16
+        kept[b, i] = c.v[b, i, 0, 5].clone()
+        c.v[b, i, 0, 5] = value
+    out, lse = c.run()
+    start = lens[0] - new[0]
+    one, both = max(first - start, 0), second - start
+    x = out[:, :, 5].float()
+    assert torch.isfinite(x[:one]).all() and (x[one:both] == INF).all()
+    assert torch.isnan(x[both:]).all() and both < new[0]
+    out[one:, :, 5] = torch.tensor(want[0][one:, :, 5], dtype=c.dt, device=DEV)
+    for (b, i), v in kept.items():
+        c.v[b, i, 0, 5] = v
+    c.check(out, lse)
