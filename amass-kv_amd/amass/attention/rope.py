@@ -13,10 +13,10 @@ Longer contexts than a model was trained on (``original_max`` positions) scale t
   "ntk"       the base becomes base * factor^(rot / (rot - 2)): the slowest pair turns
               ``factor`` times slower, the fastest as before
   "by_parts"  pair i makes ``original_max w_i / 2 pi`` turns over the trained length: at
-              ``fast`` turns or more it stays, at ``slow`` or fewer it is slowed by ``factor``,
-              linear in the number of turns between them
-  "yarn"      the same ends, linear in the pair's index between the pairs of ``fast`` and
-              ``slow`` turns, and cosines and sines times ``0.1 ln(factor) + 1``
+              ``fast`` turns (4) or more it stays, at ``slow`` (1) or fewer it is slowed by
+              ``factor``, linear in the number of turns between them
+  "yarn"      linear in the pair's index between the pairs of ``fast`` (32) and ``slow`` (1)
+              turns, and cosines and sines times ``0.1 ln(factor) + 1``
 
 Tables are computed in float64 and rounded once, so far positions keep the accuracy of near
 ones.
@@ -35,9 +35,10 @@ _pack_rope = packer(RopeArgs)
 
 
 def rope_frequencies(rot: int, *, base: float = 10000.0, scaling: str | None = None,
-                     factor: float = 1.0, original_max: int | None = None, fast: float = 4.0,
-                     slow: float = 1.0):
-    """(w (rot / 2,) float64, amplitude): the pairs' frequencies (module doc)."""
+                     factor: float = 1.0, original_max: int | None = None,
+                     fast: float | None = None, slow: float = 1.0):
+    """(w (rot / 2,) float64, amplitude): the pairs' frequencies (module doc).  ``fast`` None: 4
+    turns for "by_parts", 32 for "yarn"."""
     if rot < 2 or rot % 2:
         raise ValueError(f"rot {rot} must be even and positive")
     if not base > 1.0:
@@ -46,6 +47,8 @@ def rope_frequencies(rot: int, *, base: float = 10000.0, scaling: str | None = N
         raise ValueError(f"factor {factor} must be at least 1")
     if scaling in ("by_parts", "yarn") and not (original_max and original_max > 0):
         raise ValueError(f"scaling {scaling!r} needs original_max")
+    if fast is None:
+        fast = 32.0 if scaling == "yarn" else 4.0
     if scaling in ("by_parts", "yarn") and not fast > slow > 0.0:
         raise ValueError("fast must exceed slow, and slow zero")
     if scaling == "ntk":

@@ -199,6 +199,29 @@ def test_rope_scalings():
     assert torch.equal(table[0, :64], torch.full((64,), amp, dtype=torch.float64).float())
 
 
+@pytest.mark.parametrize("L,base", [(4096, 10000.0), (8192, 500000.0)])
+def test_rope_scalings_by_their_defaults(L, base):
+    """Without `fast` and `slow`: by parts between 4 turns and 1, yarn between 32 and 1."""
+    rot, factor = 128, 8.0
+    pairs = range(rot // 2)
+    w = [base ** (-2 * i / rot) for i in pairs]
+    turns = [L * x / (2 * math.pi) for x in w]
+    keep = [min(max((t - 1) / 3, 0.0), 1.0) for t in turns]
+    got, _ = rope_frequencies(rot, base=base, scaling="by_parts", factor=factor, original_max=L)
+    assert np.allclose(got.numpy(), [x * (k + (1 - k) / factor) for x, k in zip(w, keep)], rtol=1e-11,
+                       atol=0.0)
+    # the last pair of at least 32 turns stays, the first of at most one is slowed whole
+    first = max(i for i in pairs if turns[i] >= 32)
+    last = min(i for i in pairs if turns[i] <= 1)
+    slowed = [min(max((i - first) / (last - first), 0.0), 1.0) for i in pairs]
+    got, _ = rope_frequencies(rot, base=base, scaling="yarn", factor=factor, original_max=L)
+    assert np.allclose(got.numpy(), [x * (1 - s + s / factor) for x, s in zip(w, slowed)], rtol=1e-11,
+                       atol=0.0)
+    assert torch.equal(rope_table(rot, 9, base=base, scaling="yarn", factor=factor, original_max=L),
+                       rope_table(rot, 9, base=base, scaling="yarn", factor=factor, original_max=L,
+                                  fast=32.0, slow=1.0))
+
+
 @pytest.mark.parametrize("bad", [dict(rot=7), dict(rot=0), dict(base=1.0), dict(factor=0.5),
                                  dict(scaling="by_parts", factor=2.0), dict(scaling="other"),
                                  dict(scaling="yarn", factor=2.0),
