@@ -67,6 +67,9 @@ constexpr int CK_WORTH = 3;
 // last call left there 24.1 -> 29.1 (1 kv head) and 21.8 -> 22.1 (8).
 constexpr float CK_ONCE = 128e6f;
 constexpr float CK_LAZY = 8.f;             // a maximum may lag by this power of two
+// maxima (times c) beyond this take the products with care: there a weight may be off by 2^(1/16);
+// from 16 times as much on it may exceed fp16, from 2^11 times fp32
+constexpr float CK_FAR = 0x1p20f;
 // Weights are 2^CK_LIFT times those of the formula (sums too, so the result is the same): fp16
 // has no bits below 2^-24, and thousands of keys that far down a row count together.  2^15, the
 // largest with the lag, is below fp16's largest; bf16 has the exponents of fp32.
@@ -680,20 +683,23 @@ __device__ __forceinline__ void ordered_tile(uint32_t ks, uint32_t vs, const Lds
     st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// whether O of a row that is there is not finite: V of keys that it sees is not, or of keys that it
-// does not see (zero times that is NaN, and stays).  Asked once per row tile, 64 products a lane;
-// asking V of every tile with masks takes 160 instructions and 32 LDS reads each time.
+// whether a row that is there needs the products with care below.  Either O is not finite: V of keys
+// that the row sees is not, or of keys that it does not see (zero times that is NaN, and stays).
+// Asked once per row tile, 64 products a lane; asking V of every tile with masks takes 160
+// instructions and 32 LDS reads each time.  Or the maximum is far from zero: the weights' exponents
+// are c s less c m rounded, which is off by 2^-24 of it, and then a weight of one turns to 0 or infinity.
 template <int D>
-__device__ __forceinline__ bool not_finite(const RowState<D>& st, bool live) {
+__device__ __forceinline__ bool needs_care(const RowState<D>& st, float c, bool live) {
     float z[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < D / 32; ++x)
 #pragma unroll
         for (int i = 0; i < 16; ++i) z[i & 3] = __builtin_fmaf(st.o[x][i], 0.f, z[i & 3]);
-    return __any(live && !((z[0] + z[1]) + (z[2] + z[3]) == 0.f));
+    const bool far = st.m > -__FLT_MAX__ && fabsf(st.m) * c > CK_FAR;
+    return __any(live && (far || !((z[0] + z[1]) + (z[2] + z[3]) == 0.f)));
 }
 
-// `weigh` for V that is not finite everywhere, where the weight zero of a key that a row does not
+// `weigh` with exponents from s - m, exact where s is near m, and for V that is not finite everywhere, where the weight zero of a key that a row does not
 // see would make NaN.  The products take zeros in place of what is not finite; then products of
 // the largest bf16 values (where a row sees a key that is not finite in the channel; zeros
 // elsewhere) make an infinity of V's sign of that row's channel, and of the opposite sign too, NaN
@@ -702,7 +708,6 @@ template <int DT, int D, int NK>
 __device__ __forceinline__ void weigh_careful(uint32_t vs, const LdsLane<D>& ll,
                                               const f32x16_t (&s)[NK], float c, RowState<D>& st) {
     constexpr uint32_t MOST = 0x7F7Fu;
-    const float mc = fmaxf(st.m * c, -__FLT_MAX__) - CK_LIFT<DT>;
     const auto step = [] { __builtin_amdgcn_sched_barrier(0); };
     const auto halves = [](uint32_t tops) { return ((tops >> 15) & 0x00010001u) * 0xFFFFu; };
     float sum = 0.f;
@@ -712,8 +717,8 @@ __device__ __forceinline__ void weigh_careful(uint32_t vs, const LdsLane<D>& ll,
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
             const float s0 = s[y >> 1][8 * (y & 1) + i], s1 = s[y >> 1][8 * (y & 1) + i + 1];
-            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s0, c, -mc));
-            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s1, c, -mc));
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s0 - st.m, c, CK_LIFT<DT>));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s1 - st.m, c, CK_LIFT<DT>));
             sum += e0 + e1;
             p[i >> 1] = pack2<DT>(e0, e1);
             see[i >> 1] = (s0 != -INFINITY ? MOST : 0u) | (s1 != -INFINITY ? MOST << 16 : 0u);
@@ -852,8 +857,7 @@ __device__ __forceinline__ RowOut row_out(const amass_chunk_args& a, const Chunk
 template <int DT>
 __device__ __forceinline__ void store_lse(const RowOut& w, float m, float l, float c, int lane) {
     if (w.lse && lane < 32) {
-        const float mc = fmaxf(m * c, -__FLT_MAX__) - CK_LIFT<DT>;
-        *w.lse = l == 0.f ? -INFINITY : (mc + __log2f(l)) * 0.693147180559945309f;
+        *w.lse = l == 0.f ? -INFINITY : (m * c - CK_LIFT<DT> + __log2f(l)) * 0.693147180559945309f;
     }
 }
 
@@ -862,7 +866,7 @@ struct __align__(1024) ChunkLds {
     char kv[2 * 2 * CK_KEYS * 2 * D];              // staging, then the waves' O
     float m[CK_WAVES][WAVE], l[CK_WAVES][WAVE];
     int gaps[CK_WAVES];                            // a page without a block
-    int bad[CK_WAVES];                             // O that is not finite
+    int bad[CK_WAVES];                             // rows that need care
 };
 
 // ------------------------------------------------------------------ kernel
@@ -1011,13 +1015,14 @@ chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
                 if (seen(j)) tile(j, std::true_type());
                 if (++j < j1) turn(j);
             }
-            const bool bad = not_finite(st, live);
+            const bool bad = needs_care(st, c, live);
             if (lane == 0) lds.bad[w] = bad;
             __syncthreads();
             again = __builtin_amdgcn_readfirstlane(lds.bad[0] | lds.bad[1] | lds.bad[2] |
                                                    lds.bad[3]) != 0;
         }
-        // Pages without a block, or something that is not finite: (all over again) with care
+        // Pages without a block, something that is not finite or far from zero: (all over again) with
+        // care
         if (again) {
             reset(st);
             t_next = CK_KEYS * (sp.lo + j0) + 16 * w;
@@ -1101,7 +1106,7 @@ chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
             dma_wait<63>();
             if (more) vfull = issue_v(b + CK_WAVES);
         }
-        if (not_finite(st, live)) {                // (as above, this wave alone)
+        if (needs_care(st, c, live)) {             // (as above, this wave alone)
             reset(st);
             for (int b = b0; b < b1; b += CK_WAVES) {
                 const int t0 = 32 * b;

@@ -1,4 +1,6 @@
 """Chunk attention on the GPU at its edges: batches that are none, values that leave the ordinary."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -88,3 +90,39 @@ def test_opposite_infinities_in_v_make_nan(new, lens, first, second, dtype, d):
     for (b, i), v in kept.items():
         c.v[b, i, 0, 5] = v
     c.check(out, lse)
+
+
+@pytest.mark.parametrize("dtype,q,k,scale", [
+    ("fp16", 2.0 ** 15, 2.0 ** 15, None), ("fp16", -2.0 ** 15, 2.0 ** 14, None),
+    ("fp16", 2.0 ** 11, 2.0 ** 11, 1.0), ("bf16", 2.0 ** 25, 2.0 ** 25, None),
+    ("bf16", -2.0 ** 40, 2.0 ** 30, 0.3), ("bf16", 2.0 ** 60, 2.0 ** 58, 3.0),
+    ("bf16", 2.0 ** 60, 2.0 ** 58, 1e30), ("bf16", -2.0 ** 60, 2.0 ** 58, 1e30),
+    ("bf16", -2.0 ** 60, 2.0 ** 58, 0.1)])
+@pytest.mark.parametrize("new,lens,d", [([1], [300], 128), ([5], [9000], 128), ([100], [300], 128),
+                                        ([40], [6000], 64), ([2, 70], [40, 90], 64)])
+def test_scores_far_from_zero(new, lens, d, dtype, q, k, scale):
+    """Two keys have the largest score, every other one is thousands below: rows are the mean of the two
+    keys' V.  Scores are exact in fp32 (d q k times 11/8 and 13/8, powers of two but for that), so
+    are the two weights (1 each) and, but for 2^-24, their sum; the result is rounded once.  lse: at
+    most eight roundings (constants, products, sums) of 2^-24 of its size.  A score that times the
+    scale exceeds fp32 gives lse its infinity."""
+    announce(f"chunk attention: scores around {d * q * k:g}, scale {scale}, {new} of {lens}")
+    c = Case(new=new, lens=lens, dtype=dtype, d=d, n_kv=1, scale=scale)
+    most, least = (1.625, 1.375) if q > 0 else (1.375, 1.625)
+    c.q.fill_(q), c.k.fill_(least * k)
+    want = torch.zeros(sum(new), 4, d, dtype=torch.float64)
+    for r in range(len(new)):
+        two = [(int(c.table[r, at // 16]), at % 16) for at in (3, lens[r] - new[r])]
+        for b, i in two:
+            c.k[b, i] = most * k
+        want[int(c.qs[r]):int(c.qs[r + 1])] = sum(c.v[b, i].double() for b, i in two) / 2
+    out, lse = c.run()
+    u = torch.finfo(c.dt).eps / 2
+    err = (out.double().cpu() - want).abs()
+    size = 1.0 + 2.0 * want.abs()                   # (V is within a few of 1)
+    assert (err <= u * want.abs() * 1.01 + 2.0 ** -22 * size).all(), err.max()
+    top = most * d * q * k * c.scale
+    if abs(top) * math.log2(math.e) < 3.4e38:
+        assert ((lse.double() - (top + math.log(2.0))).abs() <= 2.0 ** -21 * abs(top) + 1e-6).all()
+    else:
+        assert (lse == math.copysign(INF, top)).all()
