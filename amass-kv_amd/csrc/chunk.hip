@@ -55,8 +55,8 @@ constexpr int ck_wgs(int d) { return d == 128 ? 2 : 3; }
 constexpr int CK_BM = 32 * CK_WAVES;       // rows of a row tile
 constexpr int CK_FEW = 32;                 // rows up to which the waves share the rows
 constexpr int CK_KEYS = 64;                // keys of a tile
-// fewest tiles of a part: joining costs what two do (5 tokens behind 4096: 13.1 us at 4, 14.7 at 2,
-// 13.7 at 8)
+// a row tile is cut in one part per this many tiles of keys at most: joining costs what two do (5
+// tokens behind 4096: 13.1 us at 4, 14.7 at 2, 13.7 at 8)
 constexpr int CK_MIN_SPLIT = 4;
 // cut tiles for parts of at most 2 / 3 of the longest (at most half: 1000 tokens behind 1600 with 7
 // heads per kv head 49.8 -> 59.8 us, ragged chunks under a sliding window 33.4 -> 32.0)
@@ -228,7 +228,8 @@ __device__ __forceinline__ int req_work(const amass_chunk_args& a, const ChunkPl
 // are left whole; the `rest` behind them (all of them where they are fewer than a round) is cut
 // so that it fills the chip once: S_r = ceil(w_r / len) parts of a request's tiles, w_r the
 // longest's tiles of keys, for the smallest len >= max(CK_MIN_SPLIT, sum_r rest_r w_r / target)
-// with at most `target` parts, none shorter than CK_MIN_SPLIT tiles of keys.  Where some
+// with at most `target` parts; a shorter tile of the request has no more of them than one per
+// CK_MIN_SPLIT tiles of keys that it begins.  Where some
 // tile is much longer than a workgroup's share of all the work, that share is `len`, and there are
 // no whole rounds.  (2100 tokens behind 60k, 66 tiles for 64: 3037 us uncut, 1951 with the rest cut.)
 // Items, slots and records are bounded by the row tiles that ascending starts can make (chunk_plan
@@ -244,7 +245,6 @@ struct Held {            // in LDS
 struct LaneReq {
     Req q;
     int tiles, rest;     // row tiles; those behind the whole rounds (the first `rest` of them)
-    int most;            // parts of at least CK_MIN_SPLIT tiles of keys that the longest has
     float cost;          // the longest's tiles of keys
 };
 __device__ __forceinline__ Held held_req(const amass_chunk_args& a, const ChunkPlan& pl, int r) {
@@ -270,17 +270,16 @@ __device__ __forceinline__ LaneReq lane_req(const amass_chunk_args& a, const Chu
     Held h;
     if (r < p.n_held) h = p.held[r];
     else h = held_req(a, pl, r);
-    LaneReq x = {h.q, h.tiles, h.tiles, 0, 0.f};
+    LaneReq x = {h.q, h.tiles, h.tiles, 0.f};
     if (p.whole > 0) {
         x.rest = min(max(before + wave_incl_scan(h.tiles) - p.whole, 0), h.tiles);
         if (x.rest < h.tiles) h.work = x.rest > 0 ? req_work(a, pl, h.q, x.rest) : 0;
     }
-    x.most = (h.work + CK_MIN_SPLIT - 1) / CK_MIN_SPLIT;
     x.cost = (float)h.work;
     return x;
 }
 __device__ __forceinline__ int parts_of(const LaneReq& x, float inv) {
-    return max(1, min(x.most, (int)ceilf(x.cost * inv)));
+    return max(1, (int)ceilf(x.cost * inv));
 }
 template <class F>
 __device__ __forceinline__ void every_req(const amass_chunk_args& a, const ChunkPlan& pl,
@@ -304,7 +303,7 @@ __device__ __forceinline__ Parts plan_parts(const amass_chunk_args& a, const Chu
                                             const Held* held, int n_held) {
     constexpr float LESS = 1.f - 0x1p-20f;
     const int lane = threadIdx.x & 63;
-    Parts p = {held, n_held, true, 0, 0.f, 0.f, {{0, 0, 0}, 0, 0, 0, 0.f}};
+    Parts p = {held, n_held, true, 0, 0.f, 0.f, {{0, 0, 0}, 0, 0, 0.f}};
     p.x0 = lane_req(a, pl, p, lane, 0);
     int tiles;
     float work, longest, share;
@@ -400,9 +399,11 @@ __device__ __forceinline__ int count_cut(const amass_chunk_args& a, const ChunkP
     return tot;
 }
 
-// tiles of keys per part of a row tile of n (a short tile has fewer parts than its request's
-// longest)
-__device__ __forceinline__ int part_len(int n, int parts) { return max(1, (n + parts - 1) / parts); }
+// tiles of keys per part of a row tile of n, of whose request's longest there are `parts`
+__device__ __forceinline__ int part_len(int n, int parts) {
+    parts = max(1, min(parts, (n + CK_MIN_SPLIT - 1) / CK_MIN_SPLIT));
+    return max(1, (n + parts - 1) / parts);
+}
 
 // ------------------------------------------------------------------ scratch
 // The number of cut row tiles, a record of each, then the slots of their parts, by kv head.  A

@@ -126,3 +126,17 @@ def test_scores_far_from_zero(new, lens, d, dtype, q, k, scale):
         assert ((lse.double() - (top + math.log(2.0))).abs() <= 2.0 ** -21 * abs(top) + 1e-6).all()
     else:
         assert (lse == math.copysign(INF, top)).all()
+
+
+@pytest.mark.parametrize("n,to", [(1024, 256), (1500, 256), (700, 224)])
+def test_short_row_tiles_stay_whole_beside_long_ones(n, to):
+    """The rows of a prompt whose longest row tiles are cut in parts: those up to 4 tiles of 64 keys are
+    as in a prompt that ends there, bit for bit."""
+    announce(f"chunk attention: first {to} tokens of {n}")
+    c = Case(new=[n], lens=[n], n_kv=1)
+    out, lse = c.run()
+    q, kv, table, lens, qs = c.dev()
+    o, e = torch.full_like(q[:to], 7.0), torch.full_like(lse[:to], 7.0)
+    paged_chunk_attention(q[:to], kv, table, torch.tensor([to], dtype=torch.int32, device=DEV),
+                          torch.tensor([0, to], dtype=torch.int32, device=DEV), o, lse=e)
+    assert torch.equal(lse[:to], e) and torch.equal(out[:to], o)
