@@ -1,5 +1,7 @@
 """Chunk attention on the GPU at its edges: batches that are none, values that leave the ordinary."""
 import math
+import os
+import re
 
 import numpy as np
 import pytest
@@ -7,7 +9,7 @@ import torch
 
 from amass.attention import chunk_scratch_bytes, paged_chunk_attention
 from helpers import announce
-from test_gpu_chunk import DEV, Case
+from test_gpu_chunk import DEV, Case, want_on_gpu
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -140,3 +142,66 @@ def test_short_row_tiles_stay_whole_beside_long_ones(n, to):
     paged_chunk_attention(q[:to], kv, table, torch.tensor([to], dtype=torch.int32, device=DEV),
                           torch.tensor([0, to], dtype=torch.int32, device=DEV), o, lse=e)
     assert torch.equal(lse[:to], e) and torch.equal(out[:to], o)
+
+
+# batches whose keys no cache keeps: K and V of requests of one row tile are loaded past the caches
+PAST = {
+    "drafts": dict(new=[4, 1, 8, 3], lens=[9001, 12345, 8200, 9999]),
+    "drafts fp16": dict(new=[3, 8, 5], lens=[17000, 10007, 9013], dtype="fp16"),
+    "drafts d64": dict(new=[5, 2, 8, 7], lens=[20011, 17203, 19999, 15000], d=64),
+    "drafts d64 fp16": dict(new=[4, 4, 8], lens=[30001, 25007, 20005], d=64, dtype="fp16", page=32),
+    "chunks": dict(new=[10, 31, 9, 32], lens=[9003, 8230, 12001, 9100], pad=5),
+    "chunks fp16": dict(new=[20, 9, 32], lens=[17005, 9012, 12300], dtype="fp16", halves_first=True),
+    "chunks d64": dict(new=[10, 32, 17, 30], lens=[20001, 17217, 19000, 16003], d=64, page=64),
+    "chunks d64 fp16": dict(new=[31, 9, 16], lens=[25011, 30030, 21001], d=64, dtype="fp16"),
+    "seven heads": dict(new=[18, 5, 1, 16], lens=[17777, 15001, 9999, 23001], n_kv=4, G=7),
+    "window": dict(new=[24, 5, 32], lens=[14001, 13007, 12345], window=11000),
+    "beside a prompt": dict(new=[1500, 12, 3], lens=[3000, 9001, 8003]),
+}
+
+
+def loaded_past_the_caches(c):
+    """Whether the requests of at most 128 rows are, by the kernel's rule: tiles of 64 keys of all row
+    tiles (each counted as its request's longest) in bytes against the limit in the source."""
+    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                           "amass-kv_amd", "csrc", "chunk.hip")) as fh:
+        limit = float(re.search(r"CK_ONCE = ([\d.e]+)f;", fh.read()).group(1))
+    n_kv, d = c.k.shape[2:]
+    G = c.q.shape[1] // n_kv
+    keys = 0
+    for n, length in zip((c.qs[1:] - c.qs[:-1]).tolist(), c.lens.tolist()):
+        tiles = -(-n * G // 128)
+        first = length - n + 128 * (tiles - 1) // G - (c.window or length) + 1    # its first key
+        keys += tiles * (-(-length // 64) - max(first, 0) // 64)
+    return keys * 64 * 4 * d * n_kv > limit
+
+
+@pytest.mark.parametrize("name", PAST)
+def test_keys_loaded_past_the_caches(name):
+    announce(f"chunk attention: {name}, loaded past the caches")
+    c = Case(**{**dict(n_kv=8, G=4), **PAST[name]})
+    assert loaded_past_the_caches(c)
+    c.want = lambda: want_on_gpu(c)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("name", ["drafts d64 fp16", "chunks", "chunks d64"])
+def test_v_that_is_not_finite_loaded_past_the_caches(name):
+    """NaN in a channel of the last token of request 1, and everywhere behind the last tokens."""
+    announce(f"chunk attention: {name}, loaded past the caches, V not finite")
+    c = Case(**{**dict(n_kv=8, G=4), **PAST[name]})
+    assert loaded_past_the_caches(c)
+    want, finite = want_on_gpu(c), c.v.clone()
+    for r, n in enumerate(c.lens.tolist()):
+        last = c.table[r, (n - 1) // c.page]
+        if n % c.page:
+            c.k[last, n % c.page:] = float("nan")
+            c.v[last, n % c.page:] = float("nan")
+    n = int(c.lens[1])
+    c.v[c.table[1, (n - 1) // c.page], (n - 1) % c.page, 2, 9] = float("nan")
+    out, lse = c.run()
+    t = int(c.qs[2]) - 1                            # the one row that sees it, by 4 heads
+    assert torch.isnan(out[t, 8:12, 9].float()).all()
+    out[t, 8:12, 9] = torch.tensor(want[0][t, 8:12, 9], dtype=c.dt, device=DEV)
+    c.want, c.v = lambda: want, finite              # (the tolerance goes by V's largest)
+    c.check(out, lse)
