@@ -29,7 +29,6 @@ CFLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-variable", "-Wno-unused-function",
-    "-Wno-inline-asm",      # (the reserved m0 among the clobbers of chunk.hip's LDS loads)
 ]
 
 

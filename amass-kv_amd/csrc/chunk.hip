@@ -115,6 +115,10 @@ __device__ __forceinline__ int swz(int row) {
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
+// (the compiler warns of m0, a reserved register, among the clobbers: the loads take their LDS address
+// there, and it has to know)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 // 16 bytes per lane from base + off (off per lane) to LDS at `to` + 16 lane (`to` uniform).
 // No register waits for it: the caller waits with dma_wait before anyone reads the place.
 __device__ __forceinline__ void dma16(uint32_t to, const char* base, uint32_t off) {
@@ -149,6 +153,7 @@ __device__ __forceinline__ void dma16_n(uint32_t to, const char* base, const uin
     else
         asm volatile(CK_LOADS2("") : : "s"(to), "s"(base), "v"(off[0]), "v"(off[1]) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 template <int N>
 __device__ __forceinline__ void dma_wait() {        // all but the last N loads have arrived
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory");
