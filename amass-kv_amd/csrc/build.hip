@@ -494,7 +494,7 @@ using namespace amass;
 
 extern "C" int amass_summary_build(const amass_build_args* a, void* stream) {
     if (!a) return AMASS_ERR_NULL;
-    if ((!a->k && !a->k_layers) || !a->blocks || !a->rec) return AMASS_ERR_NULL;
+    if ((!a->k && !a->k_layers) || (a->n > 0 && !a->blocks) || !a->rec) return AMASS_ERR_NULL;
     if (a->d != BD || a->page != BP || a->n < 0 || a->n_kv < 1) return AMASS_ERR_GEOMETRY;
     if (a->kind < 0 || a->kind > 2) return AMASS_ERR_GEOMETRY;
     if (a->rank < 1 || a->rank > 8) return AMASS_ERR_UNSUPPORTED;

@@ -115,3 +115,16 @@ def test_product_never_imports_the_oracle():
             if fn.endswith((".py", ".hip", ".h", ".cpp")):
                 with open(os.path.join(dp, fn)) as f:
                     assert not pat.search(f.read()), os.path.join(dp, fn)
+
+
+def test_summary_build_of_no_blocks():
+    """An empty list needs no address (a refresh with nothing stale); the rest is still asked for."""
+    lib = _hip.load_library()
+    b = _hip.BuildArgs(k=0x1000, rec=0x1000, rec_sb=1 << 20, n=0, n_layers=1, n_kv=2, d=128, page=16,
+                       rank=8, v_bits=8, c_bits=8)
+    assert lib.amass_summary_build(ctypes.byref(b), None) == 0
+    for over, status in ((dict(n=1), -1), (dict(rec=None), -1), (dict(k=None), -1), (dict(d=64), -2)):
+        a = _hip.BuildArgs.from_buffer_copy(b)
+        for k, v in over.items():
+            setattr(a, k, v)
+        assert lib.amass_summary_build(ctypes.byref(a), None) == status, over

@@ -283,3 +283,23 @@ def test_tail_rebuild_graph_replay():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(st.quad_rec, want)
+
+
+@pytest.mark.parametrize("kind", ["quad", "clse", "r8"])
+def test_refresh_with_nothing_stale(kind):
+    """The second refresh of the same pages finds none to build; after one key changed, one."""
+    from amass.selection.build import r8_build_refresh
+    announce(f"refresh with nothing stale: {kind}")
+    case, _ = _case(3)
+    kw = dict(num_layers=1, num_blocks=case.kv_cache.shape[0], n_kv=8, G=4, head_dim=128, page=16,
+              max_reqs=3, max_pages=case.max_pages, rank=8)
+    st = R8State(DEV, **kw) if kind == "r8" else \
+        QuadState(DEV, coords="lse" if kind == "clse" else "none", **kw)
+    refresh = r8_build_refresh if kind == "r8" else quad_build_refresh
+    args = (st, 0, case.kv_cache[:, 0], case.block_table, case.seq_lens, 3)
+    assert refresh(*args) == len(_blocks(case))
+    rec = (st.r8_rec if kind == "r8" else st.quad_rec).clone()
+    assert refresh(*args) == 0
+    assert torch.equal(rec, st.r8_rec if kind == "r8" else st.quad_rec)
+    case.kv_cache[int(case.block_table[1, 5]), 0, 15, :, 0] += 1.0
+    assert refresh(*args) == 1
