@@ -6,10 +6,15 @@ import pytest
 import torch
 
 import oracle.chunk as ochunk
+import oracle.decode as odec
+import oracle.select as osel
 from amass.attention import (ResidentVSource, dense_paged_decode, ensure_stage_b_buffers,
                              extend_block_tables, free_blocks, paged_chunk_attention,
                              release_blocks, rope_frequencies, rope_paged_write, rope_table)
-from helpers import announce
+from amass.selection import QuadState, derive_page_params
+from amass.selection.quad_build import quad_build_bulk, quad_build_delta
+from amass.selection.quad_score import select_then_attend
+from helpers import announce, npf, npi
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -152,3 +157,50 @@ def test_captured_decode_step():
         assert torch.equal(lens, other[1]) and torch.equal(s.table, other[0]), i
         assert torch.equal(out, other[5]) and torch.isfinite(out.float()).all(), i
     assert lens.tolist() == [34, 50, 21] and s.top.tolist() == other[2].tolist()
+
+
+@pytest.mark.parametrize("budget", [0.15, 1.0])
+def test_sparse_decode_over_the_cache_that_they_filled(budget):
+    """Prompts through the operators, summaries of the pages that they filled, then decode steps:
+    slots, rotary write, summaries of new pages, score, selection and sparse decode.  The pages
+    kept are those of the scores; the output is the attention over them, and over all pages
+    (budget 1) the chunk attention's of the same step.  Both kernels round their weights and results
+    once: 2 (u + u) of values up to the rows' largest."""
+    announce(f"sparse decode over the cache that the operators filled, budget {budget}")
+    R, nb, width = 3, 128, 48
+    s = Server(R=R, nb=nb, width=width, seed=7)
+    new = [600, 200, 333]
+    q, lens, qs = s.write(new, 5)
+    out = torch.zeros_like(q)
+    paged_chunk_attention(q, s.kv, s.table, lens, qs, out)
+    _near(out[:sum(new)], s.attention(new))
+    st = QuadState(DEV, num_layers=1, num_blocks=nb, n_kv=N_KV, G=G, head_dim=D, page=PAGE,
+                   max_reqs=R, max_pages=width, rank=8, budget=budget, combine="nrm")
+    ensure_stage_b_buffers(st, DEV)
+    full = sum(int(n) // PAGE for n in new)
+    assert quad_build_bulk(st, [s.kv[:, 0]], s.table, lens, R) == full
+    built = 0
+    for step in range(20):                          # every request fills a page or two
+        q, lens, qs = s.write([1] * R)
+        built += quad_build_delta(st, [s.kv[:, 0]], s.table, lens, R)
+        derive_page_params(st, lens, R)
+        got = torch.full_like(q, float("nan"))
+        select_then_attend(st, 0, q, s.kv, s.table, lens, R, D ** -0.5, got, ResidentVSource(s.kv))
+        if step % 6 and step < 19:
+            continue
+        tab, cnt, _ = osel.select(npf(st.score), npi(st.n_pages), npi(st.n_sel_hi), npi(st.b_fix),
+                                  sink=1, max_pages=width, mode=0, coverage=1.0, tie_mode=0,
+                                  score_kind=1)
+        assert np.array_equal(npi(st.page_table), tab) and np.array_equal(npi(st.page_cnt), cnt)
+        pages = -(-s.lens // PAGE)
+        assert (cnt == pages[:, None]).all() if budget == 1.0 else (cnt < pages[:, None]).all()
+        # (rows behind the last token hold NaN, and the oracle multiplies them by zero)
+        k, v = (np.nan_to_num(npf(s.kv[:, j])) for j in (0, 1))
+        want = odec.attend(npf(q), k, v, npi(s.table), npi(lens), tab, cnt, scale=D ** -0.5, G=G)
+        tol = 4 * 2.0 ** -8 * np.abs(want).max(-1, keepdims=True) + 2.0 ** -8
+        assert (np.abs(npf(got) - want) <= tol).all(), step
+        if budget == 1.0:
+            out = torch.zeros_like(q)
+            paged_chunk_attention(q, s.kv, s.table, lens, qs, out)
+            assert (np.abs(npf(got) - npf(out)) <= tol).all(), step
+    assert built == sum(int(n) // PAGE for n in s.lens) - full
