@@ -72,9 +72,10 @@ constexpr float CK_LAZY = 8.f;             // a maximum may lag by this power of
 constexpr float CK_FAR = 0x1p20f;
 // Weights are 2^CK_LIFT times those of the formula (sums too, so the result is the same): fp16
 // has no bits below 2^-24, and thousands of keys that far down a row count together.  2^15, the
-// largest with the lag, is below fp16's largest; bf16 has the exponents of fp32.
+// largest with the lag, is below fp16's largest.  bf16 has the exponents of fp32, and so has V: no
+// weight exceeds 1, or a product with V near the largest value would exceed fp32.
 template <int DT>
-constexpr float CK_LIFT = DT == AMASS_FP16 ? 7.f : 0.f;
+constexpr float CK_LIFT = DT == AMASS_FP16 ? 7.f : -CK_LAZY;
 
 // ------------------------------------------------------------------ the 16-bit types
 template <int DT>
@@ -509,7 +510,7 @@ __device__ __forceinline__ void mask_scores(f32x16_t (&s)[NK], int lo, int hi, u
 }
 
 // The running maximum after these scores, and the rescale of what was summed.  The maximum
-// may lag the true one by 2^CK_LAZY, which the weights (up to 2^8) and fp32 sums hold exactly
+// may lag the true one by 2^CK_LAZY, which the weights (of any size) and fp32 sums hold exactly
 // as well, so most tiles skip the rescale.
 __device__ __forceinline__ float row_max(const f32x16_t& s) {
     float mx = s[0];

@@ -205,3 +205,18 @@ def test_v_that_is_not_finite_loaded_past_the_caches(name):
     out[t, 8:12, 9] = torch.tensor(want[0][t, 8:12, 9], dtype=c.dt, device=DEV)
     c.want, c.v = lambda: want, finite              # (the tolerance goes by V's largest)
     c.check(out, lse)
+
+
+@pytest.mark.parametrize("new,lens", [([1], [300]), ([6], [5000]), ([100], [300]), ([300], [700])])
+def test_largest_values_of_v_under_a_maximum_that_lags(new, lens):
+    """A key whose weight is 2^7 times that of all keys before it, short of what moves the running
+    maximum, has V of 2^123: its product with a weight above 1 would exceed fp32."""
+    announce(f"chunk attention: V of 2^123, {new} of {lens}")
+    c = Case(new=new, lens=lens, n_kv=1)
+    c.q.zero_(), c.k.zero_(), c.v.zero_()
+    c.q[:, :, 0] = 1.0
+    block = int(c.table[0, 130 // 16])
+    c.k[block, 130 % 16, 0, 0] = 7.0 * math.log(2.0) / c.scale
+    c.v[block, 130 % 16, 0, 1::2] = 2.0 ** 123
+    c.v[block, 130 % 16, 0, 4::8] = -1.5 * 2.0 ** 123
+    c.check(*c.run())
