@@ -21,19 +21,20 @@
 // Two layouts, chosen per row tile (d = 128, bf16, 8 kv heads of 4 query heads unless stated):
 //   many (more than 32 rows): wave w owns rows 32 w .. 32 w + 31; the workgroup shares each
 //     64-key tile, double-buffered (2 x 32 KB at d = 128), one barrier per tile.  The matrix cores
-//     bound it: a prompt of 8192 tokens 517 us, 1.06 PFLOP/s (60 % of the matrix cores' cycles,
-//     6.7 vector instructions beside every product), 2048 tokens behind 63488
-//     1932 us, 1.12 PFLOP/s (66 %); a product of 8192^3 reaches 1.25 to 1.40 beside them.  A wave
-//     of 64 rows (O and Q in the accumulator half of the registers) took 549 and 2005 us.
+//     bound it: a prompt of 8192 tokens 536 us with both launches, 1.03 PFLOP/s (60 % of the matrix
+//     cores' cycles, 5.8 vector instructions beside every product), 2048 tokens behind 63488
+//     2007 us, 1.08 PFLOP/s (66 %), on a card whose product of 8192^3 reaches 1.24 to 1.39; 506 and
+//     1853 on the fastest met.  A wave of 64 rows (O and Q in the accumulator half of the registers)
+//     took 549 and 2005 us on one where this took 509 to 546 and 1869 to 2016.
 //   few (32 rows or less: single tokens, drafts, a chunk's remainder): the rows fit one wave,
 //     so the waves take 32 keys each in turn, each with a K and a V buffer of its own and no
 //     barrier, and merge their (m, l, O) through LDS at the end.  Memory bounds it: 8 requests of 4
-//     drafted tokens with 8k to 24k keys 104 us, 5.6 TB/s; 64 single tokens with 8k keys 330 us,
+//     drafted tokens with 8k to 24k keys 104 us, 5.6 TB/s; 64 single tokens with 8k keys 335 us,
 //     6.4 TB/s.  The many-row layout, three of four waves idle, takes 116 for the drafts.
 // Splitting.  A row tile of many keys is cut into S parts when the batch has fewer tiles
 // than the chip has room for (plan below, on the device: the launch needs no lengths on the
 // host and can be captured); parts leave (m, l, O) in scratch and a second launch joins them.
-// 5 drafted tokens behind 4096: 8.4 us of 16 parts and 3.2 us of joining.
+// 5 drafted tokens behind 4096: 9.8 us of 17 parts and 4.0 us of joining (medians; least 8.7 and 3.2).
 #include <atomic>
 #include <type_traits>
 
@@ -706,11 +707,12 @@ __device__ __forceinline__ bool needs_care(const RowState<D>& st, float c, bool 
     return __any(live && (far || !((z[0] + z[1]) + (z[2] + z[3]) == 0.f)));
 }
 
-// `weigh` with exponents from s - m, exact where s is near m, and for V that is not finite everywhere, where the weight zero of a key that a row does not
-// see would make NaN.  The products take zeros in place of what is not finite; then products of
-// the largest bf16 values (where a row sees a key that is not finite in the channel; zeros
-// elsewhere) make an infinity of V's sign of that row's channel, and of the opposite sign too, NaN
-// with the first, where V is NaN.  Rare, and written for few registers.
+// `weigh` with exponents from s - m, exact where s is near m, and for V that is not finite
+// everywhere, where the weight zero of a key that a row does not see would make NaN.  The products
+// take zeros in place of what is not finite; then products of the largest bf16 values (where a row
+// sees a key that is not finite in the channel; zeros elsewhere) make an infinity of V's sign of
+// that row's channel, and one of the opposite sign too, NaN with the first, where V is NaN.  Rare,
+// and written for few registers.
 template <int DT, int D, int NK>
 __device__ __forceinline__ void weigh_careful(uint32_t vs, const LdsLane<D>& ll,
                                               const f32x16_t (&s)[NK], float c, RowState<D>& st) {
@@ -1204,12 +1206,12 @@ chunk_kernel(const amass_chunk_args a, const ChunkPlan pl) {
 }
 
 // Joins the parts of cut row tiles, a d tile per workgroup (grid: cut tile x kv head, 32-row group, d
-// tile).  Bound by the latency of its loads: record, statistics and O, 3.3 us at 16 parts of one
-// tile, 6.2 us at 310 tiles of two or three parts (20 MB).  A wave issues the loads of
+// tile).  Bound by the latency of its loads: record, statistics and O, 4.0 us at 17 parts of one
+// tile, 6.6 us at 310 tiles of two parts (20 MB; medians).  A wave issues the loads of
 // CM_BATCH parts before it uses any.  Up to that many parts it joins a group alone, and one
 // workgroup takes all groups of the tile (a workgroup of waves with a part each, joining in LDS,
 // took 8.7 us there); beyond, wave w takes parts w, w + 4, ... of one group and the waves join
-// through LDS.  Batches without cut tiles leave a launch that reads the count, 4 us.
+// through LDS.  Batches without cut tiles leave a launch that reads the count, 4.8 us.
 constexpr int CM_WAVES = 4;
 constexpr int CM_BATCH = 4;
 
