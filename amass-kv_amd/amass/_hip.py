@@ -21,6 +21,7 @@ _F64 = C.c_double
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libamass_hip.so")
 ABI_VERSION = 11    # AMASS_ABI_VERSION of include/amass_hip.h these mirrors follow
 CHUNK_ABI_VERSION = 1    # AMASS_CHUNK_ABI_VERSION of include/amass_chunk.h
+QUANT_ABI_VERSION = 1    # AMASS_QUANT_ABI_VERSION of include/amass_quant.h
 
 
 class AmassError(RuntimeError):
@@ -168,6 +169,31 @@ class ChunkArgs(C.Structure):
         "n_kv:i32 G:i32 d:i32 page:i32 nb:i32 max_pages:i32 causal:i32 window:i32 dtype:i32")
 
 
+# include/amass_quant.h
+class QuantWriteArgs(C.Structure):
+    _fields_ = _fields(
+        "k:p k_st:i64 k_hs:i64 v:p v_st:i64 v_hs:i64 q:p q_st:i64 q_hs:i64 q_out:p qo_st:i64 "
+        "qo_hs:i64 k_codes:p v_codes:p c_sb:i64 c_st:i64 c_sh:i64 k_scale:p v_scale:p s_sb:i64 "
+        "s_sh:i64 table:p tab_st:i64 positions:p slots:p n_tokens:i32 n_heads:i32 n_kv:i32 d:i32 "
+        "rot:i32 page:i32 nb:i32 max_pos:i32 interleaved:i32 dtype:i32 code:i32")
+
+
+class QuantReadArgs(C.Structure):
+    _fields_ = _fields(
+        "k_codes:p v_codes:p c_sb:i64 c_st:i64 c_sh:i64 k_scale:p v_scale:p s_sb:i64 s_sh:i64 "
+        "k_cache:p v_cache:p o_sb:i64 o_st:i64 o_sh:i64 src:p dst:p n:i32 n_kv:i32 d:i32 page:i32 "
+        "nb:i32 nb_out:i32 dtype:i32 code:i32")
+
+
+class QuantChunkArgs(C.Structure):
+    _fields_ = _fields(
+        "q:p q_st:i64 q_hs:i64 k_codes:p v_codes:p c_sb:i64 c_st:i64 c_sh:i64 k_scale:p v_scale:p "
+        "s_sb:i64 s_sh:i64 block_table:p bt_st:i64 seq_lens:p query_start:p out:p o_st:i64 "
+        "o_hs:i64 lse:p l_st:i64 l_hs:i64 scratch:p scratch_bytes:i64 scale:f32 n_req:i32 "
+        "n_tokens:i32 n_kv:i32 G:i32 d:i32 page:i32 nb:i32 max_pages:i32 causal:i32 window:i32 "
+        "dtype:i32 code:i32")
+
+
 STRUCTS = {
     "amass_quad_score_args": (0, QuadScoreArgs),
     "amass_r8_score_args": (1, R8ScoreArgs),
@@ -193,6 +219,13 @@ CHUNK_STRUCTS = {
     "amass_chunk_args": (3, ChunkArgs),
 }
 
+# those of include/amass_quant.h (amass_quant_struct_size)
+QUANT_STRUCTS = {
+    "amass_quant_write_args": (0, QuantWriteArgs),
+    "amass_quant_read_args": (1, QuantReadArgs),
+    "amass_quant_chunk_args": (2, QuantChunkArgs),
+}
+
 # entry point -> argument struct (None = custom signature)
 ENTRY_POINTS = {
     "amass_quad_score": QuadScoreArgs,
@@ -216,6 +249,9 @@ ENTRY_POINTS = {
     "amass_release": ReleaseArgs,
     "amass_rope_write": RopeArgs,
     "amass_chunk_attention": ChunkArgs,
+    "amass_quant_write": QuantWriteArgs,
+    "amass_quant_read": QuantReadArgs,
+    "amass_quant_chunk_attention": QuantChunkArgs,
 }
 
 _CODES = {_P: "P", _I64: "q", _I32: "i", _F32: "f", _F64: "d"}
@@ -265,6 +301,14 @@ def _prototypes(lib) -> None:
     if lib.amass_chunk_abi_version() != CHUNK_ABI_VERSION:
         raise AmassError(f"{LIB_PATH} has chunk ABI version {lib.amass_chunk_abi_version()}, "
                          f"these bindings expect {CHUNK_ABI_VERSION}: rebuild it")
+    lib.amass_quant_scratch_bytes.argtypes = [C.POINTER(QuantChunkArgs)]
+    lib.amass_quant_scratch_bytes.restype = _I64
+    lib.amass_quant_abi_version.restype = C.c_int
+    lib.amass_quant_struct_size.argtypes = [C.c_int]
+    lib.amass_quant_struct_size.restype = C.c_size_t
+    if lib.amass_quant_abi_version() != QUANT_ABI_VERSION:
+        raise AmassError(f"{LIB_PATH} has quant ABI version {lib.amass_quant_abi_version()}, "
+                         f"these bindings expect {QUANT_ABI_VERSION}: rebuild it")
 
 
 def load_library(path: str = LIB_PATH) -> C.CDLL:

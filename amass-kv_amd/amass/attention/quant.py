@@ -1,0 +1,264 @@
+"""A paged cache in 8 bits: its quantising write, its attention and the way back to 16 bits
+(``amass_quant_write``, ``amass_quant_chunk_attention``, ``amass_quant_read``).
+
+  codes    (NB, 2, page, n_kv, d) or (2, NB, ...) int8 or float8_e4m3fn
+  scales   (NB, 2, n_kv) or (2, NB, n_kv) fp32, one for each block, half (K, V) and kv head
+
+A number is ``code * scale``.  Beside ``rope_paged_write`` and ``paged_chunk_attention`` it takes half the
+memory and half the bytes of every decode step.  int8 resolves a block's numbers in 254 even
+steps of its largest; e4m3 keeps 4 significant bits of each, for blocks of a few large numbers
+among small ones.
+
+A scale grows with its block: the write takes the largest magnitude of the tokens that enter the
+block now and of those that are there, and where the scale grows it rounds the earlier tokens' codes
+again.  The token in a block's first row starts the block anew.  Codes do not depend on how a
+prompt was cut into chunks where no scale grows, and differ by one step otherwise.
+
+All calls run on torch's current stream of the tensors' GPU, depend on shapes only, allocate
+nothing but the attention's scratch, never synchronise and can be captured in a HIP graph.
+"""
+from __future__ import annotations
+
+import torch
+
+from .._hip import (QuantChunkArgs, QuantReadArgs, QuantWriteArgs, cache_halves, call_on, check,
+                    device_index, load_library, packer, vector)
+from .rope import DTYPES, LAYOUTS
+
+HEAD_DIMS = (64, 128)
+CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}      # AMASS_INT8, AMASS_E4M3
+MIN_PAGE, MAX_PAGE = 16, 1024
+MAX_INT = 2 ** 31 - 1
+_pack_write = packer(QuantWriteArgs)
+_pack_read = packer(QuantReadArgs)
+_pack_chunk = packer(QuantChunkArgs)
+_SCRATCH = {}            # (GPU, requests, rows, kv heads, group, head dim) -> scratch bytes
+
+
+def quant_cache(num_blocks: int, page: int, n_kv: int, d: int, *, dtype=torch.int8,
+                device=None):
+    """(codes, scales) of a pool of ``num_blocks`` blocks, zeros with scales of one; ``dtype``
+    torch.int8 or torch.float8_e4m3fn."""
+    _geometry(page, d, dtype)
+    codes = torch.zeros(num_blocks, 2, page, n_kv, d, dtype=torch.int8, device=device).view(dtype)
+    return codes, torch.ones(num_blocks, 2, n_kv, dtype=torch.float32, device=device)
+
+
+def _geometry(page, d, dtype):
+    if dtype not in CODES:
+        raise ValueError(f"codes must be int8 or float8_e4m3fn, not {dtype}")
+    if d not in HEAD_DIMS:
+        raise ValueError(f"head dim {d} (built for {HEAD_DIMS})")
+    if page < MIN_PAGE or page > MAX_PAGE or page & (page - 1):
+        raise ValueError(f"page {page} must be a power of two from {MIN_PAGE} to {MAX_PAGE}")
+
+
+def _halves(codes, scales, writes):
+    """((blocks, page, n_kv, d), (k, v, block, row, head strides of codes), (k, v, block, head
+    strides of scales)) of a checked cache."""
+    shape, st = codes.shape, codes.stride()
+    if len(shape) != 5 or (shape[0] != 2 and shape[1] != 2):
+        raise ValueError("codes must be (NB, 2, page, n_kv, d) or (2, NB, page, n_kv, d)")
+    first = shape[0] == 2
+    nb, (page, n_kv, d) = shape[1] if first else shape[0], shape[2:]
+    _geometry(page, d, codes.dtype)
+    if scales.dtype is not torch.float32 or scales.shape != (shape[0], shape[1], n_kv):
+        raise ValueError(f"scales must be ({shape[0]}, {shape[1]}, {n_kv}) fp32")
+    sb, half = (st[1], st[0]) if first else (st[0], st[1])
+    s0, s1, s_sh = scales.stride()
+    s_sb, s_half = (s1, s0) if first else (s0, s1)
+    _, _, row, head, unit = st
+    if unit != 1:
+        raise ValueError("codes need unit stride on the head dim")
+    if writes and (not (sb or nb == 1) or not half or not row or not (head or n_kv == 1) or
+                   not (s_sb or nb == 1) or not s_half or not (s_sh or n_kv == 1)):
+        raise ValueError("rows of codes or scales share memory")
+    at, s_at = codes.data_ptr(), scales.data_ptr()
+    return ((nb, page, n_kv, d), (at, at + half, sb, row, head),
+            (s_at, s_at + 4 * s_half, s_sb, s_sh))
+
+
+def quant_paged_write(k, v, codes, scales, slots, *, q=None, positions=None, table=None,
+                      q_out=None, layout: str = "half") -> None:
+    """Quantise k and v (T, n_kv, d), bf16 or fp16, into their slots of the cache.
+
+    ``slots`` (T,) int64 from ``extend_block_tables``: the tokens of a block come as one run of
+    rows with ascending slots, and a row whose slot is outside the cache is passed over.  Two
+    runs of one call in one block leave a mixture there.  Numbers that are not finite make NaN of
+    their block, half and head (until its first row is written again).
+
+    With ``table`` (``rope_table``) and ``positions`` (T,) int32, k is turned by its position
+    first (``layout`` as ``rope_paged_write`` has it, rot a multiple of 16), in float64, rounded
+    to its type and then to a code; a row whose position is outside the table is passed over.
+    With ``q`` (T, H, d) too, q is turned into ``q_out`` (``None``: in place), as
+    ``rope_paged_write`` does.  k, v, q and codes need 16-byte aligned rows."""
+    if q is None and q_out is not None:
+        raise ValueError("q_out without q")
+    if (table is None) != (positions is None) or (q is not None and table is None):
+        raise ValueError("q needs positions and table, and each of those the other")
+    q_out = q if q_out is None else q_out
+    index = device_index(k, v, codes, scales, slots, q, positions, table, q_out)
+    dt = k.dtype
+    if not (dt in DTYPES and dt is v.dtype and (q is None or dt is q.dtype is q_out.dtype)):
+        raise ValueError("k, v, q and q_out must all be bf16 or all fp16")
+    if layout not in LAYOUTS:
+        raise ValueError(f"layout {layout!r}: 'half' or 'interleaved'")
+    (nb, page, n_kv, d), c, s = _halves(codes, scales, True)
+    T = k.shape[0]
+    if k.shape != (T, n_kv, d) or v.shape != k.shape:
+        raise ValueError(f"k and v must be (T, {n_kv}, {d})")
+    vector(slots, torch.int64, T, "slots")
+    k_st, k_hs, k_unit = k.stride()
+    v_st, v_hs, v_unit = v.stride()
+    q_at = q_st = q_hs = o_at = o_st = o_hs = H = 0
+    q_unit = o_unit = 1
+    if q is not None:
+        H = q.shape[1] if q.dim() == 3 else 0
+        if H == 0 or q.shape != (T, H, d) or q_out.shape != q.shape:
+            raise ValueError(f"q and q_out must be (T, H, {d})")
+        q_at, o_at = q.data_ptr(), q_out.data_ptr()
+        q_st, q_hs, q_unit = q.stride()
+        o_st, o_hs, o_unit = q_out.stride()
+        if not (o_st or T == 1) or not (o_hs or H == 1):
+            raise ValueError("rows or heads of q_out share memory")
+    if not k_unit == v_unit == q_unit == o_unit == 1:
+        raise ValueError("k / v / q / q_out need unit stride on the head dim")
+    tab_at = tab_st = pos_at = rot = max_pos = 0
+    if table is not None:
+        max_pos, rot = table.shape
+        tab_st, unit = table.stride()
+        if table.dtype is not torch.float32 or unit != 1 or rot % 16 or not 16 <= rot <= d:
+            raise ValueError(f"table must be (max_pos, rot) fp32, rot a multiple of 16 up to {d}")
+        vector(positions, torch.int32, T, "positions")
+        tab_at, pos_at = table.data_ptr(), positions.data_ptr()
+    if T == 0:
+        return
+    call_on(index, "amass_quant_write", _pack_write(       # in the struct's order
+        k.data_ptr(), k_st, k_hs, v.data_ptr(), v_st, v_hs, q_at, q_st, q_hs, o_at, o_st, o_hs,
+        *c, *s, tab_at, tab_st, pos_at, slots.data_ptr(), T, H, n_kv, d, rot, page, nb, max_pos,
+        LAYOUTS[layout], DTYPES[dt], CODES[codes.dtype]))
+
+
+def quant_paged_read(codes, scales, src, kv_cache, dst) -> None:
+    """Blocks ``src`` (n,) int32 of the 8-bit cache into blocks ``dst`` (n,) int32 of a bf16 or fp16
+    one with the same pages and heads, (2, NB, page, n_kv, d) or (NB, 2, ...): what the decode path,
+    the page summaries or ``paged_chunk_attention`` then read.  Pairs with a block outside its
+    cache are passed over; a block appears once in ``dst``."""
+    index = device_index(codes, scales, src, kv_cache, dst)
+    if kv_cache.dtype not in DTYPES:
+        raise ValueError("kv_cache must be bf16 or fp16")
+    (nb, page, n_kv, d), c, s = _halves(codes, scales, False)
+    (nb_out, *shape), k, v, (o_sb, o_st, o_sh, unit) = cache_halves(kv_cache)
+    if v == 0 or tuple(shape) != (page, n_kv, d):
+        raise ValueError(f"kv_cache must have V and pages of ({page}, {n_kv}, {d})")
+    if unit != 1 or not (o_sb or nb_out == 1) or not o_st or not (o_sh or n_kv == 1) or k == v:
+        raise ValueError("kv_cache needs unit stride on the head dim and rows of their own")
+    n = src.numel()
+    vector(src, torch.int32, n, "src")
+    vector(dst, torch.int32, n, "dst")
+    if dst.numel() != n:
+        raise ValueError(f"{n} blocks in src, {dst.numel()} in dst")
+    if n == 0 or nb == 0 or nb_out == 0:
+        return
+    call_on(index, "amass_quant_read", _pack_read(         # in the struct's order
+        *c, *s, k, v, o_sb, o_st, o_sh, src.data_ptr(), dst.data_ptr(), n, n_kv, d, page, nb,
+        nb_out, DTYPES[kv_cache.dtype], CODES[codes.dtype]))
+
+
+def _chunk_args(q, codes, scales, block_table, seq_lens, query_start, out, scale, causal, window,
+                lse):
+    """(the argument struct's values up to the scratch, those behind it) of a checked call."""
+    dt = q.dtype
+    if not (dt in DTYPES and dt is out.dtype):
+        raise ValueError("q and out must both be bf16 or both fp16")
+    (nb, page, n_kv, d), c, s = _halves(codes, scales, False)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != d or out.shape != shape:
+        raise ValueError(f"q and out must be (T, H, {d})")
+    T, H, _ = shape
+    if H == 0 or H % n_kv:
+        raise ValueError(f"{H} query heads are not a multiple of {n_kv} kv heads")
+    if window is not None and window < 1:
+        raise ValueError("window must be positive (None: no window)")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale <= 2e38:                 # (times log2 e it stays finite)
+        raise ValueError(f"scale {scale} must be positive and finite")
+    n_req = seq_lens.numel()
+    vector(seq_lens, torch.int32, n_req, "seq_lens")
+    vector(query_start, torch.int32, n_req + 1, "query_start")
+    rows, width = block_table.shape
+    bt_st, unit = block_table.stride()
+    if block_table.dtype is not torch.int32 or (unit != 1 and width > 1) or rows < n_req or \
+            width < 1:
+        raise ValueError("block_table must be (R, max_pages) int32 with unit column stride")
+    q_st, q_hs, q_unit = q.stride()
+    o_st, o_hs, o_unit = out.stride()
+    if not q_unit == o_unit == 1:
+        raise ValueError("q / out need unit stride on the head dim")
+    if not (o_st or T == 1) or not (o_hs or H == 1):
+        raise ValueError("rows or heads of out share memory")
+    l_at = l_st = l_hs = 0
+    if lse is not None:
+        if lse.dtype is not torch.float32 or lse.shape != (T, H):
+            raise ValueError("lse must be (T, H) fp32")
+        l_at = lse.data_ptr()
+        l_st, l_hs = lse.stride()
+        if not (l_st or T == 1) or not (l_hs or H == 1):
+            raise ValueError("rows or heads of lse share memory")
+    return ((q.data_ptr(), q_st, q_hs, *c, *s, block_table.data_ptr(), bt_st, seq_lens.data_ptr(),
+             query_start.data_ptr(), out.data_ptr(), o_st, o_hs, l_at, l_st, l_hs),
+            (scale, n_req, T, n_kv, H // n_kv, d, page, nb, width, 1 if causal else 0,
+             min(window or 0, MAX_INT), DTYPES[dt], CODES[codes.dtype]))
+
+
+def _scratch_bytes(index, head, tail) -> int:
+    key = (index, *tail[1:6])
+    n = _SCRATCH.get(key)
+    if n is None:
+        with torch.cuda.device(index):
+            n = load_library().amass_quant_scratch_bytes(_pack_chunk(*head, 0, 0, *tail))
+        if n < 0:
+            check(n, "amass_quant_scratch_bytes")
+        if len(_SCRATCH) >= 4096:
+            _SCRATCH.clear()
+        _SCRATCH[key] = n
+    return n
+
+
+def quant_scratch_bytes(q, codes, scales, block_table, seq_lens, query_start, out, *, scale=None,
+                        causal: bool = True, window=None, lse=None) -> int:
+    """Bytes of scratch that ``quant_chunk_attention`` takes for these shapes."""
+    index = device_index(q, codes, scales, block_table, seq_lens, query_start, out, lse)
+    return _scratch_bytes(index, *_chunk_args(q, codes, scales, block_table, seq_lens,
+                                              query_start, out, scale, causal, window, lse))
+
+
+def quant_chunk_attention(q, codes, scales, block_table, seq_lens, query_start, out, *,
+                          scale=None, causal: bool = True, window: int | None = None, lse=None,
+                          scratch=None) -> None:
+    """``paged_chunk_attention`` over the 8-bit cache: the rows of q (T, H, d), bf16 or fp16,
+    over their requests' keys and values, into out (which may be q).
+
+    Requests, visible positions, ``causal``, ``window``, ``scale``, ``lse`` and ``scratch`` as
+    there: row ``query_start[r] + i`` is one of the last tokens of request r's ``seq_lens[r]``,
+    whose K and V the cache holds already (``quant_paged_write``).  Rows that see nothing get zeros
+    (``lse``: -inf); rows of no request stay as they are.
+
+    Scales are positive, V's count as at least 2^-64 and those of one request and kv head lie within
+    2^80 of each other.  A scale that is not finite makes NaN of the rows that see its page, a NaN
+    code of those that see its key."""
+    index = device_index(q, codes, scales, block_table, seq_lens, query_start, out, lse, scratch)
+    head, tail = _chunk_args(q, codes, scales, block_table, seq_lens, query_start, out, scale,
+                             causal, window, lse)
+    need = _scratch_bytes(index, head, tail)
+    if scratch is None:
+        scratch = q.new_empty(need // 2)
+        size = need
+    else:
+        if scratch.dtype is not torch.uint8 or not scratch.is_contiguous():
+            raise ValueError("scratch must be a contiguous uint8 tensor")
+        size = scratch.numel()
+        if size < need:
+            raise ValueError(f"scratch of {size} bytes, {need} needed")
+    call_on(index, "amass_quant_chunk_attention",
+            _pack_chunk(*head, scratch.data_ptr(), size, *tail))

@@ -1,0 +1,361 @@
+// The paged cache in 8 bits for gfx950: the quantising write (amass_quant_write) and the reading back
+// (amass_quant_read).
+//
+// Mathematics.  Write: a run of tokens in a block has one scale per half and head, s = max(step(max
+// |x|), scale so far), and codes round(x / s).  K is turned in 64 bits first: a product of an
+// 8- or 11-bit number with an fp32 cosine is exact there and the difference rounded once, so that the 16-bit
+// key, and with it the code, is the formula's and not one of the two beside it.  The int8 scales have
+// 8 significant bits: then no quotient that is not half way between two codes lies nearer to it
+// than 2^-17, so the fp32 quotient rounds to the code of the exact one.
+//
+// One wave takes a run's numbers of one half and head (16 rows of 128: 32 a lane, in registers; a
+// longer run is read twice), so the maximum is a chain of v_max and six exchanges, and nothing waits for
+// another wave.  A workgroup belongs to a token and returns at once where no run starts, after
+// turning the token's queries.
+// Read: 16 codes a thread, two 16-byte stores.
+#include "quant_codes.h"
+
+namespace amass {
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+template <int DT>
+__device__ __forceinline__ float half_f32(uint32_t w, int hi) {
+    const uint32_t h = hi ? w >> 16 : w & 0xFFFFu;
+    return DT == AMASS_BF16 ? bf16_to_f32((uint16_t)h) : fp16_to_f32((uint16_t)h);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {       // to nearest even
+    if constexpr (DT == AMASS_BF16) return pack_bf16x2(lo, hi);
+    else return (uint32_t)__half_as_ushort(__float2half_rn(lo)) |
+                (uint32_t)__half_as_ushort(__float2half_rn(hi)) << 16;
+}
+
+// 16 channels of a head: 8 from c0 and 8 from c1
+struct Chan {
+    int c0, c1;
+    bool turn;
+};
+__device__ __forceinline__ Chan channels(const amass_quant_write_args& a, int u, bool may_turn) {
+    Chan c;
+    c.turn = may_turn && 16 * u < a.rot;
+    const bool apart = c.turn && !a.interleaved;
+    c.c0 = apart ? 8 * u : 16 * u;
+    c.c1 = apart ? (a.rot >> 1) + 8 * u : 16 * u + 8;
+    return c;
+}
+// the 8 pairs of x (c0 ..) and y (c1 ..) turned: pair i is (x[i], y[i]), or interleaved two
+// neighbours.  F: the type of the products.
+template <int DT, class F>
+__device__ __forceinline__ void turn(const amass_quant_write_args& a, const float* tab, u32x4_t& x,
+                                     u32x4_t& y) {
+    const int half = a.rot >> 1;
+    const auto pair = [&](float f, float g, int i, float& p, float& r) {
+        const F c = tab[i], s = tab[half + i];
+        p = (float)((F)f * c - (F)g * s);
+        r = (float)((F)g * c + (F)f * s);
+    };
+    if (a.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float p, r;
+            pair(half_f32<DT>(x[i], 0), half_f32<DT>(x[i], 1), i, p, r);
+            x[i] = pack_half<DT>(p, r);
+            pair(half_f32<DT>(y[i], 0), half_f32<DT>(y[i], 1), 4 + i, p, r);
+            y[i] = pack_half<DT>(p, r);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float p0, r0, p1, r1;
+            pair(half_f32<DT>(x[i], 0), half_f32<DT>(y[i], 0), 2 * i, p0, r0);
+            pair(half_f32<DT>(x[i], 1), half_f32<DT>(y[i], 1), 2 * i + 1, p1, r1);
+            x[i] = pack_half<DT>(p0, p1);
+            y[i] = pack_half<DT>(r0, r1);
+        }
+    }
+}
+
+constexpr int QW_THREADS = 256;
+constexpr int QW_ROWS = 16;              // rows that a wave holds
+
+template <int DT, int CT, int D>
+__global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_quant_write_args a, int sh) {
+    constexpr int LPR = D / 16, RPL = WAVE / LPR, N = QW_ROWS / RPL;   // lanes a row, rows a load, loads
+    const int t = blockIdx.x;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t end = (int64_t)a.nb << sh;
+    const auto has_pos = [&](int i) {
+        return !a.table || (uint32_t)a.positions[i] < (uint32_t)a.max_pos;
+    };
+    const auto enters = [&](int i) { return (uint64_t)a.slots[i] < (uint64_t)end && has_pos(i); };
+
+    if (a.q && has_pos(t)) {
+        const float* tab = a.table + (int64_t)a.positions[t] * a.tab_st;
+        for (int e = threadIdx.x; e < a.n_heads * LPR; e += QW_THREADS) {
+            const int head = e / LPR, u = e % LPR;
+            const Chan c = channels(a, u, true);
+            const uint16_t* src = (const uint16_t*)a.q + t * a.q_st + head * a.q_hs;
+            uint16_t* dst = (uint16_t*)a.q_out + t * a.qo_st + head * a.qo_hs;
+            u32x4_t x = *reinterpret_cast<const u32x4_t*>(src + c.c0);
+            u32x4_t y = *reinterpret_cast<const u32x4_t*>(src + c.c1);
+            if (c.turn) turn<DT, float>(a, tab + 8 * u, x, y);
+            *reinterpret_cast<u32x4_t*>(dst + c.c0) = x;
+            *reinterpret_cast<u32x4_t*>(dst + c.c1) = y;
+        }
+    }
+    // a run starts here: the token enters a block, and not behind its neighbour
+    if (!enters(t)) return;
+    const int64_t slot = a.slots[t];
+    const int first = (int)(slot & ((1 << sh) - 1));
+    if (first > 0 && t > 0 && a.slots[t - 1] == slot - 1 && has_pos(t - 1)) return;
+    const int64_t blk = slot >> sh;
+    const int most = min((1 << sh) - first, a.n_tokens - t);
+    int n = 0;
+    while (n < most) {
+        const int i = n + lane;
+        const unsigned long long in = __ballot(i < most && a.slots[t + i] == slot + i && has_pos(t + i));
+        if (~in) {
+            n += __ffsll((long long)~in) - 1;
+            break;
+        }
+        n += WAVE;
+    }
+    const int lr = lane / LPR, u = lane % LPR;
+    for (int unit = w; unit < 2 * a.n_kv; unit += QW_THREADS / WAVE) {
+        const bool is_k = unit < a.n_kv;
+        const int head = is_k ? unit : unit - a.n_kv;
+        const Chan c = channels(a, u, is_k && a.table);
+        const uint16_t* src = is_k ? (const uint16_t*)a.k + t * a.k_st + head * a.k_hs
+                                   : (const uint16_t*)a.v + t * a.v_st + head * a.v_hs;
+        const int64_t src_st = is_k ? a.k_st : a.v_st;
+        uint8_t* codes = (uint8_t*)(is_k ? a.k_codes : a.v_codes) + blk * a.c_sb + head * a.c_sh;
+        float* scale = (is_k ? a.k_scale : a.v_scale) + blk * a.s_sb + head * a.s_sh;
+        const float old = first > 0 ? *scale : 0.f;
+        u32x4_t x[N], y[N];
+        const auto load = [&](int r0) {                  // rows r0 .. r0 + 15 of the run
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int r = r0 + RPL * i + lr;
+                x[i] = y[i] = (u32x4_t){0u, 0u, 0u, 0u};
+                if (r < n) {
+                    x[i] = *reinterpret_cast<const u32x4_t*>(src + r * src_st + c.c0);
+                    y[i] = *reinterpret_cast<const u32x4_t*>(src + r * src_st + c.c1);
+                }
+            }
+            if (is_k && a.table) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int r = r0 + RPL * i + lr;
+                    if (r < n && c.turn)
+                        turn<DT, double>(a, a.table + (int64_t)a.positions[t + r] * a.tab_st + 8 * u, x[i], y[i]);
+                }
+            }
+        };
+        // the largest magnitude as 16 bits, NaN above infinity above every number
+        uint32_t top = 0;
+        for (int r0 = 0; r0 < n; r0 += QW_ROWS) {
+            load(r0);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t p = x[i][j] & 0x7FFF7FFFu, q = y[i][j] & 0x7FFF7FFFu;
+                    top = max(top, max(max(p & 0xFFFFu, p >> 16), max(q & 0xFFFFu, q >> 16)));
+                }
+        }
+        top = (uint32_t)wave_max_uniform((int)top);
+        const bool finite = top < (DT == AMASS_BF16 ? 0x7F80u : 0x7C00u);
+        float s = __builtin_nanf("");
+        if (finite) {
+            const float step = step_of<CT>(half_f32<DT>(top, 0));
+            s = step >= old ? step : old;                // (a NaN stays)
+        }
+        const float div = s < INFINITY ? s : 1.f, inv = 1.f / div, keep = s < INFINITY ? 1.f : 0.f;
+        for (int r0 = 0; r0 < n; r0 += QW_ROWS) {
+            if (n > QW_ROWS) load(r0);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int r = r0 + RPL * i + lr;
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t p = j < 2 ? x[i][2 * j] : y[i][2 * j - 4];
+                    const uint32_t q = j < 2 ? x[i][2 * j + 1] : y[i][2 * j - 3];
+                    o[j] = to_codes<CT>(quotient(half_f32<DT>(p, 0), div, inv), quotient(half_f32<DT>(p, 1), div, inv),
+                                        quotient(half_f32<DT>(q, 0), div, inv), quotient(half_f32<DT>(q, 1), div, inv));
+                    if (keep == 0.f) o[j] = 0u;
+                }
+                if (r < n) {
+                    uint8_t* to = codes + (first + r) * a.c_st;
+                    *reinterpret_cast<u32x2_t*>(to + c.c0) = (u32x2_t){o[0], o[1]};
+                    *reinterpret_cast<u32x2_t*>(to + c.c1) = (u32x2_t){o[2], o[3]};
+                }
+            }
+        }
+        if (first > 0 && s > old) {                      // the rows before the run, by the new scale
+            for (int r = lr; r < first; r += RPL) {
+                u32x4_t* at = reinterpret_cast<u32x4_t*>(codes + r * a.c_st + 16 * u);
+                u32x4_t z = *at;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 f = codes_f32<CT>(z[j]);
+                    z[j] = to_codes<CT>(quotient(f.x * old, div, inv), quotient(f.y * old, div, inv),
+                                        quotient(f.z * old, div, inv), quotient(f.w * old, div, inv));
+                }
+                *at = z;
+            }
+        }
+        if (lane == 0) *scale = s;
+    }
+}
+
+// grid (entry, half and 1024 units of 16 codes of the block)
+constexpr int QR_THREADS = 256;
+constexpr int QR_UNITS = 4;              // of a thread
+
+template <int DT, int CT, int D>
+__global__ __launch_bounds__(QR_THREADS) void quant_read_kernel(const amass_quant_read_args a, int sh) {
+    constexpr int LPR = D / 16;
+    const int src = a.src[blockIdx.x], dst = a.dst[blockIdx.x];
+    if ((uint32_t)src >= (uint32_t)a.nb || (uint32_t)dst >= (uint32_t)a.nb_out) return;
+    const bool is_k = !(blockIdx.y & 1);
+    const uint8_t* codes = (const uint8_t*)(is_k ? a.k_codes : a.v_codes) + src * a.c_sb;
+    const float* scale = (is_k ? a.k_scale : a.v_scale) + src * a.s_sb;
+    uint16_t* out = (uint16_t*)(is_k ? a.k_cache : a.v_cache) + dst * a.o_sb;
+    const int units = (a.n_kv << sh) * LPR;
+    int e = (blockIdx.y >> 1) * (QR_UNITS * QR_THREADS) + threadIdx.x;
+    u32x4_t z[QR_UNITS];
+    float s[QR_UNITS];
+    uint16_t* to[QR_UNITS];
+#pragma unroll
+    for (int i = 0; i < QR_UNITS; ++i, e += QR_THREADS) {
+        to[i] = nullptr;
+        if (e < units) {
+            const int rh = e / LPR, c = 16 * (e % LPR), row = rh / a.n_kv, head = rh - row * a.n_kv;
+            z[i] = *reinterpret_cast<const u32x4_t*>(codes + row * a.c_st + head * a.c_sh + c);
+            s[i] = scale[head * a.s_sh];
+            to[i] = out + row * a.o_st + head * a.o_sh + c;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < QR_UNITS; ++i) {
+        if (!to[i]) continue;
+        u32x4_t o[2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float4 f = codes_f32<CT>(z[i][j]);
+            o[j >> 1][2 * (j & 1)] = pack_half<DT>(f.x * s[i], f.y * s[i]);
+            o[j >> 1][2 * (j & 1) + 1] = pack_half<DT>(f.z * s[i], f.w * s[i]);
+        }
+        reinterpret_cast<u32x4_t*>(to[i])[0] = o[0];
+        reinterpret_cast<u32x4_t*>(to[i])[1] = o[1];
+    }
+}
+
+// ------------------------------------------------------------------ host
+static bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
+static int log2_of(int page) {
+    int sh = 0;
+    while ((1 << sh) < page) ++sh;
+    return sh;
+}
+static int check_kind(int d, int page, int dtype, int code) {
+    if ((dtype != AMASS_BF16 && dtype != AMASS_FP16) || (code != AMASS_INT8 && code != AMASS_E4M3) ||
+        (d != 64 && d != 128))
+        return AMASS_ERR_UNSUPPORTED;
+    return page < 16 || page > 1024 || (page & (page - 1)) ? AMASS_ERR_GEOMETRY : AMASS_OK;
+}
+
+static int check_write(const amass_quant_write_args& a) {
+    if (!a.k || !a.v || !a.k_codes || !a.v_codes || !a.k_scale || !a.v_scale || !a.slots ||
+        (a.q && (!a.q_out || !a.table)) || (a.table && !a.positions))
+        return AMASS_ERR_NULL;
+    const int rc = check_kind(a.d, a.page, a.dtype, a.code);
+    if (rc) return rc;
+    if (a.n_tokens < 0 || a.n_kv < 1 || a.n_kv > 4096 || a.nb < 1) return AMASS_ERR_GEOMETRY;
+    if (misaligned(a.k) || misaligned(a.v) || misaligned(a.k_codes) || misaligned(a.v_codes) ||
+        ((a.k_st | a.k_hs | a.v_st | a.v_hs) & 7) || ((a.c_sb | a.c_st | a.c_sh) & 15))
+        return AMASS_ERR_GEOMETRY;
+    if (a.table && (a.rot < 16 || (a.rot & 15) || a.rot > a.d || a.max_pos < 1 || misaligned(a.table) ||
+                    (a.tab_st & 3)))
+        return AMASS_ERR_GEOMETRY;
+    if (a.q && (a.n_heads < 1 || a.n_heads > (1 << 16) || misaligned(a.q) || misaligned(a.q_out) ||
+                ((a.q_st | a.q_hs | a.qo_st | a.qo_hs) & 7)))
+        return AMASS_ERR_GEOMETRY;
+    return (int64_t)a.n_tokens * QW_THREADS > 0xFFFFFFFFll ? AMASS_ERR_GEOMETRY : AMASS_OK;
+}
+static int check_read(const amass_quant_read_args& a) {
+    if (!a.k_codes || !a.v_codes || !a.k_scale || !a.v_scale || !a.k_cache || !a.v_cache || !a.src || !a.dst)
+        return AMASS_ERR_NULL;
+    const int rc = check_kind(a.d, a.page, a.dtype, a.code);
+    if (rc) return rc;
+    if (a.n < 0 || a.n_kv < 1 || a.n_kv > 4096 || a.nb < 1 || a.nb_out < 1) return AMASS_ERR_GEOMETRY;
+    if (misaligned(a.k_codes) || misaligned(a.v_codes) || misaligned(a.k_cache) || misaligned(a.v_cache) ||
+        ((a.c_sb | a.c_st | a.c_sh) & 15) || ((a.o_sb | a.o_st | a.o_sh) & 7))
+        return AMASS_ERR_GEOMETRY;
+    return AMASS_OK;
+}
+
+template <int DT, int CT>
+static int launch_write(const amass_quant_write_args& a, hipStream_t s) {
+    const int sh = log2_of(a.page);
+    if (a.d == 128)
+        hipLaunchKernelGGL((quant_write_kernel<DT, CT, 128>), dim3(a.n_tokens), dim3(QW_THREADS), 0, s, a, sh);
+    else
+        hipLaunchKernelGGL((quant_write_kernel<DT, CT, 64>), dim3(a.n_tokens), dim3(QW_THREADS), 0, s, a, sh);
+    return check_launch();
+}
+template <int DT, int CT>
+static int launch_read(const amass_quant_read_args& a, hipStream_t s) {
+    const int sh = log2_of(a.page);
+    const int64_t units = (int64_t)a.n_kv * a.page * (a.d / 16), of_wg = QR_UNITS * QR_THREADS;
+    const int64_t parts = 2 * ((units + of_wg - 1) / of_wg);
+    if (parts > 65535 || (int64_t)a.n * QR_THREADS > 0xFFFFFFFFll) return AMASS_ERR_GEOMETRY;
+    const dim3 grid(a.n, (unsigned)parts);
+    if (a.d == 128)
+        hipLaunchKernelGGL((quant_read_kernel<DT, CT, 128>), grid, dim3(QR_THREADS), 0, s, a, sh);
+    else
+        hipLaunchKernelGGL((quant_read_kernel<DT, CT, 64>), grid, dim3(QR_THREADS), 0, s, a, sh);
+    return check_launch();
+}
+
+}  // namespace amass
+
+using namespace amass;
+
+extern "C" int amass_quant_write(const amass_quant_write_args* ain, void* stream) {
+    if (!ain) return AMASS_ERR_NULL;
+    const amass_quant_write_args& a = *ain;
+    if (a.n_tokens == 0) return AMASS_OK;
+    const int rc = check_write(a);
+    if (rc) return rc;
+    hipStream_t s = (hipStream_t)stream;
+    if (a.dtype == AMASS_BF16)
+        return a.code == AMASS_INT8 ? launch_write<0, 0>(a, s) : launch_write<0, 1>(a, s);
+    return a.code == AMASS_INT8 ? launch_write<1, 0>(a, s) : launch_write<1, 1>(a, s);
+}
+
+extern "C" int amass_quant_read(const amass_quant_read_args* ain, void* stream) {
+    if (!ain) return AMASS_ERR_NULL;
+    const amass_quant_read_args& a = *ain;
+    if (a.n == 0) return AMASS_OK;
+    const int rc = check_read(a);
+    if (rc) return rc;
+    hipStream_t s = (hipStream_t)stream;
+    if (a.dtype == AMASS_BF16)
+        return a.code == AMASS_INT8 ? launch_read<0, 0>(a, s) : launch_read<0, 1>(a, s);
+    return a.code == AMASS_INT8 ? launch_read<1, 0>(a, s) : launch_read<1, 1>(a, s);
+}
+
+extern "C" int amass_quant_abi_version(void) { return AMASS_QUANT_ABI_VERSION; }
+
+extern "C" size_t amass_quant_struct_size(int which) {
+    switch (which) {
+        case 0: return sizeof(amass_quant_write_args);
+        case 1: return sizeof(amass_quant_read_args);
+        case 2: return sizeof(amass_quant_chunk_args);
+        default: return 0;
+    }
+}

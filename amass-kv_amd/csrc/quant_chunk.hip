@@ -1,0 +1,688 @@
+// Attention of a chunk of new tokens over a paged cache in 8 bits for gfx950
+// (amass_quant_chunk_attention).
+//
+// Mathematics.  That of chunk.hip with k_j = c_j sk and v_j = c'_j sv, where sk and sv belong to a page (16
+// keys or a multiple).  Codes are exact in 16 bits, so the matrix products take them as they are,
+// and the scales enter where a lane holds one row's scores of 16 keys of one page:
+//   x_j = (scale log2 e sk) (q . c_j) + log2 sv       one fma, as without scales
+//   w_j = 2^(x_j - M), M the running maximum of x     the weight with V's scale, rounded once
+//   O  += w_j c'_j,  l += (sum of the 16 w_j) / sv    V's scale leaves the sum again, per 16 keys
+//   out = O / l,  lse = ln 2 (M + log2 l)
+// So a page costs a few instructions per 16 keys and nothing per key.
+#include "chunk_core.h"
+#include "quant_codes.h"
+
+namespace amass {
+
+// Sums are 2^QC_UP times those of the weights: with bf16's lift, 1 / sv of the largest scale would
+// leave fp32's normal numbers.
+constexpr int QC_UP = 16;
+
+// As CK_ONCE of chunk.hip: more bytes of codes than this are loaded past the caches, where one row tile
+// alone reads them.
+constexpr float QC_ONCE = 128e6f;
+
+struct Scales {
+    const float *k, *v;
+    int64_t sb, sh;
+};
+
+// The pages of a wave's next 64 groups of 16 keys, one a lane, PER of them a step (a tile of 64
+// keys, or a wave's 32): looked up once in 64 / PER steps, a period ahead, so that no step waits for
+// a table entry or a scale.
+template <int PER>
+struct Lookup {
+    static constexpr int STEPS = WAVE / PER;
+    const int32_t* table;          // the request's row
+    const float *ks, *vs;          // of the kv head
+    int64_t sb;
+    int sh, nb, last;              // last: the last position that counts
+    int t, jump;                   // this lane's first position; positions of a period
+    float c;
+    int id, next_id;               // -1: no block
+    float sk, off, inv;            // scale log2 e sk, log2 sv, 2^QC_UP / sv
+    float next_k, next_v;
+    unsigned long long has;
+
+    __device__ __forceinline__ int find(int at) const {
+        const int e = table[max(min(at, last), 0) >> sh];
+        return at <= last && (uint32_t)e < (uint32_t)nb ? e : -1;
+    }
+    __device__ __forceinline__ void fetch(int e, float& k, float& v) const {
+        k = v = 1.f;
+        if (e >= 0) {
+            k = ks[e * sb];
+            v = vs[e * sb];
+        }
+    }
+    __device__ __forceinline__ void take(int e, float k, float v) {
+        id = e;
+        has = __ballot(e >= 0);
+        sk = k < INFINITY ? k * c : __builtin_nanf("");
+        if (v < LEAST_SCALE) v = LEAST_SCALE;
+        off = __log2f(v);
+        inv = (float)(1 << QC_UP) / v;
+    }
+    // first: this lane's first position
+    __device__ __forceinline__ void start(int first, int period) {
+        t = first;
+        jump = period;
+        float k, v;
+        const int e = find(t);
+        fetch(e, k, v);
+        take(e, k, v);
+        next_id = find(t + jump);
+    }
+    // before step s of a period
+    __device__ __forceinline__ void ahead(int s) {
+        if (s == STEPS / 2) fetch(next_id, next_k, next_v);
+    }
+    // behind its last step
+    __device__ __forceinline__ void turn() {
+        take(next_id, next_k, next_v);
+        t += jump;
+        next_id = find(t + jump);
+    }
+    // block of group g of step s (of the next period from STEPS on)
+    __device__ __forceinline__ int block(int s, int g) const {
+        return s < STEPS ? __builtin_amdgcn_readlane(id, PER * s + g)
+                         : __builtin_amdgcn_readlane(next_id, PER * (s - STEPS) + g);
+    }
+    __device__ __forceinline__ uint32_t groups(int s) const {
+        return (uint32_t)(has >> (PER * s)) & ((1u << PER) - 1);
+    }
+};
+
+// ------------------------------------------------------------------ staging
+// 16 rows of codes of a page, 16 channels of a row in each of a lane's LOADS registers of 16 bytes.  Rows go
+// to lanes so that 16 neighbouring lanes, whose chunks of 16 bytes a phase of an LDS write takes, hold
+// two rows (d 64: four) with different swizzles and fill all banks once.
+template <int D>
+struct Codes {
+    static constexpr int LPR = D / 16, RPL = WAVE / LPR, LOADS = 16 / RPL;
+    uint32_t off, st;              // of the lane's first 16 bytes in a page; bytes between rows
+    uint32_t lds;                  // its first chunk in the image
+    int row;
+
+    __device__ __forceinline__ Codes(uint32_t st_, int lane) : st(st_) {
+        const int r = lane / LPR, c = lane % LPR;
+        row = D == 128 ? (r >> 1) + 4 * (r & 1)
+                       : (r & 1) + 4 * ((r >> 1) & 1) + 2 * ((r >> 2) & 1) + 8 * (r >> 3);
+        off = (uint32_t)row * st + 16 * c;
+        lds = row * (2 * D) + (((2 * c) ^ swz<D>(row)) << 4);
+    }
+    __device__ __forceinline__ void load(u32x4_t* z, const uint8_t* page, bool once) const {
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) {
+            const u32x4_t* p = reinterpret_cast<const u32x4_t*>(page + off + n * RPL * st);
+            z[n] = once ? __builtin_nontemporal_load(p) : *p;
+        }
+    }
+    // register n, widened, to the image of its 16 rows at `to` (row + 8 turns the chunk's second bit)
+    template <int DT, int CT>
+    __device__ __forceinline__ void put(uint32_t to, int n, const u32x4_t& z) const {
+        typedef __attribute__((address_space(3))) u32x4_t* lds_t;
+        u32x4_t a, b;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            uint32_t lo, hi;
+            widen4<DT, CT>(z[j], lo, hi);
+            a[2 * j] = lo;
+            a[2 * j + 1] = hi;
+            widen4<DT, CT>(z[2 + j], lo, hi);
+            b[2 * j] = lo;
+            b[2 * j + 1] = hi;
+        }
+        const uint32_t at = ((to + lds) ^ (uint32_t)(32 * n)) + n * RPL * (2 * D);
+        *(lds_t)(uintptr_t)at = a;
+        *(lds_t)(uintptr_t)(at ^ 16u) = b;
+    }
+    // V's register n without the rows from `rows` on (what lies behind the last token may be a NaN, and the
+    // weight zero times that is one)
+    __device__ __forceinline__ void clip(u32x4_t& z, int n, int rows) const {
+        if (row + n * RPL >= rows) z = (u32x4_t){0u, 0u, 0u, 0u};
+    }
+    // a key whose V holds a NaN: its K becomes NaN instead, so that the rows that see it, and no others,
+    // become NaN
+    __device__ __forceinline__ void poison(u32x4_t& k, u32x4_t& v) const {
+        int bad = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad |= (int)(((v[j] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u);
+        if constexpr (LPR == 8) bad |= dpp_i<DPP_HALF_MIRROR>(bad);
+        bad |= dpp_i<DPP_XOR2>(bad);
+        bad |= dpp_i<DPP_XOR1>(bad);
+        if (bad) {
+            k = (u32x4_t){0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu};
+            v = (u32x4_t){0u, 0u, 0u, 0u};
+        }
+    }
+};
+
+// ------------------------------------------------------------------ a tile
+template <int N>
+struct Factors {                   // of N groups of 16 keys
+    float sk[N], off[N], inv[N];
+    template <int PER>
+    __device__ __forceinline__ Factors(const Lookup<PER>& lk, int s) {
+#pragma unroll
+        for (int g = 0; g < N; ++g) {
+            sk[g] = readlane_f(lk.sk, PER * s + g);
+            off[g] = readlane_f(lk.off, PER * s + g);
+            inv[g] = readlane_f(lk.inv, PER * s + g);
+        }
+    }
+};
+
+__device__ __forceinline__ float group_max(const f32x16_t& s, int half) {
+    float mx = s[8 * half];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[8 * half + i]);
+    return mx;
+}
+// the running maximum and sum for a higher maximum; the factor for O
+template <int D>
+__device__ __forceinline__ float lift_max(float mx, RowState<D>& st) {
+    const float m = fmaxf(st.m, mx);
+    const float al = __builtin_amdgcn_exp2f(st.m - m);
+    st.m = m;
+    st.l *= al;
+    return al;
+}
+
+// The weights of 32 NK keys, packed for the second product, and what they add to the maximum and the
+// sum.  MASKS: the row sees the keys [lo, hi) of the tile, in the groups whose bits are set.  CARE:
+// for factors that are not finite, which must not reach what a row does not see, and for
+// maxima far from zero: the difference from them first, exact where it matters.
+template <int DT, int D, int NK, bool MASKS, bool CARE>
+__device__ __forceinline__ void weigh_tile(f32x16_t (&s)[NK], const Factors<2 * NK>& f, RowState<D>& st,
+                                           u32x4_t (&p)[2 * NK], int lo, int hi, uint32_t groups,
+                                           int lane) {
+    if constexpr (MASKS) {
+        const int h4 = 4 * (lane >> 5);
+#pragma unroll
+        for (int x = 0; x < NK; ++x)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = 32 * x + 8 * (i >> 2) + (i & 3) + h4;
+                const bool see = key >= lo && key < hi && (groups >> (2 * x + (i >> 3)) & 1);
+                s[x][i] = see ? s[x][i] : -INFINITY;
+            }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 2 * NK; ++g) {
+        const float gm = group_max(s[g >> 1], g & 1);
+        const float x = __builtin_fmaf(gm, f.sk[g], f.off[g]);
+        mx = fmaxf(mx, CARE && gm == -INFINITY ? -INFINITY : x);
+    }
+    mx = xor32_maxf(mx);
+    float al = 1.f;
+    const bool lag = __any(mx - st.m > CK_LAZY);
+    if (lag) al = lift_max(mx, st);
+    scale_o(st, al);
+    const float base = CK_LIFT<DT> - st.m;
+#pragma unroll
+    for (int g = 0; g < 2 * NK; ++g) {
+        const float off = f.off[g] + base;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            float e[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float sc = s[g >> 1][8 * (g & 1) + i + j];
+                float x = __builtin_fmaf(sc, f.sk[g], CARE ? -st.m : off);
+                if constexpr (CARE) {
+                    x += f.off[g] + CK_LIFT<DT>;
+                    x = x > CK_LIFT<DT> + CK_LAZY ? CK_LIFT<DT> + CK_LAZY : x;
+                    x = sc == -INFINITY ? -INFINITY : x;
+                }
+                e[j] = __builtin_amdgcn_exp2f(x);
+                sum += e[j];
+            }
+            p[g][i >> 1] = pack2<DT>(e[0], e[1]);
+        }
+        if (!CARE || sum != 0.f) st.l = __builtin_fmaf(sum, f.inv[g], st.l);
+    }
+}
+
+template <int DT, int D, int NK>
+__device__ __forceinline__ void add_values(uint32_t vs, const LdsLane<D>& ll, const u32x4_t (&p)[2 * NK],
+                                           RowState<D>& st) {
+#pragma unroll
+    for (int y = 0; y < 2 * NK; ++y)
+#pragma unroll
+        for (int z = 0; z < D / 32; ++z) st.o[z] = mfma32<DT>(ll.v_frag(vs, z, y), p[y], st.o[z]);
+}
+
+// whether a row that is there needs all of it again with care: it is not finite, or its maximum so far
+// from zero that log2 sv less the maximum, rounded, moves the weights of one page against
+// another's (by 2^-12 at 2^12, and in fp16 beyond its largest at 2^27)
+constexpr float QC_FAR = 0x1p12f;
+template <int D>
+__device__ __forceinline__ bool needs_care(const RowState<D>& st, bool live) {
+    const bool far = st.m > -__FLT_MAX__ && fabsf(st.m) > QC_FAR;
+    float z[4] = {st.l * 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z[i & 3] = __builtin_fmaf(st.o[x][i], 0.f, z[i & 3]);
+    return __any(live && (far || !((z[0] + z[1]) + (z[2] + z[3]) == 0.f)));
+}
+
+// ------------------------------------------------------------------ results
+// A wave's own rows (`group` of 32 of the row tile): normalised, or as a part.
+template <int DT, int D, int UP>
+__device__ __forceinline__ void finish_rows(const amass_chunk_args& a, const ChunkPlan& pl,
+                                            const Item& it, int kh, const RowState<D>& st, float c,
+                                            int row, int group, bool whole, int lane) {
+    const float l = st.l + xor32_f(st.l);
+    const RowOut ro = row_out(a, pl, it.q, kh, row);
+    const float inv = row_scale<UP>(l);
+    float* g = whole ? nullptr : slot_group<D>(a, pl, kh, it.slot, group);
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) {
+        float o[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = st.o[x][i] * (whole ? inv : 1.f);
+        if (whole) store_row<DT, D>(ro.out, x, o, lane);
+        else save_tile<D>(g, x, o, lane);
+    }
+    if (whole) store_lse<DT, UP>(ro, st.m, l, c, lane);
+    else save_stats<D>(g, st.m, l, lane);
+}
+
+// The rows that all waves share: their (m, l, O) through LDS, wave w takes d tile w of all of them.
+// (The waves are past their last use of lds.kv.)
+template <int DT, int D, int UP, class Lds>
+__device__ __forceinline__ void finish_shared(const amass_chunk_args& a, const ChunkPlan& pl,
+                                              const Item& it, int kh, const RowState<D>& st, Lds& lds,
+                                              float c, int row, bool whole, int w, int lane) {
+    lds.m[w][lane] = st.m;
+    lds.l[w][lane] = st.l + xor32_f(st.l);
+    float* of = reinterpret_cast<float*>(lds.kv) + w * (32 * D);
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) {
+        float o[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = st.o[x][i];
+        save_tile<D>(of, x, o, lane);
+    }
+    __syncthreads();
+    float m = -__FLT_MAX__, l = 0.f, wt[CK_WAVES];
+#pragma unroll
+    for (int v = 0; v < CK_WAVES; ++v) m = fmaxf(m, lds.m[v][lane]);
+#pragma unroll
+    for (int v = 0; v < CK_WAVES; ++v) {
+        // (a wave without a finite score has l = 0 and O = 0)
+        wt[v] = __builtin_amdgcn_exp2f((lds.m[v][lane] - m) * c);
+        l += lds.l[v][lane] * wt[v];
+    }
+    if (w >= D / 32) return;
+    float o[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int v = 0; v < CK_WAVES; ++v) {
+            const float4 y = *reinterpret_cast<const float4*>(
+                reinterpret_cast<float*>(lds.kv) + v * (32 * D) + (w * 4 + i) * 4 * WAVE + 4 * lane);
+            z.x += y.x * wt[v];
+            z.y += y.y * wt[v];
+            z.z += y.z * wt[v];
+            z.w += y.w * wt[v];
+        }
+        o[4 * i] = z.x;
+        o[4 * i + 1] = z.y;
+        o[4 * i + 2] = z.z;
+        o[4 * i + 3] = z.w;
+    }
+    if (whole) {
+        const RowOut ro = row_out(a, pl, it.q, kh, row);
+        const float inv = row_scale<UP>(l);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] *= inv;
+        store_row<DT, D>(ro.out, w, o, lane);
+        if (w == 0) store_lse<DT, UP>(ro, m, l, c, lane);
+    } else {
+        float* g = slot_group<D>(a, pl, kh, it.slot, 0);
+        save_tile<D>(g, w, o, lane);
+        if (w == 0) save_stats<D>(g, m, l, lane);
+    }
+}
+
+template <int D>
+struct __align__(1024) QuantLds {
+    char kv[2 * 2 * CK_KEYS * 2 * D];              // widened tiles, then the waves' O
+    float m[CK_WAVES][WAVE], l[CK_WAVES][WAVE];
+    int bad[CK_WAVES];
+};
+
+// ------------------------------------------------------------------ kernel
+// grid: as chunk_kernel.
+template <int DT, int CT, int D>
+__global__ __launch_bounds__(CK_WAVES * WAVE)
+__attribute__((amdgpu_waves_per_eu(ck_wgs(D), ck_wgs(D)))) void
+quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl) {
+    __shared__ QuantLds<D> lds;
+    constexpr int KB = CK_KEYS * 2 * D;            // bytes of a widened K (or V) tile
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kh = blockIdx.x % a.n_kv;
+    Item it;
+    float keys;
+    {
+        Held* held = reinterpret_cast<Held*>(lds.kv);
+        const int n_held = a.n_req > WAVE ? min(a.n_req, (int)(sizeof(lds.kv) / sizeof(Held))) : 0;
+        for (int r = threadIdx.x; r < n_held; r += CK_WAVES * WAVE) held[r] = held_req(a, pl, r);
+        if (n_held > 0) __syncthreads();
+        const Parts p = plan_parts(a, pl, held, n_held);
+        if (blockIdx.x == 0 && w == 0) {
+            const int cuts = p.fits ? count_cut(a, pl, p) : 0;
+            if (lane == 0) *(int*)a.scratch = cuts;
+        }
+        keys = p.keys;
+        if (!p.fits || !find_item(a, pl, p, blockIdx.x / a.n_kv, it)) return;
+        if (n_held > 0) __syncthreads();           // (before the keys take its place)
+    }
+    const Span sp = tile_span(a, pl, it.q, it.tile);
+    const int per = part_len(sp.n, it.parts);
+    const int j0 = min(sp.n, it.part * per), j1 = min(sp.n, j0 + per);   // tiles of this part
+    if (it.part > 0 && j0 >= j1) return;
+    const bool whole = per >= sp.n;                // no other part has keys
+    if (it.parts > 1 && it.part == 0 && kh == 0 && threadIdx.x == 0)
+        *cut_tile(a, it.cut) = {it.r, it.tile, (sp.n + per - 1) / per, it.slot, it.q, 0};
+    const int rows = min(CK_BM, it.q.n * a.G - it.tile * CK_BM);
+    const bool few = rows <= CK_FEW;
+    const bool once = it.q.n * a.G <= CK_BM &&
+                      __builtin_amdgcn_readfirstlane(keys * (float)KB * (float)a.n_kv > QC_ONCE);
+    const int group = few ? 0 : w;                 // 32-row group of this wave
+    const int row = it.tile * CK_BM + 32 * group + (lane & 31);
+    const int last = it.tile * CK_BM + min(rows, 32 * group + 32) - 1;    // of the wave
+    const int start = it.q.len - it.q.n;
+    const int len = min(it.q.len, pl.cap);
+    // this lane's visible keys; the wave's rows see at least [lo_hi, hi_lo), at most [lo_lo, hi_hi)
+    const bool live = row < it.q.n * a.G;
+    const int tok = div_g(pl, row);
+    const int pos = start + tok;
+    const int hi = live ? key_hi(a, pl, it.q.len, pos) : 0, lo = live ? key_lo(a, pos) : 0;
+    const int first = it.tile * CK_BM + 32 * group;
+    const bool idle = first > last;
+    const int p_first = start + div_g(pl, first), p_last = start + div_g(pl, last);
+    const int hi_lo = key_hi(a, pl, it.q.len, p_first), hi_hi = key_hi(a, pl, it.q.len, p_last);
+    const int lo_lo = key_lo(a, p_first), lo_hi = key_lo(a, p_last);
+
+    u32x4_t q[D / 16];
+    {
+        const uint16_t* src = (const uint16_t*)a.q + (int64_t)(it.q.q0 + tok) * a.q_st +
+                              (int64_t)(kh * a.G + (row - tok * a.G)) * a.q_hs + 8 * (lane >> 5);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+            q[i] = live ? *reinterpret_cast<const u32x4_t*>(src + 16 * i) : (u32x4_t){0u, 0u, 0u, 0u};
+    }
+    const LdsLane<D> ll(lane);
+    const Codes<D> cd((uint32_t)a.kv_st, lane);
+    constexpr int LOADS = Codes<D>::LOADS;
+    const uint8_t* k0 = (const uint8_t*)a.k + kh * a.kv_sh;
+    const uint8_t* v0 = (const uint8_t*)a.v + kh * a.kv_sh;
+    const auto page_at = [&](int id, int t) {      // offset of position t's row
+        return (uint64_t)(uint32_t)id * (uint64_t)a.kv_sb + (uint32_t)(t & ((1 << pl.sh) - 1)) * (uint32_t)a.kv_st;
+    };
+    RowState<D> st;
+    const auto look = [&](auto& lk, int t, int period) {
+        lk.table = a.block_table + it.r * a.bt_st;
+        lk.ks = sc.k + kh * sc.sh;
+        lk.vs = sc.v + kh * sc.sh;
+        lk.sb = sc.sb;
+        lk.sh = pl.sh;
+        lk.nb = a.nb;
+        lk.last = sp.hi - 1;
+        lk.c = a.scale * 1.44269504088896341f;
+        lk.start(t, period);
+    };
+
+    if (!few) {
+        // ---- many rows: the workgroup shares the tiles -------------------------------------
+        // Wave w brings the 16 keys 64 j + 16 w .. of tile j: into registers two tiles ahead, widened
+        // into LDS one tile ahead.
+        const uint32_t base = lds_addr(lds.kv);
+        Lookup<4> lk;
+        u32x4_t kr[LOADS], vr[LOADS];
+        int lim = 0;                               // rows of the 16 that hold tokens
+        bool care = false;
+        const auto request = [&](int j, int s) {
+            const int t = CK_KEYS * (sp.lo + j) + 16 * w, id = lk.block(s, w);
+            lim = id >= 0 ? len - t : 0;
+            if (id >= 0) {
+                const uint64_t at = page_at(id, t);
+                cd.load(kr, k0 + at, once);
+                cd.load(vr, v0 + at, once);
+            } else {
+#pragma unroll
+                for (int n = 0; n < LOADS; ++n) kr[n] = vr[n] = (u32x4_t){0u, 0u, 0u, 0u};
+            }
+        };
+        const auto widen = [&](int buf) {
+            const uint32_t kd = base + 2 * KB * buf + 16 * w * 2 * D, vd = kd + KB;
+#pragma unroll
+            for (int n = 0; n < LOADS; ++n) {
+                if (lim < 16) cd.clip(vr[n], n, lim);
+                if (CT == AMASS_E4M3 && care) cd.poison(kr[n], vr[n]);
+                cd.template put<DT, CT>(kd, n, kr[n]);
+                cd.template put<DT, CT>(vd, n, vr[n]);
+            }
+        };
+        for (;;) {
+            reset(st);
+            if (j0 < j1) {
+                look(lk, CK_KEYS * (sp.lo + j0) + 16 * lane, 16 * WAVE);
+                request(j0, 0);
+                widen(0);
+                if (j0 + 1 < j1) request(j0 + 1, 1);
+            }
+            for (int j = j0, s = 0; j < j1; ++j) {
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if (j + 1 < j1) {
+                    widen((j + 1 - j0) & 1);
+                    if (j + 2 < j1) request(j + 2, s + 2);
+                }
+                lk.ahead(s);
+                const int t0 = CK_KEYS * (sp.lo + j);
+                if (!idle && t0 < hi_hi && t0 + CK_KEYS > lo_lo) {
+                    const uint32_t ks = base + 2 * KB * ((j - j0) & 1);
+                    const Factors<4> f(lk, s);
+                    f32x16_t sc2[2];
+                    u32x4_t p[4];
+                    scores<DT, D, 2>(ks, ll, q, sc2);
+                    if (care)
+                        weigh_tile<DT, D, 2, true, true>(sc2, f, st, p, lo - t0, hi - t0, lk.groups(s), lane);
+                    else
+                        weigh_tile<DT, D, 2, true, false>(sc2, f, st, p, lo - t0, hi - t0, lk.groups(s), lane);
+                    add_values<DT, D, 2>(ks + KB, ll, p, st);
+                }
+                if (++s == Lookup<4>::STEPS) {
+                    lk.turn();
+                    s = 0;
+                }
+            }
+            if (care) break;
+            const bool bad = needs_care(st, live);
+            if (lane == 0) lds.bad[w] = bad;
+            __syncthreads();
+            care = __builtin_amdgcn_readfirstlane(lds.bad[0] | lds.bad[1] | lds.bad[2] | lds.bad[3]) != 0;
+            if (!care) break;
+            __syncthreads();                       // (before `bad` is written again)
+        }
+        if (idle) return;
+        finish_rows<DT, D, QC_UP>(a, pl, it, kh, st, 1.f, row, group, whole, lane);
+        return;
+    }
+    // ---- few rows: each wave its own 32 keys, w + 4, w + 8, ... ------------------------
+    constexpr int HB = KB / 2;                     // 32 widened keys
+    const uint32_t base = lds_addr(lds.kv + 2 * HB * w);
+    const int b0 = 2 * (sp.lo + j0) + w, b1 = 2 * (sp.lo + j1);
+    Lookup<2> lk;
+    u32x4_t kr[2][LOADS], vr[2][LOADS];
+    const auto fetch = [&](u32x4_t (&z)[2][LOADS], const uint8_t* from, int b, int s) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const int id = lk.block(s, g);
+            if (id >= 0) cd.load(z[g], from + page_at(id, 32 * b + 16 * g), once);
+            else
+#pragma unroll
+                for (int n = 0; n < LOADS; ++n) z[g][n] = (u32x4_t){0u, 0u, 0u, 0u};
+        }
+    };
+    const auto widen = [&](const u32x4_t (&z)[2][LOADS], uint32_t to) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int n = 0; n < LOADS; ++n) cd.template put<DT, CT>(to + g * (HB / 2), n, z[g][n]);
+    };
+    const auto fence = [] { asm volatile("" ::: "memory"); };
+    const auto walk = [&](auto care) {
+        reset(st);
+        if (b0 < b1) {
+            look(lk, 32 * (b0 + CK_WAVES * (lane >> 1)) + 16 * (lane & 1), 32 * 32 * CK_WAVES);
+            fetch(kr, k0, b0, 0);
+            fetch(vr, v0, b0, 0);
+        }
+        for (int b = b0, s = 0; b < b1; b += CK_WAVES) {
+            const int t0 = 32 * b;
+            const bool more = b + CK_WAVES < b1;
+            if (t0 + 32 > len) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int n = 0; n < LOADS; ++n) cd.clip(vr[g][n], n, len - t0 - 16 * g);
+            }
+            if constexpr (CT == AMASS_E4M3 && care) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int n = 0; n < LOADS; ++n) cd.poison(kr[g][n], vr[g][n]);
+            }
+            widen(kr, base);
+            fence();
+            if (more) fetch(kr, k0, b + CK_WAVES, s + 1);
+            lk.ahead(s);
+            const Factors<2> f(lk, s);
+            f32x16_t sc1[1];
+            u32x4_t p[2];
+            scores<DT, D, 1>(base, ll, q, sc1);
+            const uint32_t groups = lk.groups(s);
+            if (care || t0 < lo_hi || t0 + 32 > hi_lo || groups != 3u)
+                weigh_tile<DT, D, 1, true, care>(sc1, f, st, p, lo - t0, hi - t0, groups, lane);
+            else
+                weigh_tile<DT, D, 1, false, false>(sc1, f, st, p, 0, 0, 0u, lane);
+            widen(vr, base + HB);
+            fence();
+            if (more) fetch(vr, v0, b + CK_WAVES, s + 1);
+            add_values<DT, D, 1>(base + HB, ll, p, st);
+            fence();
+            if (++s == Lookup<2>::STEPS) {
+                lk.turn();
+                s = 0;
+            }
+        }
+    };
+    walk(std::false_type());
+    if (needs_care(st, live)) walk(std::true_type());      // (this wave alone)
+    __syncthreads();
+    finish_shared<DT, D, QC_UP>(a, pl, it, kh, st, lds, 1.f, row, whole, w, lane);
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(CM_WAVES * WAVE) void quant_merge_kernel(const amass_chunk_args a,
+                                                                      const ChunkPlan pl) {
+    merge_parts<DT, D, QC_UP>(a, pl, 1.f);
+}
+
+// ------------------------------------------------------------------ host
+static bool quant_empty(const amass_quant_chunk_args& a) { return a.n_tokens == 0 || a.n_req == 0; }
+
+static int quant_check(const amass_quant_chunk_args& a) {
+    if (quant_empty(a)) return AMASS_OK;
+    if (!a.q || !a.k_codes || !a.v_codes || !a.k_scale || !a.v_scale || !a.block_table || !a.seq_lens ||
+        !a.query_start || !a.out)
+        return AMASS_ERR_NULL;
+    if ((a.dtype != AMASS_BF16 && a.dtype != AMASS_FP16) || (a.code != AMASS_INT8 && a.code != AMASS_E4M3) ||
+        (a.d != 64 && a.d != 128))
+        return AMASS_ERR_UNSUPPORTED;
+    if (a.page < 16 || a.page > 1024 || (a.page & (a.page - 1))) return AMASS_ERR_GEOMETRY;
+    if (a.n_req < 0 || a.n_tokens < 0 || a.n_kv < 1 || a.G < 1 || a.nb < 1 || a.max_pages < 1 ||
+        a.window < 0 || !(a.scale > 0.f) || a.scale > 2e38f)
+        return AMASS_ERR_GEOMETRY;
+    if (a.n_kv > 4096 || a.G > 4096 || (int64_t)a.n_tokens * a.G > (1 << 30)) return AMASS_ERR_GEOMETRY;
+    const auto off = [](const void* p) { return ((uintptr_t)p & 15) != 0; };
+    if (off(a.q) || off(a.k_codes) || off(a.v_codes) || off(a.out) ||
+        ((a.q_st | a.q_hs | a.o_st | a.o_hs) & 7) || ((a.c_sb | a.c_st | a.c_sh) & 15))
+        return AMASS_ERR_GEOMETRY;
+    // the kernel has 32 bits for a row's offset within its block
+    if (a.c_sb < 0 || a.c_sb >= (1ll << 31) || a.c_st < 0 || a.c_st * a.page >= (1ll << 31))
+        return AMASS_ERR_GEOMETRY;
+    return AMASS_OK;
+}
+
+// the arguments that the plan and the results share with amass_chunk_attention
+static amass_chunk_args chunk_args_of(const amass_quant_chunk_args& a) {
+    amass_chunk_args c = {};
+    c.q = a.q, c.q_st = a.q_st, c.q_hs = a.q_hs;
+    c.k = a.k_codes, c.v = a.v_codes, c.kv_sb = a.c_sb, c.kv_st = a.c_st, c.kv_sh = a.c_sh;
+    c.block_table = a.block_table, c.bt_st = a.bt_st;
+    c.seq_lens = a.seq_lens, c.query_start = a.query_start;
+    c.out = a.out, c.o_st = a.o_st, c.o_hs = a.o_hs;
+    c.lse = a.lse, c.l_st = a.l_st, c.l_hs = a.l_hs;
+    c.scratch = a.scratch, c.scratch_bytes = a.scratch_bytes;
+    c.scale = a.scale, c.n_req = a.n_req, c.n_tokens = a.n_tokens, c.n_kv = a.n_kv, c.G = a.G;
+    c.d = a.d, c.page = a.page, c.nb = a.nb, c.max_pages = a.max_pages;
+    c.causal = a.causal, c.window = a.window, c.dtype = a.dtype;
+    return c;
+}
+
+template <int DT, int CT, int D>
+static int launch_quant(const amass_chunk_args& a, const Scales& sc, const ChunkPlan& p, hipStream_t s) {
+    const int64_t items = (int64_t)p.items * a.n_kv;
+    if (items * CK_WAVES * WAVE > 0xFFFFFFFFll) return AMASS_ERR_GEOMETRY;    // (threads of a launch)
+    hipLaunchKernelGGL((quant_chunk_kernel<DT, CT, D>), dim3((unsigned)items), dim3(CK_WAVES * WAVE), 0, s, a,
+                       sc, p);
+    const int rc = check_launch();
+    if (rc) return rc;
+    // a cut tile has two slots at least
+    const int cuts = p.tiles_max < (p.slots + 1) / 2 ? p.tiles_max : (p.slots + 1) / 2;
+    hipLaunchKernelGGL((quant_merge_kernel<DT, D>), dim3(cuts * a.n_kv, p.slot_rows / 32, D / 32),
+                       dim3(CM_WAVES * WAVE), 0, s, a, p);
+    return check_launch();
+}
+template <int DT, int CT>
+static int launch_quant(const amass_chunk_args& a, const Scales& sc, const ChunkPlan& p, hipStream_t s) {
+    return a.d == 128 ? launch_quant<DT, CT, 128>(a, sc, p, s) : launch_quant<DT, CT, 64>(a, sc, p, s);
+}
+
+}  // namespace amass
+
+using namespace amass;
+
+extern "C" int64_t amass_quant_scratch_bytes(const amass_quant_chunk_args* a) {
+    if (!a) return AMASS_ERR_NULL;
+    const int rc = quant_check(*a);
+    if (rc || quant_empty(*a)) return rc;
+    const amass_chunk_args c = chunk_args_of(*a);
+    return chunk_scratch(c, chunk_plan(c));
+}
+
+extern "C" int amass_quant_chunk_attention(const amass_quant_chunk_args* ain, void* stream) {
+    if (!ain) return AMASS_ERR_NULL;
+    const int rc = quant_check(*ain);
+    if (rc) return rc;
+    if (quant_empty(*ain)) return AMASS_OK;
+    const amass_chunk_args a = chunk_args_of(*ain);
+    if (!a.scratch) return AMASS_ERR_NULL;
+    const ChunkPlan p = chunk_plan(a);
+    if (((uintptr_t)a.scratch & 255) || a.scratch_bytes < chunk_scratch(a, p)) return AMASS_ERR_CAPACITY;
+    const Scales sc = {ain->k_scale, ain->v_scale, ain->s_sb, ain->s_sh};
+    hipStream_t s = (hipStream_t)stream;
+    if (a.dtype == AMASS_BF16)
+        return ain->code == AMASS_INT8 ? launch_quant<0, 0>(a, sc, p, s) : launch_quant<0, 1>(a, sc, p, s);
+    return ain->code == AMASS_INT8 ? launch_quant<1, 0>(a, sc, p, s) : launch_quant<1, 1>(a, sc, p, s);
+}
