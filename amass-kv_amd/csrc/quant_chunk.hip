@@ -60,7 +60,7 @@ struct Lookup {
         has = __ballot(e >= 0);
         sk = k < INFINITY ? k * c : __builtin_nanf("");
         if (v < LEAST_SCALE) v = LEAST_SCALE;
-        off = __log2f(v);
+        off = e < 0 ? -INFINITY : __log2f(v);      // (a page without a block: weights of zero)
         inv = (float)(1 << QC_UP) / v;
     }
     // first: this lane's first position
@@ -83,7 +83,7 @@ struct Lookup {
         t += jump;
         next_id = find(t + jump);
     }
-    // block of group g of step s (of the next period from STEPS on)
+    // block of group g of step s (of the next period from STEPS on), negative for none
     __device__ __forceinline__ int block(int s, int g) const {
         return s < STEPS ? __builtin_amdgcn_readlane(id, PER * s + g)
                          : __builtin_amdgcn_readlane(next_id, PER * (s - STEPS) + g);
@@ -111,31 +111,30 @@ struct Codes {
         off = (uint32_t)row * st + 16 * c;
         lds = row * (2 * D) + (((2 * c) ^ swz<D>(row)) << 4);
     }
-    __device__ __forceinline__ void load(u32x4_t* z, const uint8_t* page, bool once) const {
+    // ONCE: what nobody reads again soon (it need not stay in a cache)
+    template <bool ONCE = false>
+    __device__ __forceinline__ void load(u32x4_t* z, const uint8_t* page) const {
 #pragma unroll
         for (int n = 0; n < LOADS; ++n) {
             const u32x4_t* p = reinterpret_cast<const u32x4_t*>(page + off + n * RPL * st);
-            z[n] = once ? __builtin_nontemporal_load(p) : *p;
+            z[n] = ONCE ? __builtin_nontemporal_load(p) : *p;
         }
     }
-    // register n, widened, to the image of its 16 rows at `to` (row + 8 turns the chunk's second bit)
+    // 8 codes of register n (the half h of it), widened, to the image of its 16 rows at `to` (row + 8 turns
+    // the chunk's second bit)
     template <int DT, int CT>
-    __device__ __forceinline__ void put(uint32_t to, int n, const u32x4_t& z) const {
-        typedef __attribute__((address_space(3))) u32x4_t* lds_t;
-        u32x4_t a, b;
+    __device__ __forceinline__ void put(uint32_t to, int n, int h, const u32x4_t& z) const {
+        u32x4_t a;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            uint32_t lo, hi;
-            widen4<DT, CT>(z[j], lo, hi);
+            uint32_t lo, hi, x = z[2 * h + j];
+            asm("" : "+v"(x));                     // (widened here, not byte by byte where it was loaded)
+            widen4<DT, CT>(x, lo, hi);
             a[2 * j] = lo;
             a[2 * j + 1] = hi;
-            widen4<DT, CT>(z[2 + j], lo, hi);
-            b[2 * j] = lo;
-            b[2 * j + 1] = hi;
         }
-        const uint32_t at = ((to + lds) ^ (uint32_t)(32 * n)) + n * RPL * (2 * D);
-        *(lds_t)(uintptr_t)at = a;
-        *(lds_t)(uintptr_t)(at ^ 16u) = b;
+        const uint32_t at = ((to + lds) ^ (uint32_t)(32 * n + 16 * h)) + n * RPL * (2 * D);
+        *(__attribute__((address_space(3))) u32x4_t*)(uintptr_t)at = a;
     }
     // V's register n without the rows from `rows` on (what lies behind the last token may be a NaN, and the
     // weight zero times that is one)
@@ -173,6 +172,9 @@ struct Factors {                   // of N groups of 16 keys
     }
 };
 
+// nothing moves across (the order is the program's, and few values wait in registers)
+__device__ __forceinline__ void step() { __builtin_amdgcn_sched_barrier(0); }
+
 __device__ __forceinline__ float group_max(const f32x16_t& s, int half) {
     float mx = s[8 * half];
 #pragma unroll
@@ -189,25 +191,29 @@ __device__ __forceinline__ float lift_max(float mx, RowState<D>& st) {
     return al;
 }
 
+// -inf for the keys (relative to the tile) outside [lo, hi) of this lane's row, and those of groups of 16
+// whose bit is not set
+template <int NK>
+__device__ __forceinline__ void mask_scores(f32x16_t (&s)[NK], int lo, int hi, uint32_t groups, int lane) {
+    const int h4 = 4 * (lane >> 5);
+    lo -= h4;
+    hi -= h4;
+#pragma unroll
+    for (int x = 0; x < NK; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int key = 32 * x + 8 * (i >> 2) + (i & 3);
+            const bool see = key >= lo && key < hi && (groups >> (2 * x + (i >> 3)) & 1);
+            s[x][i] = see ? s[x][i] : -INFINITY;
+        }
+}
+
 // The weights of 32 NK keys, packed for the second product, and what they add to the maximum and the
-// sum.  MASKS: the row sees the keys [lo, hi) of the tile, in the groups whose bits are set.  CARE:
-// for factors that are not finite, which must not reach what a row does not see, and for
+// sum.  CARE: for factors that are not finite, which must not reach what a row does not see, and for
 // maxima far from zero: the difference from them first, exact where it matters.
-template <int DT, int D, int NK, bool MASKS, bool CARE>
-__device__ __forceinline__ void weigh_tile(f32x16_t (&s)[NK], const Factors<2 * NK>& f, RowState<D>& st,
-                                           u32x4_t (&p)[2 * NK], int lo, int hi, uint32_t groups,
-                                           int lane) {
-    if constexpr (MASKS) {
-        const int h4 = 4 * (lane >> 5);
-#pragma unroll
-        for (int x = 0; x < NK; ++x)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = 32 * x + 8 * (i >> 2) + (i & 3) + h4;
-                const bool see = key >= lo && key < hi && (groups >> (2 * x + (i >> 3)) & 1);
-                s[x][i] = see ? s[x][i] : -INFINITY;
-            }
-    }
+template <int DT, int D, int NK, bool CARE>
+__device__ __forceinline__ void weigh_tile(const f32x16_t (&s)[NK], const Factors<2 * NK>& f,
+                                           RowState<D>& st, u32x4_t (&p)[2 * NK]) {
     float mx = -INFINITY;
 #pragma unroll
     for (int g = 0; g < 2 * NK; ++g) {
@@ -242,6 +248,7 @@ __device__ __forceinline__ void weigh_tile(f32x16_t (&s)[NK], const Factors<2 * 
             }
             p[g][i >> 1] = pack2<DT>(e[0], e[1]);
         }
+        step();
         if (!CARE || sum != 0.f) st.l = __builtin_fmaf(sum, f.inv[g], st.l);
     }
 }
@@ -252,7 +259,115 @@ __device__ __forceinline__ void add_values(uint32_t vs, const LdsLane<D>& ll, co
 #pragma unroll
     for (int y = 0; y < 2 * NK; ++y)
 #pragma unroll
-        for (int z = 0; z < D / 32; ++z) st.o[z] = mfma32<DT>(ll.v_frag(vs, z, y), p[y], st.o[z]);
+        for (int z = 0; z < D / 32; ++z) {
+            st.o[z] = mfma32<DT>(ll.v_frag(vs, z, y), p[y], st.o[z]);
+            if (z & 1) step();
+        }
+}
+
+// A tile of 64 keys of the many-row layout, in a fixed order (each step ends in a scheduling barrier):
+// the matrix products follow each other with four fragments in flight, and the vector work runs under them:
+//   scores of keys 0..31, the next tile's K into LDS | scores of 32..63, weights of 0..31 | maximum |
+//   products with V of 0..31, weights of 32..63 | products with V of 32..63, the next tile's V into LDS
+// The first weights are made with the maximum so far and made again in the rare tile whose scores exceed
+// it by more than it may lag.  MASKS: the lane's row sees the keys [lo, hi) of the tile; without, all.
+// bring_k, bring_v: put 8 codes a lane (the argument: which) of the next tile.
+template <int DT, int D, bool MASKS, class BringK, class BringV>
+__device__ __forceinline__ void ordered_tile(uint32_t ks, uint32_t vs, const LdsLane<D>& ll,
+                                             const u32x4_t (&q)[D / 16], const Factors<4>& fa,
+                                             RowState<D>& st, int lo, int hi, int lane, BringK bring_k,
+                                             BringV bring_v) {
+    lo -= 4 * (lane >> 5);
+    hi -= 4 * (lane >> 5);
+    const uint32_t seen = (uint32_t)max(hi - lo, 0);
+    const auto masked = [&](float v, int x, int i) {
+        const int key = 32 * x + 8 * (i >> 2) + (i & 3);
+        return !MASKS || (uint32_t)(key - lo) < seen ? v : -INFINITY;
+    };
+    constexpr int N = D / 16, Z = D / 32;      // products of 32 keys with K or V; d tiles
+    constexpr int EVERY = N / (2 * Codes<D>::LOADS);
+    u32x4_t f[4], p[4];
+    f32x16_t s[2], zero;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+    const auto k_frag = [&](int n) { return ll.k_frag(ks, n % N, n / N); };
+    float off[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
+    const auto offsets = [&] {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) off[g] = fa.off[g] + (CK_LIFT<DT> - st.m);
+    };
+    offsets();
+    const auto weight = [&](int x, int i, bool fresh = true) {    // weights 2 i and 2 i + 1 of half x
+        const int g = 2 * x + (i >> 2);
+        if (x == 0 && fresh) {                 // (half 1 is masked before the maximum)
+            s[0][2 * i] = masked(s[0][2 * i], 0, 2 * i);
+            s[0][2 * i + 1] = masked(s[0][2 * i + 1], 0, 2 * i + 1);
+        }
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][2 * i], fa.sk[g], off[g]));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][2 * i + 1], fa.sk[g], off[g]));
+        sum[g] += e0 + e1;
+        uint32_t w = pack2<DT>(e0, e1);
+        asm volatile("" : "+v"(w));            // (made here, not behind the branch below)
+        p[g][i & 3] = w;
+    };
+#pragma unroll
+    for (int n = 0; n < 4; ++n) f[n] = k_frag(n);
+    step();
+    __builtin_amdgcn_s_setprio(1);             // (products before the other wave's vector work)
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        s[0] = mfma32<DT>(f[n & 3], q[n], n ? s[0] : zero);
+        f[n & 3] = k_frag(n + 4);
+        if (n % EVERY == EVERY - 1) bring_k(n / EVERY);
+        step();
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        s[1] = mfma32<DT>(f[n & 3], q[n], n ? s[1] : zero);
+        if (n + 4 < N) f[n & 3] = k_frag(N + n + 4);
+        else f[n & 3] = ll.v_frag(vs, (n + 4 - N) % Z, (n + 4 - N) / Z);
+#pragma unroll
+        for (int i = 8 * n / N; i < 8 * (n + 1) / N; ++i) weight(0, i);
+        step();
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if constexpr (MASKS) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[1][i] = masked(s[1][i], 1, i);
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+        mx = fmaxf(mx, __builtin_fmaf(group_max(s[g >> 1], g & 1), fa.sk[g], fa.off[g]));
+    mx = xor32_maxf(mx);
+    const bool lag = __any(mx - st.m > CK_LAZY);
+    float al = 1.f;
+    if (lag) {
+        al = lift_max(mx, st);
+        offsets();
+        sum[0] = sum[1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weight(0, i, false);
+    }
+    scale_o(st, al);
+    __builtin_amdgcn_s_setprio(1);
+    step();
+    // V fragment n: 16-key step n / Z, d tile n % Z
+#pragma unroll
+    for (int n = 0; n < 2 * N; ++n) {
+        st.o[n % Z] = mfma32<DT>(f[n & 3], p[n / Z], st.o[n % Z]);
+        if (n + 4 < 2 * N) f[n & 3] = ll.v_frag(vs, (n + 4) % Z, (n + 4) / Z);
+        if (n < N) {
+#pragma unroll
+            for (int i = 8 * n / N; i < 8 * (n + 1) / N; ++i) weight(1, i);
+        } else if (n % EVERY == EVERY - 1) {
+            bring_v((n - N) / EVERY);
+        }
+        step();
+    }
+    __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) st.l = __builtin_fmaf(sum[g], fa.inv[g], st.l);
 }
 
 // whether a row that is there needs all of it again with care: it is not finite, or its maximum so far
@@ -420,6 +535,9 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
         for (int i = 0; i < D / 16; ++i)
             q[i] = live ? *reinterpret_cast<const u32x4_t*>(src + 16 * i) : (u32x4_t){0u, 0u, 0u, 0u};
     }
+    // (here, not in the loop over the keys, where a wait would also wait for the next tile's loads)
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(q[i]));
     const LdsLane<D> ll(lane);
     const Codes<D> cd((uint32_t)a.kv_st, lane);
     constexpr int LOADS = Codes<D>::LOADS;
@@ -443,61 +561,131 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
 
     if (!few) {
         // ---- many rows: the workgroup shares the tiles -------------------------------------
-        // Wave w brings the 16 keys 64 j + 16 w .. of tile j: into registers two tiles ahead, widened
-        // into LDS one tile ahead.
+        // Wave w brings the 16 keys 64 j + 16 w .. of tile j: into registers during tile j - 2, widened into
+        // LDS during tile j - 1.
         const uint32_t base = lds_addr(lds.kv);
         Lookup<4> lk;
         u32x4_t kr[LOADS], vr[LOADS];
-        int lim = 0;                               // rows of the 16 that hold tokens
-        bool care = false;
-        const auto request = [&](int j, int s) {
+        int lim = 16;                              // rows of the 16 that hold tokens
+        const uint32_t own = base + 16 * w * 2 * D;
+        uint64_t at = 0;                           // of the page in K and V
+        const auto find = [&](int j, int s) {      // (a page without a block: block 0, whose V is cut off)
             const int t = CK_KEYS * (sp.lo + j) + 16 * w, id = lk.block(s, w);
             lim = id >= 0 ? len - t : 0;
-            if (id >= 0) {
-                const uint64_t at = page_at(id, t);
-                cd.load(kr, k0 + at, once);
-                cd.load(vr, v0 + at, once);
-            } else {
+            at = page_at(max(id, 0), t);
+        };
+        const auto request_k = [&] { cd.load(kr, k0 + at); };
+        const auto request_v = [&] { cd.load(vr, v0 + at); };
+        const auto put_k = [&](int buf, int i) {
+            cd.template put<DT, CT>(own + 2 * KB * buf, i >> 1, i & 1, kr[i >> 1]);
+        };
+        const auto put_v = [&](int buf, int i) {
+            cd.template put<DT, CT>(own + 2 * KB * buf + KB, i >> 1, i & 1, vr[i >> 1]);
+        };
+        const auto clip = [&] {
+            if (lim < 16) {
 #pragma unroll
-                for (int n = 0; n < LOADS; ++n) kr[n] = vr[n] = (u32x4_t){0u, 0u, 0u, 0u};
+                for (int n = 0; n < LOADS; ++n) cd.clip(vr[n], n, lim);
             }
         };
-        const auto widen = [&](int buf) {
-            const uint32_t kd = base + 2 * KB * buf + 16 * w * 2 * D, vd = kd + KB;
+        const auto put_all = [&](int buf) {
 #pragma unroll
-            for (int n = 0; n < LOADS; ++n) {
-                if (lim < 16) cd.clip(vr[n], n, lim);
-                if (CT == AMASS_E4M3 && care) cd.poison(kr[n], vr[n]);
-                cd.template put<DT, CT>(kd, n, kr[n]);
-                cd.template put<DT, CT>(vd, n, vr[n]);
+            for (int i = 0; i < 2 * LOADS; ++i) {
+                put_k(buf, i);
+                put_v(buf, i);
+                step();
             }
         };
-        for (;;) {
-            reset(st);
-            if (j0 < j1) {
-                look(lk, CK_KEYS * (sp.lo + j0) + 16 * lane, 16 * WAVE);
-                request(j0, 0);
-                widen(0);
-                if (j0 + 1 < j1) request(j0 + 1, 1);
-            }
-            for (int j = j0, s = 0; j < j1; ++j) {
-                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                if (j + 1 < j1) {
-                    widen((j + 1 - j0) & 1);
-                    if (j + 2 < j1) request(j + 2, s + 2);
+        const auto turn = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+        const auto seen = [&](int j) {             // by some row of the wave
+            const int t0 = CK_KEYS * (sp.lo + j);
+            return !idle && t0 < hi_hi && t0 + CK_KEYS > lo_lo;
+        };
+        reset(st);
+        bool again = false;
+        if (j0 < j1) {
+            look(lk, CK_KEYS * (sp.lo + j0) + 16 * lane, 16 * WAVE);
+            find(j0, 0);
+            request_k();
+            request_v();
+            clip();
+            put_all(0);
+            find(j0 + 1, 1);                       // (past the part: its keys are there or none are)
+            request_k();
+            request_v();
+            // tiles [f0, f1) hold only keys that all of the wave's rows see
+            const int f1 = idle ? j1 : min(j1, hi_lo / CK_KEYS - sp.lo);
+            const int f0 = idle ? j1 : min(f1, max(j0, (lo_hi + CK_KEYS - 1) / CK_KEYS - sp.lo));
+            int s = 0;
+            const auto tile = [&](int j, auto masks) {
+                const uint32_t ks = base + 2 * KB * ((j - j0) & 1);
+                const int buf = (j + 1 - j0) & 1, t0 = CK_KEYS * (sp.lo + j);
+                clip();
+                find(j + 2, s + 2);
+                const Factors<4> f(lk, s);
+                ordered_tile<DT, D, masks>(
+                    ks, ks + KB, ll, q, f, st, lo - t0, hi - t0, lane,
+                    [&](int i) {
+                        put_k(buf, i);
+                        if (i == 2 * LOADS - 1) request_k();
+                    },
+                    [&](int i) { put_v(buf, i); });
+                request_v();
+            };
+            const auto pass = [&](int j) {         // a tile that none of the wave's rows see
+                clip();
+                put_all((j + 1 - j0) & 1);
+                find(j + 2, s + 2);
+                request_k();
+                request_v();
+            };
+            const auto next = [&] {
+                if (++s == Lookup<4>::STEPS) {
+                    lk.turn();
+                    s = 0;
                 }
+            };
+            const auto walk = [&](int j, int end, auto masks) {
+                for (; j < end; ++j) {
+                    turn();
+                    lk.ahead(s);
+                    if (!masks || seen(j)) tile(j, masks);
+                    else pass(j);
+                    next();
+                }
+            };
+            walk(j0, f0, std::true_type());
+            walk(max(f0, j0), f1, std::false_type());
+            walk(max(f1, j0), j1, std::true_type());     // (f1 may lie before this part)
+            const bool bad = needs_care(st, live);
+            if (lane == 0) lds.bad[w] = bad;
+            __syncthreads();
+            again = __builtin_amdgcn_readfirstlane(lds.bad[0] | lds.bad[1] | lds.bad[2] | lds.bad[3]) != 0;
+        }
+        if (again) {
+            reset(st);
+            look(lk, CK_KEYS * (sp.lo + j0) + 16 * lane, 16 * WAVE);
+            for (int j = j0, s = 0; j < j1; ++j) {
+                find(j, s);
+                request_k();
+                request_v();
+                clip();
+                if constexpr (CT == AMASS_E4M3) {
+#pragma unroll
+                    for (int n = 0; n < LOADS; ++n) cd.poison(kr[n], vr[n]);
+                }
+                put_all((j - j0) & 1);
+                turn();
                 lk.ahead(s);
-                const int t0 = CK_KEYS * (sp.lo + j);
-                if (!idle && t0 < hi_hi && t0 + CK_KEYS > lo_lo) {
+                if (seen(j)) {
                     const uint32_t ks = base + 2 * KB * ((j - j0) & 1);
+                    const int t0 = CK_KEYS * (sp.lo + j);
                     const Factors<4> f(lk, s);
                     f32x16_t sc2[2];
                     u32x4_t p[4];
                     scores<DT, D, 2>(ks, ll, q, sc2);
-                    if (care)
-                        weigh_tile<DT, D, 2, true, true>(sc2, f, st, p, lo - t0, hi - t0, lk.groups(s), lane);
-                    else
-                        weigh_tile<DT, D, 2, true, false>(sc2, f, st, p, lo - t0, hi - t0, lk.groups(s), lane);
+                    mask_scores<2>(sc2, lo - t0, hi - t0, lk.groups(s), lane);
+                    weigh_tile<DT, D, 2, true>(sc2, f, st, p);
                     add_values<DT, D, 2>(ks + KB, ll, p, st);
                 }
                 if (++s == Lookup<4>::STEPS) {
@@ -505,13 +693,6 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
                     s = 0;
                 }
             }
-            if (care) break;
-            const bool bad = needs_care(st, live);
-            if (lane == 0) lds.bad[w] = bad;
-            __syncthreads();
-            care = __builtin_amdgcn_readfirstlane(lds.bad[0] | lds.bad[1] | lds.bad[2] | lds.bad[3]) != 0;
-            if (!care) break;
-            __syncthreads();                       // (before `bad` is written again)
         }
         if (idle) return;
         finish_rows<DT, D, QC_UP>(a, pl, it, kh, st, 1.f, row, group, whole, lane);
@@ -523,38 +704,41 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
     const int b0 = 2 * (sp.lo + j0) + w, b1 = 2 * (sp.lo + j1);
     Lookup<2> lk;
     u32x4_t kr[2][LOADS], vr[2][LOADS];
-    const auto fetch = [&](u32x4_t (&z)[2][LOADS], const uint8_t* from, int b, int s) {
+    const auto fetch = [&](auto past, u32x4_t (&z)[2][LOADS], const uint8_t* from, int b, int s) {
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-            const int id = lk.block(s, g);
-            if (id >= 0) cd.load(z[g], from + page_at(id, 32 * b + 16 * g), once);
-            else
-#pragma unroll
-                for (int n = 0; n < LOADS; ++n) z[g][n] = (u32x4_t){0u, 0u, 0u, 0u};
+            // (a page without a block: block 0, whose weights are zero and V is cut off)
+            cd.template load<past>(z[g], from + page_at(max(lk.block(s, g), 0), 32 * b + 16 * g));
         }
     };
     const auto widen = [&](const u32x4_t (&z)[2][LOADS], uint32_t to) {
 #pragma unroll
         for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int n = 0; n < LOADS; ++n) cd.template put<DT, CT>(to + g * (HB / 2), n, z[g][n]);
+            for (int i = 0; i < 2 * LOADS; ++i)
+            {
+                cd.template put<DT, CT>(to + g * (HB / 2), i >> 1, i & 1, z[g][i >> 1]);
+                step();
+            }
     };
     const auto fence = [] { asm volatile("" ::: "memory"); };
-    const auto walk = [&](auto care) {
+    const auto walk = [&](auto past, auto care) {
         reset(st);
         if (b0 < b1) {
             look(lk, 32 * (b0 + CK_WAVES * (lane >> 1)) + 16 * (lane & 1), 32 * 32 * CK_WAVES);
-            fetch(kr, k0, b0, 0);
-            fetch(vr, v0, b0, 0);
+            fetch(past, kr, k0, b0, 0);
+            fetch(past, vr, v0, b0, 0);
         }
         for (int b = b0, s = 0; b < b1; b += CK_WAVES) {
             const int t0 = 32 * b;
             const bool more = b + CK_WAVES < b1;
-            if (t0 + 32 > len) {
+            const uint32_t groups = lk.groups(s);
+            if (t0 + 32 > len || groups != 3u) {
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
 #pragma unroll
-                    for (int n = 0; n < LOADS; ++n) cd.clip(vr[g][n], n, len - t0 - 16 * g);
+                    for (int n = 0; n < LOADS; ++n)
+                        cd.clip(vr[g][n], n, groups >> g & 1 ? len - t0 - 16 * g : 0);
             }
             if constexpr (CT == AMASS_E4M3 && care) {
 #pragma unroll
@@ -564,20 +748,17 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
             }
             widen(kr, base);
             fence();
-            if (more) fetch(kr, k0, b + CK_WAVES, s + 1);
+            if (more) fetch(past, kr, k0, b + CK_WAVES, s + 1);
             lk.ahead(s);
             const Factors<2> f(lk, s);
             f32x16_t sc1[1];
             u32x4_t p[2];
             scores<DT, D, 1>(base, ll, q, sc1);
-            const uint32_t groups = lk.groups(s);
-            if (care || t0 < lo_hi || t0 + 32 > hi_lo || groups != 3u)
-                weigh_tile<DT, D, 1, true, care>(sc1, f, st, p, lo - t0, hi - t0, groups, lane);
-            else
-                weigh_tile<DT, D, 1, false, false>(sc1, f, st, p, 0, 0, 0u, lane);
+            if (care || t0 < lo_hi || t0 + 32 > hi_lo) mask_scores<1>(sc1, lo - t0, hi - t0, groups, lane);
+            weigh_tile<DT, D, 1, care>(sc1, f, st, p);
             widen(vr, base + HB);
             fence();
-            if (more) fetch(vr, v0, b + CK_WAVES, s + 1);
+            if (more) fetch(past, vr, v0, b + CK_WAVES, s + 1);
             add_values<DT, D, 1>(base + HB, ll, p, st);
             fence();
             if (++s == Lookup<2>::STEPS) {
@@ -586,8 +767,9 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
             }
         }
     };
-    walk(std::false_type());
-    if (needs_care(st, live)) walk(std::true_type());      // (this wave alone)
+    if (once) walk(std::true_type(), std::false_type());
+    else walk(std::false_type(), std::false_type());
+    if (needs_care(st, live)) walk(std::false_type(), std::true_type());      // (this wave alone)
     __syncthreads();
     finish_shared<DT, D, QC_UP>(a, pl, it, kh, st, lds, 1.f, row, whole, w, lane);
 }
