@@ -8,10 +8,10 @@
 // 8 significant bits: then no quotient that is not half way between two codes lies nearer to it
 // than 2^-17, so the fp32 quotient rounds to the code of the exact one.
 //
-// One wave takes a run's numbers of one half and head (16 rows of 128: 32 a lane, in registers; a
-// longer run is read twice), so the maximum is a chain of v_max and six exchanges, and nothing waits for
-// another wave.  A workgroup belongs to a token and returns at once where no run starts, after
-// turning the token's queries.
+// A run's numbers of one half and head stay in the registers of one wave (16 rows of 128: 32 a lane), of two
+// where pages have 32 rows and of four beyond (a run of more than 64 rows is read twice), so the maximum is a chain
+// of v_max, six exchanges and at most one barrier.  Runs are found in the slots: where a block
+// starts or the one before is no neighbour.
 // Read: 16 codes a thread, two 16-byte stores.
 #include "quant_codes.h"
 
@@ -78,68 +78,97 @@ __device__ __forceinline__ void turn(const amass_quant_write_args& a, const floa
 }
 
 constexpr int QW_THREADS = 256;
+constexpr int QW_WAVES = QW_THREADS / WAVE;
 constexpr int QW_ROWS = 16;              // rows that a wave holds
+// Tokens that a workgroup looks for runs in: one where the batch is small (every token may start a run, and the runs
+// of a window follow each other), 16 beyond (a prompt's workgroups that found no run would take longer to
+// start than the others to work).
+constexpr int QW_ALONE = 1024;
+constexpr int QW_WINDOW = 16;
 
-template <int DT, int CT, int D>
-__global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_quant_write_args a, int sh) {
-    constexpr int LPR = D / 16, RPL = WAVE / LPR, N = QW_ROWS / RPL;   // lanes a row, rows a load, loads
-    const int t = blockIdx.x;
+template <int D>
+constexpr int LPR_OF = D / 16;           // lanes a row
+
+// 16 channels of a query a thread
+template <int DT, int D>
+__device__ __forceinline__ void turn_queries(const amass_quant_write_args& a, uint32_t e) {
+    const uint32_t per = (uint32_t)a.n_heads * LPR_OF<D>, t = e / per;
+    if (t >= (uint32_t)a.n_tokens) return;
+    const uint32_t rest = e - t * per, head = rest / LPR_OF<D>, u = rest % LPR_OF<D>;
+    const int pos = a.positions[t];
+    if ((uint32_t)pos >= (uint32_t)a.max_pos) return;
+    const Chan c = channels(a, u, true);
+    const uint16_t* src = (const uint16_t*)a.q + t * a.q_st + head * a.q_hs;
+    uint16_t* dst = (uint16_t*)a.q_out + t * a.qo_st + head * a.qo_hs;
+    u32x4_t x = *reinterpret_cast<const u32x4_t*>(src + c.c0);
+    u32x4_t y = *reinterpret_cast<const u32x4_t*>(src + c.c1);
+    if (c.turn) turn<DT, float>(a, a.table + pos * a.tab_st + 8 * u, x, y);
+    *reinterpret_cast<u32x4_t*>(dst + c.c0) = x;
+    *reinterpret_cast<u32x4_t*>(dst + c.c1) = y;
+}
+
+// Workgroups: `groups` for each window of tokens, then those of the queries.  A workgroup's waves are teams of
+// TEAM, a team has a run's numbers of one half and head, QW_ROWS rows a wave.
+template <int DT, int CT, int D, int TEAM>
+__global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_quant_write_args a, int sh,
+                                                                 int window, int groups, int kv_wgs) {
+    constexpr int LPR = LPR_OF<D>, RPL = WAVE / LPR, N = QW_ROWS / RPL;   // lanes a row, rows a load, loads
+    constexpr int STEP = TEAM * QW_ROWS;
+    __shared__ uint32_t tops[QW_WAVES];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if ((int)blockIdx.x >= kv_wgs) {
+        turn_queries<DT, D>(a, (blockIdx.x - kv_wgs) * QW_THREADS + threadIdx.x);
+        return;
+    }
     const int64_t end = (int64_t)a.nb << sh;
     const auto has_pos = [&](int i) {
         return !a.table || (uint32_t)a.positions[i] < (uint32_t)a.max_pos;
     };
     const auto enters = [&](int i) { return (uint64_t)a.slots[i] < (uint64_t)end && has_pos(i); };
-
-    if (a.q && has_pos(t)) {
-        const float* tab = a.table + (int64_t)a.positions[t] * a.tab_st;
-        for (int e = threadIdx.x; e < a.n_heads * LPR; e += QW_THREADS) {
-            const int head = e / LPR, u = e % LPR;
-            const Chan c = channels(a, u, true);
-            const uint16_t* src = (const uint16_t*)a.q + t * a.q_st + head * a.q_hs;
-            uint16_t* dst = (uint16_t*)a.q_out + t * a.qo_st + head * a.qo_hs;
-            u32x4_t x = *reinterpret_cast<const u32x4_t*>(src + c.c0);
-            u32x4_t y = *reinterpret_cast<const u32x4_t*>(src + c.c1);
-            if (c.turn) turn<DT, float>(a, tab + 8 * u, x, y);
-            *reinterpret_cast<u32x4_t*>(dst + c.c0) = x;
-            *reinterpret_cast<u32x4_t*>(dst + c.c1) = y;
-        }
-    }
-    // a run starts here: the token enters a block, and not behind its neighbour
-    if (!enters(t)) return;
-    const int64_t slot = a.slots[t];
-    const int first = (int)(slot & ((1 << sh) - 1));
-    if (first > 0 && t > 0 && a.slots[t - 1] == slot - 1 && has_pos(t - 1)) return;
-    const int64_t blk = slot >> sh;
-    const int most = min((1 << sh) - first, a.n_tokens - t);
-    int n = 0;
-    while (n < most) {
-        const int i = n + lane;
-        const unsigned long long in = __ballot(i < most && a.slots[t + i] == slot + i && has_pos(t + i));
-        if (~in) {
-            n += __ffsll((long long)~in) - 1;
-            break;
-        }
-        n += WAVE;
-    }
+    const int t0 = blockIdx.x / groups * window;
+    const int unit = (blockIdx.x % groups) * (QW_WAVES / TEAM) + w / TEAM, mate = w % TEAM;
+    const bool is_k = unit < a.n_kv, works = unit < 2 * a.n_kv;
+    const int head = is_k ? unit : unit - a.n_kv;
     const int lr = lane / LPR, u = lane % LPR;
-    for (int unit = w; unit < 2 * a.n_kv; unit += QW_THREADS / WAVE) {
-        const bool is_k = unit < a.n_kv;
-        const int head = is_k ? unit : unit - a.n_kv;
-        const Chan c = channels(a, u, is_k && a.table);
+    const Chan c = channels(a, u, is_k && a.table);
+
+    // the window's tokens that start a run: they enter a block, and not behind their neighbour
+    bool starts = false;
+    if (lane < window && t0 + lane < a.n_tokens && enters(t0 + lane)) {
+        const int t = t0 + lane;
+        const int64_t slot = a.slots[t];
+        starts = (slot & ((1 << sh) - 1)) == 0 || t == 0 || a.slots[t - 1] != slot - 1 || !has_pos(t - 1);
+    }
+    for (unsigned long long left = __ballot(starts); left; left &= left - 1) {
+        const int t = t0 + __ffsll((long long)left) - 1;
+        const int64_t slot = a.slots[t];
+        const int first = (int)(slot & ((1 << sh) - 1));
+        const int64_t blk = slot >> sh;
+        const int most = min((1 << sh) - first, a.n_tokens - t);
+        int n = 1;                       // the run's length
+        while (n < most) {
+            const int i = n + lane;
+            const unsigned long long in = __ballot(i < most && a.slots[t + i] == slot + i && has_pos(t + i));
+            if (~in) {
+                n += __ffsll((long long)~in) - 1;
+                break;
+            }
+            n += WAVE;
+        }
+        n = min(n, most);
         const uint16_t* src = is_k ? (const uint16_t*)a.k + t * a.k_st + head * a.k_hs
                                    : (const uint16_t*)a.v + t * a.v_st + head * a.v_hs;
         const int64_t src_st = is_k ? a.k_st : a.v_st;
         uint8_t* codes = (uint8_t*)(is_k ? a.k_codes : a.v_codes) + blk * a.c_sb + head * a.c_sh;
         float* scale = (is_k ? a.k_scale : a.v_scale) + blk * a.s_sb + head * a.s_sh;
-        const float old = first > 0 ? *scale : 0.f;
+        const float old = works && first > 0 ? *scale : 0.f;
         u32x4_t x[N], y[N];
         const auto load = [&](int r0) {                  // rows r0 .. r0 + 15 of the run
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int r = r0 + RPL * i + lr;
                 x[i] = y[i] = (u32x4_t){0u, 0u, 0u, 0u};
-                if (r < n) {
+                if (works && r < n) {
                     x[i] = *reinterpret_cast<const u32x4_t*>(src + r * src_st + c.c0);
                     y[i] = *reinterpret_cast<const u32x4_t*>(src + r * src_st + c.c1);
                 }
@@ -155,7 +184,7 @@ __global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_qua
         };
         // the largest magnitude as 16 bits, NaN above infinity above every number
         uint32_t top = 0;
-        for (int r0 = 0; r0 < n; r0 += QW_ROWS) {
+        for (int r0 = mate * QW_ROWS; r0 < n; r0 += STEP) {
             load(r0);
 #pragma unroll
             for (int i = 0; i < N; ++i)
@@ -166,15 +195,25 @@ __global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_qua
                 }
         }
         top = (uint32_t)wave_max_uniform((int)top);
+        if constexpr (TEAM > 1) {
+            if (lane == 0) tops[w] = top;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < TEAM; ++i) top = max(top, tops[w - mate + i]);
+            top = __builtin_amdgcn_readfirstlane(top);
+            __syncthreads();
+        }
+        if (!works) continue;
         const bool finite = top < (DT == AMASS_BF16 ? 0x7F80u : 0x7C00u);
         float s = __builtin_nanf("");
         if (finite) {
             const float step = step_of<CT>(half_f32<DT>(top, 0));
             s = step >= old ? step : old;                // (a NaN stays)
         }
-        const float div = s < INFINITY ? s : 1.f, inv = 1.f / div, keep = s < INFINITY ? 1.f : 0.f;
-        for (int r0 = 0; r0 < n; r0 += QW_ROWS) {
-            if (n > QW_ROWS) load(r0);
+        const bool keep = s < INFINITY;
+        const float div = keep ? s : 1.f, inv = 1.f / div;
+        for (int r0 = mate * QW_ROWS; r0 < n; r0 += STEP) {
+            if (n > STEP) load(r0);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int r = r0 + RPL * i + lr;
@@ -185,7 +224,7 @@ __global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_qua
                     const uint32_t q = j < 2 ? x[i][2 * j + 1] : y[i][2 * j - 3];
                     o[j] = to_codes<CT>(quotient(half_f32<DT>(p, 0), div, inv), quotient(half_f32<DT>(p, 1), div, inv),
                                         quotient(half_f32<DT>(q, 0), div, inv), quotient(half_f32<DT>(q, 1), div, inv));
-                    if (keep == 0.f) o[j] = 0u;
+                    if (!keep) o[j] = 0u;
                 }
                 if (r < n) {
                     uint8_t* to = codes + (first + r) * a.c_st;
@@ -195,7 +234,7 @@ __global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_qua
             }
         }
         if (first > 0 && s > old) {                      // the rows before the run, by the new scale
-            for (int r = lr; r < first; r += RPL) {
+            for (int r = mate * RPL + lr; r < first; r += TEAM * RPL) {
                 u32x4_t* at = reinterpret_cast<u32x4_t*>(codes + r * a.c_st + 16 * u);
                 u32x4_t z = *at;
 #pragma unroll
@@ -207,7 +246,7 @@ __global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_qua
                 *at = z;
             }
         }
-        if (lane == 0) *scale = s;
+        if (lane == 0 && mate == 0) *scale = s;
     }
 }
 
@@ -284,7 +323,7 @@ static int check_write(const amass_quant_write_args& a) {
     if (a.q && (a.n_heads < 1 || a.n_heads > (1 << 16) || misaligned(a.q) || misaligned(a.q_out) ||
                 ((a.q_st | a.q_hs | a.qo_st | a.qo_hs) & 7)))
         return AMASS_ERR_GEOMETRY;
-    return (int64_t)a.n_tokens * QW_THREADS > 0xFFFFFFFFll ? AMASS_ERR_GEOMETRY : AMASS_OK;
+    return AMASS_OK;
 }
 static int check_read(const amass_quant_read_args& a) {
     if (!a.k_codes || !a.v_codes || !a.k_scale || !a.v_scale || !a.k_cache || !a.v_cache || !a.src || !a.dst)
@@ -298,14 +337,26 @@ static int check_read(const amass_quant_read_args& a) {
     return AMASS_OK;
 }
 
+template <int DT, int CT, int D, int TEAM>
+static int launch_write(const amass_quant_write_args& a, hipStream_t s) {
+    const int64_t window = a.n_tokens <= QW_ALONE ? 1 : QW_WINDOW;
+    const int64_t groups = (2 * a.n_kv * TEAM + QW_WAVES - 1) / QW_WAVES;
+    const int64_t kv_wgs = (a.n_tokens + window - 1) / window * groups;
+    const int64_t units = a.q ? (int64_t)a.n_tokens * a.n_heads * LPR_OF<D> : 0;
+    const int64_t wgs = kv_wgs + (units + QW_THREADS - 1) / QW_THREADS;
+    if (wgs * QW_THREADS > 0xFFFFFFFFll) return AMASS_ERR_GEOMETRY;          // (threads of a launch)
+    hipLaunchKernelGGL((quant_write_kernel<DT, CT, D, TEAM>), dim3((unsigned)wgs), dim3(QW_THREADS), 0, s, a,
+                       log2_of(a.page), (int)window, (int)groups, (int)kv_wgs);
+    return check_launch();
+}
+template <int DT, int CT, int D>
+static int launch_write(const amass_quant_write_args& a, hipStream_t s) {
+    if (a.page == 16) return launch_write<DT, CT, D, 1>(a, s);
+    return a.page == 32 ? launch_write<DT, CT, D, 2>(a, s) : launch_write<DT, CT, D, 4>(a, s);
+}
 template <int DT, int CT>
 static int launch_write(const amass_quant_write_args& a, hipStream_t s) {
-    const int sh = log2_of(a.page);
-    if (a.d == 128)
-        hipLaunchKernelGGL((quant_write_kernel<DT, CT, 128>), dim3(a.n_tokens), dim3(QW_THREADS), 0, s, a, sh);
-    else
-        hipLaunchKernelGGL((quant_write_kernel<DT, CT, 64>), dim3(a.n_tokens), dim3(QW_THREADS), 0, s, a, sh);
-    return check_launch();
+    return a.d == 128 ? launch_write<DT, CT, 128>(a, s) : launch_write<DT, CT, 64>(a, s);
 }
 template <int DT, int CT>
 static int launch_read(const amass_quant_read_args& a, hipStream_t s) {
