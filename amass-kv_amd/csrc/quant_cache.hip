@@ -50,9 +50,13 @@ __device__ __forceinline__ Chan channels(const amass_quant_write_args& a, int u,
 template <int DT, class F>
 __device__ __forceinline__ void turn(const amass_quant_write_args& a, const float* tab, u32x4_t& x,
                                      u32x4_t& y) {
-    const int half = a.rot >> 1;
+    const float4* tc = reinterpret_cast<const float4*>(tab);
+    const float4* ts = reinterpret_cast<const float4*>(tab + (a.rot >> 1));
+    const float4 c0 = tc[0], c1 = tc[1], s0 = ts[0], s1 = ts[1];
+    const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+    const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
     const auto pair = [&](float f, float g, int i, float& p, float& r) {
-        const F c = tab[i], s = tab[half + i];
+        const F c = cs[i], s = sn[i];
         p = (float)((F)f * c - (F)g * s);
         r = (float)((F)g * c + (F)f * s);
     };
@@ -121,10 +125,6 @@ __global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_qua
         return;
     }
     const int64_t end = (int64_t)a.nb << sh;
-    const auto has_pos = [&](int i) {
-        return !a.table || (uint32_t)a.positions[i] < (uint32_t)a.max_pos;
-    };
-    const auto enters = [&](int i) { return (uint64_t)a.slots[i] < (uint64_t)end && has_pos(i); };
     const int t0 = blockIdx.x / groups * window;
     const int unit = (blockIdx.x % groups) * (QW_WAVES / TEAM) + w / TEAM, mate = w % TEAM;
     const bool is_k = unit < a.n_kv, works = unit < 2 * a.n_kv;
@@ -132,30 +132,44 @@ __global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_qua
     const int lr = lane / LPR, u = lane % LPR;
     const Chan c = channels(a, u, is_k && a.table);
 
-    // the window's tokens that start a run: they enter a block, and not behind their neighbour
-    bool starts = false;
-    if (lane < window && t0 + lane < a.n_tokens && enters(t0 + lane)) {
-        const int t = t0 + lane;
-        const int64_t slot = a.slots[t];
-        starts = (slot & ((1 << sh) - 1)) == 0 || t == 0 || a.slots[t - 1] != slot - 1 || !has_pos(t - 1);
+    // Lane i looks at token t0 + i (one round of memory): whether it enters a block, and as its
+    // neighbour's successor in it.  Runs start where it is none.
+    int64_t sl = -1, sl0 = -1;
+    int ps = 0, ps0 = 0;
+    if (t0 + lane < a.n_tokens) {
+        sl = a.slots[t0 + lane];
+        if (a.table) ps = a.positions[t0 + lane];
     }
-    for (unsigned long long left = __ballot(starts); left; left &= left - 1) {
-        const int t = t0 + __ffsll((long long)left) - 1;
-        const int64_t slot = a.slots[t];
+    if (t0 > 0) {
+        sl0 = a.slots[t0 - 1];
+        if (a.table) ps0 = a.positions[t0 - 1];
+    }
+    const auto fits = [&](int64_t slot, int pos) {
+        return (uint64_t)slot < (uint64_t)end && (!a.table || (uint32_t)pos < (uint32_t)a.max_pos);
+    };
+    const auto follows = [&](int64_t slot) { return (slot & ((1 << sh) - 1)) != 0; };
+    const unsigned long long enter = __ballot(fits(sl, ps));
+    const int64_t up = __shfl_up(sl, 1);         // (by all lanes)
+    const int64_t before = lane == 0 ? sl0 : up;
+    const bool neighbour = lane == 0 ? fits(sl0, ps0) : (enter >> (lane - 1)) & 1;
+    const unsigned long long joins = __ballot(neighbour && sl == before + 1 && follows(sl)) & enter;
+    for (unsigned long long left = enter & ~joins & ((2ull << (window - 1)) - 1); left; left &= left - 1) {
+        const int i0 = __ffsll((long long)left) - 1, t = t0 + i0;
+        const int64_t slot = (int64_t)readlane_u64((unsigned long long)sl, i0);
         const int first = (int)(slot & ((1 << sh) - 1));
         const int64_t blk = slot >> sh;
-        const int most = min((1 << sh) - first, a.n_tokens - t);
-        int n = 1;                       // the run's length
-        while (n < most) {
-            const int i = n + lane;
-            const unsigned long long in = __ballot(i < most && a.slots[t + i] == slot + i && has_pos(t + i));
-            if (~in) {
-                n += __ffsll((long long)~in) - 1;
-                break;
-            }
-            n += WAVE;
+        // the run's length: the tokens behind the first that join, past the 64 a look at the next ones
+        const unsigned long long rest = i0 < WAVE - 1 ? joins >> (i0 + 1) : 0;
+        int n = ~rest ? __ffsll((long long)~rest) : WAVE;
+        for (bool more = i0 + n == WAVE; more;) {
+            const int i = n + lane, at = min(t + i, a.n_tokens - 1);
+            const int64_t next = a.slots[at];
+            const bool in = t + i < a.n_tokens && next == slot + i && follows(next) &&
+                            fits(next, a.table ? a.positions[at] : 0);
+            const unsigned long long out = ~__ballot(in);
+            n += out ? __ffsll((long long)out) - 1 : WAVE;
+            more = !out;
         }
-        n = min(n, most);
         const uint16_t* src = is_k ? (const uint16_t*)a.k + t * a.k_st + head * a.k_hs
                                    : (const uint16_t*)a.v + t * a.v_st + head * a.v_hs;
         const int64_t src_st = is_k ? a.k_st : a.v_st;
@@ -177,8 +191,10 @@ __global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_qua
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int r = r0 + RPL * i + lr;
+                    int pos = __shfl(ps, (i0 + r) & (WAVE - 1));
+                    if (r < n && i0 + r >= WAVE) pos = a.positions[t + r];
                     if (r < n && c.turn)
-                        turn<DT, double>(a, a.table + (int64_t)a.positions[t + r] * a.tab_st + 8 * u, x[i], y[i]);
+                        turn<DT, double>(a, a.table + (int64_t)pos * a.tab_st + 8 * u, x[i], y[i]);
                 }
             }
         };
