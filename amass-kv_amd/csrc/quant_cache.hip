@@ -12,7 +12,7 @@
 // where pages have 32 rows and of four beyond (a run of more than 64 rows is read twice), so the maximum is a chain
 // of v_max, six exchanges and at most one barrier.  Runs are found in the slots: where a block
 // starts or the one before is no neighbour.
-// Read: 16 codes a thread, two 16-byte stores.
+// Read: 16 codes a thread, two 16-byte stores (two such units a thread took 86 us where one takes 82).
 #include "quant_codes.h"
 
 namespace amass {
@@ -84,11 +84,11 @@ __device__ __forceinline__ void turn(const amass_quant_write_args& a, const floa
 constexpr int QW_THREADS = 256;
 constexpr int QW_WAVES = QW_THREADS / WAVE;
 constexpr int QW_ROWS = 16;              // rows that a wave holds
-// Tokens that a workgroup looks for runs in: one where the batch is small (every token may start a run, and the runs
-// of a window follow each other), 16 beyond (a prompt's workgroups that found no run would take longer to
-// start than the others to work).
-constexpr int QW_ALONE = 1024;
-constexpr int QW_WINDOW = 16;
+// Tokens that a workgroup looks for runs in: one, 4 or 16 by the batch's tokens.  The runs of a window follow each
+// other, about 1 us each, and a workgroup that finds none costs as much of a place.  us in a graph with windows of
+// 1 / 4 / 16 (32 + 8 heads of 128): 256 single tokens 6.3 / 8.8 / 28.5, a prompt of 256 7.7 / 5.1 / 4.6; 1024: 19.9
+// / 17.5 / 32.0 and 17.2 / 10.5 / 7.1; 2048: 36.3 / 30.3 / 38.5 and 30.3 / 17.5 / 10.5.
+constexpr int window_of(int tokens) { return tokens <= 256 ? 1 : tokens <= 1024 ? 4 : 16; }
 
 template <int D>
 constexpr int LPR_OF = D / 16;           // lanes a row
@@ -266,47 +266,31 @@ __global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_qua
     }
 }
 
-// grid (entry, half and 1024 units of 16 codes of the block)
+// grid (entry, half and 256 units of 16 codes of the block)
 constexpr int QR_THREADS = 256;
-constexpr int QR_UNITS = 4;              // of a thread
 
 template <int DT, int CT, int D>
 __global__ __launch_bounds__(QR_THREADS) void quant_read_kernel(const amass_quant_read_args a, int sh) {
-    constexpr int LPR = D / 16;
+    constexpr int LPR = LPR_OF<D>;
     const int src = a.src[blockIdx.x], dst = a.dst[blockIdx.x];
     if ((uint32_t)src >= (uint32_t)a.nb || (uint32_t)dst >= (uint32_t)a.nb_out) return;
     const bool is_k = !(blockIdx.y & 1);
+    const int e = (blockIdx.y >> 1) * QR_THREADS + threadIdx.x;
+    if (e >= (a.n_kv << sh) * LPR) return;
+    const int rh = e / LPR, c = 16 * (e % LPR), row = rh / a.n_kv, head = rh - row * a.n_kv;
     const uint8_t* codes = (const uint8_t*)(is_k ? a.k_codes : a.v_codes) + src * a.c_sb;
-    const float* scale = (is_k ? a.k_scale : a.v_scale) + src * a.s_sb;
-    uint16_t* out = (uint16_t*)(is_k ? a.k_cache : a.v_cache) + dst * a.o_sb;
-    const int units = (a.n_kv << sh) * LPR;
-    int e = (blockIdx.y >> 1) * (QR_UNITS * QR_THREADS) + threadIdx.x;
-    u32x4_t z[QR_UNITS];
-    float s[QR_UNITS];
-    uint16_t* to[QR_UNITS];
+    const u32x4_t z = *reinterpret_cast<const u32x4_t*>(codes + row * a.c_st + head * a.c_sh + c);
+    const float s = (is_k ? a.k_scale : a.v_scale)[src * a.s_sb + head * a.s_sh];
+    u32x4_t o[2];
 #pragma unroll
-    for (int i = 0; i < QR_UNITS; ++i, e += QR_THREADS) {
-        to[i] = nullptr;
-        if (e < units) {
-            const int rh = e / LPR, c = 16 * (e % LPR), row = rh / a.n_kv, head = rh - row * a.n_kv;
-            z[i] = *reinterpret_cast<const u32x4_t*>(codes + row * a.c_st + head * a.c_sh + c);
-            s[i] = scale[head * a.s_sh];
-            to[i] = out + row * a.o_st + head * a.o_sh + c;
-        }
+    for (int j = 0; j < 4; ++j) {
+        const float4 f = codes_f32<CT>(z[j]);
+        o[j >> 1][2 * (j & 1)] = pack_half<DT>(f.x * s, f.y * s);
+        o[j >> 1][2 * (j & 1) + 1] = pack_half<DT>(f.z * s, f.w * s);
     }
-#pragma unroll
-    for (int i = 0; i < QR_UNITS; ++i) {
-        if (!to[i]) continue;
-        u32x4_t o[2];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float4 f = codes_f32<CT>(z[i][j]);
-            o[j >> 1][2 * (j & 1)] = pack_half<DT>(f.x * s[i], f.y * s[i]);
-            o[j >> 1][2 * (j & 1) + 1] = pack_half<DT>(f.z * s[i], f.w * s[i]);
-        }
-        reinterpret_cast<u32x4_t*>(to[i])[0] = o[0];
-        reinterpret_cast<u32x4_t*>(to[i])[1] = o[1];
-    }
+    uint16_t* to = (uint16_t*)(is_k ? a.k_cache : a.v_cache) + dst * a.o_sb + row * a.o_st + head * a.o_sh + c;
+    reinterpret_cast<u32x4_t*>(to)[0] = o[0];
+    reinterpret_cast<u32x4_t*>(to)[1] = o[1];
 }
 
 // ------------------------------------------------------------------ host
@@ -355,7 +339,7 @@ static int check_read(const amass_quant_read_args& a) {
 
 template <int DT, int CT, int D, int TEAM>
 static int launch_write(const amass_quant_write_args& a, hipStream_t s) {
-    const int64_t window = a.n_tokens <= QW_ALONE ? 1 : QW_WINDOW;
+    const int64_t window = window_of(a.n_tokens);
     const int64_t groups = (2 * a.n_kv * TEAM + QW_WAVES - 1) / QW_WAVES;
     const int64_t kv_wgs = (a.n_tokens + window - 1) / window * groups;
     const int64_t units = a.q ? (int64_t)a.n_tokens * a.n_heads * LPR_OF<D> : 0;
@@ -377,8 +361,8 @@ static int launch_write(const amass_quant_write_args& a, hipStream_t s) {
 template <int DT, int CT>
 static int launch_read(const amass_quant_read_args& a, hipStream_t s) {
     const int sh = log2_of(a.page);
-    const int64_t units = (int64_t)a.n_kv * a.page * (a.d / 16), of_wg = QR_UNITS * QR_THREADS;
-    const int64_t parts = 2 * ((units + of_wg - 1) / of_wg);
+    const int64_t units = (int64_t)a.n_kv * a.page * (a.d / 16);
+    const int64_t parts = 2 * ((units + QR_THREADS - 1) / QR_THREADS);
     if (parts > 65535 || (int64_t)a.n * QR_THREADS > 0xFFFFFFFFll) return AMASS_ERR_GEOMETRY;
     const dim3 grid(a.n, (unsigned)parts);
     if (a.d == 128)
