@@ -59,49 +59,6 @@ __device__ __forceinline__ uint32_t nan2(uint32_t x) {
     return (x & 0x7FFF7FFFu) + (DT == AMASS_BF16 ? 0x007F007Fu : 0x03FF03FFu);
 }
 
-// (the compiler warns of m0, a reserved register, among the clobbers: the loads take their LDS address
-// there, and it has to know)
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-// 16 bytes per lane from base + off (off per lane) to LDS at `to` + 16 lane (`to` uniform).
-// No register waits for it: the caller waits with dma_wait before anyone reads the place.
-__device__ __forceinline__ void dma16(uint32_t to, const char* base, uint32_t off) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(to), "v"(off), "s"(base)
-                 : "memory", "m0");
-}
-// N of them, load n from base + off[n] + 1024 n to `to` + 1024 n + 16 lane: the instruction's
-// offset counts on both sides, so `to` is set once.  ONCE: what nobody reads again soon (it need
-// not stay in a cache).
-#define CK_LOAD(n, at, hint) "\n\tglobal_load_lds_dwordx4 %" #n ", %1 offset:" #at hint
-#define CK_LOADS2(hint) "s_mov_b32 m0, %0\n\ts_nop 0" CK_LOAD(2, 0, hint) CK_LOAD(3, 1024, hint)
-#define CK_LOADS4(hint) CK_LOADS2(hint) CK_LOAD(4, 2048, hint) CK_LOAD(5, 0xc00, hint)
-template <bool ONCE, int N>
-__device__ __forceinline__ void dma16_n(uint32_t to, const char* base, const uint32_t (&off)[N]) {
-    if constexpr (N == 4 && ONCE)
-        asm volatile(CK_LOADS4(" nt")
-                     :
-                     : "s"(to), "s"(base), "v"(off[0]), "v"(off[1]), "v"(off[N - 2]), "v"(off[N - 1])
-                     : "memory", "m0");
-    else if constexpr (N == 4)
-        asm volatile(CK_LOADS4("")
-                     :
-                     : "s"(to), "s"(base), "v"(off[0]), "v"(off[1]), "v"(off[N - 2]), "v"(off[N - 1])
-                     : "memory", "m0");
-    else if constexpr (ONCE)
-        asm volatile(CK_LOADS2(" nt")
-                     :
-                     : "s"(to), "s"(base), "v"(off[0]), "v"(off[1])
-                     : "memory", "m0");
-    else
-        asm volatile(CK_LOADS2("") : : "s"(to), "s"(base), "v"(off[0]), "v"(off[1]) : "memory", "m0");
-}
-#pragma clang diagnostic pop
-template <int N>
-__device__ __forceinline__ void dma_wait() {        // all but the last N loads have arrived
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory");
-}
 // -inf for the keys (relative to the tile) outside [lo, hi) of this lane's row, and those of
 // 16-key groups without a block
 template <int NK>

@@ -94,6 +94,11 @@ struct Lookup {
 };
 
 // ------------------------------------------------------------------ staging
+// bit 7 of every byte that is an e4m3 NaN
+__device__ __forceinline__ uint32_t nan_codes(uint32_t x) {
+    return ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+}
+
 // 16 rows of codes of a page, 16 channels of a row in each of a lane's LOADS registers of 16 bytes.  Rows go
 // to lanes so that 16 neighbouring lanes, whose chunks of 16 bytes a phase of an LDS write takes, hold
 // two rows (d 64: four) with different swizzles and fill all banks once.
@@ -111,14 +116,9 @@ struct Codes {
         off = (uint32_t)row * st + 16 * c;
         lds = row * (2 * D) + (((2 * c) ^ swz<D>(row)) << 4);
     }
-    // ONCE: what nobody reads again soon (it need not stay in a cache)
-    template <bool ONCE = false>
     __device__ __forceinline__ void load(u32x4_t* z, const uint8_t* page) const {
 #pragma unroll
-        for (int n = 0; n < LOADS; ++n) {
-            const u32x4_t* p = reinterpret_cast<const u32x4_t*>(page + off + n * RPL * st);
-            z[n] = ONCE ? __builtin_nontemporal_load(p) : *p;
-        }
+        for (int n = 0; n < LOADS; ++n) z[n] = *reinterpret_cast<const u32x4_t*>(page + off + n * RPL * st);
     }
     // 8 codes of register n (the half h of it), widened, to the image of its 16 rows at `to` (row + 8 turns
     // the chunk's second bit)
@@ -146,7 +146,7 @@ struct Codes {
     __device__ __forceinline__ void poison(u32x4_t& k, u32x4_t& v) const {
         int bad = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) bad |= (int)(((v[j] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u);
+        for (int j = 0; j < 4; ++j) bad |= (int)nan_codes(v[j]);
         if constexpr (LPR == 8) bad |= dpp_i<DPP_HALF_MIRROR>(bad);
         bad |= dpp_i<DPP_XOR2>(bad);
         bad |= dpp_i<DPP_XOR1>(bad);
@@ -370,6 +370,115 @@ __device__ __forceinline__ void ordered_tile(uint32_t ks, uint32_t vs, const Lds
     for (int g = 0; g < 4; ++g) st.l = __builtin_fmaf(sum[g], fa.inv[g], st.l);
 }
 
+// ------------------------------------------------------------------ few rows: codes in LDS
+// Rows of D bytes, 16-byte chunk c of row t at c ^ turn(t): the 16 rows of a K read (one chunk) and the 8 rows of a
+// transposing V read (two chunks) fill the banks once.
+template <int D>
+struct RawRows {
+    static constexpr int ROWS = 1024 / D;          // of one 1-KB load
+    static constexpr int LOADS = 16 / ROWS;        // of 16 rows
+    static constexpr int BACK = 1024 * (LOADS - 1);
+    uint32_t off[LOADS];                           // this lane's source in 16 rows, less the load's own 1024 n,
+                                                   // from BACK before it
+    uint32_t k, v;                                 // its reads, within 32 rows
+    int lane;
+
+    static __device__ __forceinline__ int turn(int row) {
+        return D == 128 ? ((row >> 2) & 1) | (row & 2) | ((row >> 1) & 4) : (row >> 2) & 3;
+    }
+    __device__ __forceinline__ RawRows(uint32_t st, int lane_) : lane(lane_) {
+        const int chunk = lane & (D / 16 - 1), lr = lane / (D / 16);
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) {
+            const int row = ROWS * n + lr;
+            off[n] = (uint32_t)row * st + ((uint32_t)(chunk ^ turn(row)) << 4) + BACK - 1024 * n;
+        }
+        const int row = lane & 31, h = lane >> 5, i16 = lane & 15, sub = (lane >> 4) & 1;
+        k = row * D + ((h ^ turn(row)) << 4);
+        const int t = ((i16 >> 1) & 3) + 8 * (i16 >> 3) + 4 * h;
+        v = t * D + ((sub ^ turn(t)) << 4) + (i16 & 1) * 8;
+    }
+    // 16 rows to LDS
+    template <bool ONCE>
+    __device__ __forceinline__ void load(uint32_t to, const uint8_t* src) const {
+        dma16_n<ONCE>(to, (const char*)src - BACK, off);
+    }
+    // the first `rows` of them, zero behind
+    __device__ __forceinline__ void load_part(char* dst, uint32_t to, const uint8_t* src, int rows) const {
+#pragma unroll
+        for (int n = 0; n < LOADS; ++n) {
+            if (ROWS * n + lane / (D / 16) < rows)
+                dma16(to + 1024 * n, (const char*)src - BACK + 1024 * n, off[n]);
+            else *reinterpret_cast<u32x4_t*>(dst + 1024 * n + 16 * lane) = (u32x4_t){0u, 0u, 0u, 0u};
+        }
+    }
+    // channels 32 n + 16 h .. of key row % 32
+    __device__ __forceinline__ u32x4_t row_codes(uint32_t at, int n) const {
+        return *(const __attribute__((address_space(3))) u32x4_t*)(uintptr_t)((at + k) ^ (uint32_t)(n << 5));
+    }
+    // channel 32 x + lane % 32 of the keys 16 y + 4 h + 0..3 and + 8..11
+    __device__ __forceinline__ u32x2_t column_codes(uint32_t at, int x, int y) const {
+        typedef int i32x2_t __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (__attribute__((address_space(3))) i32x2_t*)(uintptr_t)(((at + v) ^ (uint32_t)(x << 5)) + y * (16 * D))));
+    }
+};
+
+// S^T of 32 keys (ks, and their V at vs).  CARE: a key whose V holds a NaN scores NaN.
+template <int DT, int CT, int D, bool CARE>
+__device__ __forceinline__ void few_scores(uint32_t ks, uint32_t vs, const RawRows<D>& raw,
+                                           const u32x4_t (&q)[D / 16], f32x16_t& s) {
+    uint32_t bad = 0;
+    if constexpr (CARE && CT == AMASS_E4M3) {
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) {
+            const u32x4_t z = raw.row_codes(vs, n);
+            bad |= nan_codes(z[0]) | nan_codes(z[1]) | nan_codes(z[2]) | nan_codes(z[3]);
+        }
+        const auto o = __builtin_amdgcn_permlane32_swap(bad, bad, false, false);
+        bad = o[0] | o[1];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) {
+        u32x4_t z = raw.row_codes(ks, n), f[2];
+        if constexpr (CARE && CT == AMASS_E4M3) {
+            if (bad) z = (u32x4_t){0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu};
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t lo, hi;
+            widen4<DT, CT>(z[j], lo, hi);
+            f[j >> 1][2 * (j & 1)] = lo;
+            f[j >> 1][2 * (j & 1) + 1] = hi;
+        }
+        s = mfma32<DT>(f[0], q[2 * n], s);
+        s = mfma32<DT>(f[1], q[2 * n + 1], s);
+    }
+}
+
+template <int DT, int CT, int D, bool CARE>
+__device__ __forceinline__ void few_values(uint32_t vs, const RawRows<D>& raw, const u32x4_t (&p)[2],
+                                           RowState<D>& st) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int z = 0; z < D / 32; ++z) {
+            u32x2_t c = raw.column_codes(vs, z, y);
+            u32x4_t f;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t lo, hi;
+                if constexpr (CARE && CT == AMASS_E4M3) c[j] &= ~((nan_codes(c[j]) >> 7) * 0xFFu);
+                widen4<DT, CT>(c[j], lo, hi);
+                f[2 * j] = lo;
+                f[2 * j + 1] = hi;
+            }
+            st.o[z] = mfma32<DT>(f, p[y], st.o[z]);
+        }
+}
+
 // whether a row that is there needs all of it again with care: it is not finite, or its maximum so far
 // from zero that log2 sv less the maximum, rounded, moves the weights of one page against
 // another's (by 2^-12 at 2^12, and in fp16 beyond its largest at 2^27)
@@ -530,10 +639,13 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
     u32x4_t q[D / 16];
     {
         const uint16_t* src = (const uint16_t*)a.q + (int64_t)(it.q.q0 + tok) * a.q_st +
-                              (int64_t)(kh * a.G + (row - tok * a.G)) * a.q_hs + 8 * (lane >> 5);
+                              (int64_t)(kh * a.G + (row - tok * a.G)) * a.q_hs;
+        const int h = lane >> 5;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-            q[i] = live ? *reinterpret_cast<const u32x4_t*>(src + 16 * i) : (u32x4_t){0u, 0u, 0u, 0u};
+        for (int i = 0; i < D / 16; ++i) {         // (in the order that K comes in: few_scores)
+            const int at = few ? 32 * (i >> 1) + 16 * h + 8 * (i & 1) : 16 * i + 8 * h;
+            q[i] = live ? *reinterpret_cast<const u32x4_t*>(src + at) : (u32x4_t){0u, 0u, 0u, 0u};
+        }
     }
     // (here, not in the loop over the keys, where a wait would also wait for the next tile's loads)
 #pragma unroll
@@ -699,73 +811,76 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
         return;
     }
     // ---- few rows: each wave its own 32 keys, w + 4, w + 8, ... ------------------------
-    constexpr int HB = KB / 2;                     // 32 widened keys
-    const uint32_t base = lds_addr(lds.kv + 2 * HB * w);
+    // Codes go from HBM to LDS as they are, two steps ahead (K and V two places each, in turn), and are widened
+    // on their way into a matrix operand: no wave shares a key with another here.
+    using Raw = RawRows<D>;
+    constexpr int SLOT = 32 * D, L = 2 * Raw::LOADS;     // bytes of 32 keys' K; its loads
+    char* own = lds.kv + 4 * SLOT * w;                   // K, K, V, V
+    const uint32_t base = lds_addr(own);
     const int b0 = 2 * (sp.lo + j0) + w, b1 = 2 * (sp.lo + j1);
+    const Raw raw((uint32_t)a.kv_st, lane);
     Lookup<2> lk;
-    u32x4_t kr[2][LOADS], vr[2][LOADS];
-    const auto fetch = [&](auto past, u32x4_t (&z)[2][LOADS], const uint8_t* from, int b, int s) {
+    // both of 32 keys of step s (b: their number); true if the usual number of loads is in flight
+    const auto issue_k = [&](auto past, int slot, int b, int s) {
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            // (a page without a block: block 0, whose weights are zero and V is cut off)
-            cd.template load<past>(z[g], from + page_at(max(lk.block(s, g), 0), 32 * b + 16 * g));
+        for (int g = 0; g < 2; ++g)       // (a page without a block: block 0, whose weights are zero)
+            raw.template load<past>(base + slot * SLOT + g * (SLOT / 2),
+                                    k0 + page_at(max(lk.block(s, g), 0), 32 * b + 16 * g));
+    };
+    const auto issue_v = [&](auto past, int slot, int b, int s) -> bool {
+        const int id0 = lk.block(s, 0), id1 = lk.block(s, 1), to = (2 + slot) * SLOT;
+        const int64_t at0 = page_at(max(id0, 0), 32 * b), at1 = page_at(max(id1, 0), 32 * b + 16);
+        if (id0 >= 0 && id1 >= 0 && 32 * b + 32 <= len) {
+            raw.template load<past>(base + to, v0 + at0);
+            raw.template load<past>(base + to + SLOT / 2, v0 + at1);
+            return true;
         }
+        raw.load_part(own + to, base + to, v0 + at0, id0 >= 0 ? len - 32 * b : 0);
+        raw.load_part(own + to + SLOT / 2, base + to + SLOT / 2, v0 + at1, id1 >= 0 ? len - 32 * b - 16 : 0);
+        return false;
     };
-    const auto widen = [&](const u32x4_t (&z)[2][LOADS], uint32_t to) {
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int i = 0; i < 2 * LOADS; ++i)
-            {
-                cd.template put<DT, CT>(to + g * (HB / 2), i >> 1, i & 1, z[g][i >> 1]);
-                step();
-            }
-    };
-    const auto fence = [] { asm volatile("" ::: "memory"); };
     const auto walk = [&](auto past, auto care) {
         reset(st);
+        bool v_now = true, v_next = true;          // the usual number of loads of this step's and the next one's V
         if (b0 < b1) {
             look(lk, 32 * (b0 + CK_WAVES * (lane >> 1)) + 16 * (lane & 1), 32 * 32 * CK_WAVES);
-            fetch(past, kr, k0, b0, 0);
-            fetch(past, vr, v0, b0, 0);
+            issue_k(past, 0, b0, 0);
+            v_now = issue_v(past, 0, b0, 0);
+            if (b0 + CK_WAVES < b1) {
+                issue_k(past, 1, b0 + CK_WAVES, 1);
+                v_next = issue_v(past, 1, b0 + CK_WAVES, 1);
+            }
         }
-        for (int b = b0, s = 0; b < b1; b += CK_WAVES) {
+        for (int b = b0, s = 0, slot = 0; b < b1; b += CK_WAVES, slot ^= 1) {
             const int t0 = 32 * b;
-            const bool more = b + CK_WAVES < b1;
-            const uint32_t groups = lk.groups(s);
-            if (t0 + 32 > len || groups != 3u) {
-#pragma unroll
-                for (int g = 0; g < 2; ++g)
-#pragma unroll
-                    for (int n = 0; n < LOADS; ++n)
-                        cd.clip(vr[g][n], n, groups >> g & 1 ? len - t0 - 16 * g : 0);
-            }
-            if constexpr (CT == AMASS_E4M3 && care) {
-#pragma unroll
-                for (int g = 0; g < 2; ++g)
-#pragma unroll
-                    for (int n = 0; n < LOADS; ++n) cd.poison(kr[g][n], vr[g][n]);
-            }
-            widen(kr, base);
-            fence();
-            if (more) fetch(past, kr, k0, b + CK_WAVES, s + 1);
-            lk.ahead(s);
-            const Factors<2> f(lk, s);
+            const bool one = b + CK_WAVES < b1, two = b + 2 * CK_WAVES < b1, even = !care && v_now && v_next;
+            const uint32_t ks = base + slot * SLOT, vs = ks + 2 * SLOT;
+            if (even && one) dma_wait<3 * L>();    // (V of this step, K and V of the next may be on their way)
+            else if (even) dma_wait<L>();
+            else dma_wait<0>();
             f32x16_t sc1[1];
             u32x4_t p[2];
-            scores<DT, D, 1>(base, ll, q, sc1);
-            if (care || t0 < lo_hi || t0 + 32 > hi_lo) mask_scores<1>(sc1, lo - t0, hi - t0, groups, lane);
+            few_scores<DT, CT, D, care>(ks, vs, raw, q, sc1[0]);
+            dma_wait<63>();                        // (the reads have returned)
+            if (two) issue_k(past, slot, b + 2 * CK_WAVES, s + 2);
+            lk.ahead(s);
+            const Factors<2> f(lk, s);
+            if (care || t0 < lo_hi || t0 + 32 > hi_lo)
+                mask_scores<1>(sc1, lo - t0, hi - t0, lk.groups(s), lane);
             weigh_tile<DT, D, 1, care>(sc1, f, st, p);
-            widen(vr, base + HB);
-            fence();
-            if (more) fetch(past, vr, v0, b + CK_WAVES, s + 1);
-            add_values<DT, D, 1>(base + HB, ll, p, st);
-            fence();
+            if (even && two) dma_wait<3 * L>();
+            else if (even && one) dma_wait<2 * L>();
+            else dma_wait<0>();
+            few_values<DT, CT, D, care>(vs, raw, p, st);
+            dma_wait<63>();
+            v_now = v_next;
+            v_next = two ? issue_v(past, slot, b + 2 * CK_WAVES, s + 2) : true;
             if (++s == Lookup<2>::STEPS) {
                 lk.turn();
                 s = 0;
             }
         }
+        dma_wait<0>();
     };
     if (once) walk(std::true_type(), std::false_type());
     else walk(std::false_type(), std::false_type());
