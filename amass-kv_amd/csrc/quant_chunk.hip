@@ -811,70 +811,63 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
         return;
     }
     // ---- few rows: each wave its own 32 keys, w + 4, w + 8, ... ------------------------
-    // Codes go from HBM to LDS as they are, two steps ahead (K and V two places each, in turn), and are widened
-    // on their way into a matrix operand: no wave shares a key with another here.
+    // Codes go from HBM to LDS as they are, a step ahead, and are widened on their way into a matrix operand: no
+    // wave shares a key with another here.  (Two steps ahead, 128 KB in flight a CU, 64 single tokens with 8k keys
+    // took 2 to 3 % longer.)
     using Raw = RawRows<D>;
-    constexpr int SLOT = 32 * D, L = 2 * Raw::LOADS;     // bytes of 32 keys' K; its loads
-    char* own = lds.kv + 4 * SLOT * w;                   // K, K, V, V
+    constexpr int HALF = 32 * D, L = 2 * Raw::LOADS;     // bytes of 32 keys' K; its loads
+    char* own = lds.kv + 2 * HALF * w;                   // K, then V
     const uint32_t base = lds_addr(own);
     const int b0 = 2 * (sp.lo + j0) + w, b1 = 2 * (sp.lo + j1);
     const Raw raw((uint32_t)a.kv_st, lane);
     Lookup<2> lk;
-    // both of 32 keys of step s (b: their number); true if the usual number of loads is in flight
-    const auto issue_k = [&](auto past, int slot, int b, int s) {
+    // 32 keys of step s (b: their number); of V true if the usual number of loads is in flight
+    const auto issue_k = [&](auto past, int b, int s) {
 #pragma unroll
         for (int g = 0; g < 2; ++g)       // (a page without a block: block 0, whose weights are zero)
-            raw.template load<past>(base + slot * SLOT + g * (SLOT / 2),
-                                    k0 + page_at(max(lk.block(s, g), 0), 32 * b + 16 * g));
+            raw.template load<past>(base + g * (HALF / 2), k0 + page_at(max(lk.block(s, g), 0), 32 * b + 16 * g));
     };
-    const auto issue_v = [&](auto past, int slot, int b, int s) -> bool {
-        const int id0 = lk.block(s, 0), id1 = lk.block(s, 1), to = (2 + slot) * SLOT;
+    const auto issue_v = [&](auto past, int b, int s) -> bool {
+        const int id0 = lk.block(s, 0), id1 = lk.block(s, 1);
         const int64_t at0 = page_at(max(id0, 0), 32 * b), at1 = page_at(max(id1, 0), 32 * b + 16);
         if (id0 >= 0 && id1 >= 0 && 32 * b + 32 <= len) {
-            raw.template load<past>(base + to, v0 + at0);
-            raw.template load<past>(base + to + SLOT / 2, v0 + at1);
+            raw.template load<past>(base + HALF, v0 + at0);
+            raw.template load<past>(base + HALF + HALF / 2, v0 + at1);
             return true;
         }
-        raw.load_part(own + to, base + to, v0 + at0, id0 >= 0 ? len - 32 * b : 0);
-        raw.load_part(own + to + SLOT / 2, base + to + SLOT / 2, v0 + at1, id1 >= 0 ? len - 32 * b - 16 : 0);
+        raw.load_part(own + HALF, base + HALF, v0 + at0, id0 >= 0 ? len - 32 * b : 0);
+        raw.load_part(own + HALF + HALF / 2, base + HALF + HALF / 2, v0 + at1, id1 >= 0 ? len - 32 * b - 16 : 0);
         return false;
     };
     const auto walk = [&](auto past, auto care) {
         reset(st);
-        bool v_now = true, v_next = true;          // the usual number of loads of this step's and the next one's V
+        bool full = true;                          // the usual number of loads of V is in flight
         if (b0 < b1) {
             look(lk, 32 * (b0 + CK_WAVES * (lane >> 1)) + 16 * (lane & 1), 32 * 32 * CK_WAVES);
-            issue_k(past, 0, b0, 0);
-            v_now = issue_v(past, 0, b0, 0);
-            if (b0 + CK_WAVES < b1) {
-                issue_k(past, 1, b0 + CK_WAVES, 1);
-                v_next = issue_v(past, 1, b0 + CK_WAVES, 1);
-            }
+            issue_k(past, b0, 0);
+            full = issue_v(past, b0, 0);
         }
-        for (int b = b0, s = 0, slot = 0; b < b1; b += CK_WAVES, slot ^= 1) {
+        for (int b = b0, s = 0; b < b1; b += CK_WAVES) {
             const int t0 = 32 * b;
-            const bool one = b + CK_WAVES < b1, two = b + 2 * CK_WAVES < b1, even = !care && v_now && v_next;
-            const uint32_t ks = base + slot * SLOT, vs = ks + 2 * SLOT;
-            if (even && one) dma_wait<3 * L>();    // (V of this step, K and V of the next may be on their way)
-            else if (even) dma_wait<L>();
+            const bool more = b + CK_WAVES < b1;
+            const uint32_t ks = base, vs = base + HALF;
+            if (!care && full) dma_wait<L>();      // (V may be on its way)
             else dma_wait<0>();
             f32x16_t sc1[1];
             u32x4_t p[2];
             few_scores<DT, CT, D, care>(ks, vs, raw, q, sc1[0]);
             dma_wait<63>();                        // (the reads have returned)
-            if (two) issue_k(past, slot, b + 2 * CK_WAVES, s + 2);
+            if (more) issue_k(past, b + CK_WAVES, s + 1);
             lk.ahead(s);
             const Factors<2> f(lk, s);
             if (care || t0 < lo_hi || t0 + 32 > hi_lo)
                 mask_scores<1>(sc1, lo - t0, hi - t0, lk.groups(s), lane);
             weigh_tile<DT, D, 1, care>(sc1, f, st, p);
-            if (even && two) dma_wait<3 * L>();
-            else if (even && one) dma_wait<2 * L>();
+            if (more && full) dma_wait<L>();       // (the next K may be)
             else dma_wait<0>();
             few_values<DT, CT, D, care>(vs, raw, p, st);
             dma_wait<63>();
-            v_now = v_next;
-            v_next = two ? issue_v(past, slot, b + 2 * CK_WAVES, s + 2) : true;
+            if (more) full = issue_v(past, b + CK_WAVES, s + 1);
             if (++s == Lookup<2>::STEPS) {
                 lk.turn();
                 s = 0;

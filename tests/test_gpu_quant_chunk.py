@@ -83,6 +83,59 @@ def test_matches_float64(name, code):
     c.check(*c.run())
 
 
+# batches of few rows only
+FEW = {
+    "one token": dict(new=[1], lens=[1]),
+    "16 rows": dict(new=[4, 2, 4], lens=[1000, 40, 129]),
+    "16 rows, one short": dict(new=[4, 1], lens=[333, 6000]),
+    "17 rows": dict(new=[4, 1], lens=[333, 500], G=17),
+    "one long row, split": dict(new=[1], lens=[9000], G=8),
+    "split, 6 heads": dict(new=[3, 1], lens=[7000, 3000], n_kv=6, G=5),
+    "past a period": dict(new=[2], lens=[20000], n_kv=2, G=1),
+    "decode step": dict(new=[1] * 40, lens=[16 * i + 7 for i in range(40)], n_kv=8),
+    "many requests": dict(new=[1 + i % 3 for i in range(150)], lens=[3 + 5 * i for i in range(150)], G=2),
+    "thousands of requests": dict(new=[1] * 3400, lens=[1 + i % 29 for i in range(3400)], G=1),
+    "empty requests": dict(new=[0, 3, 0, 4, 0], lens=[33, 9, 0, 77, 5], pad=6),
+    "heads of 64": dict(new=[4, 1, 2], lens=[700, 64, 33], d=64, n_kv=4),
+    "heads of 64, split": dict(new=[1], lens=[9000], d=64),
+    "fp16": dict(new=[4, 1], lens=[700, 64], dtype="fp16"),
+    "fp16 of 64": dict(new=[4, 1], lens=[700, 6400], dtype="fp16", d=64),
+    "window": dict(new=[4, 2], lens=[400, 500], window=50),
+    "window of one": dict(new=[4, 3], lens=[90, 70], window=1),
+    "not causal": dict(new=[4, 2], lens=[100, 333], causal=False),
+    "rows before position 0": dict(new=[4, 3], lens=[2, 3]),
+    "pages of 64": dict(new=[4, 4], lens=[145, 700], page=64, n_kv=4),
+    "pages of 1024, halves first": dict(new=[4, 4], lens=[145, 2700], page=1024, halves_first=True),
+    "peaked": dict(new=[4, 3], lens=[200, 100], loud=12.0),
+    "more than the chip takes": dict(new=[1] * 300, lens=[70 + i for i in range(300)], n_kv=8),
+    "a few far longer": dict(new=[1] * 300, lens=[70 + 9000 * (i % 150 == 3) for i in range(300)], n_kv=8, G=2),
+}
+
+
+@pytest.mark.parametrize("name", FEW)
+@pytest.mark.parametrize("code", CODES)
+def test_few_rows(name, code):
+    announce(f"quant attention: few rows, {name}, {code}")
+    c = QuantCase(code=code, **FEW[name])
+    c.check(*c.run())
+
+
+def test_other_layouts():
+    """A page of one head contiguous, and heads more than 2^30 bytes apart."""
+    announce("quant attention: strides of heads")
+    c = QuantCase(new=[4, 1, 2], lens=[700, 90, 33], n_kv=4)
+    q, codes, scales, table, lens, qs = c.dev()
+    major = codes.transpose(2, 3).contiguous().transpose(2, 3)
+    nb = codes.shape[0]
+    room = torch.empty(4, (1 << 30) + 16, dtype=torch.int8, device=DEV)
+    far = room[:, :codes[:, :, :, 0].numel()].view(4, nb, 2, 16, 128).permute(1, 2, 3, 0, 4)
+    far.copy_(codes)
+    for cache in (major, far):
+        out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device=DEV)
+        quant_chunk_attention(q, cache, scales, table, lens, qs, out, lse=lse)
+        c.check(out, lse)
+
+
 @pytest.mark.parametrize("name", ROUNDS)
 def test_more_tiles_than_the_chip_takes(name):
     announce(f"quant attention: {name}, more tiles than the chip takes at a time")
@@ -171,11 +224,43 @@ def test_scales_that_are_not_finite(new, lens, page, value, half, code):
         c.check(out, lse, rows=rest)
 
 
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("fp16", 64)])
+@pytest.mark.parametrize("half,head", [(0, 0), (0, 1), (1, 0), (1, 1)])
+@pytest.mark.parametrize("what", ["code", "scale"])
+def test_nan_of_one_head(what, half, head, dtype, d):
+    """It reaches the rows of its head that see it: not the other head's, nor rows before."""
+    announce(f"quant attention: a NaN {what} of head {head}, half {half}, {dtype}")
+    for new, lens, at in (([4], [300], 298), ([4, 2], [80, 5000], 4999), ([3], [50], 48)):
+        c = QuantCase(new=new, lens=lens, dtype=dtype, d=d, n_kv=2, G=2, code="e4m3")
+        want = c.want()
+        r = len(new) - 1
+        block, row = c.token(r, at)
+        if what == "code":
+            c.codes.view(torch.int8)[block, half, row, head, 5] = 0x7F
+        else:
+            c.scales[block, half, head] = float("nan")
+            at = at // 16 * 16
+        out, lse = c.run()
+        q0, q1 = int(c.qs[r]), int(c.qs[r + 1])
+        sees = [q0 + i for i in range(q1 - q0) if lens[r] - new[r] + i >= at]
+        heads = slice(2 * head, 2 * head + 2)
+        assert sees and torch.isnan(out[sees][:, heads].float()).all()
+        out[sees, heads] = torch.tensor(want[0][sees, heads], dtype=c.dt, device=DEV)
+        lse[sees, heads] = torch.tensor(want[1][sees, heads], dtype=torch.float32, device=DEV)
+        c.want = lambda: want
+        c.check(out, lse)
+
+
 @pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("n_kv", [1, 2])
 @pytest.mark.parametrize("new,lens", [([1, 3], [300, 200]), ([70], [300]), ([4], [5000]), ([280], [400])])
-def test_pages_without_a_block_are_masked(new, lens, code):
+def test_pages_without_a_block_are_masked(new, lens, code, n_kv):
     announce(f"quant attention: blocks outside the pool, {new} of {lens}")
-    c = QuantCase(new=new, lens=lens, n_kv=1, spare=0, code=code)
+    c = QuantCase(new=new, lens=lens, n_kv=n_kv, spare=0, code=code)
+    c.codes.view(torch.int8)[0] = 0x7F if code == "e4m3" else 99       # (block 0, read in their place)
+    c.table[c.table == 0] = -1
+    c.numbers()
+    c.k, c.v = c.k.nan_to_num(), c.v.nan_to_num()
     nb = c.codes.shape[0]
     c.table[0, 1:8:2] = torch.tensor([-1, nb, 2 ** 31 - 1, -2 ** 31], dtype=torch.int64).int()
     c.table[0, 10] = nb + 5
