@@ -59,27 +59,32 @@ def _geometry(page, d, dtype):
 
 
 def _halves(codes, scales, writes):
-    """((blocks, page, n_kv, d), (k, v, block, row, head strides of codes), (k, v, block, head
-    strides of scales)) of a checked cache."""
-    shape, st = codes.shape, codes.stride()
-    if len(shape) != 5 or (shape[0] != 2 and shape[1] != 2):
+    """((blocks, page, n_kv, d), code type, (k, v, block, row, head strides of codes), (k, v, block,
+    head strides of scales)) of a checked cache."""
+    shape, st, dt = codes.shape, codes.stride(), codes.dtype
+    if len(shape) != 5:
         raise ValueError("codes must be (NB, 2, page, n_kv, d) or (2, NB, page, n_kv, d)")
-    first = shape[0] == 2
-    nb, (page, n_kv, d) = shape[1] if first else shape[0], shape[2:]
-    _geometry(page, d, codes.dtype)
-    if scales.dtype is not torch.float32 or scales.shape != (shape[0], shape[1], n_kv):
-        raise ValueError(f"scales must be ({shape[0]}, {shape[1]}, {n_kv}) fp32")
-    sb, half = (st[1], st[0]) if first else (st[0], st[1])
-    s0, s1, s_sh = scales.stride()
-    s_sb, s_half = (s1, s0) if first else (s0, s1)
-    _, _, row, head, unit = st
+    n0, n1, page, n_kv, d = shape
+    if scales.dtype is not torch.float32 or scales.shape != (n0, n1, n_kv):
+        raise ValueError(f"scales must be ({n0}, {n1}, {n_kv}) fp32")
+    if n0 == 2:
+        nb = n1
+        half, sb, row, head, unit = st
+        s_half, s_sb, s_sh = scales.stride()
+    elif n1 == 2:
+        nb = n0
+        sb, half, row, head, unit = st
+        s_sb, s_half, s_sh = scales.stride()
+    else:
+        raise ValueError("codes must be (NB, 2, page, n_kv, d) or (2, NB, page, n_kv, d)")
+    _geometry(page, d, dt)
     if unit != 1:
         raise ValueError("codes need unit stride on the head dim")
-    if writes and (not (sb or nb == 1) or not half or not row or not (head or n_kv == 1) or
-                   not (s_sb or nb == 1) or not s_half or not (s_sh or n_kv == 1)):
+    if writes and (0 in (half, row, s_half) or (nb > 1 and 0 in (sb, s_sb)) or
+                   (n_kv > 1 and 0 in (head, s_sh))):
         raise ValueError("rows of codes or scales share memory")
     at, s_at = codes.data_ptr(), scales.data_ptr()
-    return ((nb, page, n_kv, d), (at, at + half, sb, row, head),
+    return ((nb, page, n_kv, d), CODES[dt], (at, at + half, sb, row, head),
             (s_at, s_at + 4 * s_half, s_sb, s_sh))
 
 
@@ -97,20 +102,27 @@ def quant_paged_write(k, v, codes, scales, slots, *, q=None, positions=None, tab
     to its type and then to a code; a row whose position is outside the table is passed over.
     With ``q`` (T, H, d) too, q is turned into ``q_out`` (``None``: in place), as
     ``rope_paged_write`` does.  k, v, q and codes need 16-byte aligned rows."""
-    if q is None and q_out is not None:
-        raise ValueError("q_out without q")
-    if (table is None) != (positions is None) or (q is not None and table is None):
-        raise ValueError("q needs positions and table, and each of those the other")
-    q_out = q if q_out is None else q_out
+    if q is None:
+        if q_out is not None:
+            raise ValueError("q_out without q")
+        if (table is None) != (positions is None):
+            raise ValueError("positions and table need each other")
+    else:
+        if table is None or positions is None:
+            raise ValueError("q needs positions and table")
+        if q_out is None:
+            q_out = q
     index = device_index(k, v, codes, scales, slots, q, positions, table, q_out)
     dt = k.dtype
-    if not (dt in DTYPES and dt is v.dtype and (q is None or dt is q.dtype is q_out.dtype)):
+    if dt not in DTYPES or dt is not v.dtype or \
+            (q is not None and not dt is q.dtype is q_out.dtype):
         raise ValueError("k, v, q and q_out must all be bf16 or all fp16")
     if layout not in LAYOUTS:
         raise ValueError(f"layout {layout!r}: 'half' or 'interleaved'")
-    (nb, page, n_kv, d), c, s = _halves(codes, scales, True)
-    T = k.shape[0]
-    if k.shape != (T, n_kv, d) or v.shape != k.shape:
+    (nb, page, n_kv, d), kind, c, s = _halves(codes, scales, True)
+    shape = k.shape
+    T = shape[0]
+    if shape != (T, n_kv, d) or v.shape != shape:
         raise ValueError(f"k and v must be (T, {n_kv}, {d})")
     vector(slots, torch.int64, T, "slots")
     k_st, k_hs, k_unit = k.stride()
@@ -118,13 +130,17 @@ def quant_paged_write(k, v, codes, scales, slots, *, q=None, positions=None, tab
     q_at = q_st = q_hs = o_at = o_st = o_hs = H = 0
     q_unit = o_unit = 1
     if q is not None:
-        H = q.shape[1] if q.dim() == 3 else 0
-        if H == 0 or q.shape != (T, H, d) or q_out.shape != q.shape:
+        shape = q.shape
+        if len(shape) != 3 or shape[0] != T or shape[1] == 0 or shape[2] != d or \
+                (q_out is not q and q_out.shape != shape):
             raise ValueError(f"q and q_out must be (T, H, {d})")
-        q_at, o_at = q.data_ptr(), q_out.data_ptr()
-        q_st, q_hs, q_unit = q.stride()
-        o_st, o_hs, o_unit = q_out.stride()
-        if not (o_st or T == 1) or not (o_hs or H == 1):
+        H = shape[1]
+        q_at = o_at = q.data_ptr()
+        q_st, q_hs, q_unit = o_st, o_hs, o_unit = q.stride()
+        if q_out is not q:
+            o_at = q_out.data_ptr()
+            o_st, o_hs, o_unit = q_out.stride()
+        if (o_st == 0 and T > 1) or (o_hs == 0 and H > 1):
             raise ValueError("rows or heads of q_out share memory")
     if not k_unit == v_unit == q_unit == o_unit == 1:
         raise ValueError("k / v / q / q_out need unit stride on the head dim")
@@ -141,7 +157,7 @@ def quant_paged_write(k, v, codes, scales, slots, *, q=None, positions=None, tab
     call_on(index, "amass_quant_write", _pack_write(       # in the struct's order
         k.data_ptr(), k_st, k_hs, v.data_ptr(), v_st, v_hs, q_at, q_st, q_hs, o_at, o_st, o_hs,
         *c, *s, tab_at, tab_st, pos_at, slots.data_ptr(), T, H, n_kv, d, rot, page, nb, max_pos,
-        LAYOUTS[layout], DTYPES[dt], CODES[codes.dtype]))
+        LAYOUTS[layout], DTYPES[dt], kind))
 
 
 def quant_paged_read(codes, scales, src, kv_cache, dst) -> None:
@@ -152,22 +168,22 @@ def quant_paged_read(codes, scales, src, kv_cache, dst) -> None:
     index = device_index(codes, scales, src, kv_cache, dst)
     if kv_cache.dtype not in DTYPES:
         raise ValueError("kv_cache must be bf16 or fp16")
-    (nb, page, n_kv, d), c, s = _halves(codes, scales, False)
+    (nb, page, n_kv, d), kind, c, s = _halves(codes, scales, False)
     (nb_out, *shape), k, v, (o_sb, o_st, o_sh, unit) = cache_halves(kv_cache)
     if v == 0 or tuple(shape) != (page, n_kv, d):
         raise ValueError(f"kv_cache must have V and pages of ({page}, {n_kv}, {d})")
     if unit != 1 or not (o_sb or nb_out == 1) or not o_st or not (o_sh or n_kv == 1) or k == v:
         raise ValueError("kv_cache needs unit stride on the head dim and rows of their own")
     n = src.numel()
-    vector(src, torch.int32, n, "src")
-    vector(dst, torch.int32, n, "dst")
     if dst.numel() != n:
         raise ValueError(f"{n} blocks in src, {dst.numel()} in dst")
+    vector(src, torch.int32, n, "src")
+    vector(dst, torch.int32, n, "dst")
     if n == 0 or nb == 0 or nb_out == 0:
         return
     call_on(index, "amass_quant_read", _pack_read(         # in the struct's order
         *c, *s, k, v, o_sb, o_st, o_sh, src.data_ptr(), dst.data_ptr(), n, n_kv, d, page, nb,
-        nb_out, DTYPES[kv_cache.dtype], CODES[codes.dtype]))
+        nb_out, DTYPES[kv_cache.dtype], kind))
 
 
 def _chunk_args(q, codes, scales, block_table, seq_lens, query_start, out, scale, causal, window,
@@ -176,7 +192,7 @@ def _chunk_args(q, codes, scales, block_table, seq_lens, query_start, out, scale
     dt = q.dtype
     if not (dt in DTYPES and dt is out.dtype):
         raise ValueError("q and out must both be bf16 or both fp16")
-    (nb, page, n_kv, d), c, s = _halves(codes, scales, False)
+    (nb, page, n_kv, d), kind, c, s = _halves(codes, scales, False)
     shape = q.shape
     if len(shape) != 3 or shape[2] != d or out.shape != shape:
         raise ValueError(f"q and out must be (T, H, {d})")
@@ -213,7 +229,7 @@ def _chunk_args(q, codes, scales, block_table, seq_lens, query_start, out, scale
     return ((q.data_ptr(), q_st, q_hs, *c, *s, block_table.data_ptr(), bt_st, seq_lens.data_ptr(),
              query_start.data_ptr(), out.data_ptr(), o_st, o_hs, l_at, l_st, l_hs),
             (scale, n_req, T, n_kv, H // n_kv, d, page, nb, width, 1 if causal else 0,
-             min(window or 0, MAX_INT), DTYPES[dt], CODES[codes.dtype]))
+             min(window or 0, MAX_INT), DTYPES[dt], kind))
 
 
 def _scratch_bytes(index, head, tail) -> int:
