@@ -2,7 +2,7 @@
 // (amass_quant_read).
 //
 // Mathematics.  Write: a run of tokens in a block has one scale per half and head, s = max(step(max
-// |x|), scale so far), and codes round(x / s).  K is turned in 64 bits first: a product of an
+// |x|), scale so far), and codes round(x / s).  K is turned first, as if in 64 bits: a product of an
 // 8- or 11-bit number with an fp32 cosine is exact there and the difference rounded once, so that the 16-bit
 // key, and with it the code, is the formula's and not one of the two beside it.  The int8 scales have
 // 8 significant bits: then no quotient that is not half way between two codes lies nearer to it
@@ -45,9 +45,12 @@ __device__ __forceinline__ Chan channels(const amass_quant_write_args& a, int u,
     c.c1 = apart ? (a.rot >> 1) + 8 * u : 16 * u + 8;
     return c;
 }
-// the 8 pairs of x (c0 ..) and y (c1 ..) turned: pair i is (x[i], y[i]), or interleaved two
-// neighbours.  F: the type of the products.
-template <int DT, class F>
+// the 8 pairs of x (c0 ..) and y (c1 ..) turned: pair i is (x[i], y[i]), or interleaved two neighbours.
+// EXACT: the 16-bit numbers that the products in 64 bits round to (through fp32).  The fp32 ones are off by less than
+// 2^-22 (|f| + |g|) (|c| + |s|), so they round to others only that near to a border between two, once in thousands.
+// fp16 asks 64 bits only there, bf16 always (us of three chunks of 1967 tokens: fp16 14.8 and paired 16.6 with 64 bits
+// always, 13.7 and 13.7 so; bf16 12.3 and 12.4 always, 12.7 and 12.8 so).
+template <int DT, bool EXACT>
 __device__ __forceinline__ void turn(const amass_quant_write_args& a, const float* tab, u32x4_t& x,
                                      u32x4_t& y) {
     const float4* tc = reinterpret_cast<const float4*>(tab);
@@ -55,28 +58,47 @@ __device__ __forceinline__ void turn(const amass_quant_write_args& a, const floa
     const float4 c0 = tc[0], c1 = tc[1], s0 = ts[0], s1 = ts[1];
     const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
     const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-    const auto pair = [&](float f, float g, int i, float& p, float& r) {
-        const F c = cs[i], s = sn[i];
-        p = (float)((F)f * c - (F)g * s);
-        r = (float)((F)g * c + (F)f * s);
-    };
-    if (a.interleaved) {
+    float f[8], g[8], p[8], r[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float p, r;
-            pair(half_f32<DT>(x[i], 0), half_f32<DT>(x[i], 1), i, p, r);
-            x[i] = pack_half<DT>(p, r);
-            pair(half_f32<DT>(y[i], 0), half_f32<DT>(y[i], 1), 4 + i, p, r);
-            y[i] = pack_half<DT>(p, r);
+    for (int i = 0; i < 8; ++i) {
+        f[i] = a.interleaved ? half_f32<DT>(i < 4 ? x[i] : y[i - 4], 0) : half_f32<DT>(x[i >> 1], i & 1);
+        g[i] = a.interleaved ? half_f32<DT>(i < 4 ? x[i] : y[i - 4], 1) : half_f32<DT>(y[i >> 1], i & 1);
+        if constexpr (EXACT && DT == AMASS_BF16) {
+            p[i] = (float)((double)f[i] * cs[i] - (double)g[i] * sn[i]);
+            r[i] = (float)((double)g[i] * cs[i] + (double)f[i] * sn[i]);
+        } else {
+            p[i] = f[i] * cs[i] - g[i] * sn[i];
+            r[i] = g[i] * cs[i] + f[i] * sn[i];
         }
-    } else {
+    }
+    if constexpr (EXACT && DT == AMASS_FP16) {
+        // the border within the fp32 numbers of one fp16 number; below the normal numbers they lie elsewhere
+        const auto far = [](float v) {
+            return fabsf(v - __uint_as_float((__float_as_uint(v) & ~0x1FFFu) | 0x1000u));
+        };
+        uint32_t near = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float p0, r0, p1, r1;
-            pair(half_f32<DT>(x[i], 0), half_f32<DT>(y[i], 0), 2 * i, p0, r0);
-            pair(half_f32<DT>(x[i], 1), half_f32<DT>(y[i], 1), 2 * i + 1, p1, r1);
-            x[i] = pack_half<DT>(p0, p1);
-            y[i] = pack_half<DT>(r0, r1);
+        for (int i = 0; i < 8; ++i) {
+            const float off = 0x1p-22f * (fabsf(f[i]) + fabsf(g[i])) * (fabsf(cs[i]) + fabsf(sn[i]));
+            near |= !(fminf(far(p[i]), far(r[i])) > off) || fminf(fabsf(p[i]), fabsf(r[i])) < 0x1p-14f ? 1u << i : 0u;
+        }
+        if (__any(near)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (near >> i & 1) {
+                    p[i] = (float)((double)f[i] * cs[i] - (double)g[i] * sn[i]);
+                    r[i] = (float)((double)g[i] * cs[i] + (double)f[i] * sn[i]);
+                }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (a.interleaved) {
+            x[i] = pack_half<DT>(p[i], r[i]);
+            y[i] = pack_half<DT>(p[4 + i], r[4 + i]);
+        } else {
+            x[i] = pack_half<DT>(p[2 * i], p[2 * i + 1]);
+            y[i] = pack_half<DT>(r[2 * i], r[2 * i + 1]);
         }
     }
 }
@@ -106,7 +128,7 @@ __device__ __forceinline__ void turn_queries(const amass_quant_write_args& a, ui
     uint16_t* dst = (uint16_t*)a.q_out + t * a.qo_st + head * a.qo_hs;
     u32x4_t x = *reinterpret_cast<const u32x4_t*>(src + c.c0);
     u32x4_t y = *reinterpret_cast<const u32x4_t*>(src + c.c1);
-    if (c.turn) turn<DT, float>(a, a.table + pos * a.tab_st + 8 * u, x, y);
+    if (c.turn) turn<DT, false>(a, a.table + pos * a.tab_st + 8 * u, x, y);
     *reinterpret_cast<u32x4_t*>(dst + c.c0) = x;
     *reinterpret_cast<u32x4_t*>(dst + c.c1) = y;
 }
@@ -194,7 +216,7 @@ __global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_qua
                     int pos = __shfl(ps, (i0 + r) & (WAVE - 1));
                     if (r < n && i0 + r >= WAVE) pos = a.positions[t + r];
                     if (r < n && c.turn)
-                        turn<DT, double>(a, a.table + (int64_t)pos * a.tab_st + 8 * u, x[i], y[i]);
+                        turn<DT, true>(a, a.table + (int64_t)pos * a.tab_st + 8 * u, x[i], y[i]);
                 }
             }
         };

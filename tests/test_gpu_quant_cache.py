@@ -145,6 +145,33 @@ def test_write_is_the_formula(name, dtype, code):
         assert (np.abs(q.double().cpu().numpy() - want) <= tol).all()
 
 
+@pytest.mark.parametrize("dtype,rot,interleaved", [("bf16", 128, False), ("bf16", 64, True), ("fp16", 128, True)])
+def test_turned_keys_are_rounded_as_in_64_bits(dtype, rot, interleaved):
+    """Millions of keys, of which some lie so near to a border of the 16-bit type that fp32 products round to
+    the other side: all codes are those of the products in float64."""
+    announce(f"quant write: keys at borders, {dtype}, {rot}")
+    T, H = 4096, 8
+    dt = TYPES[dtype]
+    g = torch.Generator(DEV).manual_seed(9)
+    k, v = (torch.randn(T, H, 128, generator=g, device=DEV).to(dt) for _ in range(2))
+    k[:, 1] *= 2.0 ** -15                          # fp16: below its normal numbers
+    pos = torch.randint(0, 60000, (T,), generator=g, device=DEV).int()
+    table = rope_table(rot, 60000, base=500000.0, device=DEV)
+    codes, scales = quant_cache(T // 16, 16, H, 128, device=DEV)
+    quant_paged_write(k, v, codes, scales, torch.arange(T, device=DEV), positions=pos, table=table,
+                      layout="interleaved" if interleaved else "half")
+    c, s = table[pos.long()].double()[:, None].chunk(2, -1)
+    x = k.double()
+    a, b = (x[..., 0:rot:2], x[..., 1:rot:2]) if interleaved else x[..., :rot].chunk(2, -1)
+    u, w = a * c - b * s, b * c + a * s
+    fast = a.float() * c.float() - b.float() * s.float()
+    assert (u.float().to(dt) != fast.to(dt)).any()             # (fp32 alone would not do)
+    turned = torch.stack([u, w], -1).flatten(-2) if interleaved else torch.cat([u, w], -1)
+    x = torch.cat([turned.float().to(dt).double(), x[..., rot:]], -1).view(T // 16, 16, H, 128)
+    scale = scales[:, 0].double()[:, None, :, None]
+    assert torch.equal(codes[:, 0].double(), (x / scale).round().clamp(-127, 127))
+
+
 def test_a_page_token_by_token():
     """Sixteen steps of one token: every growth of a scale rounds the earlier codes again."""
     announce("quant write: a page token by token")
