@@ -190,16 +190,18 @@ def _chunk_args(q, codes, scales, block_table, seq_lens, query_start, out, scale
                 lse):
     """(the argument struct's values up to the scratch, those behind it) of a checked call."""
     dt = q.dtype
-    if not (dt in DTYPES and dt is out.dtype):
+    if dt not in DTYPES or dt is not out.dtype:
         raise ValueError("q and out must both be bf16 or both fp16")
     (nb, page, n_kv, d), kind, c, s = _halves(codes, scales, False)
     shape = q.shape
-    if len(shape) != 3 or shape[2] != d or out.shape != shape:
+    if len(shape) != 3 or shape[2] != d or (out is not q and out.shape != shape):
         raise ValueError(f"q and out must be (T, H, {d})")
     T, H, _ = shape
     if H == 0 or H % n_kv:
         raise ValueError(f"{H} query heads are not a multiple of {n_kv} kv heads")
-    if window is not None and window < 1:
+    if window is None:
+        window = 0
+    elif window < 1:
         raise ValueError("window must be positive (None: no window)")
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale <= 2e38:                 # (times log2 e it stays finite)
@@ -214,9 +216,9 @@ def _chunk_args(q, codes, scales, block_table, seq_lens, query_start, out, scale
         raise ValueError("block_table must be (R, max_pages) int32 with unit column stride")
     q_st, q_hs, q_unit = q.stride()
     o_st, o_hs, o_unit = out.stride()
-    if not q_unit == o_unit == 1:
+    if q_unit != 1 or o_unit != 1:
         raise ValueError("q / out need unit stride on the head dim")
-    if not (o_st or T == 1) or not (o_hs or H == 1):
+    if (o_st == 0 and T > 1) or (o_hs == 0 and H > 1):
         raise ValueError("rows or heads of out share memory")
     l_at = l_st = l_hs = 0
     if lse is not None:
@@ -224,12 +226,12 @@ def _chunk_args(q, codes, scales, block_table, seq_lens, query_start, out, scale
             raise ValueError("lse must be (T, H) fp32")
         l_at = lse.data_ptr()
         l_st, l_hs = lse.stride()
-        if not (l_st or T == 1) or not (l_hs or H == 1):
+        if (l_st == 0 and T > 1) or (l_hs == 0 and H > 1):
             raise ValueError("rows or heads of lse share memory")
     return ((q.data_ptr(), q_st, q_hs, *c, *s, block_table.data_ptr(), bt_st, seq_lens.data_ptr(),
              query_start.data_ptr(), out.data_ptr(), o_st, o_hs, l_at, l_st, l_hs),
             (scale, n_req, T, n_kv, H // n_kv, d, page, nb, width, 1 if causal else 0,
-             min(window or 0, MAX_INT), DTYPES[dt], kind))
+             window if window < MAX_INT else MAX_INT, DTYPES[dt], kind))
 
 
 def _scratch_bytes(index, head, tail) -> int:
