@@ -175,11 +175,16 @@ struct Factors {                   // of N groups of 16 keys
 // nothing moves across (the order is the program's, and few values wait in registers)
 __device__ __forceinline__ void step() { __builtin_amdgcn_sched_barrier(0); }
 
+// The largest of 8 scores, by three a instruction.  (A NaN stays one: a maximum that drops it asks for
+// another instruction a score, which tells signalling ones apart.  Its row is not finite then, and is
+// done again with care.)
 __device__ __forceinline__ float group_max(const f32x16_t& s, int half) {
-    float mx = s[8 * half];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[8 * half + i]);
-    return mx;
+    const auto max3 = [](float a, float b, float c) {
+        return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+    };
+    const int i = 8 * half;
+    return max3(max3(max3(s[i], s[i + 1], s[i + 2]), s[i + 3], s[i + 4]), max3(s[i + 5], s[i + 6], s[i + 7]),
+                -INFINITY);
 }
 // the running maximum and sum for a higher maximum; the factor for O
 template <int D>
@@ -307,7 +312,7 @@ __device__ __forceinline__ void ordered_tile(uint32_t ks, uint32_t vs, const Lds
         const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][2 * i + 1], fa.sk[g], off[g]));
         sum[g] += e0 + e1;
         uint32_t w = pack2<DT>(e0, e1);
-        asm volatile("" : "+v"(w));            // (made here, not behind the branch below)
+        asm volatile("" : "+v"(w), "+v"(sum[g]));     // (made here, not behind the branch below)
         p[g][i & 3] = w;
     };
 #pragma unroll
