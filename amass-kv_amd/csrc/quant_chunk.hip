@@ -99,9 +99,10 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t x) {
     return ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
 }
 
-// 16 rows of codes of a page, 16 channels of a row in each of a lane's LOADS registers of 16 bytes.  Rows go
-// to lanes so that 16 neighbouring lanes, whose chunks of 16 bytes a phase of an LDS write takes, hold
-// two rows (d 64: four) with different swizzles and fill all banks once.
+// 16 rows of codes of a page, 16 channels of a row in each of a lane's LOADS registers of 16 bytes.  8 neighbouring
+// lanes, whose 16-byte chunks a cycle of an LDS write takes, hold 4 of each of two rows whose swizzles differ in the
+// lowest bit, so that they fill the banks once (with 8 lanes a row every write took two cycles for one, a quarter
+// of LDS' time).
 template <int D>
 struct Codes {
     static constexpr int LPR = D / 16, RPL = WAVE / LPR, LOADS = 16 / RPL;
@@ -110,9 +111,8 @@ struct Codes {
     int row;
 
     __device__ __forceinline__ Codes(uint32_t st_, int lane) : st(st_) {
-        const int r = lane / LPR, c = lane % LPR;
-        row = D == 128 ? (r >> 1) + 4 * (r & 1)
-                       : (r & 1) + 4 * ((r >> 1) & 1) + 2 * ((r >> 2) & 1) + 8 * (r >> 3);
+        const int c = (lane & 3) + (D == 128 ? (lane >> 1) & 4 : 0);
+        row = D == 128 ? (lane >> 4) + (lane & 4) : ((lane >> 3) & 3) + (lane & 4) + 8 * (lane >> 5);
         off = (uint32_t)row * st + 16 * c;
         lds = row * (2 * D) + (((2 * c) ^ swz<D>(row)) << 4);
     }
@@ -147,9 +147,9 @@ struct Codes {
         int bad = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) bad |= (int)nan_codes(v[j]);
-        if constexpr (LPR == 8) bad |= dpp_i<DPP_HALF_MIRROR>(bad);
         bad |= dpp_i<DPP_XOR2>(bad);
         bad |= dpp_i<DPP_XOR1>(bad);
+        if constexpr (LPR == 8) bad |= __shfl_xor(bad, 8);
         if (bad) {
             k = (u32x4_t){0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu};
             v = (u32x4_t){0u, 0u, 0u, 0u};
