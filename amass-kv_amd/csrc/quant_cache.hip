@@ -13,6 +13,10 @@
 // of v_max, six exchanges and at most one barrier.  Runs are found in the slots: where a block
 // starts or the one before is no neighbour.
 // Read: 16 codes a thread, two 16-byte stores (two such units a thread took 86 us where one takes 82).
+//
+// HBM bounds both: a prompt of 8192 tokens (32 + 8 heads of 128, bf16, turned; 189 MB) 44.7 us, 4.2 TB/s where a copy
+// reaches 4.8 to 5.1; its K and V alone 13 us; three chunks of 1967 tokens, fp16 in pairs, 12.0 us; 16 single tokens
+// 5 us, launch and two dependent rounds; 65536 tokens read back (403 MB) 81.5 us, 4.9 TB/s.
 #include "quant_codes.h"
 
 namespace amass {

@@ -9,6 +9,20 @@
 //   O  += w_j c'_j,  l += (sum of the 16 w_j) / sv    V's scale leaves the sum again, per 16 keys
 //   out = O / l,  lse = ln 2 (M + log2 l)
 // So a page costs a few instructions per 16 keys and nothing per key.
+//
+// Layouts, parts and results are those of chunk.hip (chunk_core.h).  Codes are widened to 16 bits on the way:
+//   many rows (more than 32): each wave brings 16 keys of a 64-key tile into registers two tiles ahead and writes
+//     them to LDS widened, one tile ahead, under the products with the tile before; an int8 takes 1.5 instructions
+//     (bf16; fp16 1.25), an e4m3 half a one, once for the four waves.  Vector work bounds it: a prompt of 8192 tokens
+//     (8 kv heads of 4 query heads, d 128, bf16) takes 577 us with int8, 10 vector instructions beside every product
+//     and 43 % of the matrix cores' cycles, 545 with e4m3, where chunk.hip over 16 bits takes 536; 2048 tokens
+//     behind 63488 2035 us with e4m3 (2007), 1.06 PFLOP/s.
+//   few rows: each wave brings its own 32 keys to LDS as they are, one step ahead, reads K by rows and V by columns
+//     of 8-bit elements, and widens them in registers.  Memory bounds it: 64 single tokens with 8k keys 196 us, 5.4 TB/s
+//     (16 bits: 335), 176 where the codes of a page of one head lie together (quant_cache), 6.1 TB/s; 8 requests of 4
+//     drafted tokens with 8k to 24k keys 67 us (104).  Tried there, to no gain: two heads a wave (256 neighbouring
+//     bytes a key, 196, and it needs more parts), all heads of a token in one workgroup (196), more in flight (206), loads
+//     that other caches keep (225).
 #include "chunk_core.h"
 #include "quant_codes.h"
 
