@@ -36,6 +36,10 @@ constexpr int QC_UP = 16;
 // alone reads them.
 constexpr float QC_ONCE = 128e6f;
 
+// Maxima beyond this take their request again with care: log2 sv less the maximum, rounded, moves the weights of
+// one page against another's by 2^-12 there, and from 2^27 on makes weights of any size.
+constexpr float QC_FAR = 0x1p12f;
+
 struct Scales {
     const float *k, *v;
     int64_t sb, sh;
@@ -228,18 +232,14 @@ __device__ __forceinline__ void mask_scores(f32x16_t (&s)[NK], int lo, int hi, u
 }
 
 // The weights of 32 NK keys, packed for the second product, and what they add to the maximum and the
-// sum.  CARE: for factors that are not finite, which must not reach what a row does not see, and for
-// maxima far from zero: the difference from them first, exact where it matters.
-template <int DT, int D, int NK, bool CARE>
+// sum.
+template <int DT, int D, int NK>
 __device__ __forceinline__ void weigh_tile(const f32x16_t (&s)[NK], const Factors<2 * NK>& f,
                                            RowState<D>& st, u32x4_t (&p)[2 * NK]) {
     float mx = -INFINITY;
 #pragma unroll
-    for (int g = 0; g < 2 * NK; ++g) {
-        const float gm = group_max(s[g >> 1], g & 1);
-        const float x = __builtin_fmaf(gm, f.sk[g], f.off[g]);
-        mx = fmaxf(mx, CARE && gm == -INFINITY ? -INFINITY : x);
-    }
+    for (int g = 0; g < 2 * NK; ++g)
+        mx = fmaxf(mx, __builtin_fmaf(group_max(s[g >> 1], g & 1), f.sk[g], f.off[g]));
     mx = xor32_maxf(mx);
     float al = 1.f;
     const bool lag = __any(mx - st.m > CK_LAZY);
@@ -252,24 +252,67 @@ __device__ __forceinline__ void weigh_tile(const f32x16_t (&s)[NK], const Factor
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + i], f.sk[g], off));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + i + 1], f.sk[g], off));
+            sum += e0 + e1;
+            p[g][i >> 1] = pack2<DT>(e0, e1);
+        }
+        step();
+        st.l = __builtin_fmaf(sum, f.inv[g], st.l);
+    }
+}
+
+// The same with care: for factors that are not finite, which must not reach what a row does not see, and for
+// scores far from zero, beside which log2 sv is lost.  The weights count from the largest key's product (st.m, rounded
+// as every product is, so that differences are exact where they matter) and its log2 sv (mo), kept apart.
+template <int DT, int D, int NK>
+__device__ __forceinline__ void weigh_careful(const f32x16_t (&s)[NK], const Factors<2 * NK>& f,
+                                              RowState<D>& st, float& mo, u32x4_t (&p)[2 * NK]) {
+#pragma clang fp contract(off)
+    float m = st.m, o = mo;
+    const auto larger = [&](float pm, float po) {      // (both half waves find the same one)
+        const float d = (pm - m) + (po - o);
+        const bool is = pm != -INFINITY && (d > 0.f || (d == 0.f && pm > m));
+        m = is ? pm : m;
+        o = is ? po : o;
+    };
+#pragma unroll
+    for (int g = 0; g < 2 * NK; ++g) larger(group_max(s[g >> 1], g & 1) * f.sk[g], f.off[g]);
+    larger(__shfl_xor(m, 32), __shfl_xor(o, 32));
+    const float al = __builtin_amdgcn_exp2f((st.m - m) + (mo - o));
+    st.m = m;
+    mo = o;
+    st.l *= al;
+    scale_o(st, al);
+#pragma unroll
+    for (int g = 0; g < 2 * NK; ++g) {
+        const float off = (f.off[g] - mo) + CK_LIFT<DT>;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
             float e[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const float sc = s[g >> 1][8 * (g & 1) + i + j];
-                float x = __builtin_fmaf(sc, f.sk[g], CARE ? -st.m : off);
-                if constexpr (CARE) {
-                    x += f.off[g] + CK_LIFT<DT>;
-                    x = x > CK_LIFT<DT> + CK_LAZY ? CK_LIFT<DT> + CK_LAZY : x;
-                    x = sc == -INFINITY ? -INFINITY : x;
-                }
-                e[j] = __builtin_amdgcn_exp2f(x);
+                const float x = (sc * f.sk[g] - m) + off;
+                e[j] = __builtin_amdgcn_exp2f(sc == -INFINITY ? -INFINITY : x);
                 sum += e[j];
             }
             p[g][i >> 1] = pack2<DT>(e[0], e[1]);
         }
         step();
-        if (!CARE || sum != 0.f) st.l = __builtin_fmaf(sum, f.inv[g], st.l);
+        if (sum != 0.f) st.l += sum * f.inv[g];
     }
+}
+// One number to count from again: the two together near zero, else the product, with the sums taken times sv
+// (2^-64 is its least; what a scale beyond 2^64 leaves goes to the product, which keeps O inside fp32).
+template <int D>
+__device__ __forceinline__ void careful_end(RowState<D>& st, float mo) {
+    const float o = fabsf(st.m) > QC_FAR ? fminf(mo, 64.f) : 0.f;
+    const float by = __builtin_amdgcn_exp2f(o);
+    st.m += mo - o;
+    st.l *= by;
+    scale_o(st, by);
 }
 
 template <int DT, int D, int NK>
@@ -498,13 +541,10 @@ __device__ __forceinline__ void few_values(uint32_t vs, const RawRows<D>& raw, c
         }
 }
 
-// whether a row that is there needs all of it again with care: it is not finite, or its maximum so far
-// from zero that log2 sv less the maximum, rounded, moves the weights of one page against
-// another's (by 2^-12 at 2^12, and in fp16 beyond its largest at 2^27)
-constexpr float QC_FAR = 0x1p12f;
+// whether a row that is there needs all of it again with care
 template <int D>
 __device__ __forceinline__ bool needs_care(const RowState<D>& st, bool live) {
-    const bool far = st.m > -__FLT_MAX__ && fabsf(st.m) > QC_FAR;
+    const bool far = st.m > -__FLT_MAX__ && fabsf(st.m) > QC_FAR;      // (it has seen something)
     float z[4] = {st.l * 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < D / 32; ++x)
@@ -794,6 +834,7 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
             again = __builtin_amdgcn_readfirstlane(lds.bad[0] | lds.bad[1] | lds.bad[2] | lds.bad[3]) != 0;
         }
         if (again) {
+            float mo = 0.f;
             reset(st);
             look(lk, CK_KEYS * (sp.lo + j0) + 16 * lane, 16 * WAVE);
             for (int j = j0, s = 0; j < j1; ++j) {
@@ -816,7 +857,7 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
                     u32x4_t p[4];
                     scores<DT, D, 2>(ks, ll, q, sc2);
                     mask_scores<2>(sc2, lo - t0, hi - t0, lk.groups(s), lane);
-                    weigh_tile<DT, D, 2, true>(sc2, f, st, p);
+                    weigh_careful<DT, D, 2>(sc2, f, st, mo, p);
                     add_values<DT, D, 2>(ks + KB, ll, p, st);
                 }
                 if (++s == Lookup<4>::STEPS) {
@@ -824,6 +865,7 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
                     s = 0;
                 }
             }
+            careful_end(st, mo);
         }
         if (idle) return;
         finish_rows<DT, D, QC_UP>(a, pl, it, kh, st, 1.f, row, group, whole, lane);
@@ -859,6 +901,7 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
         return false;
     };
     const auto walk = [&](auto past, auto care) {
+        float mo = 0.f;
         reset(st);
         bool full = true;                          // the usual number of loads of V is in flight
         if (b0 < b1) {
@@ -881,7 +924,8 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
             const Factors<2> f(lk, s);
             if (care || t0 < lo_hi || t0 + 32 > hi_lo)
                 mask_scores<1>(sc1, lo - t0, hi - t0, lk.groups(s), lane);
-            weigh_tile<DT, D, 1, care>(sc1, f, st, p);
+            if constexpr (care) weigh_careful<DT, D, 1>(sc1, f, st, mo, p);
+            else weigh_tile<DT, D, 1>(sc1, f, st, p);
             if (more && full) dma_wait<L>();       // (the next K may be)
             else dma_wait<0>();
             few_values<DT, CT, D, care>(vs, raw, p, st);
@@ -893,6 +937,7 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
             }
         }
         dma_wait<0>();
+        if constexpr (care) careful_end(st, mo);
     };
     if (once) walk(std::true_type(), std::false_type());
     else walk(std::false_type(), std::false_type());
