@@ -1,5 +1,6 @@
-"""Attention over the 8-bit cache where it could go wrong: scores beside which log2 of V's scale is lost,
-caches that are read past the GPU's own, starts that do not ascend, captured prompts that become padding."""
+"""The 8-bit cache where it could go wrong.  Attention: scores beside which log2 of V's scale is lost, caches that
+are read past the GPU's own, starts that do not ascend, captured prompts that become padding.  The write: batches
+of many tokens, whose runs start and end anywhere in the windows that are looked through."""
 import numpy as np
 import pytest
 import torch
@@ -7,6 +8,7 @@ import torch
 from amass.attention import quant_chunk_attention, quant_scratch_bytes
 from helpers import announce
 from test_gpu_chunk import want_on_gpu
+from test_gpu_quant_cache import Step
 from test_gpu_quant_chunk import CODES, DEV, QuantCase
 
 pytestmark = pytest.mark.gpu
@@ -142,3 +144,27 @@ def test_captured_prompts_become_padding_and_back(code, dtype):
             c.check(out, lse)
         else:
             assert (out == 7.0).all() and (lse == 7.0).all()
+
+
+LARGE = {         # more than 256 tokens are looked through by fours, more than 1024 by sixteens
+    "260 single tokens": dict(new=[1] * 260, had=[i % 50 for i in range(260)], n_kv=1),
+    "1100 single tokens": dict(new=[1] * 1100, had=[i * 7 % 40 for i in range(1100)], n_kv=1, d=64),
+    "runs of 1 to 21": dict(new=[1 + i * 5 % 21 for i in range(130)], had=[i * 11 % 37 for i in range(130)], n_kv=3),
+    "a prompt among drafts": dict(new=[3, 5, 1000, 2, 4, 90], had=[9, 14, 5, 15, 31, 0], rot=128),
+    "pages of 64, in pairs": dict(new=[61, 700, 1, 400], had=[3, 60, 63, 0], page=64, rot=64, interleaved=True, d=64),
+    "a run of a whole large page": dict(new=[7, 2100], had=[1, 1000], page=1024, n_kv=1, d=64, rot=32),
+}
+
+
+@pytest.mark.parametrize("dtype,code", [("bf16", "int8"), ("fp16", "e4m3")])
+@pytest.mark.parametrize("holes", [False, True])
+@pytest.mark.parametrize("name", LARGE)
+def test_writes_of_many_tokens(name, holes, dtype, code):
+    """The formula, exactly.  Holes: blocks that stay as they were, of padding in the middle of the batch."""
+    announce(f"quant write: {name}, {'holes, ' * holes}{dtype} {code}")
+    s = Step(dtype=dtype, code=code, **LARGE[name])
+    if holes:
+        s.slots[s.slots // s.page % 3 == 1] = -1
+    codes, scales = s.dev()
+    s.run(codes, scales, torch.full_like(s.q, 7.0).to(DEV))
+    s.check(codes, scales)
