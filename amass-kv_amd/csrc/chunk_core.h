@@ -539,10 +539,14 @@ __device__ __forceinline__ RowOut row_out(const amass_chunk_args& a, const Chunk
     return w;
 }
 
-// what O is multiplied by at the end (sums of 2^UP times the weights)
+// What O is multiplied by at the end, sums being 2^UP times those of the weights: ROW_UP, then row_scale.  In one, a
+// row of bf16 whose weight lies on a page of V scale s would take 2^8 s, beyond fp32 from s = 2^120 on (such a
+// page's numbers are in the type); of two, the second is 2^124 at most for any s.
+template <int UP>
+constexpr float ROW_UP = (float)(1 << (UP - UP / 4));
 template <int UP>
 __device__ __forceinline__ float row_scale(float l) {
-    return l == 0.f ? 0.f : (float)(1 << UP) / l;
+    return l == 0.f ? 0.f : (float)(1 << (UP / 4)) / l;
 }
 
 template <int DT, int UP>
@@ -649,7 +653,7 @@ __device__ __forceinline__ void merge_parts(const amass_chunk_args& a, const Chu
     const RowOut ro = row_out(a, pl, ct.q, kh, ct.tile * CK_BM + 32 * group + rl);
     const float inv = row_scale<UP>(l);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) o[j] *= inv;
+    for (int j = 0; j < 16; ++j) o[j] = o[j] * ROW_UP<UP> * inv;
     store_row<DT, D>(ro.out, x, o, lane);
     if (x == 0) store_lse<DT, UP>(ro, m, l, c, lane);
 }

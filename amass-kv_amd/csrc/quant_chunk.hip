@@ -567,7 +567,7 @@ __device__ __forceinline__ void finish_rows(const amass_chunk_args& a, const Chu
     for (int x = 0; x < D / 32; ++x) {
         float o[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = st.o[x][i] * (whole ? inv : 1.f);
+        for (int i = 0; i < 16; ++i) o[i] = whole ? st.o[x][i] * ROW_UP<UP> * inv : st.o[x][i];
         if (whole) store_row<DT, D>(ro.out, x, o, lane);
         else save_tile<D>(g, x, o, lane);
     }
@@ -624,7 +624,7 @@ __device__ __forceinline__ void finish_shared(const amass_chunk_args& a, const C
         const RowOut ro = row_out(a, pl, it.q, kh, row);
         const float inv = row_scale<UP>(l);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] *= inv;
+        for (int i = 0; i < 16; ++i) o[i] = o[i] * ROW_UP<UP> * inv;
         store_row<DT, D>(ro.out, w, o, lane);
         if (w == 0) store_lse<DT, UP>(ro, m, l, c, lane);
     } else {
