@@ -280,11 +280,7 @@ __global__ __launch_bounds__(QW_THREADS) void quant_write_kernel(const amass_qua
                 u32x4_t* at = reinterpret_cast<u32x4_t*>(codes + r * a.c_st + 16 * u);
                 u32x4_t z = *at;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float4 f = codes_f32<CT>(z[j]);
-                    z[j] = to_codes<CT>(quotient(f.x * old, div, inv), quotient(f.y * old, div, inv),
-                                        quotient(f.z * old, div, inv), quotient(f.w * old, div, inv));
-                }
+                for (int j = 0; j < 4; ++j) z[j] = round_again<CT>(z[j], old, div, inv);
                 *at = z;
             }
         }

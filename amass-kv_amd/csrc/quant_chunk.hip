@@ -112,11 +112,6 @@ struct Lookup {
 };
 
 // ------------------------------------------------------------------ staging
-// bit 7 of every byte that is an e4m3 NaN
-__device__ __forceinline__ uint32_t nan_codes(uint32_t x) {
-    return ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-}
-
 // 16 rows of codes of a page, 16 channels of a row in each of a lane's LOADS registers of 16 bytes.  8 neighbouring
 // lanes, whose 16-byte chunks a cycle of an LDS write takes, hold 4 of each of two rows whose swizzles differ in the
 // lowest bit, so that they fill the banks once (with 8 lanes a row every write took two cycles for one, a quarter

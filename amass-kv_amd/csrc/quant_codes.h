@@ -45,11 +45,16 @@ __device__ __forceinline__ float4 codes_f32(uint32_t x) {
     return make_float4(code_f32<CT, 0>(x), code_f32<CT, 1>(x), code_f32<CT, 2>(x), code_f32<CT, 3>(x));
 }
 
+// bit 7 of every byte that is an e4m3 NaN
+__device__ __forceinline__ uint32_t nan_codes(uint32_t x) {
+    return ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+}
+
 template <int CT>
 constexpr float MOST_CODE = CT == AMASS_INT8 ? 127.f : 448.f;
 
-// Four quotients as codes, half to even, at most the largest.  int8: 1.5 2^23 + y has the whole number in its
-// low byte.
+// Four quotients as codes, half to even, at most the largest (a NaN does not stay one).  int8: 1.5 2^23 + y has the
+// whole number in its low byte.
 template <int CT>
 __device__ __forceinline__ uint32_t to_codes(float y0, float y1, float y2, float y3) {
     const auto cap = [](float y) { return fminf(fmaxf(y, -MOST_CODE<CT>), MOST_CODE<CT>); };
@@ -85,6 +90,18 @@ __device__ __forceinline__ float step_of(float m) {
 __device__ __forceinline__ float quotient(float x, float s, float inv) {
     const float y = x * inv;
     return __builtin_fmaf(__builtin_fmaf(-y, s, x), inv, y);
+}
+
+// Four codes of scale `old` as those of scale s, inv = 1 / s.  An e4m3 NaN stays the code that it is: a cache that
+// was quantised elsewhere may hold some, and rows that see one are NaN.
+template <int CT>
+__device__ __forceinline__ uint32_t round_again(uint32_t z, float old, float s, float inv) {
+    const float4 f = codes_f32<CT>(z);
+    const uint32_t c = to_codes<CT>(quotient(f.x * old, s, inv), quotient(f.y * old, s, inv),
+                                    quotient(f.z * old, s, inv), quotient(f.w * old, s, inv));
+    if constexpr (CT == AMASS_INT8) return c;
+    const uint32_t nan = (nan_codes(z) >> 7) * 0xFFu;
+    return (c & ~nan) | (z & nan);
 }
 
 }  // namespace amass

@@ -34,7 +34,7 @@ extern "C" {
  *             e4m3: the smallest power of two with 448 step >= m;
  *             at least 2^-64, at most 2^121 (int8) or 2^119 (e4m3)
  *   s         step(m) where a = 0 (the block starts anew), else max(step(m), scale so far)
- *   rows < a  where s exceeds the scale so far: code = round(code * scale so far / s)
+ *   rows < a  where s exceeds the scale so far: code = round(code * scale so far / s), an e4m3 NaN as it is
  *   the run   code = round(x / s)
  *   scale     s
  * Quotients are rounded to fp32, then half to even to a code, at most the largest code.  Rows behind
