@@ -40,6 +40,14 @@ constexpr float QC_ONCE = 128e6f;
 // one page against another's by 2^-12 there, and from 2^27 on makes weights of any size.
 constexpr float QC_FAR = 0x1p12f;
 
+// fp16: V scales that are more powers of two than this from their first page's take their request with care, too.  A
+// weight with V's scale of 2^-21 of the largest has no bits to lose, so what counts in channels where a large page
+// holds zeros would.  As the rule leaves pages (12 powers of two apart), weights of a row's largest to 2^-9 of it keep
+// all bits everywhere.  Pages below 2^-35 do not count: their numbers are beneath half of fp16's least.  (With care a
+// prompt of 8192 tokens takes 1660 us for 630, 64 single tokens with 8k keys 414 for 198; the look at the scales 0.7 %.)
+constexpr float QC_APART = 6.f;
+constexpr float QC_NOUGHT = -35.f;
+
 struct Scales {
     const float *k, *v;
     int64_t sb, sh;
@@ -48,9 +56,10 @@ struct Scales {
 // The pages of a wave's next 64 groups of 16 keys, one a lane, PER of them a step (a tile of 64
 // keys, or a wave's 32): looked up once in 64 / PER steps, a period ahead, so that no step waits for
 // a table entry or a scale.
-template <int PER>
+template <int DT, int PER>
 struct Lookup {
     static constexpr int STEPS = WAVE / PER;
+    static constexpr uint32_t NO_REF = 0xFFFFFFFFu, APART = 0xFFFFFFFEu;      // (as numbers, NaN)
     const int32_t* table;          // the request's row
     const float *ks, *vs;          // of the kv head
     int64_t sb;
@@ -61,6 +70,8 @@ struct Lookup {
     float sk, off, inv;            // scale log2 e sk, log2 sv, 2^QC_UP / sv
     float next_k, next_v;
     unsigned long long has;
+    uint32_t ref;                  // fp16: log2 sv of the first page that counts (NO_REF: none so far), APART once
+                                   // a page is far from it
 
     __device__ __forceinline__ int find(int at) const {
         const int e = table[max(min(at, last), 0) >> sh];
@@ -80,11 +91,18 @@ struct Lookup {
         if (v < LEAST_SCALE) v = LEAST_SCALE;
         off = e < 0 ? -INFINITY : __log2f(v);      // (a page without a block: weights of zero)
         inv = (float)(1 << QC_UP) / v;
+        if constexpr (DT == AMASS_FP16) {
+            const unsigned long long counts = __ballot(off > QC_NOUGHT);
+            if (counts && ref == NO_REF)
+                ref = __builtin_amdgcn_readlane(__float_as_uint(off), __ffsll((long long)counts) - 1);
+            if (__any(off > QC_NOUGHT && fabsf(off - __uint_as_float(ref)) > QC_APART)) ref = APART;
+        }
     }
     // first: this lane's first position
     __device__ __forceinline__ void start(int first, int period) {
         t = first;
         jump = period;
+        ref = NO_REF;
         float k, v;
         const int e = find(t);
         fetch(e, k, v);
@@ -95,6 +113,7 @@ struct Lookup {
     __device__ __forceinline__ void ahead(int s) {
         if (s == STEPS / 2) fetch(next_id, next_k, next_v);
     }
+    __device__ __forceinline__ bool apart() const { return DT == AMASS_FP16 && ref == APART; }
     // behind its last step
     __device__ __forceinline__ void turn() {
         take(next_id, next_k, next_v);
@@ -174,8 +193,8 @@ struct Codes {
 template <int N>
 struct Factors {                   // of N groups of 16 keys
     float sk[N], off[N], inv[N];
-    template <int PER>
-    __device__ __forceinline__ Factors(const Lookup<PER>& lk, int s) {
+    template <int DT, int PER>
+    __device__ __forceinline__ Factors(const Lookup<DT, PER>& lk, int s) {
 #pragma unroll
         for (int g = 0; g < N; ++g) {
             sk[g] = readlane_f(lk.sk, PER * s + g);
@@ -257,12 +276,21 @@ __device__ __forceinline__ void weigh_tile(const f32x16_t (&s)[NK], const Factor
     }
 }
 
-// The same with care: for factors that are not finite, which must not reach what a row does not see, and for
-// scores far from zero, beside which log2 sv is lost.  The weights count from the largest key's product (st.m, rounded
-// as every product is, so that differences are exact where they matter) and its log2 sv (mo), kept apart.
+// The same with care: for factors that are not finite, which must not reach what a row does not see, for scores
+// far from zero, beside which log2 sv is lost, and for V scales far apart in fp16.  The weights count from the largest
+// key's product (st.m, rounded as every product is, so that differences are exact where they matter) and its log2 sv
+// (mo), kept apart.  Codes are exact in bf16, too, which has fp32's exponents: weights of fp16 rows are two numbers of
+// it each (16 bits together) and V's codes are widened to it.
+constexpr int CAREFUL_DT = AMASS_BF16;
+template <int DT>
+constexpr int LIMBS = DT == AMASS_FP16 ? 2 : 1;
+template <int N, int L>
+struct Weights {
+    u32x4_t p[L][N];
+};
 template <int DT, int D, int NK>
 __device__ __forceinline__ void weigh_careful(const f32x16_t (&s)[NK], const Factors<2 * NK>& f,
-                                              RowState<D>& st, float& mo, u32x4_t (&p)[2 * NK]) {
+                                              RowState<D>& st, float& mo, Weights<2 * NK, LIMBS<DT>>& wt) {
 #pragma clang fp contract(off)
     float m = st.m, o = mo;
     const auto larger = [&](float pm, float po) {      // (both half waves find the same one)
@@ -293,7 +321,13 @@ __device__ __forceinline__ void weigh_careful(const f32x16_t (&s)[NK], const Fac
                 e[j] = __builtin_amdgcn_exp2f(sc == -INFINITY ? -INFINITY : x);
                 sum += e[j];
             }
-            p[g][i >> 1] = pack2<DT>(e[0], e[1]);
+#pragma unroll
+            for (int k = 0; k < LIMBS<DT>; ++k) {
+                const uint32_t w = pack2<CAREFUL_DT>(e[0], e[1]);
+                wt.p[k][g][i >> 1] = w;
+                e[0] -= __uint_as_float(w << 16);
+                e[1] -= __uint_as_float(w & 0xFFFF0000u);
+            }
         }
         step();
         if (sum != 0.f) st.l += sum * f.inv[g];
@@ -310,14 +344,16 @@ __device__ __forceinline__ void careful_end(RowState<D>& st, float mo) {
     scale_o(st, by);
 }
 
-template <int DT, int D, int NK>
-__device__ __forceinline__ void add_values(uint32_t vs, const LdsLane<D>& ll, const u32x4_t (&p)[2 * NK],
+template <int D, int NK, int L>
+__device__ __forceinline__ void add_values(uint32_t vs, const LdsLane<D>& ll, const Weights<2 * NK, L>& wt,
                                            RowState<D>& st) {
 #pragma unroll
     for (int y = 0; y < 2 * NK; ++y)
 #pragma unroll
         for (int z = 0; z < D / 32; ++z) {
-            st.o[z] = mfma32<DT>(ll.v_frag(vs, z, y), p[y], st.o[z]);
+            const u32x4_t v = ll.v_frag(vs, z, y);
+#pragma unroll
+            for (int k = 0; k < L; ++k) st.o[z] = mfma32<CAREFUL_DT>(v, wt.p[k][y], st.o[z]);
             if (z & 1) step();
         }
 }
@@ -515,8 +551,9 @@ __device__ __forceinline__ void few_scores(uint32_t ks, uint32_t vs, const RawRo
     }
 }
 
-template <int DT, int CT, int D, bool CARE>
-__device__ __forceinline__ void few_values(uint32_t vs, const RawRows<D>& raw, const u32x4_t (&p)[2],
+// DT: the type of the weights; CARE: a NaN of V counts as zero (its key's score is NaN)
+template <int DT, int CT, int D, bool CARE, int L>
+__device__ __forceinline__ void few_values(uint32_t vs, const RawRows<D>& raw, const Weights<2, L>& wt,
                                            RowState<D>& st) {
 #pragma unroll
     for (int y = 0; y < 2; ++y)
@@ -532,20 +569,21 @@ __device__ __forceinline__ void few_values(uint32_t vs, const RawRows<D>& raw, c
                 f[2 * j] = lo;
                 f[2 * j + 1] = hi;
             }
-            st.o[z] = mfma32<DT>(f, p[y], st.o[z]);
+#pragma unroll
+            for (int k = 0; k < L; ++k) st.o[z] = mfma32<DT>(f, wt.p[k][y], st.o[z]);
         }
 }
 
 // whether a row that is there needs all of it again with care
 template <int D>
-__device__ __forceinline__ bool needs_care(const RowState<D>& st, bool live) {
+__device__ __forceinline__ bool needs_care(const RowState<D>& st, bool live, bool apart) {
     const bool far = st.m > -__FLT_MAX__ && fabsf(st.m) > QC_FAR;      // (it has seen something)
     float z[4] = {st.l * 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < D / 32; ++x)
 #pragma unroll
         for (int i = 0; i < 16; ++i) z[i & 3] = __builtin_fmaf(st.o[x][i], 0.f, z[i & 3]);
-    return __any(live && (far || !((z[0] + z[1]) + (z[2] + z[3]) == 0.f)));
+    return __any(live && (apart || far || !((z[0] + z[1]) + (z[2] + z[3]) == 0.f)));
 }
 
 // ------------------------------------------------------------------ results
@@ -730,7 +768,7 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
         // Wave w brings the 16 keys 64 j + 16 w .. of tile j: into registers during tile j - 2, widened into
         // LDS during tile j - 1.
         const uint32_t base = lds_addr(lds.kv);
-        Lookup<4> lk;
+        Lookup<DT, 4> lk;
         u32x4_t kr[LOADS], vr[LOADS];
         int lim = 16;                              // rows of the 16 that hold tokens
         const uint32_t own = base + 16 * w * 2 * D;
@@ -745,8 +783,8 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
         const auto put_k = [&](int buf, int i) {
             cd.template put<DT, CT>(own + 2 * KB * buf, i >> 1, i & 1, kr[i >> 1]);
         };
-        const auto put_v = [&](int buf, int i) {
-            cd.template put<DT, CT>(own + 2 * KB * buf + KB, i >> 1, i & 1, vr[i >> 1]);
+        const auto put_v = [&](int buf, int i, auto type) {
+            cd.template put<type, CT>(own + 2 * KB * buf + KB, i >> 1, i & 1, vr[i >> 1]);
         };
         const auto clip = [&] {
             if (lim < 16) {
@@ -754,11 +792,13 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
                 for (int n = 0; n < LOADS; ++n) cd.clip(vr[n], n, lim);
             }
         };
-        const auto put_all = [&](int buf) {
+        constexpr std::integral_constant<int, DT> usual;         // V's type in LDS
+        constexpr std::integral_constant<int, CAREFUL_DT> careful;
+        const auto put_all = [&](int buf, auto type) {
 #pragma unroll
             for (int i = 0; i < 2 * LOADS; ++i) {
                 put_k(buf, i);
-                put_v(buf, i);
+                put_v(buf, i, type);
                 step();
             }
         };
@@ -775,7 +815,7 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
             request_k();
             request_v();
             clip();
-            put_all(0);
+            put_all(0, usual);
             find(j0 + 1, 1);                       // (past the part: its keys are there or none are)
             request_k();
             request_v();
@@ -795,18 +835,18 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
                         put_k(buf, i);
                         if (i == 2 * LOADS - 1) request_k();
                     },
-                    [&](int i) { put_v(buf, i); });
+                    [&](int i) { put_v(buf, i, usual); });
                 request_v();
             };
             const auto pass = [&](int j) {         // a tile that none of the wave's rows see
                 clip();
-                put_all((j + 1 - j0) & 1);
+                put_all((j + 1 - j0) & 1, usual);
                 find(j + 2, s + 2);
                 request_k();
                 request_v();
             };
             const auto next = [&] {
-                if (++s == Lookup<4>::STEPS) {
+                if (++s == Lookup<DT, 4>::STEPS) {
                     lk.turn();
                     s = 0;
                 }
@@ -823,7 +863,7 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
             walk(j0, f0, std::true_type());
             walk(max(f0, j0), f1, std::false_type());
             walk(max(f1, j0), j1, std::true_type());     // (f1 may lie before this part)
-            const bool bad = needs_care(st, live);
+            const bool bad = needs_care(st, live, lk.apart());
             if (lane == 0) lds.bad[w] = bad;
             __syncthreads();
             again = __builtin_amdgcn_readfirstlane(lds.bad[0] | lds.bad[1] | lds.bad[2] | lds.bad[3]) != 0;
@@ -841,7 +881,7 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
 #pragma unroll
                     for (int n = 0; n < LOADS; ++n) cd.poison(kr[n], vr[n]);
                 }
-                put_all((j - j0) & 1);
+                put_all((j - j0) & 1, careful);
                 turn();
                 lk.ahead(s);
                 if (seen(j)) {
@@ -849,13 +889,13 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
                     const int t0 = CK_KEYS * (sp.lo + j);
                     const Factors<4> f(lk, s);
                     f32x16_t sc2[2];
-                    u32x4_t p[4];
+                    Weights<4, LIMBS<DT>> wt;
                     scores<DT, D, 2>(ks, ll, q, sc2);
                     mask_scores<2>(sc2, lo - t0, hi - t0, lk.groups(s), lane);
-                    weigh_careful<DT, D, 2>(sc2, f, st, mo, p);
-                    add_values<DT, D, 2>(ks + KB, ll, p, st);
+                    weigh_careful<DT, D, 2>(sc2, f, st, mo, wt);
+                    add_values<D, 2>(ks + KB, ll, wt, st);
                 }
-                if (++s == Lookup<4>::STEPS) {
+                if (++s == Lookup<DT, 4>::STEPS) {
                     lk.turn();
                     s = 0;
                 }
@@ -876,7 +916,7 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
     const uint32_t base = lds_addr(own);
     const int b0 = 2 * (sp.lo + j0) + w, b1 = 2 * (sp.lo + j1);
     const Raw raw((uint32_t)a.kv_st, lane);
-    Lookup<2> lk;
+    Lookup<DT, 2> lk;
     // 32 keys of step s (b: their number); of V true if the usual number of loads is in flight
     const auto issue_k = [&](auto past, int b, int s) {
 #pragma unroll
@@ -911,7 +951,7 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
             if (!care && full) dma_wait<L>();      // (V may be on its way)
             else dma_wait<0>();
             f32x16_t sc1[1];
-            u32x4_t p[2];
+            Weights<2, care ? LIMBS<DT> : 1> wt;
             few_scores<DT, CT, D, care>(ks, vs, raw, q, sc1[0]);
             dma_wait<63>();                        // (the reads have returned)
             if (more) issue_k(past, b + CK_WAVES, s + 1);
@@ -919,14 +959,14 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
             const Factors<2> f(lk, s);
             if (care || t0 < lo_hi || t0 + 32 > hi_lo)
                 mask_scores<1>(sc1, lo - t0, hi - t0, lk.groups(s), lane);
-            if constexpr (care) weigh_careful<DT, D, 1>(sc1, f, st, mo, p);
-            else weigh_tile<DT, D, 1>(sc1, f, st, p);
+            if constexpr (care) weigh_careful<DT, D, 1>(sc1, f, st, mo, wt);
+            else weigh_tile<DT, D, 1>(sc1, f, st, wt.p[0]);
             if (more && full) dma_wait<L>();       // (the next K may be)
             else dma_wait<0>();
-            few_values<DT, CT, D, care>(vs, raw, p, st);
+            few_values<care ? CAREFUL_DT : DT, CT, D, care>(vs, raw, wt, st);
             dma_wait<63>();
             if (more) full = issue_v(past, b + CK_WAVES, s + 1);
-            if (++s == Lookup<2>::STEPS) {
+            if (++s == Lookup<DT, 2>::STEPS) {
                 lk.turn();
                 s = 0;
             }
@@ -936,7 +976,7 @@ quant_chunk_kernel(const amass_chunk_args a, const Scales sc, const ChunkPlan pl
     };
     if (once) walk(std::true_type(), std::false_type());
     else walk(std::false_type(), std::false_type());
-    if (needs_care(st, live)) walk(std::false_type(), std::true_type());      // (this wave alone)
+    if (needs_care(st, live, lk.apart())) walk(std::false_type(), std::true_type());      // (this wave alone)
     __syncthreads();
     finish_shared<DT, D, QC_UP>(a, pl, it, kh, st, lds, 1.f, row, whole, w, lane);
 }
