@@ -4,15 +4,24 @@
   codes    (NB, 2, page, n_kv, d) or (2, NB, ...) int8 or float8_e4m3fn
   scales   (NB, 2, n_kv) or (2, NB, n_kv) fp32, one for each block, half (K, V) and kv head
 
-A number is ``code * scale``.  Beside ``rope_paged_write`` and ``paged_chunk_attention`` it takes half the
-memory and half the bytes of every decode step.  int8 resolves a block's numbers in 254 even
+A number is ``code * scale``; where both first axes are 2, the first is the halves (as a 16-bit cache is
+read).  Beside ``rope_paged_write`` and ``paged_chunk_attention`` it takes half the memory and half the
+bytes of every decode step.  int8 resolves a block's numbers in 254 even
 steps of its largest; e4m3 keeps 4 significant bits of each, for blocks of a few large numbers
 among small ones.
 
 A scale grows with its block: the write takes the largest magnitude of the tokens that enter the
 block now and of those that are there, and where the scale grows it rounds the earlier tokens' codes
-again.  The token in a block's first row starts the block anew.  Codes do not depend on how a
-prompt was cut into chunks where no scale grows, and differ by one step otherwise.
+again.  The token in a block's first row starts the block anew.  An int8 number is off by at most half
+a step of the last scale for its entry and for each growth after it.  So codes do not depend on how a
+prompt was cut into chunks where no scale grows; where it grows g times they differ by (2 + g) / 2
+steps at most (16 single tokens against one write: up to 2 steps among tokens of like size, several where
+each is 1 percent larger than the one before).  An e4m3 number keeps its 4 bits through growths until
+it is below 2^-6 of the scale.
+
+Rows behind a run keep their codes, not their numbers: a run from the block's first row, or one that
+makes the scale grow, leaves them under another scale.  So tokens enter a block in order; those that were
+taken back are written again before anyone sees them.
 
 All calls run on torch's current stream of the tensors' GPU, depend on shapes only, allocate
 nothing but the attention's scratch, never synchronise and can be captured in a HIP graph.
