@@ -14,9 +14,10 @@
 // starts or the one before is no neighbour.
 // Read: 16 codes a thread, two 16-byte stores (two such units a thread took 86 us where one takes 82).
 //
-// HBM bounds both: a prompt of 8192 tokens (32 + 8 heads of 128, bf16, turned; 189 MB) 44.7 us, 4.2 TB/s where a copy
-// reaches 4.8 to 5.1; its K and V alone 13 us; three chunks of 1967 tokens, fp16 in pairs, 12.0 us; 16 single tokens
-// 5 us, launch and two dependent rounds; 65536 tokens read back (403 MB) 81.5 us, 4.9 TB/s.
+// HBM bounds both: a prompt of 8192 tokens (32 + 8 heads of 128, bf16, turned; 189 MB) 45 us, 4.2 TB/s where a copy
+// reaches 4.8 to 5.1; its K and V alone, not turned, 13.5 us; three chunks of 1967 tokens, fp16 in pairs, 12.7 us among
+// other calls and 13.9 in a graph, where launches do not overlap; 16 single tokens 5 us, launch and two dependent
+// rounds; 65536 tokens read back (403 MB) 81.5 us, 4.9 TB/s.
 #include "quant_codes.h"
 
 namespace amass {
@@ -52,8 +53,8 @@ __device__ __forceinline__ Chan channels(const amass_quant_write_args& a, int u,
 // the 8 pairs of x (c0 ..) and y (c1 ..) turned: pair i is (x[i], y[i]), or interleaved two neighbours.
 // EXACT: the 16-bit numbers that the products in 64 bits round to (through fp32).  The fp32 ones are off by less than
 // 2^-22 (|f| + |g|) (|c| + |s|), so they round to others only that near to a border between two, once in thousands.
-// fp16 asks 64 bits only there, bf16 always (us of three chunks of 1967 tokens: fp16 14.8 and paired 16.6 with 64 bits
-// always, 13.7 and 13.7 so; bf16 12.3 and 12.4 always, 12.7 and 12.8 so).
+// fp16 asks 64 bits only there, bf16 always (us of three chunks of 1967 tokens in a graph: fp16 14.8 and paired 16.6
+// with 64 bits always, 13.7 and 13.7 so; bf16 12.3 and 12.4 always, 12.7 and 12.8 so).
 template <int DT, bool EXACT>
 __device__ __forceinline__ void turn(const amass_quant_write_args& a, const float* tab, u32x4_t& x,
                                      u32x4_t& y) {
@@ -113,7 +114,10 @@ constexpr int QW_ROWS = 16;              // rows that a wave holds
 // Tokens that a workgroup looks for runs in: one, 4 or 16 by the batch's tokens.  The runs of a window follow each
 // other, about 1 us each, and a workgroup that finds none costs as much of a place.  us in a graph with windows of
 // 1 / 4 / 16 (32 + 8 heads of 128): 256 single tokens 6.3 / 8.8 / 28.5, a prompt of 256 7.7 / 5.1 / 4.6; 1024: 19.9
-// / 17.5 / 32.0 and 17.2 / 10.5 / 7.1; 2048: 36.3 / 30.3 / 38.5 and 30.3 / 17.5 / 10.5.
+// / 17.5 / 32.0 and 17.2 / 10.5 / 7.1; 2048: 36.3 / 30.3 / 38.5 and 30.3 / 17.5 / 10.5.  The number of tokens is all that
+// the host knows (which kind they are is in the slots), so each border weighs both: up to 256 the rule is single
+// tokens' best, and costs a prompt 3 us; up to 1024 it is the least sum; beyond, a batch is a prompt's rather than
+// thousands of single tokens, which take 8 us more by it.
 constexpr int window_of(int tokens) { return tokens <= 256 ? 1 : tokens <= 1024 ? 4 : 16; }
 
 template <int D>

@@ -14,15 +14,17 @@
 //   many rows (more than 32): each wave brings 16 keys of a 64-key tile into registers two tiles ahead and writes
 //     them to LDS widened, one tile ahead, under the products with the tile before; an int8 takes 1.5 instructions
 //     (bf16; fp16 1.25), an e4m3 half a one, once for the four waves.  Vector work bounds it: a prompt of 8192 tokens
-//     (8 kv heads of 4 query heads, d 128, bf16) takes 577 us with int8, 10 vector instructions beside every product
-//     and 43 % of the matrix cores' cycles, 545 with e4m3, where chunk.hip over 16 bits takes 536; 2048 tokens
-//     behind 63488 2035 us with e4m3 (2007), 1.06 PFLOP/s.
+//     (8 kv heads of 4 query heads, d 128, bf16) takes 576 us with int8, 10 vector instructions beside every product
+//     and 43 % of the matrix cores' cycles, 539 with e4m3, where chunk.hip over the same numbers in 16 bits takes
+//     507 and 490; 2048 tokens behind 63488 2034 us with e4m3 (1820), 1.06 PFLOP/s.  Cards differ: 576 to 601,
+//     2022 to 2106.  d 64: the prompt 359 and 342 us (312 and 304).
 //   few rows: each wave brings its own 32 keys to LDS as they are, one step ahead, reads K by rows and V by columns
-//     of 8-bit elements, and widens them in registers.  Memory bounds it: 64 single tokens with 8k keys 196 us, 5.4 TB/s
-//     (16 bits: 335), 176 where the codes of a page of one head lie together (quant_cache), 6.1 TB/s; 8 requests of 4
-//     drafted tokens with 8k to 24k keys 67 us (104).  Tried there, to no gain: two heads a wave (256 neighbouring
-//     bytes a key, 196, and it needs more parts), all heads of a token in one workgroup (196), more in flight (206), loads
-//     that other caches keep (225).
+//     of 8-bit elements, and widens them in registers.  Memory bounds it: 64 single tokens with 8k keys 196 to 207 us, 5.1
+//     to 5.4 TB/s (16 bits: 341), 177 where the codes of a page of one head lie together (quant_cache), 6.0 TB/s; 8
+//     requests of 4 drafted tokens with 8k to 24k keys 68 us, in a graph over two caches in turn 73 (110) and 64.  Tried
+//     there where 64 single tokens took 196, to no gain: two heads a wave (256 neighbouring bytes a key, 196, and it
+//     needs more parts), all heads of a token in one workgroup (196), more in flight (206), loads that other caches
+//     keep (225).
 #include "chunk_core.h"
 #include "quant_codes.h"
 

@@ -38,8 +38,8 @@ extern "C" {
  *   the run   code = round(x / s)
  *   scale     s
  * Quotients are rounded to fp32, then half to even to a code, at most the largest code.  Rows behind
- * the run keep their codes, under the scale that is then the block's.  A number that is not finite makes s NaN and the run's codes zero; the
- * scale stays NaN until the block starts anew.
+ * the run keep their codes, under the scale that is then the block's.  A number that is not finite
+ * makes s NaN and the run's codes zero; the scale stays NaN until the block starts anew.
  *   x of V is v; x of K is k or, with `table` ((max_pos, rot): cos | sin, as amass_rope_write), k
  * turned by its position in 64 bits and rounded to fp32 and to the element type.  With q, q_out
  * receives q turned, as amass_rope_write turns it, for every token whose position is in the table.
