@@ -335,13 +335,15 @@ __device__ __forceinline__ void weigh_careful(const f32x16_t (&s)[NK], const Fac
         if (sum != 0.f) st.l += sum * f.inv[g];
     }
 }
-// One number to count from again: the two together near zero, else the product, with the sums taken times sv
-// (2^-64 is its least; what a scale beyond 2^64 leaves goes to the product, which keeps O inside fp32).
+// One number to count from again: the two together near zero, else the product, with the sums taken times sv.  Those
+// are 2^-QC_DOWN times that, for any sv's sake, and the number is larger by it: the same for every wave, so that what
+// is lost of it beside a product beyond 2^24 is lost of all alike.
+constexpr float QC_DOWN = 32.f;
 template <int D>
 __device__ __forceinline__ void careful_end(RowState<D>& st, float mo) {
-    const float o = fabsf(st.m) > QC_FAR ? fminf(mo, 64.f) : 0.f;
-    const float by = __builtin_amdgcn_exp2f(o);
-    st.m += mo - o;
+    const bool far = fabsf(st.m) > QC_FAR;
+    const float by = __builtin_amdgcn_exp2f(far ? mo - QC_DOWN : 0.f);
+    st.m += far ? QC_DOWN : mo;
     st.l *= by;
     scale_o(st, by);
 }

@@ -1,10 +1,12 @@
 """Attention over the 8-bit cache where V holds the largest numbers of bf16: scales up to those that the write
 makes of them (2^121 int8, 2^119 e4m3), and larger ones of caches quantised elsewhere."""
+import numpy as np
 import pytest
 import torch
 
 from helpers import announce
 from test_gpu_quant_chunk import QuantCase
+from test_gpu_quant_edges import far_case
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +60,22 @@ def test_pages_of_the_largest_numbers(new, lens, code, exponent):
     out, lse = c.run()
     assert torch.isfinite(out.float()).all()
     c.check(out, lse)
+
+
+@pytest.mark.parametrize("e", [13, 20, 31, 60])
+@pytest.mark.parametrize("new,lens", [([4], [300]), ([150], [400]), ([1], [9000]), ([40], [9000])])
+def test_scores_far_from_zero_beside_the_largest_v_scales(new, lens, e):
+    """Equal scores of 2^e, on pages of V scales from 2^56 to 2^116: the pages of the largest take all, and as much
+    each as its scale says.  Tolerances of test_scores_far_from_zero."""
+    announce(f"quant attention: scores of 2^{e}, V scales to 2^116, {new} of {lens}")
+    for sign in (1, -1):
+        c = far_case(new, lens, e, sign)
+        g = torch.Generator().manual_seed(5)
+        c.scales[:, 1] *= torch.exp2(torch.randint(62, 121, c.scales[:, 1].shape, generator=g).float())
+        c.numbers()
+        out, lse = c.run()
+        want, wlse, _, size, _ = c.want()
+        tol = torch.finfo(c.dt).eps / 2 * (1.01 * size + np.abs(want)) + 2.0 ** -14 * size
+        err = np.abs(out.double().cpu().numpy() - want)
+        assert (err <= tol).all(), (np.argwhere(~(err <= tol))[:4], (err / tol).max())
+        assert (np.abs(lse.double().cpu().numpy() - wlse) <= 5 * 2.0 ** -24 * np.abs(wlse) + 2.0 ** -14).all()
