@@ -277,7 +277,7 @@ def quant_chunk_attention(q, codes, scales, block_table, seq_lens, query_start, 
     (``lse``: -inf); rows of no request stay as they are.
 
     Scales are positive, V's count as at least 2^-64 and those of one request and kv head lie within
-    2^80 of each other.  A scale that is not finite makes NaN of the rows that see its page, a NaN
+    2^80 of each other (pages of zeros aside, beside V of up to 2^40).  A scale that is not finite makes NaN of the rows that see its page, a NaN
     code of those that see its key."""
     index = device_index(q, codes, scales, block_table, seq_lens, query_start, out, lse, scratch)
     head, tail = _chunk_args(q, codes, scales, block_table, seq_lens, query_start, out, scale,

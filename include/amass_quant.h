@@ -84,9 +84,10 @@ int amass_quant_read(const amass_quant_read_args* a, void* stream);
  * enter the products as they are, exact in the element type; K's scale multiplies the score, V's the
  * weight before its one rounding to the element type; sums and statistics are fp32.
  *   Scales are positive; V's count as at least 2^-64, and those of one request and kv head should lie
- * within 2^80 of each other (a weight that much below the largest is lost).  A scale that is not
- * finite makes NaN of the rows that see its page; a code that is NaN makes NaN of the rows that see
- * its key.  What is not visible is not used, whatever it holds.  q is finite. */
+ * within 2^80 of each other (a weight that much below the largest is lost; pages of zeros, whose scale
+ * the write makes 2^-64, count in full beside V of up to 2^40).  A scale that is not finite makes NaN of
+ * the rows that see its page; a code that is NaN makes NaN of the rows that see its key.  What is not
+ * visible is not used, whatever it holds.  q is finite. */
 typedef struct amass_quant_chunk_args {
     const void*    q; int64_t q_st, q_hs;                /* (T,H,d) */
     const void*    k_codes; const void* v_codes;         /* (NB,page,n_kv,d) views of */

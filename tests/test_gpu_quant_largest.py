@@ -79,3 +79,18 @@ def test_scores_far_from_zero_beside_the_largest_v_scales(new, lens, e):
         err = np.abs(out.double().cpu().numpy() - want)
         assert (err <= tol).all(), (np.argwhere(~(err <= tol))[:4], (err / tol).max())
         assert (np.abs(lse.double().cpu().numpy() - wlse) <= 5 * 2.0 ** -24 * np.abs(wlse) + 2.0 ** -14).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("new,lens,d", [([4, 1], [300, 90], 128), ([150], [400], 64), ([2], [9000], 128)])
+def test_pages_of_zeros_count_in_full(new, lens, d, dtype):
+    """Every other page of V is zeros under the least scale, beside numbers of 2^40 (fp16: 2^12): its keys' weights
+    are in every row's sum."""
+    announce(f"quant attention: pages of zeros beside large numbers, {new} of {lens}, {d}, {dtype}")
+    c = QuantCase(new=new, lens=lens, n_kv=2, d=d, dtype=dtype)
+    c.scales[:, 1] *= 2.0 ** (38 if dtype == "bf16" else 10)
+    for r, n in enumerate(lens):
+        zero = c.table[r, :-(-n // 16)][r % 2::2].long()
+        c.codes[zero, 1], c.scales[zero, 1] = 0, 2.0 ** -64
+    c.numbers()
+    c.check(*c.run())
