@@ -16,8 +16,8 @@
 //
 // HBM bounds both: a prompt of 8192 tokens (32 + 8 heads of 128, bf16, turned; 189 MB) 45 us, 4.2 TB/s where a copy
 // reaches 4.8 to 5.1; its K and V alone, not turned, 13.5 us; three chunks of 1967 tokens, fp16 in pairs, 12.7 us among
-// other calls and 13.9 in a graph, where launches do not overlap; 16 single tokens 5 us, launch and two dependent
-// rounds; 65536 tokens read back (403 MB) 81.5 us, 4.9 TB/s.
+// other calls, 13.9 in a graph over two batches in turn, the kernel alone 14.5 from an idle card; 16 single tokens 5 us,
+// launch and two dependent rounds; 65536 tokens read back (403 MB) 81.5 us, 4.9 TB/s.
 #include "quant_codes.h"
 
 namespace amass {

@@ -72,7 +72,7 @@ struct Lookup {
     float sk, off, inv;            // scale log2 e sk, log2 sv, 2^QC_UP / sv
     float next_k, next_v;
     unsigned long long has;
-    uint32_t ref;                  // fp16: log2 sv of the first page that counts (NO_REF: none so far), APART once
+    uint32_t ref = NO_REF;         // fp16: log2 sv of the first page that counts (NO_REF: none so far), APART once
                                    // a page is far from it
 
     __device__ __forceinline__ int find(int at) const {
